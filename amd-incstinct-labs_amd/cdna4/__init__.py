@@ -38,7 +38,8 @@ __all__ = [
     "rope_table_f32", "flash_attn", "flash_attn_decode", "CDNA4Error", "PrefillStrides", "prefill_strided",
     "scatter_kv_f16", "repack_f16", "rope_append_kv_f16", "ModelCfg", "GenerateCfg", "Session",
     "PlanInfo", "prefill_plan", "decode_plan", "scan_status", "KERNEL_NAMES", "decode_noalloc",
-    "decode_noalloc_max_bytes", "softmax_rows_f32",
+    "decode_noalloc_max_bytes", "softmax_rows_f32", "PackedPrefillCfg", "PackedStrides", "prefill_packed",
+    "prefill_packed_plan",
 ]
 
 # Element types and operators (include/cdna4_attn.h).
@@ -82,6 +83,18 @@ class DecodeCfg(ctypes.Structure):
         super().__init__(D, N, nQHeads, nKVHeads, batch, stride_kv)
 
 
+class PackedPrefillCfg(ctypes.Structure):
+    """cdna4_packed_cfg: `batch` prompts of different lengths in `total` tokens; max_seq 0 = unknown; `prefix`
+    keys that all of them see first (stride_prefix rows between kv heads, 0 = packed)."""
+    _fields_ = [(n, ctypes.c_int) for n in ("D", "nQHeads", "nKVHeads", "batch", "total", "max_seq", "prefix",
+                                            "stride_prefix")]
+
+
+class PackedStrides(ctypes.Structure):
+    """cdna4_packed_strides: element strides between tokens (row) and heads of Q, of K and V, and of O."""
+    _fields_ = [(n, ctypes.c_longlong) for n in ("q_row", "q_head", "kv_row", "kv_head", "o_row", "o_head")]
+
+
 class ModelCfg(ctypes.Structure):
     """cdna3_model_cfg: the reference's ModelConfig (runtime/model_loader.hpp:52-61) plus the
     qkv_bias flag and the norm kind and epsilon."""
@@ -108,7 +121,7 @@ class PlanInfo(ctypes.Structure):
 
 # CDNA4_KERNEL_* (include/cdna4_attn.h)
 KERNEL_NAMES = {1: "fa_mfma_8w", 2: "fa_mfma_4w", 3: "fa_small", 4: "fa_f32", 5: "decode_split", 6: "decode_wg",
-                7: "fa_mfma_keys"}
+                7: "fa_mfma_keys", 8: "fa_packed"}
 
 
 def DecodeDmeCfg(D: int, N: int, nQHeads: int, nKVHeads: int, stride_kv: int, batch: int = 1) -> DecodeCfg:
@@ -140,6 +153,10 @@ def _declare(l: ctypes.CDLL) -> None:
         "cdna3_attn_decode_noalloc_max_bytes": (c_size, []),
         "cdna3_attn_prefill_plan": (c_int, [ctypes.POINTER(PrefillCfg), c_int, ctypes.POINTER(PlanInfo)]),
         "cdna3_attn_decode_plan": (c_int, [ctypes.POINTER(DecodeCfg), c_int, c_int, ctypes.POINTER(PlanInfo)]),
+        "cdna4_attn_prefill_packed": (c_int, [vp] * 7 + [ctypes.POINTER(PackedPrefillCfg),
+                                                         ctypes.POINTER(PackedStrides), c_int, vp]),
+        "cdna4_attn_prefill_packed_plan": (c_int, [ctypes.POINTER(PackedPrefillCfg), c_int,
+                                                   ctypes.POINTER(PlanInfo)]),
         "cdna3_scan_status": (c_int, [vp, ctypes.POINTER(c_int), vp]),
         "cdna3_model_load": (c_int, [ctypes.c_char_p, ctypes.POINTER(vp)]),
         "cdna3_model_free": (None, [vp]),
@@ -281,6 +298,84 @@ def prefill_strided(Q: torch.Tensor, K: torch.Tensor, V: torch.Tensor, O: torch.
         raise ValueError("Q, K, V, O must share one dtype")
     _check(lib().cdna3_attn_prefill_strided(_ptr(Q), _ptr(K), _ptr(V), _ptr(O), ctypes.byref(cfg),
                                             ctypes.byref(strides), dt, _stream(stream)), "cdna3_attn_prefill_strided")
+
+
+def _device_of(t: torch.Tensor, *others: Optional[torch.Tensor]) -> int:
+    """Index of the GPU that t lies on; the other tensors have to lie there too."""
+    dev = t.get_device()
+    if dev < 0:
+        raise ValueError("tensors must be on the GPU")
+    for x in others:
+        if x is not None and x.get_device() != dev:
+            raise ValueError("tensors must be on one GPU")
+    return dev
+
+
+def _on_device(dev: int):
+    """Context in which dev is the current device, so that a call goes to its tensors' device."""
+    return _NO_STREAM if torch.cuda.current_device() == dev else torch.cuda.device(dev)
+
+
+def _token_major(name: str, t: torch.Tensor, T: int, heads: int, D: int):
+    """(token stride, head stride) of t [>= T][heads][D]; an axis of one element gets the packed stride."""
+    n, h, d = t.shape if t.dim() == 3 else (-1, 0, 0)
+    if n < T or h != heads or d != D:
+        raise ValueError(f"{name} must be [total][heads][D]")
+    row, head, one = t.stride()
+    if one != 1 and T:
+        raise ValueError(f"{name} must have contiguous rows of D")
+    return (row if n > 1 else heads * D), (head if h > 1 else D)
+
+
+def prefill_packed(Q: torch.Tensor, K: torch.Tensor, V: torch.Tensor, O: torch.Tensor, cu_seqlens: torch.Tensor,
+                   cfg: PackedPrefillCfg, K_prefix: Optional[torch.Tensor] = None,
+                   V_prefix: Optional[torch.Tensor] = None, stream=None) -> None:
+    """Causal attention over prompts of different lengths, packed token after token: Q, O [total][nQH][D];
+    K, V [total][nKVH][D] (fp16 or bf16, any token and head strides with contiguous rows of D: parts of
+    one projection's output, for instance); cu_seqlens int32 [batch + 1] on the device. With
+    cfg.prefix > 0 every token also sees the first `prefix` rows of K_prefix / V_prefix [nKVH][stride][D].
+    Rows of O outside cu_seqlens[0] .. cu_seqlens[batch] are left as they are."""
+    dev = _device_of(Q, K, V, O, cu_seqlens, K_prefix, V_prefix)
+    dt, dtype = _dtype(Q), Q.dtype
+    if not (K.dtype == V.dtype == O.dtype == dtype):
+        raise ValueError("Q, K, V, O must share one dtype")
+    T, D, P = cfg.total, cfg.D, cfg.prefix
+    kv = _token_major("K", K, T, cfg.nKVHeads, D)
+    if _token_major("V", V, T, cfg.nKVHeads, D) != kv:
+        raise ValueError("K and V must have the same strides")
+    st = PackedStrides(*_token_major("Q", Q, T, cfg.nQHeads, D), *kv, *_token_major("O", O, T, cfg.nQHeads, D))
+    if cu_seqlens.dtype != torch.int32 or not cu_seqlens.is_contiguous() or cu_seqlens.numel() < cfg.batch + 1:
+        raise ValueError("cu_seqlens must be contiguous int32 [batch + 1]")
+    kp = vp = 0
+    if P > 0:
+        kp, vp = _prefix_ptrs(K_prefix, V_prefix, dtype, cfg.nKVHeads * (cfg.stride_prefix or P) * D)
+    with _on_device(dev):
+        _check(lib().cdna4_attn_prefill_packed(Q.data_ptr(), K.data_ptr(), V.data_ptr(), kp, vp, O.data_ptr(),
+                                               cu_seqlens.data_ptr(), ctypes.byref(cfg), ctypes.byref(st), dt,
+                                               _stream(stream)), "cdna4_attn_prefill_packed")
+
+
+def _prefix_ptrs(K_prefix, V_prefix, dtype, need: int):
+    """Addresses of the shared prefix's K and V, checked against the `need` elements of the configuration."""
+    if K_prefix is None or V_prefix is None:
+        raise ValueError("prefix > 0 needs K_prefix and V_prefix")
+    if not (K_prefix.dtype == V_prefix.dtype == dtype):
+        raise ValueError("K_prefix, V_prefix must have the dtype of the queries")
+    if not (K_prefix.is_contiguous() and V_prefix.is_contiguous()):
+        raise ValueError("K_prefix, V_prefix must be contiguous")
+    if min(K_prefix.numel(), V_prefix.numel()) < need:
+        raise ValueError("K_prefix/V_prefix smaller than the configuration")
+    return K_prefix.data_ptr(), V_prefix.data_ptr()
+
+
+def prefill_packed_plan(cfg: PackedPrefillCfg, dtype=BF16) -> PlanInfo:
+    """The kernel cdna4_attn_prefill_packed would launch for cfg on the current device."""
+    if isinstance(dtype, torch.dtype):
+        dtype = _TORCH_DTYPES[dtype]
+    out = PlanInfo()
+    _check(lib().cdna4_attn_prefill_packed_plan(ctypes.byref(cfg), dtype, ctypes.byref(out)),
+           "cdna4_attn_prefill_packed_plan")
+    return out
 
 
 def decode_workspace_size(cfg: DecodeCfg) -> int:

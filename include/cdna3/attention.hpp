@@ -80,6 +80,27 @@ inline hipError_t prefill(const float* Q, const float* K, const float* V, float*
     return detail::prefill_any(Q, K, V, O, cfg, CDNA4_F32, stream);
 }
 
+// New: packed prompts of different lengths (cdna4_attn_prefill_packed). Token-major Q, O [total][nQH][D], K, V
+// [total][nKVH][D], or any strides; cu_seqlens int32 [batch + 1] in device memory; prefix keys [nKVH][stride][D].
+using PackedCfg = cdna4_packed_cfg;
+using PackedStrides = cdna4_packed_strides;
+inline PackedStrides packed_strides(const PackedCfg& c) {
+    return PackedStrides{(long long)c.nQHeads * c.D, c.D, (long long)c.nKVHeads * c.D, c.D, (long long)c.nQHeads * c.D, c.D};
+}
+inline hipError_t prefill_packed(const __half* Q, const __half* K, const __half* V, __half* O, const int* cu_seqlens,
+                                 const PackedCfg& cfg, const PackedStrides& strides, const __half* K_prefix = nullptr,
+                                 const __half* V_prefix = nullptr, hipStream_t stream = nullptr) {
+    return (hipError_t)cdna4_attn_prefill_packed(Q, K, V, K_prefix, V_prefix, O, cu_seqlens, &cfg, &strides, CDNA4_F16,
+                                                 (cdna4_stream_t)stream);
+}
+inline hipError_t prefill_packed(const __hip_bfloat16* Q, const __hip_bfloat16* K, const __hip_bfloat16* V,
+                                 __hip_bfloat16* O, const int* cu_seqlens, const PackedCfg& cfg,
+                                 const PackedStrides& strides, const __hip_bfloat16* K_prefix = nullptr,
+                                 const __hip_bfloat16* V_prefix = nullptr, hipStream_t stream = nullptr) {
+    return (hipError_t)cdna4_attn_prefill_packed(Q, K, V, K_prefix, V_prefix, O, cu_seqlens, &cfg, &strides, CDNA4_BF16,
+                                                 (cdna4_stream_t)stream);
+}
+
 // q[batch x nQH x D], K/V[batch x nKVH x N x D], o[batch x nQH x D].
 inline hipError_t decode(const __half* q, const __half* K, const __half* V, __half* o, const DecodeCfg& cfg,
                          hipStream_t stream = nullptr) {

@@ -123,6 +123,49 @@ int cdna3_attn_prefill_strided(const void* Q, const void* K, const void* V, void
                                const cdna3_prefill_strides* strides, int dtype,
                                cdna4_stream_t stream);
 
+/* ---- attention: packed prompts -------------------------------------------------
+ * No counterpart in the reference. Causal attention over `batch` prompts of different lengths whose
+ * tokens lie one after another: sequence s holds tokens cu_seqlens[s] .. cu_seqlens[s + 1] - 1 (int32,
+ * device memory, read when the kernel runs, so a captured call replays on other lengths; not
+ * decreasing, 0 <= cu_seqlens[s] <= total; an empty sequence has none). Token i of a sequence sees its
+ * sequence's tokens 0 .. i and, with prefix > 0, every one of the `prefix` keys that all sequences share:
+ * a system prompt whose keys are in the cache already. Query head h reads kv head h / (nQHeads / nKVHeads).
+ * Q, O: [total][nQHeads][D]; K, V: [total][nKVHeads][D], with element strides between tokens (row) and
+ * heads, so that Q, K and V may be parts of one projection's output; K_prefix, V_prefix:
+ * [nKVHeads][stride_prefix][D], the KV cache's layout, first `prefix` rows of each head read. dtype
+ * CDNA4_F16 or CDNA4_BF16; scale 1/sqrt(D), softmax and accumulation in fp32. Rows of O that belong to no
+ * sequence (before cu_seqlens[0], behind cu_seqlens[batch]) are left as they are. cu_seqlens entries
+ * outside 0 .. total or decreasing read and write nothing outside the tensors; the rows that they name
+ * wrongly are not defined. A value in V that is not finite reaches the rows of its sequence's earlier
+ * tokens too where they share 32 keys with it (a weight of zero times infinity); K may hold any value there.
+ * max_seq (0: unknown) is the longest sequence, used only to choose the kernel.
+ * batch == 0 or total == 0: nothing is done. Invalid: D not 64 or 128, nQHeads % nKVHeads != 0, negative
+ * sizes, max_seq > total, prefix + total near 2^31, stride_prefix (0: prefix) < prefix, Q/K/V strides not a multiple of 8
+ * elements, O strides not a multiple of 4, rows shorter than D, Q/K/V/prefix not 16-byte or O not 8-byte
+ * aligned. O must not overlap the inputs.
+ */
+typedef struct {
+    int D;              /* 64 or 128 */
+    int nQHeads;
+    int nKVHeads;       /* nQHeads % nKVHeads == 0 */
+    int batch;          /* sequences */
+    int total;          /* tokens in Q, K, V and O */
+    int max_seq;        /* longest sequence, 0: unknown */
+    int prefix;         /* keys that every sequence sees before its own, 0: none */
+    int stride_prefix;  /* rows between kv heads of the prefix; 0 = prefix */
+} cdna4_packed_cfg;
+
+typedef struct {
+    long long q_row, q_head;    /* Q element strides between tokens and between heads */
+    long long kv_row, kv_head;  /* K and V */
+    long long o_row, o_head;    /* O */
+} cdna4_packed_strides;
+
+int cdna4_attn_prefill_packed(const void* Q, const void* K, const void* V, const void* K_prefix,
+                              const void* V_prefix, void* O, const int* cu_seqlens,
+                              const cdna4_packed_cfg* cfg, const cdna4_packed_strides* strides, int dtype,
+                              cdna4_stream_t stream);
+
 /* ---- attention: decode (one query per sequence, split-K) --------------------
  * Replaces cdna3::attn::decode (attention.hpp:117-137) and cdna3::attn::decode_dme
  * (attention.hpp:152-173); the reference has no batch dimension (batch == 1 here).
@@ -174,8 +217,9 @@ enum {
     CDNA4_KERNEL_PREFILL_F32 = 4,      /* fa_f32: fp32 matrix-core kernel */
     CDNA4_KERNEL_DECODE_SPLIT = 5,     /* decode_mfma split-K grid + decode_merge */
     CDNA4_KERNEL_DECODE_WG = 6,        /* decode_wg: one launch, no workspace */
-    CDNA4_KERNEL_PREFILL_KEYS = 7      /* fa_mfma_keys: 8 waves, `rows` 128, 64 or 32 queries with the keys
+    CDNA4_KERNEL_PREFILL_KEYS = 7,     /* fa_mfma_keys: 8 waves, `rows` 128, 64 or 32 queries with the keys
                                           split over 2, 4 or 8 groups of waves */
+    CDNA4_KERNEL_PACKED_4W = 8         /* fa_packed: 4 waves x 32 queries, two workgroups per CU */
 };
 
 typedef struct {
@@ -190,6 +234,9 @@ typedef struct {
 int cdna3_attn_prefill_plan(const cdna3_prefill_cfg* cfg, int dtype, cdna3_plan_info* out);
 int cdna3_attn_decode_plan(const cdna3_decode_cfg* cfg, int dtype, int with_workspace,
                            cdna3_plan_info* out);
+/* cdna4_attn_prefill_packed: `grid` counts a workgroup for every block that the sequences could need
+ * (those past the last block end at once). */
+int cdna4_attn_prefill_packed_plan(const cdna4_packed_cfg* cfg, int dtype, cdna3_plan_info* out);
 
 /* ---- device-wide reduce / scan on the wave64 DPP primitives ------------------
  * Device-wide counterparts of wave::dpp::reduce_* / scan_inclusive_* (research/

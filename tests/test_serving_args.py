@@ -1,0 +1,75 @@
+"""CPU checks of the batched serving entry points: exported, and refusing what they do not support before any
+GPU work."""
+import ctypes
+import os
+import re
+import subprocess
+
+import pytest
+import torch
+
+import cdna4
+
+ROOT = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+P = ctypes.c_void_p(64)   # aligned, never dereferenced: validation fails first
+
+
+def test_cdna4_symbols_exported():
+    text = open(os.path.join(ROOT, "include", "cdna4_attn.h")).read()
+    names = set(re.findall(r"\b(cdna4_[a-z0-9_]+)\s*\(", text))
+    out = subprocess.run(["nm", "-D", "--defined-only", cdna4.library_path()], capture_output=True, text=True, check=True).stdout
+    assert names <= set(re.findall(r"\bT (cdna4_\w+)", out)), names
+
+
+def packed(cfg=(64, 8, 4, 3, 100, 50, 0, 0), strides=(512, 64, 256, 64, 512, 64), dtype=cdna4.F16, Q=P, K=P, V=P, Kp=None, Vp=None, O=P, cu=P):
+    c, s = cdna4.PackedPrefillCfg(*cfg), cdna4.PackedStrides(*strides)
+    return cdna4.lib().cdna4_attn_prefill_packed(Q, K, V, Kp, Vp, O, cu, ctypes.byref(c), ctypes.byref(s), dtype, None)
+
+
+@pytest.mark.parametrize("cfg", [
+    (96, 8, 4, 3, 100, 50, 0, 0), (64, 8, 3, 3, 100, 50, 0, 0), (64, 0, 4, 3, 100, 50, 0, 0), (64, 8, 0, 3, 100, 50, 0, 0),
+    (64, 8, 4, -1, 100, 50, 0, 0), (64, 8, 4, 3, -1, 50, 0, 0), (64, 8, 4, 3, 100, 101, 0, 0), (64, 8, 4, 3, 100, -1, 0, 0),
+    (64, 8, 4, 3, 100, 50, -1, 0), (64, 8, 4, 3, 100, 50, 2 ** 31 - 100, 0)])
+def test_packed_refuses_configurations(cfg):
+    assert packed(cfg) == 1
+    info = cdna4.PlanInfo()
+    c = cdna4.PackedPrefillCfg(*cfg)
+    if cfg[6] < 2 ** 30:
+        assert cdna4.lib().cdna4_attn_prefill_packed_plan(ctypes.byref(c), cdna4.F16, ctypes.byref(info)) == 1
+
+
+def test_packed_refuses_arguments():
+    good = (64, 8, 4, 3, 100, 50, 0, 0)
+    pre = (64, 8, 4, 3, 100, 50, 20, 0)
+    odd = ctypes.c_void_p(72)
+    assert packed(good, dtype=cdna4.F32) == 1 and packed(good, dtype=9) == 1
+    for name in ("Q", "K", "V", "O", "cu"):
+        assert packed(good, **{name: None}) == 1, name
+    for name in ("Q", "K", "V"):
+        assert packed(good, **{name: odd}) == 1, name            # 8 bytes off 16
+    assert packed(good, O=ctypes.c_void_p(68)) == 1 and packed(good, cu=ctypes.c_void_p(66)) == 1
+    assert packed(pre) == 1 and packed(pre, Kp=P) == 1 and packed(pre, Kp=P, Vp=odd) == 1
+    assert packed((64, 8, 4, 3, 100, 50, 20, 19), Kp=P, Vp=P) == 1    # rows between heads below the prefix
+    for i, bad in ((0, 60), (0, 516), (1, 4), (2, 56), (2, 260), (3, -64), (4, 60), (4, 510), (5, 2)):
+        st = [512, 64, 256, 64, 512, 64]
+        st[i] = bad
+        assert packed(good, strides=st) == 1, (i, bad)
+    l = cdna4.lib()
+    assert l.cdna4_attn_prefill_packed(P, P, P, None, None, P, P, None, None, cdna4.F16, None) == 1
+    # nothing to do: no pointer is needed
+    assert packed((64, 8, 4, 0, 100, 50, 0, 0), Q=None, K=None, V=None, O=None, cu=None) == 0
+    assert packed((64, 8, 4, 3, 0, 0, 0, 0), Q=None, K=None, V=None, O=None, cu=None) == 0
+
+
+def test_packed_plan():
+    for D, dt in ((64, torch.float16), (128, torch.bfloat16)):
+        p = cdna4.prefill_packed_plan(cdna4.PackedPrefillCfg(D, 32, 8, 24, 12961, 2048, 0, 0), dt)
+        assert p.name.startswith("fa_packed") and p.workspace == 0 and p.grid >= 32 * 12961 // p.rows
+    with pytest.raises(cdna4.CDNA4Error):
+        cdna4.prefill_packed_plan(cdna4.PackedPrefillCfg(64, 8, 3, 1, 10, 0, 0, 0))
+
+
+def test_packed_python_refuses_cpu_tensors():
+    x = torch.zeros(10, 4, 64, dtype=torch.float16)
+    with pytest.raises(ValueError):
+        cdna4.prefill_packed(x, x, x, x, torch.zeros(2, dtype=torch.int32), cdna4.PackedPrefillCfg(64, 4, 4, 1, 10, 10, 0, 0))
