@@ -39,7 +39,7 @@ __all__ = [
     "scatter_kv_f16", "repack_f16", "rope_append_kv_f16", "ModelCfg", "GenerateCfg", "Session",
     "PlanInfo", "prefill_plan", "decode_plan", "scan_status", "KERNEL_NAMES", "decode_noalloc",
     "decode_noalloc_max_bytes", "softmax_rows_f32", "PackedPrefillCfg", "PackedStrides", "prefill_packed",
-    "prefill_packed_plan",
+    "prefill_packed_plan", "LogitsArgs", "process_logits",
 ]
 
 # Element types and operators (include/cdna4_attn.h).
@@ -93,6 +93,17 @@ class PackedPrefillCfg(ctypes.Structure):
 class PackedStrides(ctypes.Structure):
     """cdna4_packed_strides: element strides between tokens (row) and heads of Q, of K and V, and of O."""
     _fields_ = [(n, ctypes.c_longlong) for n in ("q_row", "q_head", "kv_row", "kv_head", "o_row", "o_head")]
+
+
+class LogitsArgs(ctypes.Structure):
+    """cdna4_logits_args: the pointers, sizes and strides of one cdna4_process_logits call."""
+    _fields_ = [("logits", ctypes.c_void_p), ("out", ctypes.c_void_p), ("M", ctypes.c_int), ("V", ctypes.c_int),
+                ("logits_stride", ctypes.c_longlong), ("out_stride", ctypes.c_longlong),
+                ("history", ctypes.c_void_p), ("history_len", ctypes.c_void_p), ("prompt_len", ctypes.c_void_p),
+                ("history_max", ctypes.c_int), ("n_bias", ctypes.c_int), ("history_stride", ctypes.c_longlong),
+                ("repetition", ctypes.c_void_p), ("frequency", ctypes.c_void_p), ("presence", ctypes.c_void_p),
+                ("bias_ids", ctypes.c_void_p), ("bias_values", ctypes.c_void_p), ("mask", ctypes.c_void_p),
+                ("mask_stride", ctypes.c_longlong)]
 
 
 class ModelCfg(ctypes.Structure):
@@ -166,6 +177,7 @@ def _declare(l: ctypes.CDLL) -> None:
         "cdna3_reduce": (c_int, [c_int, c_int, vp, c_size, vp, vp, c_size, vp]),
         "cdna3_scan_workspace_size": (c_size, [c_size, c_int]),
         "cdna3_scan_inclusive": (c_int, [c_int, c_int, vp, c_size, vp, vp, c_size, vp]),
+        "cdna4_process_logits": (c_int, [ctypes.POINTER(LogitsArgs), c_int, vp]),
         "cdna3_rmsnorm_f32": (c_int, [vp, vp, vp, c_int, c_int, c_float, vp]),
         "cdna3_layernorm_f32": (c_int, [vp, vp, vp, vp, c_int, c_int, c_float, vp]),
         "cdna4_gemm_f16_nt": (c_int, [vp, vp, vp, c_int, c_int, c_int, c_int, c_int, c_int, vp]),
@@ -553,6 +565,68 @@ def softmax_rows_f32(X: torch.Tensor, out: Optional[torch.Tensor] = None, stream
     with _on_stream(stream):
         out = torch.empty_like(X) if out is None else out
     _check(lib().cdna3_softmax_rows_f32(_ptr(X), _ptr(out), M, H, _stream(stream)), "cdna3_softmax_rows_f32")
+    return out
+
+
+def _row_values(name: str, t: Optional[torch.Tensor], dtype, shape) -> int:
+    """Address of an optional contiguous tensor of `shape`; 0 for None."""
+    if t is None:
+        return 0
+    if t.dtype != dtype or tuple(t.shape) != shape or not t.is_contiguous():
+        raise ValueError(f"{name} must be contiguous {dtype} {list(shape)}")
+    return t.data_ptr()
+
+
+def process_logits(logits: torch.Tensor, out: Optional[torch.Tensor] = None, *,
+                   history: Optional[torch.Tensor] = None, history_len: Optional[torch.Tensor] = None,
+                   prompt_len: Optional[torch.Tensor] = None, repetition: Optional[torch.Tensor] = None,
+                   frequency: Optional[torch.Tensor] = None, presence: Optional[torch.Tensor] = None,
+                   bias_ids: Optional[torch.Tensor] = None, bias_values: Optional[torch.Tensor] = None,
+                   mask: Optional[torch.Tensor] = None, stream=None) -> torch.Tensor:
+    """Penalties for repeated tokens, biases and a grammar mask on logits [M][V] (fp32, fp16 or bf16; rows may be
+    apart) -> fp32 [M][V] into out (may be logits itself where those are fp32):
+    history int32 [M][H] (ids outside 0 .. V - 1 are padding), history_len, prompt_len int32 [M]; repetition,
+    frequency, presence fp32 [M]; bias_ids int32, bias_values fp32 [M][n]; mask int32 [M][>= ceil(V / 32)],
+    bit j % 32 of word j / 32 set: token j is allowed. The formula: cdna4_process_logits in cdna4_attn.h."""
+    dev = _device_of(logits, out, history, history_len, prompt_len, repetition, frequency, presence, bias_ids,
+                     bias_values, mask)
+    if logits.dim() != 2 or (logits.stride(1) != 1 and logits.numel()):
+        raise ValueError("logits must be [M][V] with contiguous rows")
+    dt = _dtype(logits)
+    M, V = logits.shape
+    i32, f32, rows = torch.int32, torch.float32, (M,)
+    a = LogitsArgs()
+    if history is not None:
+        a.history = _row_values("history", history, i32, (M, history.shape[-1]))
+        a.history_max = a.history_stride = history.shape[1]
+        a.history_len = _row_values("history_len", history_len, i32, rows)
+        a.prompt_len = _row_values("prompt_len", prompt_len, i32, rows)
+        a.repetition = _row_values("repetition", repetition, f32, rows)
+        a.frequency = _row_values("frequency", frequency, f32, rows)
+        a.presence = _row_values("presence", presence, f32, rows)
+    elif not (history_len is prompt_len is repetition is frequency is presence is None):
+        raise ValueError("lengths and penalties need a history")
+    if (bias_ids is None) != (bias_values is None):
+        raise ValueError("bias_ids and bias_values go together")
+    if bias_ids is not None:
+        a.n_bias = bias_ids.shape[-1]
+        a.bias_ids = _row_values("bias_ids", bias_ids, i32, (M, a.n_bias))
+        a.bias_values = _row_values("bias_values", bias_values, f32, (M, a.n_bias))
+    if mask is not None:
+        a.mask_stride = mask.shape[-1]
+        if 32 * a.mask_stride < V:   # an empty mask has a null address, which would allow everything
+            raise ValueError("mask must have a bit for each of the V tokens")
+        a.mask = _row_values("mask", mask, i32, (M, a.mask_stride))
+    with _on_device(dev):
+        if out is None:
+            with _on_stream(stream):
+                out = torch.empty((M, V), dtype=f32, device=logits.device)
+        elif out.dtype != f32 or out.shape != logits.shape or (out.stride(1) != 1 and out.numel()):
+            raise ValueError("out must be fp32 [M][V] with contiguous rows")
+        a.logits, a.out, a.M, a.V = logits.data_ptr(), out.data_ptr(), M, V
+        a.logits_stride = logits.stride(0) if M > 1 else V
+        a.out_stride = out.stride(0) if M > 1 else V
+        _check(lib().cdna4_process_logits(ctypes.byref(a), dt, _stream(stream)), "cdna4_process_logits")
     return out
 
 

@@ -278,6 +278,42 @@ int cdna3_scan_status(const void* workspace, int* status, cdna4_stream_t stream)
  */
 int cdna3_softmax_rows_f32(const float* X, float* Y, int M, int H, cdna4_stream_t stream);
 
+/* ---- logits for the sampler --------------------------------------------------------
+ * No counterpart in the reference (its runtime takes the argmax of the logits as they are). Penalties for
+ * repeated tokens, biases and a grammar mask on M rows of V logits (fp32, fp16 or bf16), computed in fp32
+ * and written as fp32 (to the logits themselves where those are fp32 and out_stride == logits_stride). With
+ * s whether token j is among the first history_len[m] entries of row m's history and c how many of them from
+ * prompt_len[m] on are j:
+ *   x = logit;  s: x = x > 0 ? x / repetition[m] : x * repetition[m];
+ *   x -= c * frequency[m];  c > 0: x -= presence[m];  x += bias of j;  not allowed: x = -inf
+ * A null pointer leaves its part out (history: no penalties; history_len: history_max entries; prompt_len: 0,
+ * all generated; repetition: 1, frequency, presence: 0; mask: all allowed). Lengths are cut to
+ * 0 .. history_max; ids outside 0 .. V - 1 in the history or the biases are passed over (padding); of several
+ * biases for one token the last counts. The mask holds token j of row m in bit j % 32 of word
+ * mask[m * mask_stride + j / 32] (1: allowed); a row that allows nothing is all -inf. repetition must not be 0.
+ * Invalid: V < 1, M < 0 or > 65,535, strides below V (mask: below ceil(V / 32); history: below history_max),
+ * history_max or n_bias negative or above 2^24, null logits or out, misaligned pointers.
+ */
+typedef struct {
+    const void* logits;          /* [M][logits_stride] */
+    float* out;                  /* [M][out_stride] */
+    int M, V;
+    long long logits_stride, out_stride;   /* elements between rows, >= V */
+    const int* history;          /* [M][history_stride] token ids: the prompt's, then the generated ones */
+    const int* history_len;      /* [M] */
+    const int* prompt_len;       /* [M] */
+    int history_max;             /* entries per row that may be read */
+    int n_bias;                  /* biases per row, 0: none */
+    long long history_stride;
+    const float *repetition, *frequency, *presence;   /* [M] */
+    const int* bias_ids;         /* [M][n_bias] */
+    const float* bias_values;    /* [M][n_bias] */
+    const uint32_t* mask;        /* [M][mask_stride] */
+    long long mask_stride;       /* words between rows */
+} cdna4_logits_args;
+
+int cdna4_process_logits(const cdna4_logits_args* args, int dtype, cdna4_stream_t stream);
+
 /* ---- runtime norms and RoPE ---------------------------------------------------
  * cdna3_rmsnorm_f32 replaces rmsnorm_f32_kernel (cdna3-prims/include/cdna3/runtime/
  * forward.hpp:34-56): Y[m][i] = X[m][i] * rsqrt(mean_i(X[m][:]^2) + eps) * W[i],

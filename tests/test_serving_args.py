@@ -73,3 +73,34 @@ def test_packed_python_refuses_cpu_tensors():
     x = torch.zeros(10, 4, 64, dtype=torch.float16)
     with pytest.raises(ValueError):
         cdna4.prefill_packed(x, x, x, x, torch.zeros(2, dtype=torch.int32), cdna4.PackedPrefillCfg(64, 4, 4, 1, 10, 10, 0, 0))
+
+
+def logits_args(**kw):
+    a = cdna4.LogitsArgs()
+    a.logits = a.out = a.history = a.bias_ids = a.bias_values = a.mask = 64
+    a.M, a.V, a.logits_stride, a.out_stride = 3, 100, 100, 104
+    a.history_max, a.history_stride, a.n_bias, a.mask_stride = 5, 5, 2, 4
+    for k, v in kw.items():
+        setattr(a, k, v)
+    return a
+
+
+@pytest.mark.parametrize("bad", [
+    dict(V=0), dict(V=-1), dict(V=2 ** 31 - 1), dict(M=-1), dict(M=65536), dict(logits_stride=99), dict(out_stride=99),
+    dict(history_stride=4), dict(history_max=-1), dict(history_max=2 ** 24 + 1), dict(n_bias=-1), dict(n_bias=2 ** 24 + 1),
+    dict(mask_stride=3), dict(logits=None), dict(out=None), dict(bias_ids=None), dict(bias_values=None), dict(logits=65),
+    dict(out=66), dict(history=66), dict(repetition=66), dict(mask=65), dict(prompt_len=63)])
+def test_logits_refuses(bad):
+    a = logits_args(**bad)
+    assert cdna4.lib().cdna4_process_logits(ctypes.byref(a), cdna4.F16, None) == 1
+
+
+def test_logits_refuses_dtypes_and_null():
+    a = logits_args()
+    for dt in (cdna4.F64, cdna4.I32, 9, -1):
+        assert cdna4.lib().cdna4_process_logits(ctypes.byref(a), dt, None) == 1
+    assert cdna4.lib().cdna4_process_logits(None, cdna4.F16, None) == 1
+    a = logits_args(logits=66)
+    assert cdna4.lib().cdna4_process_logits(ctypes.byref(a), cdna4.F32, None) == 1   # fp32 rows are 4-byte aligned
+    a = logits_args(M=0, logits=None, out=None)
+    assert cdna4.lib().cdna4_process_logits(ctypes.byref(a), cdna4.F32, None) == 0   # nothing to do
