@@ -39,7 +39,8 @@ __all__ = [
     "scatter_kv_f16", "repack_f16", "rope_append_kv_f16", "ModelCfg", "GenerateCfg", "Session",
     "PlanInfo", "prefill_plan", "decode_plan", "scan_status", "KERNEL_NAMES", "decode_noalloc",
     "decode_noalloc_max_bytes", "softmax_rows_f32", "PackedPrefillCfg", "PackedStrides", "prefill_packed",
-    "prefill_packed_plan", "LogitsArgs", "process_logits",
+    "prefill_packed_plan", "LogitsArgs", "process_logits", "SharedDecodeCfg",
+    "decode_shared", "decode_shared_plan", "decode_shared_workspace_size",
 ]
 
 # Element types and operators (include/cdna4_attn.h).
@@ -95,6 +96,13 @@ class PackedStrides(ctypes.Structure):
     _fields_ = [(n, ctypes.c_longlong) for n in ("q_row", "q_head", "kv_row", "kv_head", "o_row", "o_head")]
 
 
+class SharedDecodeCfg(ctypes.Structure):
+    """cdna4_shared_decode_cfg: `batch` sequences behind `prefix` shared keys, with up to max_own keys of their own
+    (strides: rows between kv heads, 0 = packed)."""
+    _fields_ = [(n, ctypes.c_int) for n in ("D", "nQHeads", "nKVHeads", "batch", "prefix", "stride_prefix", "max_own",
+                                            "stride_kv")]
+
+
 class LogitsArgs(ctypes.Structure):
     """cdna4_logits_args: the pointers, sizes and strides of one cdna4_process_logits call."""
     _fields_ = [("logits", ctypes.c_void_p), ("out", ctypes.c_void_p), ("M", ctypes.c_int), ("V", ctypes.c_int),
@@ -132,7 +140,7 @@ class PlanInfo(ctypes.Structure):
 
 # CDNA4_KERNEL_* (include/cdna4_attn.h)
 KERNEL_NAMES = {1: "fa_mfma_8w", 2: "fa_mfma_4w", 3: "fa_small", 4: "fa_f32", 5: "decode_split", 6: "decode_wg",
-                7: "fa_mfma_keys", 8: "fa_packed"}
+                7: "fa_mfma_keys", 8: "fa_packed", 9: "decode_shared"}
 
 
 def DecodeDmeCfg(D: int, N: int, nQHeads: int, nKVHeads: int, stride_kv: int, batch: int = 1) -> DecodeCfg:
@@ -177,6 +185,9 @@ def _declare(l: ctypes.CDLL) -> None:
         "cdna3_reduce": (c_int, [c_int, c_int, vp, c_size, vp, vp, c_size, vp]),
         "cdna3_scan_workspace_size": (c_size, [c_size, c_int]),
         "cdna3_scan_inclusive": (c_int, [c_int, c_int, vp, c_size, vp, vp, c_size, vp]),
+        "cdna4_attn_decode_shared_workspace_size": (c_size, [ctypes.POINTER(SharedDecodeCfg)]),
+        "cdna4_attn_decode_shared": (c_int, [vp] * 7 + [ctypes.POINTER(SharedDecodeCfg), c_int, vp, c_size, vp]),
+        "cdna4_attn_decode_shared_plan": (c_int, [ctypes.POINTER(SharedDecodeCfg), c_int, ctypes.POINTER(PlanInfo)]),
         "cdna4_process_logits": (c_int, [ctypes.POINTER(LogitsArgs), c_int, vp]),
         "cdna3_rmsnorm_f32": (c_int, [vp, vp, vp, c_int, c_int, c_float, vp]),
         "cdna3_layernorm_f32": (c_int, [vp, vp, vp, vp, c_int, c_int, c_float, vp]),
@@ -443,6 +454,61 @@ def decode_noalloc(q: torch.Tensor, K: torch.Tensor, V: torch.Tensor, o: torch.T
 
 def decode_noalloc_max_bytes() -> int:
     return int(lib().cdna3_attn_decode_noalloc_max_bytes())
+
+
+def decode_shared_workspace_size(cfg: SharedDecodeCfg) -> int:
+    return int(lib().cdna4_attn_decode_shared_workspace_size(ctypes.byref(cfg)))
+
+
+def decode_shared(q: torch.Tensor, K_prefix: Optional[torch.Tensor], V_prefix: Optional[torch.Tensor],
+                  K: Optional[torch.Tensor], V: Optional[torch.Tensor], lens: Optional[torch.Tensor],
+                  o: torch.Tensor, cfg: SharedDecodeCfg, workspace="auto", stream=None) -> None:
+    """One query per sequence over a prefix that the batch shares and the sequence's own keys: q, o [batch][nQH][D];
+    K_prefix, V_prefix [nKVH][stride_prefix][D] (None with prefix 0); K, V [batch][nKVH][stride_kv][D] with lens[b]
+    keys each, int32 on the device (None with max_own 0); fp16 or bf16. `workspace`: "auto" allocates
+    decode_shared_workspace_size(cfg) bytes on the stream the call launches on; a uint8 tensor is used as given."""
+    dev = _device_of(q, K_prefix, V_prefix, K, V, lens, o)
+    dt, dtype = _dtype(q), q.dtype
+    B, D = cfg.batch, cfg.D
+    if o.dtype != dtype:
+        raise ValueError("q and o must share one dtype")
+    if not (q.is_contiguous() and o.is_contiguous()):
+        raise ValueError("tensors must be contiguous")
+    if min(q.numel(), o.numel()) < B * cfg.nQHeads * D:
+        raise ValueError("q/o smaller than the configuration")
+    kp = vp = k = v = n = 0
+    if cfg.prefix > 0:
+        kp, vp = _prefix_ptrs(K_prefix, V_prefix, dtype, cfg.nKVHeads * (cfg.stride_prefix or cfg.prefix) * D)
+    if cfg.max_own > 0:
+        if K is None or V is None or lens is None:
+            raise ValueError("max_own > 0 needs K, V and lens")
+        if not (K.dtype == V.dtype == dtype) or not (K.is_contiguous() and V.is_contiguous()):
+            raise ValueError("K, V must be contiguous and have the dtype of q")
+        if min(K.numel(), V.numel()) < B * cfg.nKVHeads * (cfg.stride_kv or cfg.max_own) * D:
+            raise ValueError("K/V smaller than the configuration")
+        if lens.dtype != torch.int32 or not lens.is_contiguous() or lens.numel() < B:
+            raise ValueError("lens must be contiguous int32 [batch]")
+        k, v, n = K.data_ptr(), V.data_ptr(), lens.data_ptr()
+    if workspace is None or (isinstance(workspace, str) and workspace != "auto"):
+        raise ValueError("workspace must be 'auto' or a uint8 tensor")
+    with _on_device(dev), _on_stream(stream):
+        if isinstance(workspace, str):
+            workspace = torch.empty(max(1, decode_shared_workspace_size(cfg)), dtype=torch.uint8, device=q.device)
+        elif workspace.get_device() != dev or not workspace.is_contiguous():
+            raise ValueError("workspace must be contiguous on the GPU of the tensors")
+        _check(lib().cdna4_attn_decode_shared(q.data_ptr(), kp, vp, k, v, n, o.data_ptr(), ctypes.byref(cfg), dt,
+                                              workspace.data_ptr(), workspace.numel() * workspace.element_size(),
+                                              _stream(stream)), "cdna4_attn_decode_shared")
+
+
+def decode_shared_plan(cfg: SharedDecodeCfg, dtype=F16) -> PlanInfo:
+    """The kernels cdna4_attn_decode_shared would launch for cfg on the current device."""
+    if isinstance(dtype, torch.dtype):
+        dtype = _TORCH_DTYPES[dtype]
+    out = PlanInfo()
+    _check(lib().cdna4_attn_decode_shared_plan(ctypes.byref(cfg), dtype, ctypes.byref(out)),
+           "cdna4_attn_decode_shared_plan")
+    return out
 
 
 def prefill_plan(cfg: PrefillCfg, dtype=BF16) -> PlanInfo:

@@ -16,13 +16,14 @@
 
 #include "attn_tile.hpp"
 #include "attn_stream.hpp"
-#include "attn_pipe.hpp"
+#include "attn_block.hpp"
 
 namespace cdna4 {
 namespace {
 
 using namespace tile;
 using namespace pipe;
+using block::Keys;
 using wave::xlane::allreduce;
 using wave::xlane::Max;
 using wave::xlane::Sum;
@@ -114,58 +115,6 @@ __device__ __forceinline__ int item_head(int i, int nQH) {
     return (nQH & 7) ? i : (i & 7) * (nQH >> 3) + (i >> 3);
 }
 
-// Keys of one sequence and kv head on the joint axis: k < P in the prefix, else own row k - P.
-template <bool kPrefix>
-struct Keys {
-    const uint16_t *own, *pre;
-    long long rs;
-    int P, S;   // prefix keys, all keys
-    template <int D>
-    __device__ __forceinline__ const uint16_t* row(int k) const {
-        k = min(k, S - 1);   // rows past the end re-read the last key (masked)
-        if constexpr (!kPrefix) return own + k * rs;
-        else return k < P ? pre + (long long)k * D : own + (k - P) * rs;
-    }
-};
-
-// Copy of `rows` keys from k0 on into an LDS slot by W waves, each lane's address formed by itself.
-template <int D, int W, bool kIsK, bool kPrefix>
-__device__ __forceinline__ void copy_any(const Keys<kPrefix>& k, int k0, int rows, uint16_t* dst, int wave, int lane) {
-    constexpr int CPR = D / 8;
-#pragma unroll
-    for (int j = 0; j < rows * CPR / (64 * W); ++j) {
-        const int p0 = (j * W + wave) * 64, p = p0 + lane, r = p / CPR;
-        stream::dma16(k.template row<D>(k0 + r) + ((p % CPR) ^ swz<D, kIsK>(r)) * 8, dst + p0 * 8);
-    }
-}
-
-// The copies of a whole step of K or of V, all in one source, that a region issues between its MFMAs: a
-// wave-uniform base that moves on by whole rows per instruction, and per-lane offsets, of which two differ (a
-// row's swizzle repeats every 32 rows, two instructions at D = 128).
-template <int D, int W, int NI>
-struct StepCopy {
-    static constexpr int kCount = NI;
-    static constexpr int kRows = 512 * W / D;   // rows of one instruction of all waves
-    const uint16_t* base;
-    uint16_t* dst;
-    const uint32_t* off;   // [2]
-    long long rs;
-    int wave;
-    __device__ __forceinline__ void issue(int c) const {
-        stream::dma16_s(base + c * (kRows * rs), off[c & 1], dst + (c * W + wave) * 512);
-    }
-    template <bool kIsK>
-    static __device__ __forceinline__ void offsets(long long rs, int wave, int lane, uint32_t (&off)[2]) {
-        static_assert(kRows % 16 == 0, "rows 2 kRows apart have one swizzle");
-        constexpr int CPR = D / 8;
-#pragma unroll
-        for (int j = 0; j < 2; ++j) {
-            const int p = wave * 64 + lane, r = p / CPR, c = p % CPR;
-            off[j] = (uint32_t)((r * rs + (c ^ swz<D, kIsK>(r + j * kRows)) * 8) * 2);
-        }
-    }
-};
-
 template <int D, bool kBf16>
 __device__ __forceinline__ void store_rows(const f32x4 (&o)[D / 16], float l, uint16_t* dst) {
     const float inv = l > 0.f ? 1.f / l : 1.f;
@@ -183,9 +132,8 @@ __device__ __forceinline__ void store_rows(const f32x4 (&o)[D / 16], float l, ui
 // so each copy has the time of two regions to land.
 template <int D, bool kBf16, bool kPrefix>
 __global__ __launch_bounds__(256, 2) void fa_packed(PackedArgs a) {
-    constexpr int W = 4, QT = 2, ND = D / 32, NDT = D / 16, BM = W * QT * 16;
-    constexpr int kTile = kBc * D, NI = kBc * (D / 8) / (64 * W);
-    __shared__ __attribute__((aligned(16))) uint16_t lds[4 * kTile];   // K slots 0, 1, V slots 0, 1
+    constexpr int QT = block::kQT, ND = D / 32, NDT = D / 16, BM = block::kRows;
+    __shared__ __attribute__((aligned(16))) uint16_t lds[block::lds_elems<D>()];
     const int lane = (int)(threadIdx.x & 63u);
     const int wave = __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
     const int li = lane & 15, g = lane >> 4;
@@ -214,114 +162,16 @@ __global__ __launch_bounds__(256, 2) void fa_packed(PackedArgs a) {
     const int ntiles = (P + min(q0 + BM, len) + kBc - 1) / kBc;
     const int wave_end = min(qw0 + QT * 16, len);                     // one past this wave's last query
     const int nch = wave_end > qw0 ? (P + wave_end + 31) / 32 : 0;     // the wave's chunks; 0: no queries
-    const int qv0 = P + qw0;                                          // the first query on the key axis
     // Main tiles: chunks 2t + 1 and 2t + 2 lie below the workgroup's first query, and the copies of
     // V (t + 1) and K (t + 2) are whole tiles that exist.
     int t_main = P + q0 >= 95 ? (P + q0 - 95) / 64 + 1 : 0;
     t_main = min(t_main, min(ntiles - 2, S / kBc - 2));
     if (!a.copy32) t_main = 0;
 
-    uint16_t* const vlds = lds + 2 * kTile;
-    auto copy_k = [&](int t) { copy_any<D, W, true>(keys_k, t * kBc, kBc, lds + (t & 1) * kTile, wave, lane); };
-    auto copy_v = [&](int t) { copy_any<D, W, false>(keys_v, t * kBc, kBc, vlds + (t & 1) * kTile, wave, lane); };
-    copy_k(0);
-    copy_v(0);
-    if (ntiles > 1) copy_k(1);
-    using CP = StepCopy<D, W, NI>;
-    uint32_t koff[2], voff[2];
-    const float inv_sc = 1.f / a.sc;
     f32x4 o[QT][NDT], lacc[QT];
-    float m[QT], thr[QT];
-#pragma unroll
-    for (int t = 0; t < QT; ++t) {
-        m[t] = kInitM;
-        thr[t] = (kInitM + kTau) * inv_sc;
-        lacc[t] = f32x4{0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-        for (int d = 0; d < NDT; ++d) o[t][d] = f32x4{0.f, 0.f, 0.f, 0.f};
-    }
-    const LdsOffsets off = lds_offsets<D>(li, g);
-    u32x4 ones;
-    {
-        const uint32_t one2 = kBf16 ? 0x3F803F80u : 0x3C003C00u;
-        ones = u32x4{one2, one2, one2, one2};
-        asm volatile("" : "+v"(ones));
-    }
-    if (ntiles > 1) asm volatile("s_waitcnt vmcnt(%0)" : : "n"(2 * NI) : "memory");   // K 0 (V 0, K 1 newer)
-    else asm volatile("s_waitcnt vmcnt(0)" : : : "memory");
-    __syncthreads();
-    f32x4 s[QT][2];
-    qk_chunk<D, QT, kBf16>((const char*)lds, off, qb, s, 0);
-    {
-        float lm[QT];
-        if (31 > qv0) mask_chunk<QT>(s, 0, qv0, S, 1, li, g);
-        const bool need = check_raw<QT>(s, thr, lm) && nch > 0;
-        if (__builtin_amdgcn_ballot_w64(need)) rescale_pipe<D, QT>(lm, m, thr, o, lacc, a.sc, inv_sc);
-    }
-    auto tile_iter = [&](int t, auto tail, auto two, int sl, const uint16_t* kb, const uint16_t* vb, long long rs) {
-        constexpr bool kTail = decltype(tail)::value;
-        constexpr bool kTwo = decltype(two)::value;
-        const char* Kt = (const char*)(lds + sl * kTile);
-        const char* Kn = (const char*)(lds + (sl ^ 1) * kTile);
-        const char* Vt = (const char*)(vlds + sl * kTile);
-        // V t landed (K t + 1 may be in flight); every wave is past region 2t - 1, the last reader of V t - 1
-        if (kTail && t + 1 >= ntiles) asm volatile("s_waitcnt vmcnt(0)" : : : "memory");
-        else asm volatile("s_waitcnt vmcnt(%0)" : : "n"(NI) : "memory");
-        __syncthreads();
-        if (kTail && t + 1 < ntiles) copy_v(t + 1);
-        const int j0 = 2 * t;
-        const CP cv{vb, vlds + (sl ^ 1) * kTile, voff, rs, wave};
-        if (!kTail)
-            pipe_region<D, QT, kBf16, false, true, NI, false, CP>(Kt, 1, Vt, 0, off, qb, s, o, m, thr, lacc, ones, true, (j0 + 1) * 32,
-                                                                  qv0, S, 1, a.sc, inv_sc, li, g, cv);
-        else if (j0 < nch)
-            pipe_region<D, QT, kBf16, true, false, NI, kTwo, CP, kPrefix>(Kt, 1, Vt, 0, off, qb, s, o, m, thr, lacc, ones, j0 + 1 < nch,
-                                                                 (j0 + 1) * 32, qv0, S, 1, a.sc, inv_sc, li, g, cv);
-        // K t + 1 landed (V t + 1 may be in flight); every wave is past region 2t, the last reader of K t
-        if (!kTail || t + 1 < ntiles) {
-            asm volatile("s_waitcnt vmcnt(%0)" : : "n"(NI) : "memory");
-            __syncthreads();
-            if (kTail && t + 2 < ntiles) copy_k(t + 2);
-        }
-        const int j1 = 2 * t + 1;
-        const CP ck{kb, lds + sl * kTile, koff, rs, wave};
-        if (!kTail)
-            pipe_region<D, QT, kBf16, false, true, NI, false, CP>(Kn, 0, Vt, 1, off, qb, s, o, m, thr, lacc, ones, true, (j1 + 1) * 32,
-                                                                  qv0, S, 1, a.sc, inv_sc, li, g, ck);
-        else if (j1 < nch)
-            pipe_region<D, QT, kBf16, true, false, NI, kTwo, CP, kPrefix>(Kn, 0, Vt, 1, off, qb, s, o, m, thr, lacc, ones, j1 + 1 < nch,
-                                                                 (j1 + 1) * 32, qv0, S, 1, a.sc, inv_sc, li, g, ck);
-    };
-    int t = 0;
-    // bf16: keys 0..63 enter with their weights' second bf16 term where the queries see few keys
-    if constexpr (kBf16) {
-        if (t_main <= 0) {
-            tile_iter(0, std::true_type{}, std::true_type{}, 0, nullptr, nullptr, 0);
-            t = 1;
-        }
-    }
-    // The joint axis in two passes: main tiles whose copies lie in the prefix, then (past the tiles whose
-    // copies straddle its end, to an even tile) those whose copies lie in the sequence.
-    bool pre = kPrefix;
-    for (;;) {
-        const long long rs = pre ? D : a.k_rs;
-        const uint16_t* kb = (pre ? keys_k.pre : own_k - (long long)P * a.k_rs) + 2LL * kBc * rs;
-        const uint16_t* vb = (pre ? keys_v.pre : own_v - (long long)P * a.k_rs) + (long long)kBc * rs;
-        const int t1 = pre ? min(t_main, P / kBc - 2) : t_main;   // main tiles of this source: t < t1
-        CP::template offsets<true>(rs, wave, lane, koff);
-        CP::template offsets<false>(rs, wave, lane, voff);
-#pragma unroll 1
-        for (; t + 2 <= t1; t += 2) {
-            tile_iter(t, std::false_type{}, std::false_type{}, 0, kb + (long long)t * kBc * rs, vb + (long long)t * kBc * rs, rs);
-            tile_iter(t + 1, std::false_type{}, std::false_type{}, 1, kb + (long long)(t + 1) * kBc * rs, vb + (long long)(t + 1) * kBc * rs, rs);
-        }
-        // own main tiles begin where K (t + 2) and V (t + 1) lie past the prefix, at an even tile
-        const int t2 = pre ? min(ntiles, ((P + kBc - 1) / kBc) & ~1) : ntiles;
-#pragma unroll 1
-        for (; t < t2; ++t) tile_iter(t, std::true_type{}, std::false_type{}, t & 1, nullptr, nullptr, 0);
-        if (!pre) break;
-        pre = false;
-    }
+    float m[QT];
+    block::attend<D, kBf16, kPrefix, true>(keys_k, keys_v, block::Shape{S, ntiles, nch, P + qw0, t_main}, qb, o, lacc, m,
+                                           lds, a.sc, wave, lane);
 
     uint16_t* Oh = a.O + start * a.o_rs + h * a.o_hs;
 #pragma unroll

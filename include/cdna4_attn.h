@@ -204,6 +204,36 @@ size_t cdna3_attn_decode_noalloc_max_bytes(void);
 int cdna3_attn_decode_noalloc(const void* q, const void* K, const void* V, void* o,
                               const cdna3_decode_cfg* cfg, int dtype, cdna4_stream_t stream);
 
+/* ---- attention: decode of a batch that shares a prefix ------------------------------
+ * No counterpart in the reference. One query per sequence over `prefix` keys that all sequences share (read
+ * once for the batch) and the sequence's own lens[b] keys (int32, device memory, read when the kernel runs and cut to
+ * 0 .. max_own): q, o [batch][nQHeads][D]; K_prefix, V_prefix [nKVHeads][stride_prefix][D]; K, V
+ * [batch][nKVHeads][stride_kv][D]; dtype CDNA4_F16 or CDNA4_BF16. prefix == 0 is a decode of caches of
+ * different lengths (K_prefix, V_prefix may be null), max_own == 0 one of the prefix alone (K, V, lens may be
+ * null); a row that sees no key gets zeros. Own rows from lens[b] on are never read into a result, whatever they
+ * hold. The workspace (cdna4_attn_decode_shared_workspace_size(cfg) bytes, 16-byte aligned, no
+ * initialisation) holds the parts' results; calls that overlap must not share one. A captured call replays
+ * on other lengths up to max_own. The plan is sized to the current device, so query the size with the device
+ * current that the call will run on. batch == 0: nothing is done.
+ * Invalid: D not 64 or 128, nQHeads % nKVHeads != 0, negative sizes, a stride below its rows (0: packed),
+ * q/K/V/prefix not 16-byte or o not 4-byte aligned, a missing or small workspace.
+ */
+typedef struct {
+    int D;              /* 64 or 128 */
+    int nQHeads;
+    int nKVHeads;       /* nQHeads % nKVHeads == 0 */
+    int batch;
+    int prefix;         /* shared keys, 0: none */
+    int stride_prefix;  /* rows between kv heads of the prefix; 0 = prefix */
+    int max_own;        /* most own keys a sequence can have */
+    int stride_kv;      /* rows between kv heads of the own keys; 0 = max_own */
+} cdna4_shared_decode_cfg;
+
+size_t cdna4_attn_decode_shared_workspace_size(const cdna4_shared_decode_cfg* cfg);
+int cdna4_attn_decode_shared(const void* q, const void* K_prefix, const void* V_prefix, const void* K,
+                             const void* V, const int* lens, void* o, const cdna4_shared_decode_cfg* cfg,
+                             int dtype, void* workspace, size_t ws_bytes, cdna4_stream_t stream);
+
 /* ---- kernel plans (introspection) ---------------------------------------------
  * No counterpart in the reference (its launchers had one kernel each). Report which kernel a
  * call with the same arguments would launch on the current device, without launching it, so
@@ -219,7 +249,8 @@ enum {
     CDNA4_KERNEL_DECODE_WG = 6,        /* decode_wg: one launch, no workspace */
     CDNA4_KERNEL_PREFILL_KEYS = 7,     /* fa_mfma_keys: 8 waves, `rows` 128, 64 or 32 queries with the keys
                                           split over 2, 4 or 8 groups of waves */
-    CDNA4_KERNEL_PACKED_4W = 8         /* fa_packed: 4 waves x 32 queries, two workgroups per CU */
+    CDNA4_KERNEL_PACKED_4W = 8,        /* fa_packed: 4 waves x 32 queries, two workgroups per CU */
+    CDNA4_KERNEL_DECODE_SHARED = 9     /* shared_parts + shared_join */
 };
 
 typedef struct {
@@ -237,6 +268,8 @@ int cdna3_attn_decode_plan(const cdna3_decode_cfg* cfg, int dtype, int with_work
 /* cdna4_attn_prefill_packed: `grid` counts a workgroup for every block that the sequences could need
  * (those past the last block end at once). */
 int cdna4_attn_prefill_packed_plan(const cdna4_packed_cfg* cfg, int dtype, cdna3_plan_info* out);
+/* cdna4_attn_decode_shared: `rows` prefix keys per part, `partials` parts per query head at most. */
+int cdna4_attn_decode_shared_plan(const cdna4_shared_decode_cfg* cfg, int dtype, cdna3_plan_info* out);
 
 /* ---- device-wide reduce / scan on the wave64 DPP primitives ------------------
  * Device-wide counterparts of wave::dpp::reduce_* / scan_inclusive_* (research/

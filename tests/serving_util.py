@@ -79,3 +79,23 @@ def cu_of(lens, first=0):
     for n in lens:
         cu.append(cu[-1] + n)
     return cu
+
+
+def shared_reference(q, Kp, Vp, K, V, lens, G, dtype, P=0):
+    """(o, bound) of one query per sequence; lens a host list."""
+    B, HQ, D = q.shape
+    O = torch.zeros(B, HQ, D, dtype=torch.float64, device=q.device)
+    bound = torch.zeros_like(O)
+    for b in range(B):
+        for h in range(HQ // G):
+            k, v = [], []
+            if P:
+                k.append(Kp[h, :P]), v.append(Vp[h, :P])
+            if lens is not None and lens[b] > 0:
+                k.append(K[b, h, :lens[b]]), v.append(V[b, h, :lens[b]])
+            if not k:
+                continue
+            k, v = torch.cat(k), torch.cat(v)
+            sl = slice(h * G, (h + 1) * G)
+            O[b, sl], bound[b, sl] = attend(q[b, sl], k, v, torch.ones(G, k.shape[0], dtype=torch.bool, device=q.device), dtype)
+    return O, bound

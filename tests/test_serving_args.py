@@ -104,3 +104,39 @@ def test_logits_refuses_dtypes_and_null():
     assert cdna4.lib().cdna4_process_logits(ctypes.byref(a), cdna4.F32, None) == 1   # fp32 rows are 4-byte aligned
     a = logits_args(M=0, logits=None, out=None)
     assert cdna4.lib().cdna4_process_logits(ctypes.byref(a), cdna4.F32, None) == 0   # nothing to do
+
+
+def shared(cfg=(128, 8, 2, 4, 100, 0, 50, 0), dtype=cdna4.F16, q=P, Kp=P, Vp=P, K=P, V=P, lens=P, o=P, ws=P, n=None):
+    c = cdna4.SharedDecodeCfg(*cfg)
+    if n is None:
+        n = cdna4.decode_shared_workspace_size(c)
+    return cdna4.lib().cdna4_attn_decode_shared(q, Kp, Vp, K, V, lens, o, ctypes.byref(c), dtype, ws, n, None)
+
+
+@pytest.mark.parametrize("cfg", [
+    (96, 8, 2, 4, 100, 0, 50, 0), (128, 8, 3, 4, 100, 0, 50, 0), (128, 0, 2, 4, 100, 0, 50, 0), (128, 8, 0, 4, 100, 0, 50, 0),
+    (128, 8, 2, -1, 100, 0, 50, 0), (128, 8, 2, 4, -1, 0, 50, 0), (128, 8, 2, 4, 100, 99, 50, 0), (128, 8, 2, 4, 100, 0, -1, 0),
+    (128, 8, 2, 4, 100, 0, 50, 49), (128, 8, 2, 4, 2 ** 31 - 1, 0, 50, 0), (128, 8, 2, 4, 100, 0, 2 ** 31 - 1, 0),
+    (128, 2 ** 20, 1, 2 ** 20, 100, 0, 50, 0)])
+def test_shared_refuses_configurations(cfg):
+    assert shared(cfg, n=1 << 60) == 1
+    assert cdna4.decode_shared_workspace_size(cdna4.SharedDecodeCfg(*cfg)) == 0
+    info = cdna4.PlanInfo()
+    c = cdna4.SharedDecodeCfg(*cfg)
+    assert cdna4.lib().cdna4_attn_decode_shared_plan(ctypes.byref(c), cdna4.F16, ctypes.byref(info)) == 1
+
+
+def test_shared_refuses_arguments():
+    odd = ctypes.c_void_p(72)
+    for name in ("q", "Kp", "Vp", "K", "V", "lens", "o", "ws"):
+        assert shared(**{name: None}) == 1, name
+    for name in ("q", "Kp", "Vp", "K", "V", "ws"):
+        assert shared(**{name: odd}) == 1, name
+    assert shared(o=ctypes.c_void_p(66)) == 1 and shared(lens=ctypes.c_void_p(66)) == 1
+    assert shared(dtype=cdna4.F32) == 1 and shared(dtype=9) == 1
+    need = cdna4.decode_shared_workspace_size(cdna4.SharedDecodeCfg(128, 8, 2, 4, 100, 0, 50, 0))
+    assert need > 0 and shared(n=need - 1) == 1
+    assert shared((128, 8, 2, 0, 100, 0, 50, 0), q=None, o=None, ws=None, n=0) == 0     # nothing to do
+    p = cdna4.decode_shared_plan(cdna4.SharedDecodeCfg(128, 32, 8, 64, 8192, 0, 1024, 0))
+    assert p.name == "decode_shared" and p.workspace == cdna4.decode_shared_workspace_size(cdna4.SharedDecodeCfg(128, 32, 8, 64, 8192, 0, 1024, 0))
+    assert p.grid * 256 < 2 ** 32
