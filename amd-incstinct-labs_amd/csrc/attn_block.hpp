@@ -12,15 +12,18 @@ namespace block {
 using namespace tile;
 using namespace pipe;
 
-constexpr int kWaves = 4, kQT = 2, kRows = kWaves * kQT * 16;   // queries per block
+constexpr int kWaves = 4, kQT = 2, kRowsLog2 = 7, kRows = 1 << kRowsLog2;   // queries per block
+static_assert(kRows == kWaves * kQT * 16, "");
 template <int D> constexpr int lds_elems() { return 4 * kBc * D; }   // K slots 0, 1, V slots 0, 1
+template <int D> constexpr int lds_v() { return 2 * kBc * D; }
 
 // Keys of one sequence and kv head on the joint axis: k < P in the prefix, else own row k - P.
 template <bool kPrefix>
 struct Keys {
     const uint16_t *own, *pre;
     long long rs;
-    int P, S;   // prefix keys, all keys
+    int P, S;     // prefix keys, all keys
+    int copy32;   // a tile's own rows span < 4 GiB: 32-bit offsets
     template <int D>
     __device__ __forceinline__ const uint16_t* row(int k) const {
         k = min(k, S - 1);   // rows past the end re-read the last key (masked)
@@ -67,12 +70,54 @@ struct StepCopy {
     }
 };
 
+// The per-lane offsets of whole tiles' copies from own rows; those from a prefix (rows of D) are formed on use.
+struct Offsets { uint32_t k[2], v[2]; };
+template <int D>
+__device__ __forceinline__ Offsets own_offsets(long long rs, int wave, int lane) {
+    using CP = StepCopy<D, kWaves, kBc * (D / 8) / (64 * kWaves)>;
+    Offsets o;
+    CP::template offsets<true>(rs, wave, lane, o.k);
+    CP::template offsets<false>(rs, wave, lane, o.v);
+    return o;
+}
+
+// Copy of tile t into a slot: a whole tile of one source by a wave-uniform base and 32-bit offsets (a few scalar
+// instructions), the others lane by lane.
+template <int D, bool kIsK, bool kPrefix>
+__device__ __forceinline__ void copy_tile(const Keys<kPrefix>& k, int t, const Offsets& own, uint16_t* dst, int wave, int lane) {
+    constexpr int NI = kBc * (D / 8) / (64 * kWaves);
+    using CP = StepCopy<D, kWaves, NI>;
+    const int k0 = t * kBc;
+    if (k.copy32 && k0 >= k.P && k0 + kBc <= k.S) {
+        const CP c{k.own + (k0 - k.P) * k.rs, dst, kIsK ? own.k : own.v, k.rs, wave};
+#pragma unroll
+        for (int j = 0; j < NI; ++j) c.issue(j);
+    } else if (kPrefix && k0 + kBc <= k.P) {
+        uint32_t off[2];
+        CP::template offsets<kIsK>(D, wave, lane, off);
+        const CP c{k.pre + (long long)k0 * D, dst, off, D, wave};
+#pragma unroll
+        for (int j = 0; j < NI; ++j) c.issue(j);
+    } else {
+        copy_any<D, kWaves, kIsK>(k, k0, kBc, dst, wave, lane);
+    }
+}
+
 // What the loop needs to know of a block: keys S on the joint axis, tiles ntiles, this wave's chunks nch (0:
 // it has no queries), its first query on the key axis qv0 (causal), and main tiles t < t_main, whose chunks
 // 2t + 1 and 2t + 2 every query sees and whose copies of V (t + 1) and K (t + 2) are whole tiles that exist.
 struct Shape { int S, ntiles, nch, qv0, t_main; };
 
-// Leaves the running base-2 maxima m, the sums lacc and O^T of the wave's queries (attn_tile.hpp's layout).
+// The copies of K 0, V 0 and K 1, which attend waits for.
+template <int D, bool kPrefix>
+__device__ __forceinline__ void first_copies(const Keys<kPrefix>& keys_k, const Keys<kPrefix>& keys_v, int ntiles,
+                                             const Offsets& own, uint16_t* lds, int wave, int lane) {
+    copy_tile<D, true>(keys_k, 0, own, lds, wave, lane);
+    copy_tile<D, false>(keys_v, 0, own, lds + lds_v<D>(), wave, lane);
+    if (ntiles > 1) copy_tile<D, true>(keys_k, 1, own, lds + kBc * D, wave, lane);
+}
+
+// After first_copies: leaves the running base-2 maxima m, the sums lacc and O^T of the wave's queries (attn_tile.hpp's layout).
 // Tile t's regions (attn_pipe.hpp), with a barrier before each:
 //   region 2t     S of chunk 2t + 1 (K t), P.V of chunk 2t (V t); copies V (t + 1) into the slot of V (t - 1)
 //   region 2t + 1 S of chunk 2t + 2 (K t + 1), P.V of chunk 2t + 1; copies K (t + 2) into the slot of K t
@@ -80,19 +125,17 @@ struct Shape { int S, ntiles, nch, qv0, t_main; };
 template <int D, bool kBf16, bool kPrefix, bool kCausal>
 __device__ __forceinline__ void attend(const Keys<kPrefix>& keys_k, const Keys<kPrefix>& keys_v, const Shape& shape,
                                        const u32x4 (&qb)[kQT][D / 32], f32x4 (&o)[kQT][D / 16], f32x4 (&lacc)[kQT],
-                                       float (&m)[kQT], uint16_t* lds, float sc, int wave, int lane) {
+                                       float (&m)[kQT], const Offsets& own, uint16_t* lds, float sc, int wave,
+                                       int lane) {
     constexpr int W = kWaves, QT = kQT, NDT = D / 16;
     constexpr int kTile = kBc * D, NI = kBc * (D / 8) / (64 * W);
     const int li = lane & 15, g = lane >> 4;
     const int P = keys_k.P, S = shape.S, ntiles = shape.ntiles, nch = shape.nch, qv0 = shape.qv0, t_main = shape.t_main;
-    uint16_t* const vlds = lds + 2 * kTile;
-    auto copy_k = [&](int t) { copy_any<D, W, true>(keys_k, t * kBc, kBc, lds + (t & 1) * kTile, wave, lane); };
-    auto copy_v = [&](int t) { copy_any<D, W, false>(keys_v, t * kBc, kBc, vlds + (t & 1) * kTile, wave, lane); };
-    copy_k(0);
-    copy_v(0);
-    if (ntiles > 1) copy_k(1);
+    uint16_t* const vlds = lds + lds_v<D>();
+    auto copy_k = [&](int t) { copy_tile<D, true>(keys_k, t, own, lds + (t & 1) * kTile, wave, lane); };
+    auto copy_v = [&](int t) { copy_tile<D, false>(keys_v, t, own, vlds + (t & 1) * kTile, wave, lane); };
     using CP = StepCopy<D, W, NI>;
-    uint32_t koff[2], voff[2];
+    uint32_t koff[2] = {own.k[0], own.k[1]}, voff[2] = {own.v[0], own.v[1]};
     const float inv_sc = 1.f / sc;
     float thr[QT];
 #pragma unroll
@@ -171,8 +214,10 @@ __device__ __forceinline__ void attend(const Keys<kPrefix>& keys_k, const Keys<k
         const uint16_t* kb = (pre ? keys_k.pre : keys_k.own - (long long)P * keys_k.rs) + 2LL * kBc * rs;
         const uint16_t* vb = (pre ? keys_v.pre : keys_v.own - (long long)P * keys_k.rs) + (long long)kBc * rs;
         const int t1 = pre ? min(t_main, P / kBc - 2) : t_main;   // main tiles of this source: t < t1
-        CP::template offsets<true>(rs, wave, lane, koff);
-        CP::template offsets<false>(rs, wave, lane, voff);
+        if (pre) {
+            CP::template offsets<true>(D, wave, lane, koff);
+            CP::template offsets<false>(D, wave, lane, voff);
+        }
 #pragma unroll 1
         for (; t + 2 <= t1; t += 2) {
             tile_iter(t, std::false_type{}, std::false_type{}, 0, kb + (long long)t * kBc * rs, vb + (long long)t * kBc * rs, rs);
@@ -184,6 +229,8 @@ __device__ __forceinline__ void attend(const Keys<kPrefix>& keys_k, const Keys<k
         for (; t < t2; ++t) tile_iter(t, std::true_type{}, std::false_type{}, t & 1, nullptr, nullptr, 0);
         if (!pre) break;
         pre = false;
+#pragma unroll
+        for (int j = 0; j < 2; ++j) { koff[j] = own.k[j]; voff[j] = own.v[j]; }
     }
 }
 

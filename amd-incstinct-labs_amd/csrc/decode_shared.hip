@@ -80,11 +80,13 @@ __device__ __forceinline__ void prefix_part(const SharedArgs& a, int item, uint1
     }
     const int ntiles = (S + pipe::kBc - 1) / pipe::kBc;
     const int t_main = min(S >= 96 ? (S - 96) / 64 + 1 : 0, min(ntiles, S / pipe::kBc) - 2);
-    const block::Keys<false> kk{Kh, nullptr, D, 0, S}, kv{Vh, nullptr, D, 0, S};
+    const block::Keys<false> kk{Kh, nullptr, D, 0, S, 1}, kv{Vh, nullptr, D, 0, S, 1};
+    const block::Offsets own = block::own_offsets<D>(D, wave, lane);
+    block::first_copies<D, false>(kk, kv, ntiles, own, lds, wave, lane);
     f32x4 o[QT][NDT], lacc[QT];
     float m[QT];
     block::attend<D, kBf16, false, false>(kk, kv, block::Shape{S, ntiles, r0 < rows ? (S + 31) / 32 : 0, 0, t_main}, qb, o,
-                                          lacc, m, lds, a.sc, wave, lane);
+                                          lacc, m, own, lds, a.sc, wave, lane);
     const int PT = a.Pp + a.Po;
 #pragma unroll
     for (int t = 0; t < QT; ++t) {

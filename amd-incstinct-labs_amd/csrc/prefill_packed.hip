@@ -35,78 +35,125 @@ struct PackedArgs {
     long long q_rs, q_hs, k_rs, k_hs, o_rs, o_hs;   // row (token) and head strides, elements
     long long p_hs;                                  // head stride of the prefix (rows are D elements apart)
     int nQH, G, batch, total, prefix;
+    int hp;       // log2 of the query heads per workgroup
     int copy32;   // 1: a step's rows span < 4 GiB (32-bit copy offsets)
     float sc;     // log2(e) / sqrt(D)
 };
 
 // ---- work items ----------------------------------------------------------------------------------
-// Blocks of sequence s with `rows` queries each; cu outside 0 .. total or decreasing is cut to it, so that
-// no contents of cu lead outside the tensors.
+// Rows of sequence s; cu outside 0 .. total or decreasing is cut to it, so that no contents of cu lead
+// outside the tensors.
 __device__ __forceinline__ void seq_rows(const PackedArgs& a, int s, int& start, int& len) {
     start = min(max(a.cu[s], 0), a.total);
     len = min(max(a.cu[s + 1], start), a.total) - start;   // cut before the difference, which then cannot wrap
 }
 
-// Entry idx of the list of blocks, block index descending and sequences ascending within one index:
-// f(d) = sum_s max(0, n_s - d) blocks have an index of d or more, so idx lies at the largest d with
-// f(d) > idx, found by bisection; each lane holds the block counts of sequences lane, lane + 64, ..
-// (kHeld in registers, the rest read again). Six wave sums at 64 blocks a sequence, ~0.3 us.
-// False past the last block.
-constexpr int kHeld = 4;
-template <int kRows>
-__device__ __forceinline__ bool packed_item(const PackedArgs& a, int idx, int lane, int& start, int& len, int& blk) {
-    int n[kHeld];
-    auto blocks = [&](int s) {
-        int st, ln;
-        if (s >= a.batch) return 0;
-        seq_rows(a, s, st, ln);
-        return (ln + kRows - 1) / kRows;
-    };
-    int most = 0, sum = 0;
-#pragma unroll
-    for (int i = 0; i < kHeld; ++i) {
-        n[i] = 0;
-        if (64 * i < a.batch) n[i] = blocks(64 * i + lane);
-        most = max(most, n[i]);
-        sum += n[i];
+// The list of blocks, block index descending and sequences ascending within one index. With n_s the blocks of
+// sequence s, f(d) = sum_s max(0, n_s - d) blocks have an index of d or more, so entry idx of the list has
+// the largest index d with f(d) > idx, and is the (idx - f(d + 1))-th sequence with more than d blocks. A
+// workgroup forms f once, in LDS: a histogram of the n_s, summed twice from the top (the sequences with more
+// than d blocks, then their blocks).
+constexpr int kLevels = 1024;   // block indices held: sequences of 32,768 tokens and more (rows_log2)
+constexpr int kSeqs = 512;      // sequences held; the rows of others are read again
+struct Items {
+    int f[kLevels];
+    int2 seq[kSeqs];   // first row, rows
+    int levels;
+};
+
+__device__ __forceinline__ int scalar(int x) { return __builtin_amdgcn_readfirstlane(x); }   // the same in every lane
+
+__device__ __forceinline__ int blocks_of(const PackedArgs& a, const Items& it, int s, int rows_log2) {
+    int start, len;
+    if (s >= a.batch) return 0;
+    if (s < kSeqs) len = it.seq[s].y;
+    else seq_rows(a, s, start, len);
+    return (len + (1 << rows_log2) - 1) >> rows_log2;
+}
+
+// hist: kLevels + 1 words of LDS, free until the barrier at the end.
+__device__ __forceinline__ void list_items(const PackedArgs& a, int rows_log2, Items& it, int* hist, int tid) {
+    for (int i = tid; i <= kLevels; i += 256) hist[i] = 0;
+    __syncthreads();
+    for (int s = tid; s < a.batch; s += 256) {
+        int start, len;
+        seq_rows(a, s, start, len);
+        if (s < kSeqs) it.seq[s] = make_int2(start, len);
+        const int n = (len + (1 << rows_log2) - 1) >> rows_log2;
+        if (n > 0) {
+            atomicAdd(&hist[min(n, kLevels)], 1);
+            atomicMax(&hist[0], n);   // entry 0 is not a count
+        }
     }
-    for (int s = 64 * kHeld; s < a.batch; s += 64) {
-        const int x = blocks(s + lane);
-        most = max(most, x);
-        sum += x;
+    __syncthreads();
+    if (tid < 64) {
+        const int levels = scalar(hist[0]);
+        if (tid == 0) it.levels = levels;
+        int more = 0, f = 0;   // of the levels above
+        for (int d0 = (min(levels, kLevels) - 1) & ~63; d0 >= 0; d0 -= 64) {
+            const int d = d0 + 63 - tid;
+            const int g = wave::xlane::scan_inclusive(d < kLevels ? hist[d + 1] : 0, Sum{}) + more;
+            const int x = wave::xlane::scan_inclusive(g, Sum{}) + f;
+            it.f[d] = x;
+            more = __builtin_amdgcn_readlane(g, 63);
+            f = __builtin_amdgcn_readlane(x, 63);
+        }
     }
-    // every lane holds a wave sum: readfirstlane keeps what follows from it scalar
-    auto scalar = [](int x) { return __builtin_amdgcn_readfirstlane(x); };
-    if (idx >= scalar(allreduce(sum, Sum{}))) return false;
-    auto above = [&](int d) {   // f(d)
-        int x = 0;
-#pragma unroll
-        for (int i = 0; i < kHeld; ++i) x += max(n[i] - d, 0);
-        for (int s = 64 * kHeld; s < a.batch; s += 64) x += max(blocks(s + lane) - d, 0);
-        return scalar(allreduce(x, Sum{}));
-    };
-    int lo = 0, hi = scalar(allreduce(most, Max{})), f_hi = 0;   // f(lo) > idx >= f(hi)
-    while (hi - lo > 1) {
-        const int mid = (lo + hi) >> 1, f = above(mid);
-        if (f > idx) lo = mid;
-        else { hi = mid; f_hi = f; }
+    __syncthreads();
+}
+
+// Entry idx of the list; false past its end.
+__device__ __forceinline__ bool find_item(const PackedArgs& a, int rows_log2, const Items& it, int idx, int lane, int& start,
+                                          int& len, int& blk) {
+    const int levels = scalar(it.levels);
+    if (levels == 0) return false;
+    int f_above;
+    if (levels <= kLevels) {
+        if (idx >= scalar(it.f[0])) return false;
+        constexpr int kStep = kLevels / 64;
+        const int seg = kStep * (__popcll(__builtin_amdgcn_ballot_w64(kStep * lane < levels && it.f[kStep * lane] > idx)) - 1);
+        const int d = seg + lane;
+        blk = seg + __popcll(__builtin_amdgcn_ballot_w64(lane < kStep && d < levels && it.f[min(d, kLevels - 1)] > idx)) - 1;
+        f_above = blk + 1 < levels ? scalar(it.f[blk + 1]) : 0;
+    } else {   // longer than the levels held: f by bisection, each from all sequences
+        auto f = [&](int d) {
+            int x = 0;
+            for (int s = lane; s < a.batch; s += 64) x += max(blocks_of(a, it, s, rows_log2) - d, 0);
+            return scalar(allreduce(x, Sum{}));
+        };
+        if (idx >= f(0)) return false;
+        int lo = 0, hi = levels;   // f(lo) > idx >= f(hi)
+        f_above = 0;
+        while (hi - lo > 1) {
+            const int mid = (lo + hi) >> 1, x = f(mid);
+            if (x > idx) lo = mid;
+            else { hi = mid; f_above = x; }
+        }
+        blk = lo;
     }
-    blk = lo;
-    int r = idx - f_hi, seq = -1;   // the r-th sequence with more than blk blocks
-    auto pick = [&](int s0, int cnt) {
-        const uint64_t mask = __builtin_amdgcn_ballot_w64(cnt > blk);
-        const int before = __builtin_amdgcn_mbcnt_hi((uint32_t)(mask >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)mask, 0u));
-        const uint64_t here = __builtin_amdgcn_ballot_w64(cnt > blk && before == r);
-        if (here != 0 && seq < 0) seq = s0 + __builtin_ctzll(here);
-        r -= __popcll(mask);
-    };
-#pragma unroll
-    for (int i = 0; i < kHeld; ++i) pick(64 * i, n[i]);
-    for (int s = 64 * kHeld; s < a.batch && seq < 0; s += 64) pick(s, blocks(s + lane));
-    seq_rows(a, max(seq, 0), start, len);
+    int r = idx - f_above, seq = 0;
+    for (int s0 = 0; s0 < a.batch; s0 += 64) {
+        const bool has = blocks_of(a, it, s0 + lane, rows_log2) > blk;
+        const uint64_t mask = __builtin_amdgcn_ballot_w64(has);
+        const int c = __popcll(mask);
+        if (r < c) {
+            const int before = __builtin_amdgcn_mbcnt_hi((uint32_t)(mask >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)mask, 0u));
+            const uint64_t here = __builtin_amdgcn_ballot_w64(has && before == r);
+            seq = s0 + (here ? __builtin_ctzll(here) : 0);
+            break;
+        }
+        r -= c;
+    }
+    if (seq < kSeqs) {
+        const int2 sl = it.seq[seq];
+        start = sl.x;
+        len = sl.y;
+    } else {
+        seq_rows(a, seq, start, len);
+    }
     start = scalar(start);
     len = scalar(len);
-    return blk * kRows < len;   // always, but for counts of overlapping sequences that pass 32 bits
+    return (blk << rows_log2) < len;   // always, but for counts of overlapping sequences that pass 32 bits
 }
 
 // Head of workgroup i within one entry's nQH workgroups. Workgroups go to the XCDs round-robin: with nQH a
@@ -115,69 +162,116 @@ __device__ __forceinline__ int item_head(int i, int nQH) {
     return (nQH & 7) ? i : (i & 7) * (nQH >> 3) + (i >> 3);
 }
 
+// O^T / l of 16 queries as 16-bit rows: lane (li, g) holds elements 16 dt + 4 g + e of query li. A swap between
+// neighbouring rows of lanes gives each lane eight neighbouring elements, so that a store writes 64 contiguous
+// bytes per query instead of 32, in half the instructions.
 template <int D, bool kBf16>
-__device__ __forceinline__ void store_rows(const f32x4 (&o)[D / 16], float l, uint16_t* dst) {
+__device__ __forceinline__ void store_rows(const f32x4 (&o)[D / 16], float l, uint16_t* row, int g, bool valid) {
+    typedef uint32_t u32x4_8 __attribute__((ext_vector_type(4), aligned(8)));   // O is 8-byte aligned
     const float inv = l > 0.f ? 1.f / l : 1.f;
+    uint16_t* dst = row + (g & 1) * 16 + (g >> 1) * 8;
 #pragma unroll
-    for (int dt = 0; dt < D / 16; ++dt)
-        *(u32x2*)(dst + dt * 16) = u32x2{pack2<kBf16>(o[dt][0] * inv, o[dt][1] * inv), pack2<kBf16>(o[dt][2] * inv, o[dt][3] * inv)};
+    for (int dt = 0; dt < D / 16; dt += 2) {
+        u32x4_8 w;
+#pragma unroll
+        for (int x = 0; x < 2; ++x) {
+            const uint32_t even = pack2<kBf16>(o[dt][2 * x] * inv, o[dt][2 * x + 1] * inv);
+            const uint32_t odd = pack2<kBf16>(o[dt + 1][2 * x] * inv, o[dt + 1][2 * x + 1] * inv);
+            const auto r = __builtin_amdgcn_permlane16_swap(even, odd, false, false);
+            w[x] = r[0];
+            w[2 + x] = r[1];
+        }
+        if (valid) *(u32x4_8*)(dst + dt * 16) = w;
+    }
 }
 
-// ---- 128 queries per workgroup, two workgroups per CU ---------------------------------------------
+// ---- 128 rows per workgroup, two workgroups per CU -------------------------------------------------
 // Four waves of 32 queries share 64-key K/V tiles in LDS, two slots each for K and V (64 KiB at D = 128), so
-// that two workgroups fit a CU: while one fills its first tiles, masks its diagonal or stores, the other has
-// the matrix cores. Tile t's regions (attn_pipe.hpp), with a barrier before each:
-//   region 2t     S of chunk 2t + 1 (K t), P.V of chunk 2t (V t); copies V (t + 1) into the slot of V (t - 1)
-//   region 2t + 1 S of chunk 2t + 2 (K t + 1), P.V of chunk 2t + 1; copies K (t + 2) into the slot of K t
-// so each copy has the time of two regions to land.
+// that two workgroups fit a CU: while one waits for its first tiles, masks its diagonal or stores, the other
+// has the matrix cores. The grid is one round of them; workgroup p takes entries p, 2 G - 1 - p, 2 G + p, ..
+// of the list times the heads (G workgroups), which evens out what a round's order costs, and loads the next
+// item's queries and first tiles before it stores its results: an item of one tile took 12.4 us as a
+// workgroup of its own, of which 2.4 to find it, 3.0 for the first loads and 2.9 for the stores.
 template <int D, bool kBf16, bool kPrefix>
 __global__ __launch_bounds__(256, 2) void fa_packed(PackedArgs a) {
-    constexpr int QT = block::kQT, ND = D / 32, NDT = D / 16, BM = block::kRows;
+    constexpr int QT = block::kQT, ND = D / 32, NDT = D / 16;
     __shared__ __attribute__((aligned(16))) uint16_t lds[block::lds_elems<D>()];
+    __shared__ Items items;
+    static_assert((kLevels + 1) * 4 <= (int)sizeof(lds), "the histogram fits the tiles' LDS");
     const int lane = (int)(threadIdx.x & 63u);
-    const int wave = __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
+    const int wave = scalar((int)(threadIdx.x >> 6));
     const int li = lane & 15, g = lane >> 4;
-
-    const int entry = (int)blockIdx.x / a.nQH;
-    const int h = item_head((int)blockIdx.x - entry * a.nQH, a.nQH);
-    int start, len, blk;
-    if (!packed_item<BM>(a, entry, lane, start, len, blk)) return;
+    // The workgroup's waves serve 1 << hp query heads of one kv head, block::kRows >> hp tokens each
+    const int hp = a.hp, rows_log2 = block::kRowsLog2 - hp, nh = a.nQH >> hp;
     const int P = kPrefix ? a.prefix : 0;
-    const int q0 = blk * BM, qw0 = q0 + wave * QT * 16, S = P + len;
-    const int kvh = h / a.G;
-    const uint16_t* own_k = a.K + start * a.k_rs + kvh * a.k_hs;
-    const uint16_t* own_v = a.V + start * a.k_rs + kvh * a.k_hs;
-    const Keys<kPrefix> keys_k{own_k, a.Kp + kvh * a.p_hs, a.k_rs, P, S};
-    const Keys<kPrefix> keys_v{own_v, a.Vp + kvh * a.p_hs, a.k_rs, P, S};
+    list_items(a, rows_log2, items, (int*)lds, (int)threadIdx.x);
+
+    // Each wave finds the item of another of the next four rounds.
+    __shared__ int4 next_s[4];
+    auto find = [&](int round) {
+        const int G = (int)gridDim.x, p = (int)blockIdx.x;
+        const int idx = round * G + ((round & 1) ? G - 1 - p : p), entry = idx / nh;
+        int start = 0, len = 0, blk = 0;
+        const bool ok = find_item(a, rows_log2, items, entry, lane, start, len, blk);
+        if (lane == 0) next_s[round & 3] = make_int4(start, ok ? len : 0, blk << rows_log2, item_head(idx - entry * nh, nh) << hp);
+    };
+    struct Item { int start, len, q0, h0; };
+    auto item_at = [&](int round) {   // len 0: none
+        const int4 x = next_s[round & 3];
+        return Item{scalar(x.x), scalar(x.y), scalar(x.z), scalar(x.w)};
+    };
+    const block::Offsets own = block::own_offsets<D>(a.k_rs, wave, lane);
     u32x4 qb[QT][ND];
-    {
-        const uint16_t* Qh = a.Q + start * a.q_rs + h * a.q_hs;
+    auto keys = [&](const Item& it, const uint16_t* own, const uint16_t* pre) {
+        const int kvh = it.h0 / a.G;
+        return Keys<kPrefix>{own + it.start * a.k_rs + kvh * a.k_hs, pre + kvh * a.p_hs, a.k_rs, P, P + it.len, a.copy32};
+    };
+    auto tiles = [&](const Item& it) { return (P + min(it.q0 + (1 << rows_log2), it.len) + kBc - 1) / kBc; };
+    const int dq = (wave & ((4 >> hp) - 1)) * QT * 16, dh = wave >> (2 - hp);   // of this wave in the block
+    auto load = [&](const Item& it) {   // the queries and the first tiles
+        const uint16_t* Qh = a.Q + it.start * a.q_rs + (it.h0 + dh) * a.q_hs;
 #pragma unroll
         for (int t = 0; t < QT; ++t) {
-            const int q = min(qw0 + t * 16 + li, len - 1);
+            const int q = min(it.q0 + dq + t * 16 + li, it.len - 1);
 #pragma unroll
             for (int c = 0; c < ND; ++c) qb[t][c] = *(const u32x4*)(Qh + q * a.q_rs + c * 32 + g * 8);
         }
-    }
-    const int ntiles = (P + min(q0 + BM, len) + kBc - 1) / kBc;
-    const int wave_end = min(qw0 + QT * 16, len);                     // one past this wave's last query
-    const int nch = wave_end > qw0 ? (P + wave_end + 31) / 32 : 0;     // the wave's chunks; 0: no queries
-    // Main tiles: chunks 2t + 1 and 2t + 2 lie below the workgroup's first query, and the copies of
-    // V (t + 1) and K (t + 2) are whole tiles that exist.
-    int t_main = P + q0 >= 95 ? (P + q0 - 95) / 64 + 1 : 0;
-    t_main = min(t_main, min(ntiles - 2, S / kBc - 2));
-    if (!a.copy32) t_main = 0;
-
-    f32x4 o[QT][NDT], lacc[QT];
-    float m[QT];
-    block::attend<D, kBf16, kPrefix, true>(keys_k, keys_v, block::Shape{S, ntiles, nch, P + qw0, t_main}, qb, o, lacc, m,
-                                           lds, a.sc, wave, lane);
-
-    uint16_t* Oh = a.O + start * a.o_rs + h * a.o_hs;
+        block::first_copies<D, kPrefix>(keys(it, a.K, a.Kp), keys(it, a.V, a.Vp), tiles(it), own, lds, wave, lane);
+    };
+    find(wave);
+    __syncthreads();
+    Item it = item_at(0);
+    if (it.len == 0) return;
+    load(it);
+    for (int round = 1;; ++round) {
+        const int qw0 = it.q0 + dq, S = P + it.len, ntiles = tiles(it);
+        const int wave_end = min(qw0 + QT * 16, it.len);                  // one past this wave's last query
+        const int nch = wave_end > qw0 ? (P + wave_end + 31) / 32 : 0;     // the wave's chunks; 0: no queries
+        // Main tiles: chunks 2t + 1 and 2t + 2 lie below the workgroup's first query, and the copies of
+        // V (t + 1) and K (t + 2) are whole tiles that exist.
+        int t_main = P + it.q0 >= 95 ? (P + it.q0 - 95) / 64 + 1 : 0;
+        t_main = min(t_main, min(ntiles - 2, S / kBc - 2));
+        if (!a.copy32) t_main = 0;
+        f32x4 o[QT][NDT], lacc[QT];
+        float m[QT];
+        block::attend<D, kBf16, kPrefix, true>(keys(it, a.K, a.Kp), keys(it, a.V, a.Vp), block::Shape{S, ntiles, nch, P + qw0, t_main},
+                                               qb, o, lacc, m, own, lds, a.sc, wave, lane);
+        uint16_t* Oh = a.O + it.start * a.o_rs + (it.h0 + dh) * a.o_hs;
+        const int len = it.len;
+        // What lies between two items is short and holds the matrix cores up: ahead of the CU's other waves
+        __builtin_amdgcn_s_setprio(3);
+        if ((round & 3) == 0) find(round + wave);
+        __syncthreads();   // every wave is done with the tiles; the next items are there
+        it = item_at(round);
+        const bool more = it.len > 0;
+        if (more) load(it);
 #pragma unroll
-    for (int x = 0; x < QT; ++x) {
-        const int q = qw0 + x * 16 + li;
-        if (q < len) store_rows<D, kBf16>(o[x], lacc[x][0], Oh + q * a.o_rs + g * 4);
+        for (int x = 0; x < QT; ++x) {
+            const int q = qw0 + x * 16 + li;
+            store_rows<D, kBf16>(o[x], lacc[x][0], Oh + q * a.o_rs, g, q < len);
+        }
+        if (!more) break;
+        __builtin_amdgcn_s_setprio(0);
     }
 }
 
@@ -209,16 +303,23 @@ int check_packed(const cdna4_packed_cfg* cfg, const cdna4_packed_strides* st, co
     return 0;
 }
 
-struct PackedPlan { int kernel, waves, rows; long long grid; };
+struct PackedPlan { int kernel, waves, rows, hp; long long grid; };
 
 template <int D>
 PackedPlan plan_packed(const cdna4_packed_cfg& c) {
     PackedPlan p{};
     p.kernel = CDNA4_KERNEL_PACKED_4W;
     p.waves = 4;
-    p.rows = 128;
+    // Query heads of one kv head side by side, up to one per wave: a block then has 128, 64 or 32 tokens, its
+    // waves end at the same key or nearly so (with 128 tokens they pass the last two tiles as a staircase), and
+    // short sequences fill it.
+    const int G = c.nQHeads / c.nKVHeads;
+    p.hp = G % 4 == 0 ? 2 : G % 2 == 0 ? 1 : 0;
+    p.rows = block::kRows >> p.hp;
     // sum of ceil(len / rows) is at most total / rows + the sequences that are not empty
-    p.grid = (long long)c.nQHeads * (c.total / p.rows + std::min(c.batch, c.total));
+    p.grid = (long long)(c.nQHeads >> p.hp) * (c.total / p.rows + std::min(c.batch, c.total));
+    // one round of resident workgroups
+    p.grid = std::min(p.grid, 2LL * (device_cus() & ~3));
     return p;
 }
 
@@ -233,7 +334,7 @@ int launch_packed(const cdna4_packed_cfg& c, const cdna4_packed_strides& st, con
     a.cu = cu;
     a.q_rs = st.q_row; a.q_hs = st.q_head; a.k_rs = st.kv_row; a.k_hs = st.kv_head; a.o_rs = st.o_row; a.o_hs = st.o_head;
     a.p_hs = (long long)(c.stride_prefix ? c.stride_prefix : c.prefix) * D;
-    a.nQH = c.nQHeads; a.G = c.nQHeads / c.nKVHeads; a.batch = c.batch; a.total = c.total; a.prefix = c.prefix;
+    a.nQH = c.nQHeads; a.G = c.nQHeads / c.nKVHeads; a.batch = c.batch; a.total = c.total; a.prefix = c.prefix; a.hp = p.hp;
     a.copy32 = 256 * st.kv_row * 2 < (1LL << 32) ? 1 : 0;
     a.sc = kLog2e / sqrtf((float)D);
     const unsigned grid = (unsigned)p.grid;
