@@ -35,7 +35,7 @@ struct SharedArgs {
     int nQH, nKVH, G, HB, batch, prefix, max_own;
     int blocks, kpp, Pp;       // row blocks per kv head, keys per prefix part, prefix parts
     int Po, kmin;              // own parts per row at most, keys per own part at least
-    int prefix_groups, groups; // groups of 8 workgroups: those of prefix parts, all
+    int prefix_groups;         // groups of 8 workgroups of prefix parts
     float sc;
 };
 
@@ -159,17 +159,16 @@ __device__ __forceinline__ void own_part(const SharedArgs& a, int item, uint16_t
     }
 }
 
-// Workgroups come in groups of 8, one per XCD; the prefix parts' groups are spread evenly over all groups.
+// Workgroups of prefix parts first, in groups of 8, one per XCD: with own keys in the call they are one per CU
+// (plan_shared), and the own parts that follow take the CUs' other places.
 template <int D, bool kBf16, bool kNT>
 __global__ __launch_bounds__(256, 2) void shared_parts(SharedArgs a) {
     __shared__ __attribute__((aligned(16))) uint16_t lds[shared_lds<D>()];
     const int lane = (int)(threadIdx.x & 63u);
     const int wave = __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
-    const int gi = (int)blockIdx.x >> 3, x = (int)blockIdx.x & 7;
-    const int before = (int)((long long)gi * a.prefix_groups / a.groups);
-    const int after = (int)((long long)(gi + 1) * a.prefix_groups / a.groups);
-    if (after > before) prefix_part<D, kBf16>(a, before * 8 + x, lds, wave, lane);
-    else own_part<D, kBf16, kNT>(a, (gi - before) * 8 + x, lds, wave, lane);
+    const int own = (int)blockIdx.x - a.prefix_groups * 8;
+    if (own < 0) prefix_part<D, kBf16>(a, (int)blockIdx.x, lds, wave, lane);
+    else own_part<D, kBf16, kNT>(a, own, lds, wave, lane);
 }
 
 // One wave per (batch, query head): its n parts joined (Pp of the prefix, then the own ones that exist).
@@ -231,9 +230,10 @@ bool plan_shared(const cdna4_shared_decode_cfg& c, SharedPlan& p) {
     if (c.prefix > 0x7fffffff - 1024 || c.max_own > 0x7fffffff - 1024) return false;
     if (c.stride_prefix != 0 && c.stride_prefix < c.prefix) return false;
     if (c.stride_kv != 0 && c.stride_kv < c.max_own) return false;
-    const long long slots = 2LL * device_cus();
+    const long long cus = device_cus(), slots = 2 * cus;
     p.G = c.nQHeads / c.nKVHeads;
     p.HB = (p.G + 15) / 16;
+    const long long own_rows = (long long)c.batch * c.nKVHeads * p.HB;
     const long long rows = (long long)c.batch * p.G;
     if (rows > 0x7fffffff - block::kRows || (long long)c.batch * c.nQHeads > 0x7fffffff) return false;
     p.blocks = (int)((rows + block::kRows - 1) / block::kRows);
@@ -242,22 +242,32 @@ bool plan_shared(const cdna4_shared_decode_cfg& c, SharedPlan& p) {
     p.kpp = 64;
     if (c.prefix > 0) {
         const long long tiles = (c.prefix + 63) / 64, all = tiles * c.nKVHeads * p.blocks;
-        long long per = std::max(2LL, (all + slots - 1) / slots);
+        // One part per CU (a CU with two runs each of them slower, and the parts' results are written and read
+        // again: 64 sequences behind 8,192 keys, 32/8 heads D 128, 22.3 us with 256 parts, 27.5 with 128, 29.1
+        // with 512), two where the parts stay long (256 behind 16,384: 73.8 against 81.4 us). With about as many
+        // own keys, three quarters of that: their parts get the other CUs (64 behind 8,192 with 20-1,000 own
+        // 29.6 against 32.2 us, 256 behind 16,384 with 64-2,048 142 against 151 us). Half the capacity is taken
+        // for the own keys, whose number is on the device.
+        const long long own = c.max_own / 2 / 64 * own_rows;
+        const long long want = all >= 32 * slots && 8 * own < all ? slots : 2 * own >= all ? cus * 3 / 4 : cus;
+        long long per = std::max(2LL, (all + want - 1) / want);
         per = std::min(per, tiles);
         p.kpp = (int)per * 64;
         p.Pp = (int)((tiles + per - 1) / per);
     }
     p.prefix_groups = ((long long)c.nKVHeads * p.Pp + 7) / 8 * p.blocks;
     // own keys
-    const long long own_rows = (long long)c.batch * c.nKVHeads * p.HB;
     p.Po = 0;
     p.kmin = 64;
     if (c.max_own > 0) {
-        long long keys = (c.max_own * own_rows + 4 * slots - 1) / (4 * slots);
-        keys = std::min(std::max(keys, 64LL), 512LL);
+        // Two rounds of parts at full lengths, of 64 to 1,024 keys, and up to 32 parts a row (more cost the join
+        // more than they save: one sequence of 8,192 keys 10.7 us with 32, 17.5 with 128). 256 sequences of 64-2,048
+        // keys: 108.8 us with 512 keys a part, 108.1 with 1,024, 113.7 with 2,048, 152 with 128.
+        long long keys = (c.max_own * own_rows + 2 * slots - 1) / (2 * slots);
+        keys = std::max({std::min(keys, 1024LL), 64LL, (c.max_own + 31LL) / 32});
         keys = (keys + 63) / 64 * 64;
         p.kmin = (int)keys;
-        p.Po = (int)std::min((c.max_own + keys - 1) / keys, 1024LL);
+        p.Po = (int)((c.max_own + keys - 1) / keys);
     }
     p.groups = p.prefix_groups + (own_rows * p.Po + 7) / 8;
     if (p.groups * 8 * 256 > 0xffffffffLL) return false;
@@ -279,7 +289,7 @@ int launch_shared(const cdna4_shared_decode_cfg& c, const SharedPlan& p, const v
     a.kv_hs = (long long)(c.stride_kv ? c.stride_kv : c.max_own) * D;
     a.nQH = c.nQHeads; a.nKVH = c.nKVHeads; a.G = p.G; a.HB = p.HB; a.batch = c.batch; a.prefix = c.prefix; a.max_own = c.max_own;
     a.blocks = p.blocks; a.kpp = p.kpp; a.Pp = p.Pp; a.Po = std::max(p.Po, 0); a.kmin = p.kmin;
-    a.prefix_groups = (int)p.prefix_groups; a.groups = (int)p.groups;
+    a.prefix_groups = (int)p.prefix_groups;
     a.sc = kLog2e / sqrtf((float)D);
     if (p.groups > 0) {
         const unsigned grid = (unsigned)(p.groups * 8);
