@@ -39,7 +39,7 @@ __all__ = [
     "scatter_kv_f16", "repack_f16", "rope_append_kv_f16", "ModelCfg", "GenerateCfg", "Session",
     "PlanInfo", "prefill_plan", "decode_plan", "scan_status", "KERNEL_NAMES", "decode_noalloc",
     "decode_noalloc_max_bytes", "softmax_rows_f32", "PackedPrefillCfg", "PackedStrides", "prefill_packed",
-    "prefill_packed_plan", "LogitsArgs", "process_logits", "SharedDecodeCfg",
+    "prefill_packed_plan", "prefill_packed_workspace_size", "LogitsArgs", "process_logits", "SharedDecodeCfg",
     "decode_shared", "decode_shared_plan", "decode_shared_workspace_size",
 ]
 
@@ -173,7 +173,8 @@ def _declare(l: ctypes.CDLL) -> None:
         "cdna3_attn_prefill_plan": (c_int, [ctypes.POINTER(PrefillCfg), c_int, ctypes.POINTER(PlanInfo)]),
         "cdna3_attn_decode_plan": (c_int, [ctypes.POINTER(DecodeCfg), c_int, c_int, ctypes.POINTER(PlanInfo)]),
         "cdna4_attn_prefill_packed": (c_int, [vp] * 7 + [ctypes.POINTER(PackedPrefillCfg),
-                                                         ctypes.POINTER(PackedStrides), c_int, vp]),
+                                                         ctypes.POINTER(PackedStrides), c_int, vp, c_size, vp]),
+        "cdna4_attn_prefill_packed_workspace_size": (c_size, [ctypes.POINTER(PackedPrefillCfg)]),
         "cdna4_attn_prefill_packed_plan": (c_int, [ctypes.POINTER(PackedPrefillCfg), c_int,
                                                    ctypes.POINTER(PlanInfo)]),
         "cdna3_scan_status": (c_int, [vp, ctypes.POINTER(c_int), vp]),
@@ -352,12 +353,14 @@ def _token_major(name: str, t: torch.Tensor, T: int, heads: int, D: int):
 
 def prefill_packed(Q: torch.Tensor, K: torch.Tensor, V: torch.Tensor, O: torch.Tensor, cu_seqlens: torch.Tensor,
                    cfg: PackedPrefillCfg, K_prefix: Optional[torch.Tensor] = None,
-                   V_prefix: Optional[torch.Tensor] = None, stream=None) -> None:
+                   V_prefix: Optional[torch.Tensor] = None, workspace="auto", stream=None) -> None:
     """Causal attention over prompts of different lengths, packed token after token: Q, O [total][nQH][D];
     K, V [total][nKVH][D] (fp16 or bf16, any token and head strides with contiguous rows of D: parts of
     one projection's output, for instance); cu_seqlens int32 [batch + 1] on the device. With
     cfg.prefix > 0 every token also sees the first `prefix` rows of K_prefix / V_prefix [nKVH][stride][D].
-    Rows of O outside cu_seqlens[0] .. cu_seqlens[batch] are left as they are."""
+    Rows of O outside cu_seqlens[0] .. cu_seqlens[batch] are left as they are. `workspace`: "auto" (default)
+    allocates prefill_packed_workspace_size(cfg) bytes, where that is not 0, on the stream the call launches on; a
+    uint8 tensor is used as given; None runs in one launch, which needs none."""
     dev = _device_of(Q, K, V, O, cu_seqlens, K_prefix, V_prefix)
     dt, dtype = _dtype(Q), Q.dtype
     if not (K.dtype == V.dtype == O.dtype == dtype):
@@ -372,9 +375,21 @@ def prefill_packed(Q: torch.Tensor, K: torch.Tensor, V: torch.Tensor, O: torch.T
     kp = vp = 0
     if P > 0:
         kp, vp = _prefix_ptrs(K_prefix, V_prefix, dtype, cfg.nKVHeads * (cfg.stride_prefix or P) * D)
-    with _on_device(dev):
+    if isinstance(workspace, str) and workspace != "auto":
+        raise ValueError("workspace must be 'auto', None or a uint8 tensor")
+    with _on_device(dev), _on_stream(stream):
+        ws = n = 0
+        if isinstance(workspace, str):
+            n = lib().cdna4_attn_prefill_packed_workspace_size(ctypes.byref(cfg))
+            if n:
+                workspace = torch.empty(n, dtype=torch.uint8, device=Q.device)
+                ws = workspace.data_ptr()
+        elif workspace is not None:
+            if workspace.get_device() != dev or not workspace.is_contiguous():
+                raise ValueError("workspace must be contiguous on the GPU of the tensors")
+            ws, n = workspace.data_ptr(), workspace.numel() * workspace.element_size()
         _check(lib().cdna4_attn_prefill_packed(Q.data_ptr(), K.data_ptr(), V.data_ptr(), kp, vp, O.data_ptr(),
-                                               cu_seqlens.data_ptr(), ctypes.byref(cfg), ctypes.byref(st), dt,
+                                               cu_seqlens.data_ptr(), ctypes.byref(cfg), ctypes.byref(st), dt, ws, n,
                                                _stream(stream)), "cdna4_attn_prefill_packed")
 
 
@@ -389,6 +404,10 @@ def _prefix_ptrs(K_prefix, V_prefix, dtype, need: int):
     if min(K_prefix.numel(), V_prefix.numel()) < need:
         raise ValueError("K_prefix/V_prefix smaller than the configuration")
     return K_prefix.data_ptr(), V_prefix.data_ptr()
+
+
+def prefill_packed_workspace_size(cfg: PackedPrefillCfg) -> int:
+    return int(lib().cdna4_attn_prefill_packed_workspace_size(ctypes.byref(cfg)))
 
 
 def prefill_packed_plan(cfg: PackedPrefillCfg, dtype=BF16) -> PlanInfo:

@@ -1,5 +1,5 @@
-// A block of 128 queries against a key axis, the core of the packed prompt kernel (prefill_packed.hip) and of the
-// shared prefix's part of a decode step (decode_shared.hip): four waves of 32 queries over 64-key K/V tiles
+// A block of 128 (or 64) queries against a key axis, the core of the packed prompt kernel (prefill_packed.hip) and of the
+// shared prefix's part of a decode step (decode_shared.hip): four waves of 32 (16) queries over 64-key K/V tiles
 // in LDS, the pipelined regions of attn_pipe.hpp, asynchronous copies two regions ahead.
 #pragma once
 #include <type_traits>
@@ -12,8 +12,8 @@ namespace block {
 using namespace tile;
 using namespace pipe;
 
-constexpr int kWaves = 4, kQT = 2, kRowsLog2 = 7, kRows = 1 << kRowsLog2;   // queries per block
-static_assert(kRows == kWaves * kQT * 16, "");
+constexpr int kWaves = 4;
+template <int QT> constexpr int rows_log2() { return QT == 2 ? 7 : 6; }   // queries per block: QT tiles of 16 per wave
 template <int D> constexpr int lds_elems() { return 4 * kBc * D; }   // K slots 0, 1, V slots 0, 1
 template <int D> constexpr int lds_v() { return 2 * kBc * D; }
 
@@ -122,12 +122,13 @@ __device__ __forceinline__ void first_copies(const Keys<kPrefix>& keys_k, const 
 //   region 2t     S of chunk 2t + 1 (K t), P.V of chunk 2t (V t); copies V (t + 1) into the slot of V (t - 1)
 //   region 2t + 1 S of chunk 2t + 2 (K t + 1), P.V of chunk 2t + 1; copies K (t + 2) into the slot of K t
 // so each copy has the time of two regions to land.
-template <int D, bool kBf16, bool kPrefix, bool kCausal>
+template <int D, int QT, bool kBf16, bool kPrefix, bool kCausal>
 __device__ __forceinline__ void attend(const Keys<kPrefix>& keys_k, const Keys<kPrefix>& keys_v, const Shape& shape,
-                                       const u32x4 (&qb)[kQT][D / 32], f32x4 (&o)[kQT][D / 16], f32x4 (&lacc)[kQT],
-                                       float (&m)[kQT], const Offsets& own, uint16_t* lds, float sc, int wave,
+                                       const u32x4 (&qb)[QT][D / 32], f32x4 (&o)[QT][D / 16], f32x4 (&lacc)[QT],
+                                       float (&m)[QT], const Offsets& own, uint16_t* lds, float sc, int wave,
                                        int lane) {
-    constexpr int W = kWaves, QT = kQT, NDT = D / 16;
+    constexpr int W = kWaves, NDT = D / 16;
+    constexpr bool kAnyDiag = kPrefix || QT == 1;   // a wave's first query is no multiple of 32 on the key axis
     constexpr int kTile = kBc * D, NI = kBc * (D / 8) / (64 * W);
     const int li = lane & 15, g = lane >> 4;
     const int P = keys_k.P, S = shape.S, ntiles = shape.ntiles, nch = shape.nch, qv0 = shape.qv0, t_main = shape.t_main;
@@ -181,7 +182,7 @@ __device__ __forceinline__ void attend(const Keys<kPrefix>& keys_k, const Keys<k
             pipe_region<D, QT, kBf16, false, true, NI, false, CP>(Kt, 1, Vt, 0, off, qb, s, o, m, thr, lacc, ones, true, (j0 + 1) * 32,
                                                                   qv0, S, kCausal, sc, inv_sc, li, g, cv);
         else if (j0 < nch)
-            pipe_region<D, QT, kBf16, true, false, NI, kTwo, CP, kPrefix>(Kt, 1, Vt, 0, off, qb, s, o, m, thr, lacc, ones, j0 + 1 < nch,
+            pipe_region<D, QT, kBf16, true, false, NI, kTwo, CP, kAnyDiag>(Kt, 1, Vt, 0, off, qb, s, o, m, thr, lacc, ones, j0 + 1 < nch,
                                                                  (j0 + 1) * 32, qv0, S, kCausal, sc, inv_sc, li, g, cv);
         // K t + 1 landed (V t + 1 may be in flight); every wave is past region 2t, the last reader of K t
         if (!kTail || t + 1 < ntiles) {
@@ -195,7 +196,7 @@ __device__ __forceinline__ void attend(const Keys<kPrefix>& keys_k, const Keys<k
             pipe_region<D, QT, kBf16, false, true, NI, false, CP>(Kn, 0, Vt, 1, off, qb, s, o, m, thr, lacc, ones, true, (j1 + 1) * 32,
                                                                   qv0, S, kCausal, sc, inv_sc, li, g, ck);
         else if (j1 < nch)
-            pipe_region<D, QT, kBf16, true, false, NI, kTwo, CP, kPrefix>(Kn, 0, Vt, 1, off, qb, s, o, m, thr, lacc, ones, j1 + 1 < nch,
+            pipe_region<D, QT, kBf16, true, false, NI, kTwo, CP, kAnyDiag>(Kn, 0, Vt, 1, off, qb, s, o, m, thr, lacc, ones, j1 + 1 < nch,
                                                                  (j1 + 1) * 32, qv0, S, kCausal, sc, inv_sc, li, g, ck);
     };
     int t = 0;

@@ -107,7 +107,7 @@ __device__ __forceinline__ void pipe_region(const char* Kn, int kcn, const char*
     constexpr int NP = QT * 8;         // P_j values per lane
     constexpr int SL = NP / NK;        // P values per interleave slot
     constexpr int kAhead = 2;          // LDS operand reads issued ahead of their MFMAs
-    static_assert(NP % NK == 0 && SL % 2 == 0, "softmax slices must pair up for the packing");
+    static_assert(NP % NK == 0, "the exponentials spread evenly over the slots");
     if constexpr (kTwo) {
         // Chunk j's keys lie below kLoKeys: first the P.V product of its weights' second bf16 term
         // (s holds chunk j's masked scores, m is the reference P_j is formed against; the sum into

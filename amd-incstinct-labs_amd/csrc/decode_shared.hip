@@ -25,6 +25,8 @@ using wave::xlane::allreduce;
 using wave::xlane::Max;
 using wave::xlane::Sum;
 
+constexpr int kBlockRows = 1 << block::rows_log2<2>();   // rows of a prefix part's workgroup
+
 struct SharedArgs {
     const uint16_t *q, *Kp, *Vp, *K, *V;
     uint16_t* o;
@@ -58,7 +60,7 @@ template <int D> constexpr int shared_lds() { return 32768; }   // elements: 64 
 
 template <int D, bool kBf16>
 __device__ __forceinline__ void prefix_part(const SharedArgs& a, int item, uint16_t* lds, int wave, int lane) {
-    constexpr int QT = block::kQT, ND = D / 32, NDT = D / 16;
+    constexpr int QT = 2, ND = D / 32, NDT = D / 16;
     const int li = lane & 15, g = lane >> 4;
     // item = ((column / 8) * blocks + row block) * 8 + column % 8: the row blocks of a column (kv head and key
     // range) run on one XCD, which workgroups go to round-robin, and share the range in its L2
@@ -66,7 +68,7 @@ __device__ __forceinline__ void prefix_part(const SharedArgs& a, int item, uint1
     if (col >= a.nKVH * a.Pp) return;
     const int kvh = col % a.nKVH, part = col / a.nKVH;
     const int k0 = part * a.kpp, S = min(a.kpp, a.prefix - k0);
-    const int rows = a.batch * a.G, r0 = blk * block::kRows + wave * QT * 16;
+    const int rows = a.batch * a.G, r0 = blk * kBlockRows + wave * QT * 16;
     const uint16_t* Kh = a.Kp + kvh * a.p_hs + (long long)k0 * D;
     const uint16_t* Vh = a.Vp + kvh * a.p_hs + (long long)k0 * D;
     // row r of the kv head: sequence r / G, query head kvh G + r % G
@@ -85,7 +87,7 @@ __device__ __forceinline__ void prefix_part(const SharedArgs& a, int item, uint1
     block::first_copies<D, false>(kk, kv, ntiles, own, lds, wave, lane);
     f32x4 o[QT][NDT], lacc[QT];
     float m[QT];
-    block::attend<D, kBf16, false, false>(kk, kv, block::Shape{S, ntiles, r0 < rows ? (S + 31) / 32 : 0, 0, t_main}, qb, o,
+    block::attend<D, QT, kBf16, false, false>(kk, kv, block::Shape{S, ntiles, r0 < rows ? (S + 31) / 32 : 0, 0, t_main}, qb, o,
                                           lacc, m, own, lds, a.sc, wave, lane);
     const int PT = a.Pp + a.Po;
 #pragma unroll
@@ -235,8 +237,8 @@ bool plan_shared(const cdna4_shared_decode_cfg& c, SharedPlan& p) {
     p.HB = (p.G + 15) / 16;
     const long long own_rows = (long long)c.batch * c.nKVHeads * p.HB;
     const long long rows = (long long)c.batch * p.G;
-    if (rows > 0x7fffffff - block::kRows || (long long)c.batch * c.nQHeads > 0x7fffffff) return false;
-    p.blocks = (int)((rows + block::kRows - 1) / block::kRows);
+    if (rows > 0x7fffffff - kBlockRows || (long long)c.batch * c.nQHeads > 0x7fffffff) return false;
+    p.blocks = (int)((rows + kBlockRows - 1) / kBlockRows);
     // prefix: parts of whole tiles
     p.Pp = 0;
     p.kpp = 64;

@@ -36,6 +36,9 @@ struct PackedArgs {
     long long p_hs;                                  // head stride of the prefix (rows are D elements apart)
     int nQH, G, batch, total, prefix;
     int hp;       // log2 of the query heads per workgroup
+    int single;   // 1: a workgroup per item, at most
+    struct ListHead* head;   // the work list, if there is one
+    int4* items;
     int copy32;   // 1: a step's rows span < 4 GiB (32-bit copy offsets)
     float sc;     // log2(e) / sqrt(D)
 };
@@ -156,6 +159,189 @@ __device__ __forceinline__ bool find_item(const PackedArgs& a, int rows_log2, co
     return (blk << rows_log2) < len;   // always, but for counts of overlapping sequences that pass 32 bits
 }
 
+// ---- work lists -----------------------------------------------------------------------------------
+// Many items (several rounds of the chip's workgroups) are listed by a launch of one workgroup and handed out
+// while the kernel runs. Eight queues, one per XCD, so that the blocks of one sequence and kv head, which read
+// the same K and V, run on one XCD at about the same time and find them in its L2; longest sequences first, the
+// last blocks of a sequence first; a workgroup whose queue is empty takes from the others. Against the list
+// in LDS (longest blocks of all sequences first, dealt out in turn): 64 prompts of 512 tokens, 32/8 heads
+// D 128, read their 134 MB of K and V again for every block index there, 260 us against 215 in this order; and
+// the same 24 prompts of 33-2,048 tokens end 6 % earlier by a model of their items when handed out.
+constexpr int kListSeqs = 2048;   // sequences of the listing kernel's LDS
+struct ListHead {
+    int next[8][32];   // of the queue's entries, a cache line each
+    int begin[8], end[8];
+    int pad[48];
+};
+static_assert(sizeof(ListHead) % 256 == 0, "");
+
+// Heads (nh per entry) of the sequence at place q that go to queue x: cnt of them, the c-th is head(c).
+struct QueueHeads {
+    int first, step, cnt;
+    __device__ __forceinline__ QueueHeads(int q, int nh, int x) {
+        if ((nh & 7) == 0) {   // neighbouring heads, which share K and V
+            cnt = nh >> 3;
+            first = x * cnt;
+            step = 1;
+        } else {               // the sequences' heads in turn
+            first = (x - q * nh) & 7;
+            step = 8;
+            cnt = first < nh ? (nh - first + 7) >> 3 : 0;
+        }
+    }
+};
+
+__global__ __launch_bounds__(1024) void packed_list(PackedArgs a, int per_queue) {
+    __shared__ int hist[kLevels + 1];
+    __shared__ int2 seq[kListSeqs];            // by place: longest first
+    __shared__ int blocks[kListSeqs];
+    __shared__ int pre[8][kListSeqs + 1];      // entries of the queue before place q
+    __shared__ int placed;
+    const int tid = (int)threadIdx.x, lane = tid & 63, wave = tid >> 6;
+    const int rows_log2 = block::rows_log2<2>() - a.hp, nh = a.nQH >> a.hp;
+    for (int i = tid; i <= kLevels; i += 1024) hist[i] = 0;
+    __syncthreads();
+    int2 mine[kListSeqs / 1024];
+    int n[kListSeqs / 1024];
+#pragma unroll
+    for (int k = 0; k < kListSeqs / 1024; ++k) {
+        const int s = k * 1024 + tid;
+        n[k] = 0;
+        if (s < a.batch) {
+            seq_rows(a, s, mine[k].x, mine[k].y);
+            n[k] = (mine[k].y + (1 << rows_log2) - 1) >> rows_log2;
+            if (n[k] > 0) {
+                atomicAdd(&hist[min(n[k], kLevels)], 1);
+                atomicMax(&hist[0], min(n[k], kLevels));   // entry 0 is not a count
+            }
+        }
+    }
+    __syncthreads();
+    if (wave == 0) {   // hist[i] becomes the places before the sequences of i blocks
+        int more = 0;
+        for (int d0 = (hist[0] - 1) & ~63; d0 >= 0; d0 -= 64) {
+            const int i = d0 + 64 - lane, h = hist[i];
+            const int g = wave::xlane::scan_inclusive(h, Sum{}) + more;
+            hist[i] = g - h;
+            more = __builtin_amdgcn_readlane(g, 63);
+        }
+        if (lane == 0) placed = more;
+    }
+    __syncthreads();
+#pragma unroll
+    for (int k = 0; k < kListSeqs / 1024; ++k) {
+        if (n[k] == 0) continue;
+        const int q = atomicAdd(&hist[min(n[k], kLevels)], 1);   // equal counts in any order: no result depends on it
+        seq[q] = mine[k];
+        blocks[q] = n[k];
+    }
+    __syncthreads();
+    const int nseq = placed;
+    if (wave < 8) {
+        int sum = 0;
+        for (int q0 = 0; q0 < nseq; q0 += 64) {
+            const int q = q0 + lane;
+            const int v = q < nseq ? blocks[q] * QueueHeads(q, nh, wave).cnt : 0;
+            const int g = wave::xlane::scan_inclusive(v, Sum{}) + sum;
+            if (q < nseq) pre[wave][q] = g - v;
+            sum = __builtin_amdgcn_readlane(g, 63);
+        }
+        if (lane == 0) pre[wave][nseq] = sum;
+    }
+    __syncthreads();
+    int begin[8];
+    begin[0] = 0;
+#pragma unroll
+    for (int x = 1; x < 8; ++x) begin[x] = begin[x - 1] + pre[x - 1][nseq];
+    if (tid == 0) {
+#pragma unroll
+        for (int x = 0; x < 8; ++x) {
+            const int len = pre[x][nseq];
+            a.head->begin[x] = begin[x];
+            a.head->end[x] = begin[x] + len;
+            a.head->next[x][0] = begin[x] + min(len, per_queue);   // the workgroups' first items
+        }
+    }
+    // one thread per entry: its queue from the eight lengths, its sequence by bisection
+    const int all = begin[7] + pre[7][nseq];
+    for (int i = tid; i < all; i += 1024) {
+        int x = 0;
+#pragma unroll
+        for (int y = 1; y < 8; ++y) x += i >= begin[y];
+        int e = i;
+#pragma unroll
+        for (int y = 1; y < 8; ++y) e = x == y ? i - begin[y] : e;
+        int lo = 0, hi = nseq;   // pre[lo] <= e < pre[hi]
+        while (hi - lo > 1) {
+            const int mid = (lo + hi) >> 1;
+            if (pre[x][mid] <= e) lo = mid;
+            else hi = mid;
+        }
+        const QueueHeads qh(lo, nh, x);
+        e -= pre[x][lo];
+        const int d = e / qh.cnt, c = e - d * qh.cnt;
+        const int2 sl = seq[lo];
+        a.items[i] = make_int4(sl.x, sl.y, (blocks[lo] - 1 - d) << rows_log2, (qh.first + c * qh.step) << a.hp);
+    }
+}
+
+// Entry idx of the list for a workgroup that takes one item: f by bisection, from the block counts that the
+// lanes hold (sequences lane, lane + 64, ..: kHeld in registers, others read again). False past the list's end.
+constexpr int kHeld = 4;
+__device__ __forceinline__ bool packed_item(const PackedArgs& a, int rows_log2, int idx, int lane, int& start, int& len,
+                                            int& blk) {
+    int n[kHeld];
+    auto blocks = [&](int s) {
+        int st, ln;
+        if (s >= a.batch) return 0;
+        seq_rows(a, s, st, ln);
+        return (ln + (1 << rows_log2) - 1) >> rows_log2;
+    };
+    int most = 0, sum = 0;
+#pragma unroll
+    for (int i = 0; i < kHeld; ++i) {
+        n[i] = 0;
+        if (64 * i < a.batch) n[i] = blocks(64 * i + lane);
+        most = max(most, n[i]);
+        sum += n[i];
+    }
+    for (int s = 64 * kHeld; s < a.batch; s += 64) {
+        const int x = blocks(s + lane);
+        most = max(most, x);
+        sum += x;
+    }
+    if (idx >= scalar(allreduce(sum, Sum{}))) return false;
+    auto above = [&](int d) {
+        int x = 0;
+#pragma unroll
+        for (int i = 0; i < kHeld; ++i) x += max(n[i] - d, 0);
+        for (int s = 64 * kHeld; s < a.batch; s += 64) x += max(blocks(s + lane) - d, 0);
+        return scalar(allreduce(x, Sum{}));
+    };
+    int lo = 0, hi = scalar(allreduce(most, Max{})), f_hi = 0;   // f(lo) > idx >= f(hi)
+    while (hi - lo > 1) {
+        const int mid = (lo + hi) >> 1, f = above(mid);
+        if (f > idx) lo = mid;
+        else { hi = mid; f_hi = f; }
+    }
+    blk = lo;
+    int r = idx - f_hi, seq = -1;   // the r-th sequence with more than blk blocks
+    auto pick = [&](int s0, int cnt) {
+        const uint64_t mask = __builtin_amdgcn_ballot_w64(cnt > blk);
+        const int before = __builtin_amdgcn_mbcnt_hi((uint32_t)(mask >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)mask, 0u));
+        const uint64_t here = __builtin_amdgcn_ballot_w64(cnt > blk && before == r);
+        if (here != 0 && seq < 0) seq = s0 + __builtin_ctzll(here);
+        r -= __popcll(mask);
+    };
+#pragma unroll
+    for (int i = 0; i < kHeld; ++i) pick(64 * i, n[i]);
+    for (int s = 64 * kHeld; s < a.batch && seq < 0; s += 64) pick(s, blocks(s + lane));
+    seq_rows(a, max(seq, 0), start, len);
+    start = scalar(start);
+    len = scalar(len);
+    return (blk << rows_log2) < len;   // always, but for counts of overlapping sequences that pass 32 bits
+}
+
 // Head of workgroup i within one entry's nQH workgroups. Workgroups go to the XCDs round-robin: with nQH a
 // multiple of 8 each XCD takes nQH / 8 neighbouring query heads, which share K and V heads in its L2.
 __device__ __forceinline__ int item_head(int i, int nQH) {
@@ -185,6 +371,9 @@ __device__ __forceinline__ void store_rows(const f32x4 (&o)[D / 16], float l, ui
     }
 }
 
+// Workgroups of fa_packed that a CU holds (registers and LDS).
+template <int D, int QT> constexpr int resident() { return D == 64 ? 3 : 2; }
+
 // ---- 128 rows per workgroup, two workgroups per CU -------------------------------------------------
 // Four waves of 32 queries share 64-key K/V tiles in LDS, two slots each for K and V (64 KiB at D = 128), so
 // that two workgroups fit a CU: while one waits for its first tiles, masks its diagonal or stores, the other
@@ -192,34 +381,66 @@ __device__ __forceinline__ void store_rows(const f32x4 (&o)[D / 16], float l, ui
 // of the list times the heads (G workgroups), which evens out what a round's order costs, and loads the next
 // item's queries and first tiles before it stores its results: an item of one tile took 12.4 us as a
 // workgroup of its own, of which 2.4 to find it, 3.0 for the first loads and 2.9 for the stores.
-template <int D, bool kBf16, bool kPrefix>
-__global__ __launch_bounds__(256, 2) void fa_packed(PackedArgs a) {
-    constexpr int QT = block::kQT, ND = D / 32, NDT = D / 16;
+template <int D, int QT, bool kBf16, bool kPrefix, bool kListed>
+__global__ __launch_bounds__(256, (resident<D, QT>())) void fa_packed(PackedArgs a) {
+    constexpr int ND = D / 32, NDT = D / 16;
     __shared__ __attribute__((aligned(16))) uint16_t lds[block::lds_elems<D>()];
-    __shared__ Items items;
     static_assert((kLevels + 1) * 4 <= (int)sizeof(lds), "the histogram fits the tiles' LDS");
     const int lane = (int)(threadIdx.x & 63u);
     const int wave = scalar((int)(threadIdx.x >> 6));
     const int li = lane & 15, g = lane >> 4;
-    // The workgroup's waves serve 1 << hp query heads of one kv head, block::kRows >> hp tokens each
-    const int hp = a.hp, rows_log2 = block::kRowsLog2 - hp, nh = a.nQH >> hp;
+    // The workgroup's waves serve 1 << hp query heads of one kv head, a block's rows >> hp tokens each
+    const int hp = a.hp, rows_log2 = block::rows_log2<QT>() - hp, nh = a.nQH >> hp;
     const int P = kPrefix ? a.prefix : 0;
-    list_items(a, rows_log2, items, (int*)lds, (int)threadIdx.x);
-
-    // Each wave finds the item of another of the next four rounds.
+    struct Item { int start, len, q0, h0; };   // len 0: none
     __shared__ int4 next_s[4];
-    auto find = [&](int round) {
-        const int G = (int)gridDim.x, p = (int)blockIdx.x;
-        const int idx = round * G + ((round & 1) ? G - 1 - p : p), entry = idx / nh;
-        int start = 0, len = 0, blk = 0;
-        const bool ok = find_item(a, rows_log2, items, entry, lane, start, len, blk);
-        if (lane == 0) next_s[round & 3] = make_int4(start, ok ? len : 0, blk << rows_log2, item_head(idx - entry * nh, nh) << hp);
-    };
-    struct Item { int start, len, q0, h0; };
-    auto item_at = [&](int round) {   // len 0: none
-        const int4 x = next_s[round & 3];
+    auto item_at = [&](int round) {
+        const int4 x = next_s[kListed ? 0 : round & 3];
         return Item{scalar(x.x), scalar(x.y), scalar(x.z), scalar(x.w)};
     };
+    // Listed: the first item is the workgroup's place in its XCD's queue, the others are claimed by wave 0 ahead
+    // of an item's last tiles.
+    int queue = (int)blockIdx.x & 7, claimed = -1;   // of wave 0
+    auto claim = [&]() {
+        if (!kListed || wave != 0) return;
+        claimed = -1;
+        for (int k = 0; k < 8; ++k) {
+            int i = 0;
+            if (lane == 0) i = atomicAdd(&a.head->next[queue][0], 1);
+            i = scalar(i);
+            if (i < scalar(a.head->end[queue])) {
+                claimed = i;
+                break;
+            }
+            queue = (queue + 1) & 7;
+        }
+    };
+    auto publish = [&]() {
+        if (kListed && wave == 0 && lane == 0) next_s[0] = claimed >= 0 ? a.items[claimed] : make_int4(0, 0, 0, 0);
+    };
+    // Not listed: each wave finds the item of another of the next four rounds.
+    struct NoItems {};
+    __shared__ std::conditional_t<kListed, NoItems, Items> items;
+    auto find = [&](int round) {
+        if constexpr (!kListed) {
+            const int G = (int)gridDim.x, p = (int)blockIdx.x;
+            const int idx = round * G + ((round & 1) ? G - 1 - p : p), entry = idx / nh;
+            int start = 0, len = 0, blk = 0;
+            const bool ok = find_item(a, rows_log2, items, entry, lane, start, len, blk);
+            if (lane == 0) next_s[round & 3] = make_int4(start, ok ? len : 0, blk << rows_log2, item_head(idx - entry * nh, nh) << hp);
+        }
+    };
+    if constexpr (kListed) {
+        if (wave == 0) {
+            const int i = scalar(a.head->begin[queue]) + ((int)blockIdx.x >> 3);
+            if (i < scalar(a.head->end[queue])) claimed = i;
+            else claim();
+            publish();
+        }
+    } else if (!a.single) {
+        list_items(a, rows_log2, items, (int*)lds, (int)threadIdx.x);
+        find(wave);
+    }
     const block::Offsets own = block::own_offsets<D>(a.k_rs, wave, lane);
     u32x4 qb[QT][ND];
     auto keys = [&](const Item& it, const uint16_t* own, const uint16_t* pre) {
@@ -238,10 +459,18 @@ __global__ __launch_bounds__(256, 2) void fa_packed(PackedArgs a) {
         }
         block::first_copies<D, kPrefix>(keys(it, a.K, a.Kp), keys(it, a.V, a.Vp), tiles(it), own, lds, wave, lane);
     };
-    find(wave);
-    __syncthreads();
-    Item it = item_at(0);
-    if (it.len == 0) return;
+    Item it;
+    if (!kListed && a.single) {   // no list to form: every wave finds the one item
+        const int entry = (int)blockIdx.x / nh;
+        int blk;
+        if (!packed_item(a, rows_log2, entry, lane, it.start, it.len, blk)) return;
+        it.q0 = blk << rows_log2;
+        it.h0 = item_head((int)blockIdx.x - entry * nh, nh) << hp;
+    } else {
+        __syncthreads();
+        it = item_at(0);
+        if (it.len == 0) return;
+    }
     load(it);
     for (int round = 1;; ++round) {
         const int qw0 = it.q0 + dq, S = P + it.len, ntiles = tiles(it);
@@ -254,17 +483,21 @@ __global__ __launch_bounds__(256, 2) void fa_packed(PackedArgs a) {
         if (!a.copy32) t_main = 0;
         f32x4 o[QT][NDT], lacc[QT];
         float m[QT];
-        block::attend<D, kBf16, kPrefix, true>(keys(it, a.K, a.Kp), keys(it, a.V, a.Vp), block::Shape{S, ntiles, nch, P + qw0, t_main},
+        block::attend<D, QT, kBf16, kPrefix, true>(keys(it, a.K, a.Kp), keys(it, a.V, a.Vp), block::Shape{S, ntiles, nch, P + qw0, t_main},
                                                qb, o, lacc, m, own, lds, a.sc, wave, lane);
         uint16_t* Oh = a.O + it.start * a.o_rs + (it.h0 + dh) * a.o_hs;
         const int len = it.len;
         // What lies between two items is short and holds the matrix cores up: ahead of the CU's other waves
         __builtin_amdgcn_s_setprio(3);
-        if ((round & 3) == 0) find(round + wave);
-        __syncthreads();   // every wave is done with the tiles; the next items are there
-        it = item_at(round);
-        const bool more = it.len > 0;
-        if (more) load(it);
+        bool more = kListed || !a.single;
+        if (more) {
+            if (kListed) { claim(); publish(); }
+            else if ((round & 3) == 0) find(round + wave);
+            __syncthreads();   // every wave is done with the tiles; the next items are there
+            it = item_at(round);
+            more = it.len > 0;
+            if (more) load(it);
+        }
 #pragma unroll
         for (int x = 0; x < QT; ++x) {
             const int q = qw0 + x * 16 + li;
@@ -303,43 +536,69 @@ int check_packed(const cdna4_packed_cfg* cfg, const cdna4_packed_strides* st, co
     return 0;
 }
 
-struct PackedPlan { int kernel, waves, rows, hp; long long grid; };
+struct PackedPlan { int kernel, waves, rows, hp, qt; long long grid, items; size_t ws_bytes; };
 
 template <int D>
 PackedPlan plan_packed(const cdna4_packed_cfg& c) {
     PackedPlan p{};
-    p.kernel = CDNA4_KERNEL_PACKED_4W;
+    p.kernel = CDNA4_KERNEL_PACKED;
     p.waves = 4;
     // Query heads of one kv head side by side, up to one per wave: a block then has 128, 64 or 32 tokens, its
     // waves end at the same key or nearly so (with 128 tokens they pass the last two tiles as a staircase), and
     // short sequences fill it.
     const int G = c.nQHeads / c.nKVHeads;
     p.hp = G % 4 == 0 ? 2 : G % 2 == 0 ? 1 : 0;
-    p.rows = block::kRows >> p.hp;
     // sum of ceil(len / rows) is at most total / rows + the sequences that are not empty
-    p.grid = (long long)(c.nQHeads >> p.hp) * (c.total / p.rows + std::min(c.batch, c.total));
-    // one round of resident workgroups
-    p.grid = std::min(p.grid, 2LL * (device_cus() & ~3));
+    auto items = [&](int rows) { return (long long)(c.nQHeads >> p.hp) * (c.total / rows + std::min(c.batch, c.total)); };
+    const long long cus = device_cus() & ~7;
+    const long long slots = resident<D, 2>() * cus;   // resident workgroups: the grid is one round of them
+    // Blocks of half as many rows for calls of about one round of blocks and less, whose time is that of their
+    // longest block: one sequence of 1,024 tokens, 32/8 heads D 128, 21.4 against 25.7 us; above that they read K and V
+    // more often and fill the matrix cores less: four of 512-1,024 (808 blocks of 128) 40.0 against 34.8 us. Half a
+    // block per sequence is taken for the last ones.
+    p.qt = (long long)(c.nQHeads >> p.hp) * (2LL * c.total / (128 >> p.hp) + std::min(c.batch, c.total)) <= 4 * cus ? 1 : 2;
+    p.rows = (p.qt == 2 ? 128 : 64) >> p.hp;
+    p.items = items(p.rows);
+    p.grid = std::min(p.items, p.qt == 2 ? slots : resident<D, 1>() * cus);
+    p.ws_bytes = D == 128 && p.qt == 2 && p.items >= 2 * slots && c.batch <= kListSeqs && p.items < (1LL << 30)
+                     ? sizeof(ListHead) + (size_t)p.items * sizeof(int4) : 0;
     return p;
 }
 
 template <int D, bool kBf16>
 int launch_packed(const cdna4_packed_cfg& c, const cdna4_packed_strides& st, const void* Q, const void* K, const void* V,
-                  const void* Kp, const void* Vp, void* O, const int* cu, hipStream_t s) {
+                  const void* Kp, const void* Vp, void* O, const int* cu, void* ws, hipStream_t s) {
     const PackedPlan p = plan_packed<D>(c);
-    if (p.grid * 64 * p.waves > 0xffffffffLL) return CDNA4_ERR_INVALID_VALUE;
+    if (p.items > 0x7fffffffLL) return CDNA4_ERR_INVALID_VALUE;   // items are counted in 32 bits
     PackedArgs a;
     a.Q = (const uint16_t*)Q; a.K = (const uint16_t*)K; a.V = (const uint16_t*)V; a.O = (uint16_t*)O;
     a.Kp = (const uint16_t*)Kp; a.Vp = (const uint16_t*)Vp;
     a.cu = cu;
     a.q_rs = st.q_row; a.q_hs = st.q_head; a.k_rs = st.kv_row; a.k_hs = st.kv_head; a.o_rs = st.o_row; a.o_hs = st.o_head;
     a.p_hs = (long long)(c.stride_prefix ? c.stride_prefix : c.prefix) * D;
-    a.nQH = c.nQHeads; a.G = c.nQHeads / c.nKVHeads; a.batch = c.batch; a.total = c.total; a.prefix = c.prefix; a.hp = p.hp;
+    a.nQH = c.nQHeads; a.G = c.nQHeads / c.nKVHeads; a.batch = c.batch; a.total = c.total; a.prefix = c.prefix; a.hp = p.hp; a.single = p.grid == p.items;
     a.copy32 = 256 * st.kv_row * 2 < (1LL << 32) ? 1 : 0;
     a.sc = kLog2e / sqrtf((float)D);
     const unsigned grid = (unsigned)p.grid;
-    if (c.prefix) fa_packed<D, kBf16, true><<<grid, 256, 0, s>>>(a);
-    else fa_packed<D, kBf16, false><<<grid, 256, 0, s>>>(a);
+    a.head = nullptr;
+    a.items = nullptr;
+    if constexpr (D == 128) {
+        if (ws && p.ws_bytes) {
+            a.head = (ListHead*)ws;
+            a.items = (int4*)(a.head + 1);
+            packed_list<<<1, 1024, 0, s>>>(a, (int)(grid >> 3));
+            if (c.prefix) fa_packed<D, 2, kBf16, true, true><<<grid, 256, 0, s>>>(a);
+            else fa_packed<D, 2, kBf16, false, true><<<grid, 256, 0, s>>>(a);
+            return launch_status();
+        }
+    }
+    if (p.qt == 2) {
+        if (c.prefix) fa_packed<D, 2, kBf16, true, false><<<grid, 256, 0, s>>>(a);
+        else fa_packed<D, 2, kBf16, false, false><<<grid, 256, 0, s>>>(a);
+    } else {
+        if (c.prefix) fa_packed<D, 1, kBf16, true, false><<<grid, 256, 0, s>>>(a);
+        else fa_packed<D, 1, kBf16, false, false><<<grid, 256, 0, s>>>(a);
+    }
     return launch_status();
 }
 
@@ -350,17 +609,24 @@ using namespace cdna4;
 
 extern "C" int cdna4_attn_prefill_packed(const void* Q, const void* K, const void* V, const void* K_prefix,
                                          const void* V_prefix, void* O, const int* cu_seqlens, const cdna4_packed_cfg* cfg,
-                                         const cdna4_packed_strides* strides, int dtype, cdna4_stream_t stream) {
+                                         const cdna4_packed_strides* strides, int dtype, void* workspace,
+                                         size_t ws_bytes, cdna4_stream_t stream) {
     if (int e = check_packed(cfg, strides, Q, K, V, K_prefix, V_prefix, O, cu_seqlens, dtype)) return e;
     if (cfg->batch == 0 || cfg->total == 0) return 0;
+    if (workspace && (((uintptr_t)workspace & 15u) || ws_bytes < cdna4_attn_prefill_packed_workspace_size(cfg))) return CDNA4_ERR_INVALID_VALUE;
     if (int e = check_device()) return e;
     hipStream_t s = (hipStream_t)stream;
     const bool bf = dtype == CDNA4_BF16;
     if (cfg->D == 128)
-        return bf ? launch_packed<128, true>(*cfg, *strides, Q, K, V, K_prefix, V_prefix, O, cu_seqlens, s)
-                  : launch_packed<128, false>(*cfg, *strides, Q, K, V, K_prefix, V_prefix, O, cu_seqlens, s);
-    return bf ? launch_packed<64, true>(*cfg, *strides, Q, K, V, K_prefix, V_prefix, O, cu_seqlens, s)
-              : launch_packed<64, false>(*cfg, *strides, Q, K, V, K_prefix, V_prefix, O, cu_seqlens, s);
+        return bf ? launch_packed<128, true>(*cfg, *strides, Q, K, V, K_prefix, V_prefix, O, cu_seqlens, workspace, s)
+                  : launch_packed<128, false>(*cfg, *strides, Q, K, V, K_prefix, V_prefix, O, cu_seqlens, workspace, s);
+    return bf ? launch_packed<64, true>(*cfg, *strides, Q, K, V, K_prefix, V_prefix, O, cu_seqlens, workspace, s)
+              : launch_packed<64, false>(*cfg, *strides, Q, K, V, K_prefix, V_prefix, O, cu_seqlens, workspace, s);
+}
+
+extern "C" size_t cdna4_attn_prefill_packed_workspace_size(const cdna4_packed_cfg* cfg) {
+    cdna3_plan_info info;
+    return cdna4_attn_prefill_packed_plan(cfg, CDNA4_F16, &info) == 0 ? info.workspace : 0;
 }
 
 extern "C" int cdna4_attn_prefill_packed_plan(const cdna4_packed_cfg* cfg, int dtype, cdna3_plan_info* out) {
@@ -375,6 +641,6 @@ extern "C" int cdna4_attn_prefill_packed_plan(const cdna4_packed_cfg* cfg, int d
     out->rows = p.rows;
     out->grid = p.grid;
     out->partials = 1;
-    out->workspace = 0;
+    out->workspace = p.ws_bytes;
     return 0;
 }

@@ -89,16 +89,18 @@ inline PackedStrides packed_strides(const PackedCfg& c) {
 }
 inline hipError_t prefill_packed(const __half* Q, const __half* K, const __half* V, __half* O, const int* cu_seqlens,
                                  const PackedCfg& cfg, const PackedStrides& strides, const __half* K_prefix = nullptr,
-                                 const __half* V_prefix = nullptr, hipStream_t stream = nullptr) {
+                                 const __half* V_prefix = nullptr, hipStream_t stream = nullptr, void* workspace = nullptr,
+                                 size_t ws_bytes = 0) {
     return (hipError_t)cdna4_attn_prefill_packed(Q, K, V, K_prefix, V_prefix, O, cu_seqlens, &cfg, &strides, CDNA4_F16,
-                                                 (cdna4_stream_t)stream);
+                                                 workspace, ws_bytes, (cdna4_stream_t)stream);
 }
 inline hipError_t prefill_packed(const __hip_bfloat16* Q, const __hip_bfloat16* K, const __hip_bfloat16* V,
                                  __hip_bfloat16* O, const int* cu_seqlens, const PackedCfg& cfg,
                                  const PackedStrides& strides, const __hip_bfloat16* K_prefix = nullptr,
-                                 const __hip_bfloat16* V_prefix = nullptr, hipStream_t stream = nullptr) {
+                                 const __hip_bfloat16* V_prefix = nullptr, hipStream_t stream = nullptr,
+                                 void* workspace = nullptr, size_t ws_bytes = 0) {
     return (hipError_t)cdna4_attn_prefill_packed(Q, K, V, K_prefix, V_prefix, O, cu_seqlens, &cfg, &strides, CDNA4_BF16,
-                                                 (cdna4_stream_t)stream);
+                                                 workspace, ws_bytes, (cdna4_stream_t)stream);
 }
 
 // q[batch x nQH x D], K/V[batch x nKVH x N x D], o[batch x nQH x D].

@@ -139,6 +139,10 @@ int cdna3_attn_prefill_strided(const void* Q, const void* K, const void* V, void
  * wrongly are not defined. A value in V that is not finite reaches the rows of its sequence's earlier
  * tokens too where they share 32 keys with it (a weight of zero times infinity); K may hold any value there.
  * max_seq (0: unknown) is the longest sequence, used only to choose the kernel.
+ * With a workspace (cdna4_attn_prefill_packed_workspace_size(cfg) bytes, 16-byte aligned, no initialisation; calls
+ * that overlap must not share one) a call of many blocks first lists them, in an order that finds K and V in the L2
+ * caches, and its workgroups claim them one by one; without one (NULL), or where the size is 0, the blocks are
+ * dealt out in a fixed order in one launch. Both give the same bits.
  * batch == 0 or total == 0: nothing is done. Invalid: D not 64 or 128, nQHeads % nKVHeads != 0, negative
  * sizes, max_seq > total, prefix + total near 2^31, stride_prefix (0: prefix) < prefix, Q/K/V strides not a multiple of 8
  * elements, O strides not a multiple of 4, rows shorter than D, Q/K/V/prefix not 16-byte or O not 8-byte
@@ -161,10 +165,11 @@ typedef struct {
     long long o_row, o_head;    /* O */
 } cdna4_packed_strides;
 
+size_t cdna4_attn_prefill_packed_workspace_size(const cdna4_packed_cfg* cfg);
 int cdna4_attn_prefill_packed(const void* Q, const void* K, const void* V, const void* K_prefix,
                               const void* V_prefix, void* O, const int* cu_seqlens,
                               const cdna4_packed_cfg* cfg, const cdna4_packed_strides* strides, int dtype,
-                              cdna4_stream_t stream);
+                              void* workspace, size_t ws_bytes, cdna4_stream_t stream);
 
 /* ---- attention: decode (one query per sequence, split-K) --------------------
  * Replaces cdna3::attn::decode (attention.hpp:117-137) and cdna3::attn::decode_dme
@@ -249,7 +254,8 @@ enum {
     CDNA4_KERNEL_DECODE_WG = 6,        /* decode_wg: one launch, no workspace */
     CDNA4_KERNEL_PREFILL_KEYS = 7,     /* fa_mfma_keys: 8 waves, `rows` 128, 64 or 32 queries with the keys
                                           split over 2, 4 or 8 groups of waves */
-    CDNA4_KERNEL_PACKED_4W = 8,        /* fa_packed: 4 waves x 32 queries, two workgroups per CU */
+    CDNA4_KERNEL_PACKED = 8,           /* fa_packed: 4 waves x 32 or 16 queries, `rows` tokens of 128 / rows or 64 /
+                                          rows query heads */
     CDNA4_KERNEL_DECODE_SHARED = 9     /* shared_parts + shared_join */
 };
 

@@ -96,6 +96,74 @@ def test_many_sequences(batch):
     verify(args, args[-1], F16, run(*args[:5], *args[6:]))
 
 
+LISTED = {   # calls of two rounds of blocks and more, whose blocks are listed first
+    "docs": ([2100, 1, 900, 0, 1300, 77, 4000], 40, 8, 128, BF16, 0),
+    "docs_prefix": ([700, 0, 1200, 3], 64, 16, 128, F16, 300),
+    "heads_in_turn": ([300, 1, 0, 500, 64, 65] * 4, 20, 10, 64, F16, 0),       # 10 pairs of heads over 8 queues
+    "three_heads": ([129] * 350, 3, 1, 64, BF16, 0),
+    "one_long": ([9000], 16, 16, 64, BF16, 0),
+    "equal": ([64] * 40, 64, 8, 128, F16, 0),
+    "most_sequences": ([1, 2, 40] * 682 + [5, 9], 4, 4, 64, F16, 40),          # 2,048
+    "more_sequences": ([1, 2, 40] * 683, 4, 4, 64, BF16, 0),                   # 2,049: not listed
+    "docs_prefix_listed": ([700, 0, 1200, 300], 64, 16, 128, F16, 300),
+    "heads_in_turn_listed": ([300, 1, 0, 500, 64, 65] * 6, 20, 10, 128, F16, 0),
+    "three_heads_listed": ([129] * 350, 3, 1, 128, BF16, 0),
+    "one_long_listed": ([9000], 16, 16, 128, BF16, 0),
+    "most_sequences_listed": ([1, 2, 40] * 682 + [5, 9], 4, 4, 128, F16, 40),  # 2,048
+    "more_sequences_128": ([1, 2, 40] * 683, 4, 4, 128, BF16, 0),              # 2,049: not listed
+}
+# not listed: D = 64, too many sequences, or below two rounds
+UNLISTED = {n for n, c in LISTED.items() if c[3] == 64} | {"docs_prefix", "more_sequences_128"}
+
+
+@pytest.mark.parametrize("name", list(LISTED))
+def test_listed_blocks(name):
+    lens, HQ, HK, D, dtype, prefix = LISTED[name]
+    args = make(lens, HQ, HK, D, dtype, prefix=prefix, spare=2, seed=len(lens))
+    need = cdna4.prefill_packed_workspace_size(args[-1])
+    assert (need > 0) == (name not in UNLISTED)
+    one = run(*args[:5], *args[6:], workspace=None)
+    for fill in (0, 255):
+        ws = torch.full((need + 16,), fill, dtype=torch.uint8, device=DEV)
+        assert torch.equal(one, run(*args[:5], *args[6:], workspace=ws[:need] if need else None))
+        assert bool((ws[need:] == fill).all())
+    assert torch.equal(one, run(*args[:5], *args[6:]))
+    verify(args, args[-1], dtype, one, name)
+
+
+def test_listed_blocks_replayed():
+    """The queues start over in every replay, on other lengths."""
+    T = 4200
+    Q, K, V, _, _, _, _, cfg0 = make([T], 32, 8, 128, F16, seed=21)
+    cfg = cdna4.PackedPrefillCfg(128, 32, 8, 5, T, 0, 0, 0)
+    ws = torch.empty(cdna4.prefill_packed_workspace_size(cfg), dtype=torch.uint8, device=DEV)
+    cu_d = torch.tensor([0, 1, 2, 3, 4, 5], dtype=torch.int32, device=DEV)
+    O = torch.full((T, 32, 128), 7.0, dtype=F16, device=DEV)
+    run(Q, K, V, None, None, cu_d, cfg, O=O, workspace=ws)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        run(Q, K, V, None, None, cu_d, cfg, O=O, workspace=ws)
+    for lens in ([4200, 0, 0, 0, 0], [600] * 5, [1, 1, 1, 1, 1], [0, 0, 0, 0, 0], [17, 2000, 900, 3, 80]):
+        cu = cu_of(lens)
+        cu_d.copy_(torch.tensor(cu, dtype=torch.int32))
+        O.fill_(7.0)
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(O, run(Q, K, V, None, None, cu_d, cfg, workspace=None)), lens
+        verify((Q, K, V, None, None, cu, cu_d, cfg), cfg, F16, O, str(lens))
+
+
+def test_workspace_refusals():
+    args = make([1900, 1300], 64, 16, 128, F16, seed=22)
+    need = cdna4.prefill_packed_workspace_size(args[-1])
+    with pytest.raises(cdna4.CDNA4Error):
+        run(*args[:5], *args[6:], workspace=torch.empty(need - 1, dtype=torch.uint8, device=DEV))
+    for bad in ("none", torch.empty(need, dtype=torch.uint8)):
+        with pytest.raises(ValueError):
+            run(*args[:5], *args[6:], workspace=bad)
+
+
 def test_first_row_not_zero():
     args = make([30, 129], 4, 4, 128, BF16, first=11, spare=4, seed=5)
     verify(args, args[-1], BF16, run(*args[:5], *args[6:]))

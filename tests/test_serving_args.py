@@ -21,9 +21,9 @@ def test_cdna4_symbols_exported():
     assert names <= set(re.findall(r"\bT (cdna4_\w+)", out)), names
 
 
-def packed(cfg=(64, 8, 4, 3, 100, 50, 0, 0), strides=(512, 64, 256, 64, 512, 64), dtype=cdna4.F16, Q=P, K=P, V=P, Kp=None, Vp=None, O=P, cu=P):
+def packed(cfg=(64, 8, 4, 3, 100, 50, 0, 0), strides=(512, 64, 256, 64, 512, 64), dtype=cdna4.F16, Q=P, K=P, V=P, Kp=None, Vp=None, O=P, cu=P, ws=None, n=0):
     c, s = cdna4.PackedPrefillCfg(*cfg), cdna4.PackedStrides(*strides)
-    return cdna4.lib().cdna4_attn_prefill_packed(Q, K, V, Kp, Vp, O, cu, ctypes.byref(c), ctypes.byref(s), dtype, None)
+    return cdna4.lib().cdna4_attn_prefill_packed(Q, K, V, Kp, Vp, O, cu, ctypes.byref(c), ctypes.byref(s), dtype, ws, n, None)
 
 
 @pytest.mark.parametrize("cfg", [
@@ -55,7 +55,7 @@ def test_packed_refuses_arguments():
         st[i] = bad
         assert packed(good, strides=st) == 1, (i, bad)
     l = cdna4.lib()
-    assert l.cdna4_attn_prefill_packed(P, P, P, None, None, P, P, None, None, cdna4.F16, None) == 1
+    assert l.cdna4_attn_prefill_packed(P, P, P, None, None, P, P, None, None, cdna4.F16, None, 0, None) == 1
     # nothing to do: no pointer is needed
     assert packed((64, 8, 4, 0, 100, 50, 0, 0), Q=None, K=None, V=None, O=None, cu=None) == 0
     assert packed((64, 8, 4, 3, 0, 0, 0, 0), Q=None, K=None, V=None, O=None, cu=None) == 0
@@ -63,8 +63,15 @@ def test_packed_refuses_arguments():
 
 def test_packed_plan():
     for D, dt in ((64, torch.float16), (128, torch.bfloat16)):
-        p = cdna4.prefill_packed_plan(cdna4.PackedPrefillCfg(D, 32, 8, 24, 12961, 2048, 0, 0), dt)
-        assert p.name.startswith("fa_packed") and p.workspace == 0 and p.grid >= 32 * 12961 // p.rows
+        c = cdna4.PackedPrefillCfg(D, 32, 8, 24, 12961, 2048, 0, 0)
+        p = cdna4.prefill_packed_plan(c, dt)
+        assert p.name == "fa_packed" and p.workspace == cdna4.prefill_packed_workspace_size(c)
+        assert (p.workspace > 0) == (D == 128)
+        small = cdna4.PackedPrefillCfg(D, 12, 12, 7, 161, 61, 0, 0)
+        assert cdna4.prefill_packed_workspace_size(small) == 0
+        # a workspace that is too small or misaligned is refused, a missing one is not needed (checked on the GPU)
+        for ws, n in ((P, p.workspace - 1), (ctypes.c_void_p(72), p.workspace)) if p.workspace else ():
+            assert packed((D, 32, 8, 24, 12961, 2048, 0, 0), (32 * D, D, 8 * D, D, 32 * D, D), ws=ws, n=n) == 1
     with pytest.raises(cdna4.CDNA4Error):
         cdna4.prefill_packed_plan(cdna4.PackedPrefillCfg(64, 8, 3, 1, 10, 0, 0, 0))
 
