@@ -331,7 +331,7 @@ int cdna3_softmax_rows_f32(const float* X, float* Y, int M, int H, cdna4_stream_
  * biases for one token the last counts. The mask holds token j of row m in bit j % 32 of word
  * mask[m * mask_stride + j / 32] (1: allowed); a row that allows nothing is all -inf. repetition must not be 0.
  * Invalid: V < 1, M < 0 or > 65,535, strides below V (mask: below ceil(V / 32); history: below history_max),
- * history_max or n_bias negative or above 2^24, null logits or out, misaligned pointers.
+ * history_max negative or above 2^24, n_bias negative or above 8,192, null logits or out, misaligned pointers.
  */
 typedef struct {
     const void* logits;          /* [M][logits_stride] */

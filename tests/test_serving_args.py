@@ -94,7 +94,7 @@ def logits_args(**kw):
 
 @pytest.mark.parametrize("bad", [
     dict(V=0), dict(V=-1), dict(V=2 ** 31 - 1), dict(M=-1), dict(M=65536), dict(logits_stride=99), dict(out_stride=99),
-    dict(history_stride=4), dict(history_max=-1), dict(history_max=2 ** 24 + 1), dict(n_bias=-1), dict(n_bias=2 ** 24 + 1),
+    dict(history_stride=4), dict(history_max=-1), dict(history_max=2 ** 24 + 1), dict(n_bias=-1), dict(n_bias=8193),
     dict(mask_stride=3), dict(logits=None), dict(out=None), dict(bias_ids=None), dict(bias_values=None), dict(logits=65),
     dict(out=66), dict(history=66), dict(repetition=66), dict(mask=65), dict(prompt_len=63)])
 def test_logits_refuses(bad):
