@@ -324,31 +324,40 @@ def prefill_strided(Q: torch.Tensor, K: torch.Tensor, V: torch.Tensor, O: torch.
                                             ctypes.byref(strides), dt, _stream(stream)), "cdna3_attn_prefill_strided")
 
 
-def _device_of(t: torch.Tensor, *others: Optional[torch.Tensor]) -> int:
-    """Index of the GPU that t lies on; the other tensors have to lie there too."""
+# The batched serving calls keep their Python short: their kernels take a few microseconds.
+_I32, _F32 = torch.int32, torch.float32
+
+
+def _gpu_of(t: torch.Tensor) -> int:
     dev = t.get_device()
     if dev < 0:
         raise ValueError("tensors must be on the GPU")
-    for x in others:
-        if x is not None and x.get_device() != dev:
-            raise ValueError("tensors must be on one GPU")
     return dev
 
 
 def _on_device(dev: int):
     """Context in which dev is the current device, so that a call goes to its tensors' device."""
-    return _NO_STREAM if torch.cuda.current_device() == dev else torch.cuda.device(dev)
+    return _NO_STREAM if torch._C._cuda_getDevice() == dev else torch.cuda.device(dev)
+
+
+def _arg(name: str, t: Optional[torch.Tensor], dtype, n: int, dev: int) -> int:
+    """Address of a contiguous tensor of at least n elements on GPU dev."""
+    if t is None:
+        raise ValueError(f"{name} is missing")
+    if t.dtype is not dtype or t.numel() < n or t.get_device() != dev or not t.is_contiguous():
+        raise ValueError(f"{name} must be contiguous {dtype} with {n} elements on GPU {dev}")
+    return t.data_ptr()
 
 
 def _token_major(name: str, t: torch.Tensor, T: int, heads: int, D: int):
     """(token stride, head stride) of t [>= T][heads][D]; an axis of one element gets the packed stride."""
-    n, h, d = t.shape if t.dim() == 3 else (-1, 0, 0)
-    if n < T or h != heads or d != D:
+    s = t.shape
+    if len(s) != 3 or s[0] < T or s[1] != heads or s[2] != D:
         raise ValueError(f"{name} must be [total][heads][D]")
     row, head, one = t.stride()
     if one != 1 and T:
         raise ValueError(f"{name} must have contiguous rows of D")
-    return (row if n > 1 else heads * D), (head if h > 1 else D)
+    return (row if s[0] > 1 else heads * D), (head if heads > 1 else D)
 
 
 def prefill_packed(Q: torch.Tensor, K: torch.Tensor, V: torch.Tensor, O: torch.Tensor, cu_seqlens: torch.Tensor,
@@ -361,49 +370,34 @@ def prefill_packed(Q: torch.Tensor, K: torch.Tensor, V: torch.Tensor, O: torch.T
     Rows of O outside cu_seqlens[0] .. cu_seqlens[batch] are left as they are. `workspace`: "auto" (default)
     allocates prefill_packed_workspace_size(cfg) bytes, where that is not 0, on the stream the call launches on; a
     uint8 tensor is used as given; None runs in one launch, which needs none."""
-    dev = _device_of(Q, K, V, O, cu_seqlens, K_prefix, V_prefix)
-    dt, dtype = _dtype(Q), Q.dtype
-    if not (K.dtype == V.dtype == O.dtype == dtype):
-        raise ValueError("Q, K, V, O must share one dtype")
-    T, D, P = cfg.total, cfg.D, cfg.prefix
-    kv = _token_major("K", K, T, cfg.nKVHeads, D)
-    if _token_major("V", V, T, cfg.nKVHeads, D) != kv:
-        raise ValueError("K and V must have the same strides")
-    st = PackedStrides(*_token_major("Q", Q, T, cfg.nQHeads, D), *kv, *_token_major("O", O, T, cfg.nQHeads, D))
-    if cu_seqlens.dtype != torch.int32 or not cu_seqlens.is_contiguous() or cu_seqlens.numel() < cfg.batch + 1:
-        raise ValueError("cu_seqlens must be contiguous int32 [batch + 1]")
+    dev, dtype = _gpu_of(Q), Q.dtype
+    dt = _dtype(Q)
+    T, HQ, HK, D, P = cfg.total, cfg.nQHeads, cfg.nKVHeads, cfg.D, cfg.prefix
+    for x in (K, V, O):
+        if x.dtype is not dtype or x.get_device() != dev:
+            raise ValueError("Q, K, V, O must share one dtype and GPU")
+    q, kv, o = _token_major("Q", Q, T, HQ, D), _token_major("K", K, T, HK, D), _token_major("O", O, T, HQ, D)
+    if V.shape != K.shape or _token_major("V", V, T, HK, D) != kv:
+        raise ValueError("K and V must have the same shape and strides")
+    cu = _arg("cu_seqlens", cu_seqlens, _I32, cfg.batch + 1, dev)
     kp = vp = 0
     if P > 0:
-        kp, vp = _prefix_ptrs(K_prefix, V_prefix, dtype, cfg.nKVHeads * (cfg.stride_prefix or P) * D)
+        need = HK * (cfg.stride_prefix or P) * D
+        kp, vp = _arg("K_prefix", K_prefix, dtype, need, dev), _arg("V_prefix", V_prefix, dtype, need, dev)
     if isinstance(workspace, str) and workspace != "auto":
         raise ValueError("workspace must be 'auto', None or a uint8 tensor")
+    l, c, ws, n = lib(), ctypes.byref(cfg), 0, 0
     with _on_device(dev), _on_stream(stream):
-        ws = n = 0
         if isinstance(workspace, str):
-            n = lib().cdna4_attn_prefill_packed_workspace_size(ctypes.byref(cfg))
+            n = l.cdna4_attn_prefill_packed_workspace_size(c)
             if n:
                 workspace = torch.empty(n, dtype=torch.uint8, device=Q.device)
                 ws = workspace.data_ptr()
         elif workspace is not None:
-            if workspace.get_device() != dev or not workspace.is_contiguous():
-                raise ValueError("workspace must be contiguous on the GPU of the tensors")
-            ws, n = workspace.data_ptr(), workspace.numel() * workspace.element_size()
-        _check(lib().cdna4_attn_prefill_packed(Q.data_ptr(), K.data_ptr(), V.data_ptr(), kp, vp, O.data_ptr(),
-                                               cu_seqlens.data_ptr(), ctypes.byref(cfg), ctypes.byref(st), dt, ws, n,
-                                               _stream(stream)), "cdna4_attn_prefill_packed")
-
-
-def _prefix_ptrs(K_prefix, V_prefix, dtype, need: int):
-    """Addresses of the shared prefix's K and V, checked against the `need` elements of the configuration."""
-    if K_prefix is None or V_prefix is None:
-        raise ValueError("prefix > 0 needs K_prefix and V_prefix")
-    if not (K_prefix.dtype == V_prefix.dtype == dtype):
-        raise ValueError("K_prefix, V_prefix must have the dtype of the queries")
-    if not (K_prefix.is_contiguous() and V_prefix.is_contiguous()):
-        raise ValueError("K_prefix, V_prefix must be contiguous")
-    if min(K_prefix.numel(), V_prefix.numel()) < need:
-        raise ValueError("K_prefix/V_prefix smaller than the configuration")
-    return K_prefix.data_ptr(), V_prefix.data_ptr()
+            ws, n = _arg("workspace", workspace, torch.uint8, 0, dev), workspace.numel()
+        _check(l.cdna4_attn_prefill_packed(Q.data_ptr(), K.data_ptr(), V.data_ptr(), kp, vp, O.data_ptr(), cu, c,
+                                           ctypes.byref(PackedStrides(*q, *kv, *o)), dt, ws, n, _stream(stream)),
+               "cdna4_attn_prefill_packed")
 
 
 def prefill_packed_workspace_size(cfg: PackedPrefillCfg) -> int:
@@ -486,37 +480,25 @@ def decode_shared(q: torch.Tensor, K_prefix: Optional[torch.Tensor], V_prefix: O
     K_prefix, V_prefix [nKVH][stride_prefix][D] (None with prefix 0); K, V [batch][nKVH][stride_kv][D] with lens[b]
     keys each, int32 on the device (None with max_own 0); fp16 or bf16. `workspace`: "auto" allocates
     decode_shared_workspace_size(cfg) bytes on the stream the call launches on; a uint8 tensor is used as given."""
-    dev = _device_of(q, K_prefix, V_prefix, K, V, lens, o)
-    dt, dtype = _dtype(q), q.dtype
-    B, D = cfg.batch, cfg.D
-    if o.dtype != dtype:
-        raise ValueError("q and o must share one dtype")
-    if not (q.is_contiguous() and o.is_contiguous()):
-        raise ValueError("tensors must be contiguous")
-    if min(q.numel(), o.numel()) < B * cfg.nQHeads * D:
-        raise ValueError("q/o smaller than the configuration")
-    kp = vp = k = v = n = 0
-    if cfg.prefix > 0:
-        kp, vp = _prefix_ptrs(K_prefix, V_prefix, dtype, cfg.nKVHeads * (cfg.stride_prefix or cfg.prefix) * D)
-    if cfg.max_own > 0:
-        if K is None or V is None or lens is None:
-            raise ValueError("max_own > 0 needs K, V and lens")
-        if not (K.dtype == V.dtype == dtype) or not (K.is_contiguous() and V.is_contiguous()):
-            raise ValueError("K, V must be contiguous and have the dtype of q")
-        if min(K.numel(), V.numel()) < B * cfg.nKVHeads * (cfg.stride_kv or cfg.max_own) * D:
-            raise ValueError("K/V smaller than the configuration")
-        if lens.dtype != torch.int32 or not lens.is_contiguous() or lens.numel() < B:
-            raise ValueError("lens must be contiguous int32 [batch]")
-        k, v, n = K.data_ptr(), V.data_ptr(), lens.data_ptr()
+    dev, dtype = _gpu_of(q), q.dtype
+    dt = _dtype(q)
+    B, D, HK, P, own = cfg.batch, cfg.D, cfg.nKVHeads, cfg.prefix, cfg.max_own
+    n = B * cfg.nQHeads * D
+    qp, op = _arg("q", q, dtype, n, dev), _arg("o", o, dtype, n, dev)
+    kp = vp = k = v = at = 0
+    if P > 0:
+        n = HK * (cfg.stride_prefix or P) * D
+        kp, vp = _arg("K_prefix", K_prefix, dtype, n, dev), _arg("V_prefix", V_prefix, dtype, n, dev)
+    if own > 0:
+        n = B * HK * (cfg.stride_kv or own) * D
+        k, v, at = _arg("K", K, dtype, n, dev), _arg("V", V, dtype, n, dev), _arg("lens", lens, _I32, B, dev)
     if workspace is None or (isinstance(workspace, str) and workspace != "auto"):
         raise ValueError("workspace must be 'auto' or a uint8 tensor")
     with _on_device(dev), _on_stream(stream):
         if isinstance(workspace, str):
             workspace = torch.empty(max(1, decode_shared_workspace_size(cfg)), dtype=torch.uint8, device=q.device)
-        elif workspace.get_device() != dev or not workspace.is_contiguous():
-            raise ValueError("workspace must be contiguous on the GPU of the tensors")
-        _check(lib().cdna4_attn_decode_shared(q.data_ptr(), kp, vp, k, v, n, o.data_ptr(), ctypes.byref(cfg), dt,
-                                              workspace.data_ptr(), workspace.numel() * workspace.element_size(),
+        ws = _arg("workspace", workspace, torch.uint8, 0, dev)
+        _check(lib().cdna4_attn_decode_shared(qp, kp, vp, k, v, at, op, ctypes.byref(cfg), dt, ws, workspace.numel(),
                                               _stream(stream)), "cdna4_attn_decode_shared")
 
 
@@ -653,15 +635,6 @@ def softmax_rows_f32(X: torch.Tensor, out: Optional[torch.Tensor] = None, stream
     return out
 
 
-def _row_values(name: str, t: Optional[torch.Tensor], dtype, shape) -> int:
-    """Address of an optional contiguous tensor of `shape`; 0 for None."""
-    if t is None:
-        return 0
-    if t.dtype != dtype or tuple(t.shape) != shape or not t.is_contiguous():
-        raise ValueError(f"{name} must be contiguous {dtype} {list(shape)}")
-    return t.data_ptr()
-
-
 def process_logits(logits: torch.Tensor, out: Optional[torch.Tensor] = None, *,
                    history: Optional[torch.Tensor] = None, history_len: Optional[torch.Tensor] = None,
                    prompt_len: Optional[torch.Tensor] = None, repetition: Optional[torch.Tensor] = None,
@@ -673,44 +646,47 @@ def process_logits(logits: torch.Tensor, out: Optional[torch.Tensor] = None, *,
     history int32 [M][H] (ids outside 0 .. V - 1 are padding), history_len, prompt_len int32 [M]; repetition,
     frequency, presence fp32 [M]; bias_ids int32, bias_values fp32 [M][n]; mask int32 [M][>= ceil(V / 32)],
     bit j % 32 of word j / 32 set: token j is allowed. The formula: cdna4_process_logits in cdna4_attn.h."""
-    dev = _device_of(logits, out, history, history_len, prompt_len, repetition, frequency, presence, bias_ids,
-                     bias_values, mask)
-    if logits.dim() != 2 or (logits.stride(1) != 1 and logits.numel()):
+    dev, dt = _gpu_of(logits), _dtype(logits)
+    M, V = logits.shape if logits.dim() == 2 else (-1, 0)
+    row, one = logits.stride() if M >= 0 else (0, 0)
+    if M < 0 or (one != 1 and M):
         raise ValueError("logits must be [M][V] with contiguous rows")
-    dt = _dtype(logits)
-    M, V = logits.shape
-    i32, f32, rows = torch.int32, torch.float32, (M,)
-    a = LogitsArgs()
+    h = hl = pl = r = f = p = H = 0
     if history is not None:
-        a.history = _row_values("history", history, i32, (M, history.shape[-1]))
-        a.history_max = a.history_stride = history.shape[1]
-        a.history_len = _row_values("history_len", history_len, i32, rows)
-        a.prompt_len = _row_values("prompt_len", prompt_len, i32, rows)
-        a.repetition = _row_values("repetition", repetition, f32, rows)
-        a.frequency = _row_values("frequency", frequency, f32, rows)
-        a.presence = _row_values("presence", presence, f32, rows)
+        H = history.shape[-1]
+        h = _arg("history", history, _I32, M * H, dev)
+        if history_len is not None:
+            hl = _arg("history_len", history_len, _I32, M, dev)
+        if prompt_len is not None:
+            pl = _arg("prompt_len", prompt_len, _I32, M, dev)
+        if repetition is not None:
+            r = _arg("repetition", repetition, _F32, M, dev)
+        if frequency is not None:
+            f = _arg("frequency", frequency, _F32, M, dev)
+        if presence is not None:
+            p = _arg("presence", presence, _F32, M, dev)
     elif not (history_len is prompt_len is repetition is frequency is presence is None):
         raise ValueError("lengths and penalties need a history")
-    if (bias_ids is None) != (bias_values is None):
-        raise ValueError("bias_ids and bias_values go together")
-    if bias_ids is not None:
-        a.n_bias = bias_ids.shape[-1]
-        a.bias_ids = _row_values("bias_ids", bias_ids, i32, (M, a.n_bias))
-        a.bias_values = _row_values("bias_values", bias_values, f32, (M, a.n_bias))
+    ids = vals = n = words = bits = 0
+    if bias_ids is not None or bias_values is not None:
+        n = bias_ids.shape[-1] if bias_ids is not None else 0
+        ids, vals = _arg("bias_ids", bias_ids, _I32, M * n, dev), _arg("bias_values", bias_values, _F32, M * n, dev)
     if mask is not None:
-        a.mask_stride = mask.shape[-1]
-        if 32 * a.mask_stride < V:   # an empty mask has a null address, which would allow everything
+        words = mask.shape[-1]
+        if 32 * words < V:   # an empty mask has a null address, which would allow everything
             raise ValueError("mask must have a bit for each of the V tokens")
-        a.mask = _row_values("mask", mask, i32, (M, a.mask_stride))
+        bits = _arg("mask", mask, _I32, M * words, dev)
     with _on_device(dev):
         if out is None:
             with _on_stream(stream):
-                out = torch.empty((M, V), dtype=f32, device=logits.device)
-        elif out.dtype != f32 or out.shape != logits.shape or (out.stride(1) != 1 and out.numel()):
-            raise ValueError("out must be fp32 [M][V] with contiguous rows")
-        a.logits, a.out, a.M, a.V = logits.data_ptr(), out.data_ptr(), M, V
-        a.logits_stride = logits.stride(0) if M > 1 else V
-        a.out_stride = out.stride(0) if M > 1 else V
+                out = torch.empty((M, V), dtype=_F32, device=logits.device)
+        if out.dtype is not _F32 or out.get_device() != dev or out.shape != logits.shape:
+            raise ValueError("out must be fp32 [M][V] on the GPU of the logits")
+        to, one = out.stride()
+        if one != 1 and M:
+            raise ValueError("out must have contiguous rows")
+        a = LogitsArgs(logits.data_ptr(), out.data_ptr(), M, V, row if M > 1 else V, to if M > 1 else V, h, hl, pl, H, n,
+                       H, r, f, p, ids, vals, bits, words)
         _check(lib().cdna4_process_logits(ctypes.byref(a), dt, _stream(stream)), "cdna4_process_logits")
     return out
 
