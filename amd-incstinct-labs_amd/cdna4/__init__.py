@@ -335,9 +335,18 @@ def _gpu_of(t: torch.Tensor) -> int:
     return dev
 
 
-def _on_device(dev: int):
-    """Context in which dev is the current device, so that a call goes to its tensors' device."""
-    return _NO_STREAM if torch._C._cuda_getDevice() == dev else torch.cuda.device(dev)
+def _elsewhere(dev: int, stream) -> bool:
+    """Whether a call has to enter its device or stream first (_entered)."""
+    return stream is not None or torch._C._cuda_getDevice() != dev
+
+
+@contextlib.contextmanager
+def _entered(dev: int, stream):
+    """The tensors' device and the call's stream made current."""
+    if isinstance(stream, torch.cuda.Stream) and stream.device_index != dev:
+        raise ValueError("stream must be on the GPU of the tensors")
+    with torch.cuda.device(dev), _on_stream(stream):
+        yield
 
 
 def _arg(name: str, t: Optional[torch.Tensor], dtype, n: int, dev: int) -> int:
@@ -371,6 +380,9 @@ def prefill_packed(Q: torch.Tensor, K: torch.Tensor, V: torch.Tensor, O: torch.T
     allocates prefill_packed_workspace_size(cfg) bytes, where that is not 0, on the stream the call launches on; a
     uint8 tensor is used as given; None runs in one launch, which needs none."""
     dev, dtype = _gpu_of(Q), Q.dtype
+    if _elsewhere(dev, stream):
+        with _entered(dev, stream):
+            return prefill_packed(Q, K, V, O, cu_seqlens, cfg, K_prefix, V_prefix, workspace)
     dt = _dtype(Q)
     T, HQ, HK, D, P = cfg.total, cfg.nQHeads, cfg.nKVHeads, cfg.D, cfg.prefix
     for x in (K, V, O):
@@ -387,17 +399,18 @@ def prefill_packed(Q: torch.Tensor, K: torch.Tensor, V: torch.Tensor, O: torch.T
     if isinstance(workspace, str) and workspace != "auto":
         raise ValueError("workspace must be 'auto', None or a uint8 tensor")
     l, c, ws, n = lib(), ctypes.byref(cfg), 0, 0
-    with _on_device(dev), _on_stream(stream):
-        if isinstance(workspace, str):
-            n = l.cdna4_attn_prefill_packed_workspace_size(c)
-            if n:
-                workspace = torch.empty(n, dtype=torch.uint8, device=Q.device)
-                ws = workspace.data_ptr()
-        elif workspace is not None:
-            ws, n = _arg("workspace", workspace, torch.uint8, 0, dev), workspace.numel()
-        _check(l.cdna4_attn_prefill_packed(Q.data_ptr(), K.data_ptr(), V.data_ptr(), kp, vp, O.data_ptr(), cu, c,
-                                           ctypes.byref(PackedStrides(*q, *kv, *o)), dt, ws, n, _stream(stream)),
-               "cdna4_attn_prefill_packed")
+    if isinstance(workspace, str):
+        n = l.cdna4_attn_prefill_packed_workspace_size(c)
+        if n:
+            workspace = torch.empty(n, dtype=torch.uint8, device=Q.device)
+            ws = workspace.data_ptr()
+    elif workspace is not None:
+        ws, n = _arg("workspace", workspace, torch.uint8, 0, dev), workspace.numel()
+    rc = l.cdna4_attn_prefill_packed(Q.data_ptr(), K.data_ptr(), V.data_ptr(), kp, vp, O.data_ptr(), cu, c,
+                                     ctypes.byref(PackedStrides(*q, *kv, *o)), dt, ws, n,
+                                     torch._C._cuda_getCurrentRawStream(dev))
+    if rc:
+        raise CDNA4Error("cdna4_attn_prefill_packed", rc)
 
 
 def prefill_packed_workspace_size(cfg: PackedPrefillCfg) -> int:
@@ -481,6 +494,9 @@ def decode_shared(q: torch.Tensor, K_prefix: Optional[torch.Tensor], V_prefix: O
     keys each, int32 on the device (None with max_own 0); fp16 or bf16. `workspace`: "auto" allocates
     decode_shared_workspace_size(cfg) bytes on the stream the call launches on; a uint8 tensor is used as given."""
     dev, dtype = _gpu_of(q), q.dtype
+    if _elsewhere(dev, stream):
+        with _entered(dev, stream):
+            return decode_shared(q, K_prefix, V_prefix, K, V, lens, o, cfg, workspace)
     dt = _dtype(q)
     B, D, HK, P, own = cfg.batch, cfg.D, cfg.nKVHeads, cfg.prefix, cfg.max_own
     n = B * cfg.nQHeads * D
@@ -494,12 +510,13 @@ def decode_shared(q: torch.Tensor, K_prefix: Optional[torch.Tensor], V_prefix: O
         k, v, at = _arg("K", K, dtype, n, dev), _arg("V", V, dtype, n, dev), _arg("lens", lens, _I32, B, dev)
     if workspace is None or (isinstance(workspace, str) and workspace != "auto"):
         raise ValueError("workspace must be 'auto' or a uint8 tensor")
-    with _on_device(dev), _on_stream(stream):
-        if isinstance(workspace, str):
-            workspace = torch.empty(max(1, decode_shared_workspace_size(cfg)), dtype=torch.uint8, device=q.device)
-        ws = _arg("workspace", workspace, torch.uint8, 0, dev)
-        _check(lib().cdna4_attn_decode_shared(qp, kp, vp, k, v, at, op, ctypes.byref(cfg), dt, ws, workspace.numel(),
-                                              _stream(stream)), "cdna4_attn_decode_shared")
+    if isinstance(workspace, str):
+        workspace = torch.empty(max(1, decode_shared_workspace_size(cfg)), dtype=torch.uint8, device=q.device)
+    rc = lib().cdna4_attn_decode_shared(qp, kp, vp, k, v, at, op, ctypes.byref(cfg), dt,
+                                        _arg("workspace", workspace, torch.uint8, 0, dev), workspace.numel(),
+                                        torch._C._cuda_getCurrentRawStream(dev))
+    if rc:
+        raise CDNA4Error("cdna4_attn_decode_shared", rc)
 
 
 def decode_shared_plan(cfg: SharedDecodeCfg, dtype=F16) -> PlanInfo:
@@ -646,7 +663,13 @@ def process_logits(logits: torch.Tensor, out: Optional[torch.Tensor] = None, *,
     history int32 [M][H] (ids outside 0 .. V - 1 are padding), history_len, prompt_len int32 [M]; repetition,
     frequency, presence fp32 [M]; bias_ids int32, bias_values fp32 [M][n]; mask int32 [M][>= ceil(V / 32)],
     bit j % 32 of word j / 32 set: token j is allowed. The formula: cdna4_process_logits in cdna4_attn.h."""
-    dev, dt = _gpu_of(logits), _dtype(logits)
+    dev = _gpu_of(logits)
+    if _elsewhere(dev, stream):
+        with _entered(dev, stream):
+            return process_logits(logits, out, history=history, history_len=history_len, prompt_len=prompt_len,
+                                  repetition=repetition, frequency=frequency, presence=presence, bias_ids=bias_ids,
+                                  bias_values=bias_values, mask=mask)
+    dt = _dtype(logits)
     M, V = logits.shape if logits.dim() == 2 else (-1, 0)
     row, one = logits.stride() if M >= 0 else (0, 0)
     if M < 0 or (one != 1 and M):
@@ -676,18 +699,18 @@ def process_logits(logits: torch.Tensor, out: Optional[torch.Tensor] = None, *,
         if 32 * words < V:   # an empty mask has a null address, which would allow everything
             raise ValueError("mask must have a bit for each of the V tokens")
         bits = _arg("mask", mask, _I32, M * words, dev)
-    with _on_device(dev):
-        if out is None:
-            with _on_stream(stream):
-                out = torch.empty((M, V), dtype=_F32, device=logits.device)
-        if out.dtype is not _F32 or out.get_device() != dev or out.shape != logits.shape:
-            raise ValueError("out must be fp32 [M][V] on the GPU of the logits")
-        to, one = out.stride()
-        if one != 1 and M:
-            raise ValueError("out must have contiguous rows")
-        a = LogitsArgs(logits.data_ptr(), out.data_ptr(), M, V, row if M > 1 else V, to if M > 1 else V, h, hl, pl, H, n,
-                       H, r, f, p, ids, vals, bits, words)
-        _check(lib().cdna4_process_logits(ctypes.byref(a), dt, _stream(stream)), "cdna4_process_logits")
+    if out is None:
+        out = torch.empty((M, V), dtype=_F32, device=logits.device)
+    if out.dtype is not _F32 or out.get_device() != dev or out.shape != logits.shape:
+        raise ValueError("out must be fp32 [M][V] on the GPU of the logits")
+    to, one = out.stride()
+    if one != 1 and M:
+        raise ValueError("out must have contiguous rows")
+    a = LogitsArgs(logits.data_ptr(), out.data_ptr(), M, V, row if M > 1 else V, to if M > 1 else V, h, hl, pl, H, n, H,
+                   r, f, p, ids, vals, bits, words)
+    rc = lib().cdna4_process_logits(ctypes.byref(a), dt, torch._C._cuda_getCurrentRawStream(dev))
+    if rc:
+        raise CDNA4Error("cdna4_process_logits", rc)
     return out
 
 
