@@ -19,7 +19,7 @@
 //     same shapes (decode_workspace_size gives the bytes, 1.06 MB there). Use them whenever
 //     batch x nKVHeads is well below the device's CU count.
 // New overloads: bf16 tensors, a batch dimension (DecodeCfg::batch), fp32 prefill, split-K
-// workspaces.
+// workspaces. New: prefill_packed (prompts of different lengths) and decode_shared (a batch behind one prefix).
 #include <hip/hip_runtime_api.h>
 #include <hip/hip_fp16.h>
 #include <hip/hip_bf16.h>
@@ -87,6 +87,7 @@ using PackedStrides = cdna4_packed_strides;
 inline PackedStrides packed_strides(const PackedCfg& c) {
     return PackedStrides{(long long)c.nQHeads * c.D, c.D, (long long)c.nKVHeads * c.D, c.D, (long long)c.nQHeads * c.D, c.D};
 }
+inline size_t prefill_packed_workspace_size(const PackedCfg& cfg) { return cdna4_attn_prefill_packed_workspace_size(&cfg); }
 inline hipError_t prefill_packed(const __half* Q, const __half* K, const __half* V, __half* O, const int* cu_seqlens,
                                  const PackedCfg& cfg, const PackedStrides& strides, const __half* K_prefix = nullptr,
                                  const __half* V_prefix = nullptr, hipStream_t stream = nullptr, void* workspace = nullptr,
@@ -145,6 +146,25 @@ inline hipError_t decode_dme(const __half* q, const __half* K, const __half* V, 
                              void* workspace, size_t ws_bytes, hipStream_t stream) {
     return detail::decode_any(q, K, V, o, cdna3_decode_cfg{cfg.D, cfg.N, cfg.nQHeads, cfg.nKVHeads, 1, cfg.stride_kv},
                               CDNA4_F16, workspace, ws_bytes, stream);
+}
+
+// New: decode of a batch behind a shared prefix (cdna4_attn_decode_shared): q, o [batch][nQH][D], prefix
+// [nKVH][stride_prefix][D], own keys [batch][nKVH][stride_kv][D] with lens[b] of them (device memory); a workspace of
+// decode_shared_workspace_size(cfg) bytes.
+using SharedDecodeCfg = cdna4_shared_decode_cfg;
+inline size_t decode_shared_workspace_size(const SharedDecodeCfg& cfg) { return cdna4_attn_decode_shared_workspace_size(&cfg); }
+inline hipError_t decode_shared(const __half* q, const __half* K_prefix, const __half* V_prefix, const __half* K,
+                                const __half* V, const int* lens, __half* o, const SharedDecodeCfg& cfg,
+                                void* workspace, size_t ws_bytes, hipStream_t stream = nullptr) {
+    return (hipError_t)cdna4_attn_decode_shared(q, K_prefix, V_prefix, K, V, lens, o, &cfg, CDNA4_F16, workspace, ws_bytes,
+                                                (cdna4_stream_t)stream);
+}
+inline hipError_t decode_shared(const __hip_bfloat16* q, const __hip_bfloat16* K_prefix, const __hip_bfloat16* V_prefix,
+                                const __hip_bfloat16* K, const __hip_bfloat16* V, const int* lens, __hip_bfloat16* o,
+                                const SharedDecodeCfg& cfg, void* workspace, size_t ws_bytes,
+                                hipStream_t stream = nullptr) {
+    return (hipError_t)cdna4_attn_decode_shared(q, K_prefix, V_prefix, K, V, lens, o, &cfg, CDNA4_BF16, workspace, ws_bytes,
+                                                (cdna4_stream_t)stream);
 }
 
 }  // namespace attn

@@ -36,6 +36,11 @@ inline hipError_t layernorm_f32(const float* X, const float* gamma, const float*
 inline hipError_t softmax_rows_f32(const float* X, float* Y, int M, int H, hipStream_t stream = nullptr) {
     return (hipError_t)cdna3_softmax_rows_f32(X, Y, M, H, (cdna4_stream_t)stream);
 }
+// New: logits of a batch made ready for the sampler (cdna4_process_logits). dtype: CDNA4_F32, CDNA4_F16 or CDNA4_BF16.
+using LogitsArgs = cdna4_logits_args;
+inline hipError_t process_logits(const LogitsArgs& args, int dtype, hipStream_t stream = nullptr) {
+    return (hipError_t)cdna4_process_logits(&args, dtype, (cdna4_stream_t)stream);
+}
 inline hipError_t rope_f16(__half* T, const float* cos, const float* sin, int seq, int heads, int D,
                            hipStream_t stream = nullptr) {
     return (hipError_t)cdna3_rope_f16(T, cos, sin, seq, heads, D, (cdna4_stream_t)stream);

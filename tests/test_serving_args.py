@@ -147,3 +147,41 @@ def test_shared_refuses_arguments():
     p = cdna4.decode_shared_plan(cdna4.SharedDecodeCfg(128, 32, 8, 64, 8192, 0, 1024, 0))
     assert p.name == "decode_shared" and p.workspace == cdna4.decode_shared_workspace_size(cdna4.SharedDecodeCfg(128, 32, 8, 64, 8192, 0, 1024, 0))
     assert p.grid * 256 < 2 ** 32
+
+
+CALLER = r"""
+#include <cdna3/attention.hpp>
+#include <cdna3/runtime/forward.hpp>
+using namespace cdna3;
+int main() {
+    attn::PackedCfg p{64, 8, 4, 3, 100, 50, 0, 0};
+    attn::PackedStrides st = attn::packed_strides(p);
+    if (st.q_row != 512 || st.kv_row != 256 || st.o_head != 64) return 1;
+    const __half* h = nullptr;
+    const __hip_bfloat16* b = nullptr;
+    if (attn::prefill_packed(h, h, h, (__half*)nullptr, nullptr, p, st) != hipErrorInvalidValue) return 2;
+    if (attn::prefill_packed(b, b, b, (__hip_bfloat16*)nullptr, nullptr, p, st, b, b, nullptr, nullptr, 0) != hipErrorInvalidValue) return 3;
+    if (attn::prefill_packed_workspace_size(p) != 0) return 4;
+    attn::SharedDecodeCfg s{128, 8, 2, 4, 100, 0, 50, 0};
+    if (attn::decode_shared_workspace_size(s) == 0) return 5;
+    if (attn::decode_shared(h, h, h, h, h, nullptr, (__half*)nullptr, s, nullptr, 0) != hipErrorInvalidValue) return 6;
+    if (attn::decode_shared(b, b, b, b, b, nullptr, (__hip_bfloat16*)nullptr, s, nullptr, 0) != hipErrorInvalidValue) return 7;
+    runtime::LogitsArgs a{};
+    if (runtime::process_logits(a, CDNA4_F16) != hipErrorInvalidValue) return 8;
+    return 0;
+}
+"""
+
+
+def test_cxx_callers(tmp_path):
+    clang = "/opt/rocm/llvm/bin/clang++"
+    if not os.path.exists(clang):
+        pytest.skip("no clang++")
+    src, exe = tmp_path / "caller.cpp", tmp_path / "caller"
+    src.write_text(CALLER)
+    lib = os.path.dirname(cdna4.library_path())
+    r = subprocess.run([clang, "-std=c++17", "-Wall", "-Werror", "-D__HIP_PLATFORM_AMD__", "-I/opt/rocm/include", "-I" + os.path.join(ROOT, "include"),
+                        str(src), "-o", str(exe), "-L" + lib, "-lcdna4_attn", "-Wl,-rpath," + lib, "-L/opt/rocm/lib", "-lamdhip64",
+                        "-Wl,-rpath,/opt/rocm/lib"], capture_output=True, text=True)
+    assert r.returncode == 0, r.stderr[-3000:]
+    assert subprocess.run([str(exe)]).returncode == 0
