@@ -39,6 +39,7 @@ struct PackedArgs {
     int single;   // 1: a workgroup per item, at most
     struct ListHead* head;   // the work list, if there is one
     int4* items;
+    int max_items;           // blocks times groups of heads that the sequences can have; the list's room
     int copy32;   // 1: a step's rows span < 4 GiB (32-bit copy offsets)
     float sc;     // log2(e) / sqrt(D)
 };
@@ -165,8 +166,8 @@ __device__ __forceinline__ bool find_item(const PackedArgs& a, int rows_log2, co
 // the same K and V, run on one XCD at about the same time and find them in its L2; longest sequences first, the
 // last blocks of a sequence first; a workgroup whose queue is empty takes from the others. Against the list
 // in LDS (longest blocks of all sequences first, dealt out in turn): 64 prompts of 512 tokens, 32/8 heads
-// D 128, read their 134 MB of K and V again for every block index there, 260 us against 215 in this order; and
-// the same 24 prompts of 33-2,048 tokens end 6 % earlier by a model of their items when handed out.
+// D 128, read their 134 MB of K and V again for every block index there, 258 us against 224 in this order; 12 of
+// 512-8,192 tokens 945 against 925 us.
 constexpr int kListSeqs = 2048;   // sequences of the listing kernel's LDS
 struct ListHead {
     int next[8][32];   // of the queue's entries, a cache line each
@@ -238,32 +239,35 @@ __global__ __launch_bounds__(1024) void packed_list(PackedArgs a, int per_queue)
     __syncthreads();
     const int nseq = placed;
     if (wave < 8) {
-        int sum = 0;
+        // Sequences of a wrong cu may overlap and have more blocks than the list has room for (a.max_items, up to
+        // 2^30): sums in 64 bits, cut to it.
+        long long sum = 0;
+        const long long most = a.max_items;
         for (int q0 = 0; q0 < nseq; q0 += 64) {
             const int q = q0 + lane;
-            const int v = q < nseq ? blocks[q] * QueueHeads(q, nh, wave).cnt : 0;
-            const int g = wave::xlane::scan_inclusive(v, Sum{}) + sum;
-            if (q < nseq) pre[wave][q] = g - v;
-            sum = __builtin_amdgcn_readlane(g, 63);
+            const long long v = q < nseq ? (long long)blocks[q] * QueueHeads(q, nh, wave).cnt : 0;
+            const long long g = wave::xlane::scan_inclusive(v, Sum{}) + sum;
+            if (q < nseq) pre[wave][q] = (int)min(g - v, most);
+            sum = __shfl(g, 63);
         }
-        if (lane == 0) pre[wave][nseq] = sum;
+        if (lane == 0) pre[wave][nseq] = (int)min(sum, most);
     }
     __syncthreads();
     int begin[8];
     begin[0] = 0;
 #pragma unroll
-    for (int x = 1; x < 8; ++x) begin[x] = begin[x - 1] + pre[x - 1][nseq];
+    for (int x = 1; x < 8; ++x) begin[x] = min(begin[x - 1] + pre[x - 1][nseq], a.max_items);
     if (tid == 0) {
 #pragma unroll
         for (int x = 0; x < 8; ++x) {
-            const int len = pre[x][nseq];
+            const int len = min(pre[x][nseq], a.max_items - begin[x]);
             a.head->begin[x] = begin[x];
             a.head->end[x] = begin[x] + len;
             a.head->next[x][0] = begin[x] + min(len, per_queue);   // the workgroups' first items
         }
     }
     // one thread per entry: its queue from the eight lengths, its sequence by bisection
-    const int all = begin[7] + pre[7][nseq];
+    const int all = min(begin[7] + pre[7][nseq], a.max_items);
     for (int i = tid; i < all; i += 1024) {
         int x = 0;
 #pragma unroll
@@ -426,7 +430,8 @@ __global__ __launch_bounds__(256, (resident<D, QT>())) void fa_packed(PackedArgs
             const int G = (int)gridDim.x, p = (int)blockIdx.x;
             const int idx = round * G + ((round & 1) ? G - 1 - p : p), entry = idx / nh;
             int start = 0, len = 0, blk = 0;
-            const bool ok = find_item(a, rows_log2, items, entry, lane, start, len, blk);
+            // overlapping sequences of a wrong cu can have more items than lengths that add up to the tokens: no more
+            const bool ok = idx < a.max_items && find_item(a, rows_log2, items, entry, lane, start, len, blk);
             if (lane == 0) next_s[round & 3] = make_int4(start, ok ? len : 0, blk << rows_log2, item_head(idx - entry * nh, nh) << hp);
         }
     };
@@ -512,16 +517,23 @@ __global__ __launch_bounds__(256, (resident<D, QT>())) void fa_packed(PackedArgs
 
 namespace {
 
+// Every call reads cu in each of its workgroups, and a block's keys and the blocks are counted in 32 bits.
+constexpr int kMaxBatch = 1 << 20;
+constexpr long long kMaxItems = 1LL << 30;
+
+bool valid_cfg(const cdna4_packed_cfg& c) {
+    if (c.D != 64 && c.D != 128) return false;
+    if (c.nQHeads < 1 || c.nKVHeads < 1 || c.nQHeads % c.nKVHeads) return false;
+    if (c.batch < 0 || c.batch > kMaxBatch || c.total < 0 || c.max_seq < 0 || c.max_seq > c.total || c.prefix < 0) return false;
+    if (c.total > 0x7fffffff - 1024 || c.prefix > 0x7fffffff - 1024 - c.total) return false;
+    return c.stride_prefix == 0 || c.stride_prefix >= c.prefix;
+}
+
 int check_packed(const cdna4_packed_cfg* cfg, const cdna4_packed_strides* st, const void* Q, const void* K, const void* V,
                  const void* Kp, const void* Vp, const void* O, const int* cu, int dtype) {
-    if (!cfg || !st) return CDNA4_ERR_INVALID_VALUE;
+    if (!cfg || !st || !valid_cfg(*cfg)) return CDNA4_ERR_INVALID_VALUE;
     const cdna4_packed_cfg& c = *cfg;
-    if (c.D != 64 && c.D != 128) return CDNA4_ERR_INVALID_VALUE;
     if (dtype != CDNA4_F16 && dtype != CDNA4_BF16) return CDNA4_ERR_INVALID_VALUE;
-    if (c.nQHeads < 1 || c.nKVHeads < 1 || c.nQHeads % c.nKVHeads) return CDNA4_ERR_INVALID_VALUE;
-    if (c.batch < 0 || c.total < 0 || c.max_seq < 0 || c.max_seq > c.total || c.prefix < 0) return CDNA4_ERR_INVALID_VALUE;
-    if (c.total > 0 && c.prefix > 0x7fffffff - 1024 - c.total) return CDNA4_ERR_INVALID_VALUE;   // keys are counted in 32 bits
-    if (c.stride_prefix != 0 && c.stride_prefix < c.prefix) return CDNA4_ERR_INVALID_VALUE;
     const long long in[4] = {st->q_row, st->q_head, st->kv_row, st->kv_head};
     for (long long x : in)
         if (x < 0 || (x & 7)) return CDNA4_ERR_INVALID_VALUE;
@@ -560,7 +572,7 @@ PackedPlan plan_packed(const cdna4_packed_cfg& c) {
     p.rows = (p.qt == 2 ? 128 : 64) >> p.hp;
     p.items = items(p.rows);
     p.grid = std::min(p.items, p.qt == 2 ? slots : resident<D, 1>() * cus);
-    p.ws_bytes = D == 128 && p.qt == 2 && p.items >= 2 * slots && c.batch <= kListSeqs && p.items < (1LL << 30)
+    p.ws_bytes = D == 128 && p.qt == 2 && p.items >= 2 * slots && c.batch <= kListSeqs && p.items <= kMaxItems
                      ? sizeof(ListHead) + (size_t)p.items * sizeof(int4) : 0;
     return p;
 }
@@ -569,7 +581,7 @@ template <int D, bool kBf16>
 int launch_packed(const cdna4_packed_cfg& c, const cdna4_packed_strides& st, const void* Q, const void* K, const void* V,
                   const void* Kp, const void* Vp, void* O, const int* cu, void* ws, hipStream_t s) {
     const PackedPlan p = plan_packed<D>(c);
-    if (p.items > 0x7fffffffLL) return CDNA4_ERR_INVALID_VALUE;   // items are counted in 32 bits
+    if (p.items > kMaxItems) return CDNA4_ERR_INVALID_VALUE;
     PackedArgs a;
     a.Q = (const uint16_t*)Q; a.K = (const uint16_t*)K; a.V = (const uint16_t*)V; a.O = (uint16_t*)O;
     a.Kp = (const uint16_t*)Kp; a.Vp = (const uint16_t*)Vp;
@@ -582,6 +594,7 @@ int launch_packed(const cdna4_packed_cfg& c, const cdna4_packed_strides& st, con
     const unsigned grid = (unsigned)p.grid;
     a.head = nullptr;
     a.items = nullptr;
+    a.max_items = (int)p.items;   // up to kMaxItems
     if constexpr (D == 128) {
         if (ws && p.ws_bytes) {
             a.head = (ListHead*)ws;
@@ -632,10 +645,9 @@ extern "C" size_t cdna4_attn_prefill_packed_workspace_size(const cdna4_packed_cf
 extern "C" int cdna4_attn_prefill_packed_plan(const cdna4_packed_cfg* cfg, int dtype, cdna3_plan_info* out) {
     if (!cfg || !out) return CDNA4_ERR_INVALID_VALUE;
     const cdna4_packed_cfg& c = *cfg;
-    if ((c.D != 64 && c.D != 128) || (dtype != CDNA4_F16 && dtype != CDNA4_BF16)) return CDNA4_ERR_INVALID_VALUE;
-    if (c.nQHeads < 1 || c.nKVHeads < 1 || c.nQHeads % c.nKVHeads) return CDNA4_ERR_INVALID_VALUE;
-    if (c.batch < 1 || c.total < 1 || c.max_seq < 0 || c.max_seq > c.total || c.prefix < 0) return CDNA4_ERR_INVALID_VALUE;
+    if (!valid_cfg(c) || c.batch < 1 || c.total < 1 || (dtype != CDNA4_F16 && dtype != CDNA4_BF16)) return CDNA4_ERR_INVALID_VALUE;
     const PackedPlan p = c.D == 128 ? plan_packed<128>(c) : plan_packed<64>(c);
+    if (p.items > kMaxItems) return CDNA4_ERR_INVALID_VALUE;
     out->kernel = p.kernel;
     out->waves = p.waves;
     out->rows = p.rows;

@@ -138,13 +138,13 @@ int cdna3_attn_prefill_strided(const void* Q, const void* K, const void* V, void
  * outside 0 .. total or decreasing read and write nothing outside the tensors; the rows that they name
  * wrongly are not defined. A value in V that is not finite reaches the rows of its sequence's earlier
  * tokens too where they share 32 keys with it (a weight of zero times infinity); K may hold any value there.
- * max_seq (0: unknown) is the longest sequence, used only to choose the kernel.
+ * max_seq (0: unknown) is the longest sequence; it is checked against total, and no kernel depends on it.
  * With a workspace (cdna4_attn_prefill_packed_workspace_size(cfg) bytes, 16-byte aligned, no initialisation; calls
  * that overlap must not share one) a call of many blocks first lists them, in an order that finds K and V in the L2
  * caches, and its workgroups claim them one by one; without one (NULL), or where the size is 0, the blocks are
  * dealt out in a fixed order in one launch. Both give the same bits.
  * batch == 0 or total == 0: nothing is done. Invalid: D not 64 or 128, nQHeads % nKVHeads != 0, negative
- * sizes, max_seq > total, prefix + total near 2^31, stride_prefix (0: prefix) < prefix, Q/K/V strides not a multiple of 8
+ * sizes, more than 2^20 sequences or 2^30 blocks of queries, max_seq > total, prefix + total near 2^31, stride_prefix (0: prefix) < prefix, Q/K/V strides not a multiple of 8
  * elements, O strides not a multiple of 4, rows shorter than D, Q/K/V/prefix not 16-byte or O not 8-byte
  * aligned. O must not overlap the inputs.
  */

@@ -215,6 +215,35 @@ def test_lengths_outside_the_tensors_stay_inside():
     check(guard[:T], ref, bound)
 
 
+def test_wrong_lengths_stay_inside_the_list():
+    """Overlapping sequences, which have many times the blocks that the workspace lists: nothing outside it, or outside
+    the tensors, is written, and the next call is right."""
+    T, n = 4200, 64
+    x = torch.randn(T, 8, 128, device=DEV).to(F16)
+    guard = torch.full((T + 64, 32, 128), 7.0, dtype=F16, device=DEV)
+    q = torch.randn(T, 32, 128, device=DEV).to(F16)
+    cfg = cdna4.PackedPrefillCfg(128, 32, 8, n, T, 0, 0, 0)
+    need = cdna4.prefill_packed_workspace_size(cfg)
+    assert need > 0
+    ws = torch.full((need + 4096,), 255, dtype=torch.uint8, device=DEV)
+    for cu in ([0, T] * (n // 2) + [0], [0, T, -5] * 21 + [0, T], [T, 0] * (n // 2) + [2 ** 31 - 1]):
+        cu_d = torch.tensor(cu, dtype=torch.int32, device=DEV)
+        assert cu_d.numel() == n + 1
+        for w in (ws[:need], None):
+            cdna4.prefill_packed(q, x, x, guard[:T], cu_d, cfg, workspace=w)
+        torch.cuda.synchronize()
+        assert bool((ws[need:] == 255).all()) and bool((guard[T:] == 7.0).all())
+    cu = cu_of([64] * (n - 1) + [T - 64 * (n - 1)])
+    cu_d = torch.tensor(cu, dtype=torch.int32, device=DEV)
+    guard[:T] = 7.0
+    cdna4.prefill_packed(q, x, x, guard[:T], cu_d, cfg, workspace=ws[:need])
+    one = torch.empty_like(q)
+    cdna4.prefill_packed(q, x, x, one, cu_d, cfg, workspace=None)
+    assert torch.equal(one, guard[:T])
+    ref, bound, _ = packed_reference(q, x, x, cu, 128, 4, F16)
+    check(one, ref, bound)
+
+
 def test_equal_lengths_as_the_uniform_call():
     """Sequences of one length: what prefill gives for them, within both calls' bounds."""
     B, S, H, D = 3, 333, 8, 128

@@ -76,6 +76,21 @@ def test_packed_plan():
         cdna4.prefill_packed_plan(cdna4.PackedPrefillCfg(64, 8, 3, 1, 10, 0, 0, 0))
 
 
+@pytest.mark.parametrize("cfg", [
+    (64, 8, 4, 3, 100, 50, 2 ** 31 - 100, 0), (64, 8, 4, 3, 2 ** 31 - 1, 50, 0, 0), (64, 8, 4, 3, 100, 50, 20, 19),
+    (64, 8, 4, 2 ** 20 + 1, 100, 50, 0, 0), (64, 8, 4, 2 ** 31 - 1, 2 ** 30, 0, 0, 0),
+    (128, 1025, 1025, 2 ** 20, 2 ** 20, 0, 0, 0)])
+def test_packed_refuses_sizes_past_32_bits(cfg):
+    """Key indices, sequences and blocks that 32-bit counters could not hold: the plan and the size refuse what the
+    call refuses."""
+    info, c = cdna4.PlanInfo(), cdna4.PackedPrefillCfg(*cfg)
+    assert cdna4.lib().cdna4_attn_prefill_packed_plan(ctypes.byref(c), cdna4.F16, ctypes.byref(info)) == 1
+    assert cdna4.prefill_packed_workspace_size(c) == 0
+    row = cfg[1] * cfg[0]
+    if cfg[1] == 8:   # the blocks of the last are counted when the device is known
+        assert packed(cfg, (row, cfg[0], row, cfg[0], row, cfg[0]), Kp=P, Vp=P) == 1
+
+
 def test_packed_python_refuses_cpu_tensors():
     x = torch.zeros(10, 4, 64, dtype=torch.float16)
     with pytest.raises(ValueError):
