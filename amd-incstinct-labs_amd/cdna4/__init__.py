@@ -378,7 +378,8 @@ def prefill_packed(Q: torch.Tensor, K: torch.Tensor, V: torch.Tensor, O: torch.T
     cfg.prefix > 0 every token also sees the first `prefix` rows of K_prefix / V_prefix [nKVH][stride][D].
     Rows of O outside cu_seqlens[0] .. cu_seqlens[batch] are left as they are. `workspace`: "auto" (default)
     allocates prefill_packed_workspace_size(cfg) bytes, where that is not 0, on the stream the call launches on; a
-    uint8 tensor is used as given; None runs in one launch, which needs none."""
+    uint8 tensor is used as given; None runs in one launch, which needs none (few prompts behind a long prefix
+    are faster with one)."""
     dev, dtype = _gpu_of(Q), Q.dtype
     if _elsewhere(dev, stream):
         with _entered(dev, stream):

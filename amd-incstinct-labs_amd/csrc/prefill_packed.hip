@@ -39,6 +39,9 @@ struct PackedArgs {
     int single;   // 1: a workgroup per item, at most
     struct ListHead* head;   // the work list, if there is one
     int4* items;
+    struct Cut* split;         // cut items, if any can be: how, their places, the parts' results
+    int4* cut;
+    float *part_ml, *part_o;   // [part][rows][2], [part][rows][D]
     int max_items;           // blocks times groups of heads that the sequences can have; the list's room
     int copy32;   // 1: a step's rows span < 4 GiB (32-bit copy offsets)
     float sc;     // log2(e) / sqrt(D)
@@ -375,8 +378,45 @@ __device__ __forceinline__ void store_rows(const f32x4 (&o)[D / 16], float l, ui
     }
 }
 
+// ---- items cut along their keys --------------------------------------------------------------------
+// Behind a long prefix all items take about as long, so the rounds of the chip's workgroups count: the items past
+// the last full round, where they are few, are cut into `each` parts along their keys, one to a workgroup, and
+// packed_join joins the parts. Part y of the tail's item e goes to workgroup y tail + e: the items of one kv head stay on
+// one XCD, whose L2 their prefix comes through.
+enum { kDealt, kFromList, kDealtCut };   // fa_packed: how workgroups get their items
+constexpr int kMinTiles = 16;   // tiles of an item that is cut
+constexpr int kMaxParts = 32;   // of an item
+struct Cut { int rounds, tail, each; };   // rounds of whole items before the cut ones; tail 0: none is cut
+
 // Workgroups of fa_packed that a CU holds (registers and LDS).
 template <int D, int QT> constexpr int resident() { return D == 64 ? 3 : 2; }
+
+// Whether and how the items past the last full round of G workgroups (per_cu to a CU) of 64 qt rows behind `tiles` tiles
+// are cut, by estimated times in eighths of a tile's (0.7 us at D = 128): a workgroup that has its CU to itself
+// takes 8 per tile, all that fit it together 13 (two) or 19 (three); the join costs five tiles for its launch and a
+// sixth per part and 64 rows for the results' way through memory (512 parts of 128 rows: 68 MB). Measured at 32/8 heads,
+// D 128, bf16: one sequence of 64 tokens behind 8,192 keys 93 -> 27 us, four of 16 behind 32,768 350 -> 59, ten of
+// 200 behind 8,192 (560 items on 512 workgroups) 369 -> 275; cut all the same, six of 70 behind 2,048 30.5 -> 48.
+__host__ __device__ __forceinline__ Cut cut_items(int items, int G, int tiles, int per_cu, int qt) {
+    const int rounds = items / G, tail = items - rounds * G, cus = G / per_cu;
+    const int full = per_cu == 2 ? 13 : 19;
+    Cut best{rounds, 0, 0};
+    if (tail == 0 || tiles < kMinTiles) return best;
+    int most = 1;   // parts of an item, about the root of its tiles
+    while (most < kMaxParts && (most + 1) * (most + 1) <= tiles) ++most;
+    long long time = (long long)tiles * (tail > cus ? full : 8);
+    for (int k = 0; k < 2; ++k) {   // to one workgroup per CU, or to as many as fit
+        int each = (k ? G : cus) / tail;
+        if (each > most) each = most;
+        if (each < 2) continue;
+        const long long t = (long long)tiles * (each * tail > cus ? full : 8) / each + 40 + each * tail * qt / 6;
+        if (t < time) {
+            time = t;
+            best = Cut{rounds, tail, each};
+        }
+    }
+    return best;
+}
 
 // ---- 128 rows per workgroup, two workgroups per CU -------------------------------------------------
 // Four waves of 32 queries share 64-key K/V tiles in LDS, two slots each for K and V (64 KiB at D = 128), so
@@ -385,8 +425,9 @@ template <int D, int QT> constexpr int resident() { return D == 64 ? 3 : 2; }
 // of the list times the heads (G workgroups), which evens out what a round's order costs, and loads the next
 // item's queries and first tiles before it stores its results: an item of one tile took 12.4 us as a
 // workgroup of its own, of which 2.4 to find it, 3.0 for the first loads and 2.9 for the stores.
-template <int D, int QT, bool kBf16, bool kPrefix, bool kListed>
+template <int D, int QT, bool kBf16, bool kPrefix, int kOrder>
 __global__ __launch_bounds__(256, (resident<D, QT>())) void fa_packed(PackedArgs a) {
+    constexpr bool kListed = kOrder == kFromList, kCut = kOrder == kDealtCut;
     constexpr int ND = D / 32, NDT = D / 16;
     __shared__ __attribute__((aligned(16))) uint16_t lds[block::lds_elems<D>()];
     static_assert((kLevels + 1) * 4 <= (int)sizeof(lds), "the histogram fits the tiles' LDS");
@@ -396,11 +437,25 @@ __global__ __launch_bounds__(256, (resident<D, QT>())) void fa_packed(PackedArgs
     // The workgroup's waves serve 1 << hp query heads of one kv head, a block's rows >> hp tokens each
     const int hp = a.hp, rows_log2 = block::rows_log2<QT>() - hp, nh = a.nQH >> hp;
     const int P = kPrefix ? a.prefix : 0;
-    struct Item { int start, len, q0, h0; };   // len 0: none
+    struct Item {
+        int start, len, q0, h0;   // len 0: none
+        int t0, t1, part;         // its tiles of keys, part >= 0: where its results go for packed_join
+    };
     __shared__ int4 next_s[4];
+    __shared__ int4 piece_s[kCut ? 4 : 1];
+    auto all_tiles = [&](int q0, int len) { return (P + min(q0 + (1 << rows_log2), len) + kBc - 1) / kBc; };
     auto item_at = [&](int round) {
         const int4 x = next_s[kListed ? 0 : round & 3];
-        return Item{scalar(x.x), scalar(x.y), scalar(x.z), scalar(x.w)};
+        Item it{scalar(x.x), scalar(x.y), scalar(x.z), scalar(x.w), 0, 0, -1};
+        if (kCut) {
+            const int4 y = piece_s[round & 3];
+            it.t0 = scalar(y.x);
+            it.t1 = scalar(y.y);
+            it.part = scalar(y.z);
+        } else {
+            it.t1 = all_tiles(it.q0, it.len);
+        }
+        return it;
     };
     // Listed: the first item is the workgroup's place in its XCD's queue, the others are claimed by wave 0 ahead
     // of an item's last tiles.
@@ -425,14 +480,27 @@ __global__ __launch_bounds__(256, (resident<D, QT>())) void fa_packed(PackedArgs
     // Not listed: each wave finds the item of another of the next four rounds.
     struct NoItems {};
     __shared__ std::conditional_t<kListed, NoItems, Items> items;
+    Cut cut{0, 0, 0};
     auto find = [&](int round) {
         if constexpr (!kListed) {
             const int G = (int)gridDim.x, p = (int)blockIdx.x;
-            const int idx = round * G + ((round & 1) ? G - 1 - p : p), entry = idx / nh;
+            int idx = round * G + ((round & 1) ? G - 1 - p : p);
+            const bool part = kCut && cut.tail > 0 && round >= cut.rounds;
+            const int y = part ? p / cut.tail : 0;
+            if (part) idx = round == cut.rounds && y < cut.each ? cut.rounds * G + p - y * cut.tail : a.max_items;
+            const int entry = idx / nh;
             int start = 0, len = 0, blk = 0;
             // overlapping sequences of a wrong cu can have more items than lengths that add up to the tokens: no more
             const bool ok = idx < a.max_items && find_item(a, rows_log2, items, entry, lane, start, len, blk);
-            if (lane == 0) next_s[round & 3] = make_int4(start, ok ? len : 0, blk << rows_log2, item_head(idx - entry * nh, nh) << hp);
+            const int4 x = make_int4(start, ok ? len : 0, blk << rows_log2, item_head(idx - entry * nh, nh) << hp);
+            if (lane == 0) next_s[round & 3] = x;
+            if constexpr (kCut) {
+                const int n = all_tiles(x.z, x.y);   // no fewer than the prefix has, so no part is empty
+                if (lane == 0) {
+                    piece_s[round & 3] = part ? make_int4(n * y / cut.each, n * (y + 1) / cut.each, p, 0) : make_int4(0, n, -1, 0);
+                    if (part && y == 0) a.cut[p] = x;   // p = e
+                }
+            }
         }
     };
     if constexpr (kListed) {
@@ -444,15 +512,27 @@ __global__ __launch_bounds__(256, (resident<D, QT>())) void fa_packed(PackedArgs
         }
     } else if (!a.single) {
         list_items(a, rows_log2, items, (int*)lds, (int)threadIdx.x);
+        if constexpr (kCut) {
+            cut = cut_items(scalar(items.levels) ? min(scalar(items.f[0]) * nh, a.max_items) : 0, (int)gridDim.x, P / kBc, resident<D, QT>(), QT);
+            if (blockIdx.x == 0 && threadIdx.x == 0) *a.split = cut;
+        }
         find(wave);
     }
     const block::Offsets own = block::own_offsets<D>(a.k_rs, wave, lane);
     u32x4 qb[QT][ND];
+    // keys from a part's first on: all that are left for an item's last part, whose tiles end with the block
+    auto keys_of = [&](const Item& it) {
+        const int left = P + it.len - it.t0 * kBc;
+        return kCut && it.t1 < all_tiles(it.q0, it.len) ? (it.t1 - it.t0) * kBc : left;
+    };
     auto keys = [&](const Item& it, const uint16_t* own, const uint16_t* pre) {
         const int kvh = it.h0 / a.G;
-        return Keys<kPrefix>{own + it.start * a.k_rs + kvh * a.k_hs, pre + kvh * a.p_hs, a.k_rs, P, P + it.len, a.copy32};
+        const uint16_t* o = own + it.start * a.k_rs + kvh * a.k_hs;
+        const uint16_t* p = pre + kvh * a.p_hs;
+        if (!kCut) return Keys<kPrefix>{o, p, a.k_rs, P, P + it.len, a.copy32};
+        const int k0 = it.t0 * kBc;   // the axis of a part begins at its first key
+        return Keys<kPrefix>{o + max(k0 - P, 0) * a.k_rs, p + (long long)min(k0, P) * D, a.k_rs, max(P - k0, 0), keys_of(it), a.copy32};
     };
-    auto tiles = [&](const Item& it) { return (P + min(it.q0 + (1 << rows_log2), it.len) + kBc - 1) / kBc; };
     const int dq = (wave & ((4 >> hp) - 1)) * QT * 16, dh = wave >> (2 - hp);   // of this wave in the block
     auto load = [&](const Item& it) {   // the queries and the first tiles
         const uint16_t* Qh = a.Q + it.start * a.q_rs + (it.h0 + dh) * a.q_hs;
@@ -462,7 +542,7 @@ __global__ __launch_bounds__(256, (resident<D, QT>())) void fa_packed(PackedArgs
 #pragma unroll
             for (int c = 0; c < ND; ++c) qb[t][c] = *(const u32x4*)(Qh + q * a.q_rs + c * 32 + g * 8);
         }
-        block::first_copies<D, kPrefix>(keys(it, a.K, a.Kp), keys(it, a.V, a.Vp), tiles(it), own, lds, wave, lane);
+        block::first_copies<D, kPrefix>(keys(it, a.K, a.Kp), keys(it, a.V, a.Vp), it.t1 - it.t0, own, lds, wave, lane);
     };
     Item it;
     if (!kListed && a.single) {   // no list to form: every wave finds the one item
@@ -471,6 +551,9 @@ __global__ __launch_bounds__(256, (resident<D, QT>())) void fa_packed(PackedArgs
         if (!packed_item(a, rows_log2, entry, lane, it.start, it.len, blk)) return;
         it.q0 = blk << rows_log2;
         it.h0 = item_head((int)blockIdx.x - entry * nh, nh) << hp;
+        it.t0 = 0;
+        it.t1 = all_tiles(it.q0, it.len);
+        it.part = -1;
     } else {
         __syncthreads();
         it = item_at(0);
@@ -478,20 +561,21 @@ __global__ __launch_bounds__(256, (resident<D, QT>())) void fa_packed(PackedArgs
     }
     load(it);
     for (int round = 1;; ++round) {
-        const int qw0 = it.q0 + dq, S = P + it.len, ntiles = tiles(it);
+        const int qw0 = it.q0 + dq, S = keys_of(it), ntiles = it.t1 - it.t0, P0 = P - it.t0 * kBc;
         const int wave_end = min(qw0 + QT * 16, it.len);                  // one past this wave's last query
-        const int nch = wave_end > qw0 ? (P + wave_end + 31) / 32 : 0;     // the wave's chunks; 0: no queries
+        int nch = wave_end > qw0 ? (P0 + wave_end + 31) / 32 : 0;          // the wave's chunks; 0: no queries
+        if (kCut) nch = max(min(nch, 2 * ntiles), 0);
         // Main tiles: chunks 2t + 1 and 2t + 2 lie below the workgroup's first query, and the copies of
         // V (t + 1) and K (t + 2) are whole tiles that exist.
-        int t_main = P + it.q0 >= 95 ? (P + it.q0 - 95) / 64 + 1 : 0;
+        int t_main = P0 + it.q0 >= 95 ? (P0 + it.q0 - 95) / 64 + 1 : 0;
         t_main = min(t_main, min(ntiles - 2, S / kBc - 2));
         if (!a.copy32) t_main = 0;
         f32x4 o[QT][NDT], lacc[QT];
         float m[QT];
-        block::attend<D, QT, kBf16, kPrefix, true>(keys(it, a.K, a.Kp), keys(it, a.V, a.Vp), block::Shape{S, ntiles, nch, P + qw0, t_main},
+        block::attend<D, QT, kBf16, kPrefix, true>(keys(it, a.K, a.Kp), keys(it, a.V, a.Vp), block::Shape{S, ntiles, nch, P0 + qw0, t_main},
                                                qb, o, lacc, m, own, lds, a.sc, wave, lane);
         uint16_t* Oh = a.O + it.start * a.o_rs + (it.h0 + dh) * a.o_hs;
-        const int len = it.len;
+        const int len = it.len, part = it.part;
         // What lies between two items is short and holds the matrix cores up: ahead of the CU's other waves
         __builtin_amdgcn_s_setprio(3);
         bool more = kListed || !a.single;
@@ -503,14 +587,75 @@ __global__ __launch_bounds__(256, (resident<D, QT>())) void fa_packed(PackedArgs
             more = it.len > 0;
             if (more) load(it);
         }
+        if (kCut && part >= 0) {
 #pragma unroll
-        for (int x = 0; x < QT; ++x) {
-            const int q = qw0 + x * 16 + li;
-            store_rows<D, kBf16>(o[x], lacc[x][0], Oh + q * a.o_rs, g, q < len);
+            for (int x = 0; x < QT; ++x) {
+                const size_t row = (size_t)part * (64 * QT) + (wave * QT + x) * 16 + li;
+                float* dst = a.part_o + row * D + g * 4;
+#pragma unroll
+                for (int dt = 0; dt < NDT; ++dt) *(f32x4*)(dst + dt * 16) = o[x][dt];
+                if (g == 0) *(float2*)(a.part_ml + row * 2) = make_float2(m[x], lacc[x][0]);
+            }
+        } else {
+#pragma unroll
+            for (int x = 0; x < QT; ++x) {
+                const int q = qw0 + x * 16 + li;
+                store_rows<D, kBf16>(o[x], lacc[x][0], Oh + q * a.o_rs, g, q < len);
+            }
         }
         if (!more) break;
         __builtin_amdgcn_s_setprio(0);
     }
+}
+
+// The rows of the cut items: o = sum_p 2^(m_p - M) O_p / sum_p 2^(m_p - M) l_p over an item's parts, D / 4 lanes per row.
+template <int D, int QT, bool kBf16>
+__global__ __launch_bounds__(256) void packed_join(PackedArgs a) {
+    constexpr int kRows = 64 * QT, kLanes = D / 4, kStep = 256 / kLanes;
+    const Cut cut = *a.split;
+    const int e = (int)blockIdx.x / (kRows / kStep);
+    if (e >= cut.tail) return;
+    const int4 it = a.cut[e];   // first row, rows, first query, first head
+    const int r = (int)blockIdx.x % (kRows / kStep) * kStep + (int)threadIdx.x / kLanes, d = 4 * ((int)threadIdx.x % kLanes);
+    const int wave = r / (16 * QT), hp = a.hp;
+    const int q = it.z + (wave & ((4 >> hp) - 1)) * (16 * QT) + r % (16 * QT), head = it.w + (wave >> (2 - hp));
+    if (q >= it.y) return;
+    const int n = cut.each;
+    const size_t step = (size_t)cut.tail * kRows;   // rows from one part to the next
+    const float* ml = a.part_ml + ((size_t)e * kRows + r) * 2;
+    const float* po = a.part_o + ((size_t)e * kRows + r) * D + d;
+    constexpr int kFlight = 8;
+    float M = kInitM, L = 0.f;
+    f32x4 acc{0.f, 0.f, 0.f, 0.f};
+    for (int i0 = 0; i0 < n; i0 += kFlight) {   // parts in flight; those past the last re-read it, weighted 0
+        f32x4 v[kFlight];
+        float2 s[kFlight];
+#pragma unroll
+        for (int i = 0; i < kFlight; ++i) {
+            const size_t x = min(i0 + i, n - 1);
+            s[i] = *(const float2*)(ml + x * step * 2);
+            v[i] = *(const f32x4*)(po + x * step * D);
+        }
+        float top = M;
+#pragma unroll
+        for (int i = 0; i < kFlight; ++i) top = fmaxf(top, s[i].x);
+        const float old = __builtin_amdgcn_exp2f(M - top);
+        M = top;
+        L *= old;
+        acc *= old;
+#pragma unroll
+        for (int i = 0; i < kFlight; ++i) {
+            const float w = i0 + i < n ? __builtin_amdgcn_exp2f(s[i].x - M) : 0.f;
+            L = fmaf(w, s[i].y, L);
+#pragma unroll
+            for (int k = 0; k < 4; ++k) acc[k] = fmaf(w, v[i][k], acc[k]);
+        }
+    }
+    const float inv = L > 0.f ? 1.f / L : 1.f;
+    uint2 o;
+    o.x = pack2<kBf16>(acc[0] * inv, acc[1] * inv);
+    o.y = pack2<kBf16>(acc[2] * inv, acc[3] * inv);
+    *(uint2*)(a.O + (it.x + q) * a.o_rs + head * a.o_hs + d) = o;
 }
 
 }  // namespace
@@ -548,10 +693,16 @@ int check_packed(const cdna4_packed_cfg* cfg, const cdna4_packed_strides* st, co
     return 0;
 }
 
-struct PackedPlan { int kernel, waves, rows, hp, qt; long long grid, items; size_t ws_bytes; };
+size_t align256(size_t n) { return (n + 255) & ~(size_t)255; }
+
+struct PackedPlan {
+    int kernel, waves, rows, hp, qt, order;
+    long long grid, items, cut, parts;   // cut: items that may be cut, parts: their parts
+    size_t ws_bytes;
+};
 
 template <int D>
-PackedPlan plan_packed(const cdna4_packed_cfg& c) {
+PackedPlan plan_packed(const cdna4_packed_cfg& c, bool with_ws) {
     PackedPlan p{};
     p.kernel = CDNA4_KERNEL_PACKED;
     p.waves = 4;
@@ -569,18 +720,40 @@ PackedPlan plan_packed(const cdna4_packed_cfg& c) {
     // more often and fill the matrix cores less: four of 512-1,024 (808 blocks of 128) 40.0 against 34.8 us. Half a
     // block per sequence is taken for the last ones.
     p.qt = (long long)(c.nQHeads >> p.hp) * (2LL * c.total / (128 >> p.hp) + std::min(c.batch, c.total)) <= 4 * cus ? 1 : 2;
+    p.order = kDealt;
+    // Behind a prefix, items may be cut along their keys (cut_items) where the blocks that the call probably has, or
+    // the most it can have, would be. Whole blocks where long shares leave them their better use of K and V: one
+    // sequence of 512 tokens behind 8,192 keys 82 against 88 us.
+    bool cut = false;
+    if (with_ws && c.prefix >= kMinTiles * kBc && items(128 >> p.hp) < 2 * slots && ((long long)c.total << p.hp) / 64 < kLevels) {
+        const int tiles = c.prefix / kBc, seqs = std::min(c.batch, c.total);
+        auto blocks = [&](int rows) { return (long long)(c.nQHeads >> p.hp) * (2LL * c.total / rows + seqs) / 2; };
+        const long long n = blocks(128 >> p.hp);
+        if (((long long)c.total << p.hp) >= 128LL * seqs && n <= slots / 2 && n * tiles >= 32 * slots) p.qt = 2;
+        const int round = (int)(p.qt == 2 ? slots : resident<D, 1>() * cus), rows = (64 * p.qt) >> p.hp;
+        for (long long x : {blocks(rows), items(rows)})
+            if (cut_items((int)x, round, tiles, (int)(round / cus), p.qt).tail > 0) cut = true;
+        if (cut) p.order = kDealtCut;
+    }
     p.rows = (p.qt == 2 ? 128 : 64) >> p.hp;
     p.items = items(p.rows);
-    p.grid = std::min(p.items, p.qt == 2 ? slots : resident<D, 1>() * cus);
-    p.ws_bytes = D == 128 && p.qt == 2 && p.items >= 2 * slots && c.batch <= kListSeqs && p.items <= kMaxItems
-                     ? sizeof(ListHead) + (size_t)p.items * sizeof(int4) : 0;
+    const long long round = p.qt == 2 ? slots : resident<D, 1>() * cus;
+    p.grid = cut ? round : std::min(p.items, round);
+    if (cut) {
+        p.cut = std::min(p.items, round / 2);
+        p.parts = std::min(round, kMaxParts * p.cut);
+        p.ws_bytes = 256 + align256(p.cut * sizeof(int4)) + (size_t)p.parts * (64 * p.qt) * (D + 2) * sizeof(float);
+    } else if (with_ws && D == 128 && p.qt == 2 && p.items >= 2 * slots && c.batch <= kListSeqs && p.items <= kMaxItems) {
+        p.order = kFromList;
+        p.ws_bytes = sizeof(ListHead) + (size_t)p.items * sizeof(int4);
+    }
     return p;
 }
 
 template <int D, bool kBf16>
 int launch_packed(const cdna4_packed_cfg& c, const cdna4_packed_strides& st, const void* Q, const void* K, const void* V,
                   const void* Kp, const void* Vp, void* O, const int* cu, void* ws, hipStream_t s) {
-    const PackedPlan p = plan_packed<D>(c);
+    const PackedPlan p = plan_packed<D>(c, ws != nullptr);
     if (p.items > kMaxItems) return CDNA4_ERR_INVALID_VALUE;
     PackedArgs a;
     a.Q = (const uint16_t*)Q; a.K = (const uint16_t*)K; a.V = (const uint16_t*)V; a.O = (uint16_t*)O;
@@ -588,29 +761,47 @@ int launch_packed(const cdna4_packed_cfg& c, const cdna4_packed_strides& st, con
     a.cu = cu;
     a.q_rs = st.q_row; a.q_hs = st.q_head; a.k_rs = st.kv_row; a.k_hs = st.kv_head; a.o_rs = st.o_row; a.o_hs = st.o_head;
     a.p_hs = (long long)(c.stride_prefix ? c.stride_prefix : c.prefix) * D;
-    a.nQH = c.nQHeads; a.G = c.nQHeads / c.nKVHeads; a.batch = c.batch; a.total = c.total; a.prefix = c.prefix; a.hp = p.hp; a.single = p.grid == p.items;
+    a.nQH = c.nQHeads; a.G = c.nQHeads / c.nKVHeads; a.batch = c.batch; a.total = c.total; a.prefix = c.prefix; a.hp = p.hp; a.single = p.order == kDealt && p.grid == p.items;
     a.copy32 = 256 * st.kv_row * 2 < (1LL << 32) ? 1 : 0;
     a.sc = kLog2e / sqrtf((float)D);
     const unsigned grid = (unsigned)p.grid;
     a.head = nullptr;
     a.items = nullptr;
     a.max_items = (int)p.items;   // up to kMaxItems
+    a.split = nullptr;
+    a.cut = nullptr;
+    a.part_ml = a.part_o = nullptr;
     if constexpr (D == 128) {
-        if (ws && p.ws_bytes) {
+        if (p.order == kFromList) {
             a.head = (ListHead*)ws;
             a.items = (int4*)(a.head + 1);
             packed_list<<<1, 1024, 0, s>>>(a, (int)(grid >> 3));
-            if (c.prefix) fa_packed<D, 2, kBf16, true, true><<<grid, 256, 0, s>>>(a);
-            else fa_packed<D, 2, kBf16, false, true><<<grid, 256, 0, s>>>(a);
+            if (c.prefix) fa_packed<D, 2, kBf16, true, kFromList><<<grid, 256, 0, s>>>(a);
+            else fa_packed<D, 2, kBf16, false, kFromList><<<grid, 256, 0, s>>>(a);
             return launch_status();
         }
     }
+    if (p.order == kDealtCut) {
+        a.split = (Cut*)ws;
+        a.cut = (int4*)((char*)ws + 256);
+        a.part_o = (float*)((char*)a.cut + align256(p.cut * sizeof(int4)));
+        a.part_ml = a.part_o + (size_t)p.parts * (64 * p.qt) * D;
+        const unsigned join = (unsigned)(p.cut * (64 * p.qt) / (1024 / D));
+        if (p.qt == 2) {
+            fa_packed<D, 2, kBf16, true, kDealtCut><<<grid, 256, 0, s>>>(a);
+            packed_join<D, 2, kBf16><<<join, 256, 0, s>>>(a);
+        } else {
+            fa_packed<D, 1, kBf16, true, kDealtCut><<<grid, 256, 0, s>>>(a);
+            packed_join<D, 1, kBf16><<<join, 256, 0, s>>>(a);
+        }
+        return launch_status();
+    }
     if (p.qt == 2) {
-        if (c.prefix) fa_packed<D, 2, kBf16, true, false><<<grid, 256, 0, s>>>(a);
-        else fa_packed<D, 2, kBf16, false, false><<<grid, 256, 0, s>>>(a);
+        if (c.prefix) fa_packed<D, 2, kBf16, true, kDealt><<<grid, 256, 0, s>>>(a);
+        else fa_packed<D, 2, kBf16, false, kDealt><<<grid, 256, 0, s>>>(a);
     } else {
-        if (c.prefix) fa_packed<D, 1, kBf16, true, false><<<grid, 256, 0, s>>>(a);
-        else fa_packed<D, 1, kBf16, false, false><<<grid, 256, 0, s>>>(a);
+        if (c.prefix) fa_packed<D, 1, kBf16, true, kDealt><<<grid, 256, 0, s>>>(a);
+        else fa_packed<D, 1, kBf16, false, kDealt><<<grid, 256, 0, s>>>(a);
     }
     return launch_status();
 }
@@ -646,7 +837,7 @@ extern "C" int cdna4_attn_prefill_packed_plan(const cdna4_packed_cfg* cfg, int d
     if (!cfg || !out) return CDNA4_ERR_INVALID_VALUE;
     const cdna4_packed_cfg& c = *cfg;
     if (!valid_cfg(c) || c.batch < 1 || c.total < 1 || (dtype != CDNA4_F16 && dtype != CDNA4_BF16)) return CDNA4_ERR_INVALID_VALUE;
-    const PackedPlan p = c.D == 128 ? plan_packed<128>(c) : plan_packed<64>(c);
+    const PackedPlan p = c.D == 128 ? plan_packed<128>(c, true) : plan_packed<64>(c, true);
     if (p.items > kMaxItems) return CDNA4_ERR_INVALID_VALUE;
     out->kernel = p.kernel;
     out->waves = p.waves;

@@ -141,8 +141,11 @@ int cdna3_attn_prefill_strided(const void* Q, const void* K, const void* V, void
  * max_seq (0: unknown) is the longest sequence; it is checked against total, and no kernel depends on it.
  * With a workspace (cdna4_attn_prefill_packed_workspace_size(cfg) bytes, 16-byte aligned, no initialisation; calls
  * that overlap must not share one) a call of many blocks first lists them, in an order that finds K and V in the L2
- * caches, and its workgroups claim them one by one; without one (NULL), or where the size is 0, the blocks are
- * dealt out in a fixed order in one launch. Both give the same bits.
+ * caches, and its workgroups claim them one by one; a call of few blocks behind a prefix of 1,024 keys and more cuts
+ * them along their keys and joins the parts in a second launch. Without one (NULL), or where the size is 0, the blocks
+ * are dealt out in a fixed order in one launch: the bits are those of the listed blocks, and differ from the cut ones'
+ * by the order of their sums. The plan is sized to the current device, so query the size with the device current that
+ * the call will run on.
  * batch == 0 or total == 0: nothing is done. Invalid: D not 64 or 128, nQHeads % nKVHeads != 0, negative
  * sizes, more than 2^20 sequences or 2^30 blocks of queries, max_seq > total, prefix + total near 2^31, stride_prefix (0: prefix) < prefix, Q/K/V strides not a multiple of 8
  * elements, O strides not a multiple of 4, rows shorter than D, Q/K/V/prefix not 16-byte or O not 8-byte
@@ -272,7 +275,8 @@ int cdna3_attn_prefill_plan(const cdna3_prefill_cfg* cfg, int dtype, cdna3_plan_
 int cdna3_attn_decode_plan(const cdna3_decode_cfg* cfg, int dtype, int with_workspace,
                            cdna3_plan_info* out);
 /* cdna4_attn_prefill_packed: `grid` counts a workgroup for every block that the sequences could need
- * (those past the last block end at once). */
+ * (those past the last block end at once) or, with more of them and for cut blocks, one round of the chip's;
+ * `rows` and `workspace` are those of a call with a workspace. */
 int cdna4_attn_prefill_packed_plan(const cdna4_packed_cfg* cfg, int dtype, cdna3_plan_info* out);
 /* cdna4_attn_decode_shared: `rows` prefix keys per part, `partials` parts per query head at most. */
 int cdna4_attn_decode_shared_plan(const cdna4_shared_decode_cfg* cfg, int dtype, cdna3_plan_info* out);

@@ -131,6 +131,67 @@ def test_listed_blocks(name):
     verify(args, args[-1], dtype, one, name)
 
 
+CUT = {   # calls behind a prefix of 1,024 keys and more with fewer than two rounds of blocks: cut along their keys
+    "one_token": ([1], 8, 2, 128, BF16, 2048),
+    "few_tokens": ([3, 0, 17, 1], 12, 12, 64, F16, 2049),
+    "short_block": ([64], 4, 1, 128, F16, 40000),                     # 32 parts
+    "one_head": ([200], 1, 1, 64, BF16, 5000),
+    "ragged": ([17, 300, 64, 129, 1], 32, 8, 128, BF16, 4001),
+    "more_than_a_round": ([600, 17, 701, 333, 450], 32, 8, 128, F16, 2500),
+    "own_longer": ([5000, 20], 8, 2, 64, F16, 2048),
+    "heads": ([33] * 9, 10, 5, 128, BF16, 3001),
+    "a_round_and_more": ([130] * 40, 16, 4, 64, BF16, 2111),
+    "ragged_less": ([17, 60, 64, 40, 1], 32, 8, 128, BF16, 4001),
+    "short": ([30, 30], 32, 8, 128, F16, 1025),
+    "round_of_half_blocks": ([100] * 11, 32, 8, 128, F16, 2048),
+    "own_longer_cut": ([500, 20], 8, 2, 64, F16, 2048),
+    "a_round_and_few": ([130] * 39, 16, 4, 64, BF16, 3111),
+}
+UNCUT = {"ragged", "own_longer"}   # more than half a round of blocks
+
+
+@pytest.mark.parametrize("name", list(CUT))
+def test_cut_blocks(name):
+    lens, HQ, HK, D, dtype, prefix = CUT[name]
+    args = make(lens, HQ, HK, D, dtype, prefix=prefix, spare=2, seed=len(lens))
+    need = cdna4.prefill_packed_workspace_size(args[-1])
+    assert (need > 0) == (name not in UNCUT)
+    outs = []
+    for fill in (0, 255):
+        ws = torch.full((need + 16,), fill, dtype=torch.uint8, device=DEV)
+        outs.append(run(*args[:5], *args[6:], workspace=ws[:need] if need else None))
+        assert bool((ws[need:] == fill).all())
+    assert torch.equal(*outs) and torch.equal(outs[0], run(*args[:5], *args[6:]))
+    verify(args, args[-1], dtype, outs[0], name)
+    verify(args, args[-1], dtype, run(*args[:5], *args[6:], workspace=None), name)
+
+
+def test_cut_blocks_replayed():
+    """Which items are cut, and how, follows the lengths in every replay; wrong lengths stay inside."""
+    T, P = 1100, 2600
+    Q, K, V, Kp, Vp, _, _, _ = make([T], 32, 8, 128, F16, prefix=P, seed=31)
+    cfg = cdna4.PackedPrefillCfg(128, 32, 8, 5, T, 0, P, Kp.shape[1])
+    need = cdna4.prefill_packed_workspace_size(cfg)
+    ws = torch.full((need + 4096,), 255, dtype=torch.uint8, device=DEV)
+    cu_d = torch.tensor([0, 1, 2, 3, 4, 5], dtype=torch.int32, device=DEV)
+    O = torch.full((T + 8, 32, 128), 7.0, dtype=F16, device=DEV)
+    run(Q, K, V, Kp, Vp, cu_d, cfg, O=O[:T], workspace=ws[:need])
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        run(Q, K, V, Kp, Vp, cu_d, cfg, O=O[:T], workspace=ws[:need])
+    for lens in ([1100, 0, 0, 0, 0], [60] * 5, [1, 1, 1, 1, 1], [0, 0, 0, 0, 0], None, [17, 700, 300, 3, 80], [40, 0, 0, 0, 0]):
+        cu = cu_of(lens) if lens else [0, T, 0, T, -3, T]
+        cu_d.copy_(torch.tensor(cu, dtype=torch.int32))
+        O.fill_(7.0)
+        graph.replay()
+        torch.cuda.synchronize()
+        assert bool((ws[need:] == 255).all()) and bool((O[T:] == 7.0).all())
+        if lens:
+            assert torch.equal(O[:T], run(Q, K, V, Kp, Vp, cu_d, cfg)), lens
+            verify((Q, K, V, Kp, Vp, cu, cu_d, cfg), cfg, F16, O[:T], str(lens))
+
+
 def test_listed_blocks_replayed():
     """The queues start over in every replay, on other lengths."""
     T = 4200
