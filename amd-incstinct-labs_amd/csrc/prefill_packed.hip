@@ -11,6 +11,10 @@
 // one block of queries of one sequence and head, from cu alone. Blocks are ordered by their index in the
 // sequence, the last ones (the most keys) first, so that the hardware's in-order dispatch gives the chip a
 // longest-first schedule whatever the lengths are.
+//
+// Bound by the matrix cores: four prompts of 2,011-8,192 tokens, 32/8 heads D 128 bf16, 925 us in a graph (1,220 TFLOP/s,
+// matrix cores 65 % busy), 24 of 33-2,048 148 us (865 TFLOP/s: a block's start and end take a quarter of its time), 16 of
+// 90-1,024, 12 heads D 64 fp16, 24 us (the longest block's 16 tiles one after another).
 #include <type_traits>
 #include <algorithm>
 
@@ -169,8 +173,8 @@ __device__ __forceinline__ bool find_item(const PackedArgs& a, int rows_log2, co
 // the same K and V, run on one XCD at about the same time and find them in its L2; longest sequences first, the
 // last blocks of a sequence first; a workgroup whose queue is empty takes from the others. Against the list
 // in LDS (longest blocks of all sequences first, dealt out in turn): 64 prompts of 512 tokens, 32/8 heads
-// D 128, read their 134 MB of K and V again for every block index there, 258 us against 224 in this order; 12 of
-// 512-8,192 tokens 945 against 925 us.
+// D 128, read their 134 MB of K and V again for every block index there, 258 us against 224 in this order; four of
+// 2,011-8,192 tokens 945 against 925 us.
 constexpr int kListSeqs = 2048;   // sequences of the listing kernel's LDS
 struct ListHead {
     int next[8][32];   // of the queue's entries, a cache line each
