@@ -21,12 +21,14 @@
 #include "attn_tile.hpp"
 #include "attn_stream.hpp"
 #include "attn_block.hpp"
+#include "packed_cut.hpp"
 
 namespace cdna4 {
 namespace {
 
 using namespace tile;
 using namespace pipe;
+using namespace packed;
 using block::Keys;
 using wave::xlane::allreduce;
 using wave::xlane::Max;
@@ -43,7 +45,7 @@ struct PackedArgs {
     int single;   // 1: a workgroup per item, at most
     struct ListHead* head;   // the work list, if there is one
     int4* items;
-    struct Cut* split;         // cut items, if any can be: how, their places, the parts' results
+    Cut* split;                // cut items, if any can be: how, their places, the parts' results
     int4* cut;
     float *part_ml, *part_o;   // [part][rows][2], [part][rows][D]
     int max_items;           // blocks times groups of heads that the sequences can have; the list's room
@@ -382,45 +384,11 @@ __device__ __forceinline__ void store_rows(const f32x4 (&o)[D / 16], float l, ui
     }
 }
 
-// ---- items cut along their keys --------------------------------------------------------------------
-// Behind a long prefix all items take about as long, so the rounds of the chip's workgroups count: the items past
-// the last full round, where they are few, are cut into `each` parts along their keys, one to a workgroup, and
-// packed_join joins the parts. Part y of the tail's item e goes to workgroup y tail + e: the items of one kv head stay on
-// one XCD, whose L2 their prefix comes through.
-enum { kDealt, kFromList, kDealtCut };   // fa_packed: how workgroups get their items
-constexpr int kMinTiles = 16;   // tiles of an item that is cut
-constexpr int kMaxParts = 32;   // of an item
-struct Cut { int rounds, tail, each; };   // rounds of whole items before the cut ones; tail 0: none is cut
+// How fa_packed's workgroups get their items (packed_cut.hpp: dealt out, and cut along their keys)
+enum { kDealt, kFromList, kDealtCut };
 
 // Workgroups of fa_packed that a CU holds (registers and LDS).
 template <int D, int QT> constexpr int resident() { return D == 64 ? 3 : 2; }
-
-// Whether and how the items past the last full round of G workgroups (per_cu to a CU) of 64 qt rows behind `tiles` tiles
-// are cut, by estimated times in eighths of a tile's (0.7 us at D = 128): a workgroup that has its CU to itself
-// takes 8 per tile, all that fit it together 13 (two) or 19 (three); the join costs five tiles for its launch and a
-// sixth per part and 64 rows for the results' way through memory (512 parts of 128 rows: 68 MB). Measured at 32/8 heads,
-// D 128, bf16: one sequence of 64 tokens behind 8,192 keys 93 -> 27 us, four of 16 behind 32,768 350 -> 59, ten of
-// 200 behind 8,192 (560 items on 512 workgroups) 369 -> 275; cut all the same, six of 70 behind 2,048 30.5 -> 48.
-__host__ __device__ __forceinline__ Cut cut_items(int items, int G, int tiles, int per_cu, int qt) {
-    const int rounds = items / G, tail = items - rounds * G, cus = G / per_cu;
-    const int full = per_cu == 2 ? 13 : 19;
-    Cut best{rounds, 0, 0};
-    if (tail == 0 || tiles < kMinTiles) return best;
-    int most = 1;   // parts of an item, about the root of its tiles
-    while (most < kMaxParts && (most + 1) * (most + 1) <= tiles) ++most;
-    long long time = (long long)tiles * (tail > cus ? full : 8);
-    for (int k = 0; k < 2; ++k) {   // to one workgroup per CU, or to as many as fit
-        int each = (k ? G : cus) / tail;
-        if (each > most) each = most;
-        if (each < 2) continue;
-        const long long t = (long long)tiles * (each * tail > cus ? full : 8) / each + 40 + each * tail * qt / 6;
-        if (t < time) {
-            time = t;
-            best = Cut{rounds, tail, each};
-        }
-    }
-    return best;
-}
 
 // ---- 128 rows per workgroup, two workgroups per CU -------------------------------------------------
 // Four waves of 32 queries share 64-key K/V tiles in LDS, two slots each for K and V (64 KiB at D = 128), so
@@ -487,22 +455,19 @@ __global__ __launch_bounds__(256, (resident<D, QT>())) void fa_packed(PackedArgs
     Cut cut{0, 0, 0};
     auto find = [&](int round) {
         if constexpr (!kListed) {
-            const int G = (int)gridDim.x, p = (int)blockIdx.x;
-            int idx = round * G + ((round & 1) ? G - 1 - p : p);
-            const bool part = kCut && cut.tail > 0 && round >= cut.rounds;
-            const int y = part ? p / cut.tail : 0;
-            if (part) idx = round == cut.rounds && y < cut.each ? cut.rounds * G + p - y * cut.tail : a.max_items;
-            const int entry = idx / nh;
+            const Turn turn = turn_of(cut, round, (int)blockIdx.x, (int)gridDim.x);
+            const int entry = turn.idx / nh;
             int start = 0, len = 0, blk = 0;
             // overlapping sequences of a wrong cu can have more items than lengths that add up to the tokens: no more
-            const bool ok = idx < a.max_items && find_item(a, rows_log2, items, entry, lane, start, len, blk);
-            const int4 x = make_int4(start, ok ? len : 0, blk << rows_log2, item_head(idx - entry * nh, nh) << hp);
+            const bool ok = turn.idx < a.max_items && find_item(a, rows_log2, items, entry, lane, start, len, blk);
+            const int4 x = make_int4(start, ok ? len : 0, blk << rows_log2, item_head(turn.idx - entry * nh, nh) << hp);
             if (lane == 0) next_s[round & 3] = x;
             if constexpr (kCut) {
                 const int n = all_tiles(x.z, x.y);   // no fewer than the prefix has, so no part is empty
                 if (lane == 0) {
-                    piece_s[round & 3] = part ? make_int4(n * y / cut.each, n * (y + 1) / cut.each, p, 0) : make_int4(0, n, -1, 0);
-                    if (part && y == 0) a.cut[p] = x;   // p = e
+                    piece_s[round & 3] = turn.part >= 0 ? make_int4(n * turn.y / cut.each, n * (turn.y + 1) / cut.each, turn.part, 0)
+                                                        : make_int4(0, n, -1, 0);
+                    if (turn.place >= 0) a.cut[turn.place] = x;   // one wave of one workgroup for each place
                 }
             }
         }
