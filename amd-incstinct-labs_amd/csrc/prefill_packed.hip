@@ -21,7 +21,7 @@
 #include "attn_tile.hpp"
 #include "attn_stream.hpp"
 #include "attn_block.hpp"
-#include "packed_cut.hpp"
+#include "packed_plan.hpp"
 
 namespace cdna4 {
 namespace {
@@ -66,7 +66,6 @@ __device__ __forceinline__ void seq_rows(const PackedArgs& a, int s, int& start,
 // the largest index d with f(d) > idx, and is the (idx - f(d + 1))-th sequence with more than d blocks. A
 // workgroup forms f once, in LDS: a histogram of the n_s, summed twice from the top (the sequences with more
 // than d blocks, then their blocks).
-constexpr int kLevels = 1024;   // block indices held: sequences of 32,768 tokens and more (rows_log2)
 constexpr int kSeqs = 512;      // sequences held; the rows of others are read again
 struct Items {
     int f[kLevels];
@@ -177,13 +176,12 @@ __device__ __forceinline__ bool find_item(const PackedArgs& a, int rows_log2, co
 // in LDS (longest blocks of all sequences first, dealt out in turn): 64 prompts of 512 tokens, 32/8 heads
 // D 128, read their 134 MB of K and V again for every block index there, 258 us against 224 in this order; four of
 // 2,011-8,192 tokens 945 against 925 us.
-constexpr int kListSeqs = 2048;   // sequences of the listing kernel's LDS
 struct ListHead {
     int next[8][32];   // of the queue's entries, a cache line each
     int begin[8], end[8];
     int pad[48];
 };
-static_assert(sizeof(ListHead) % 256 == 0, "");
+static_assert(sizeof(ListHead) == kListHeadBytes && sizeof(int4) == kItemBytes, "the plan's sizes");
 
 // Heads (nh per entry) of the sequence at place q that go to queue x: cnt of them, the c-th is head(c).
 struct QueueHeads {
@@ -383,12 +381,6 @@ __device__ __forceinline__ void store_rows(const f32x4 (&o)[D / 16], float l, ui
         if (valid) *(u32x4_8*)(dst + dt * 16) = w;
     }
 }
-
-// How fa_packed's workgroups get their items (packed_cut.hpp: dealt out, and cut along their keys)
-enum { kDealt, kFromList, kDealtCut };
-
-// Workgroups of fa_packed that a CU holds (registers and LDS).
-template <int D, int QT> constexpr int resident() { return D == 64 ? 3 : 2; }
 
 // ---- 128 rows per workgroup, two workgroups per CU -------------------------------------------------
 // Four waves of 32 queries share 64-key K/V tiles in LDS, two slots each for K and V (64 KiB at D = 128), so
@@ -633,7 +625,6 @@ namespace {
 
 // Every call reads cu in each of its workgroups, and a block's keys and the blocks are counted in 32 bits.
 constexpr int kMaxBatch = 1 << 20;
-constexpr long long kMaxItems = 1LL << 30;
 
 bool valid_cfg(const cdna4_packed_cfg& c) {
     if (c.D != 64 && c.D != 128) return false;
@@ -662,67 +653,10 @@ int check_packed(const cdna4_packed_cfg* cfg, const cdna4_packed_strides* st, co
     return 0;
 }
 
-size_t align256(size_t n) { return (n + 255) & ~(size_t)255; }
-
-struct PackedPlan {
-    int kernel, waves, rows, hp, qt, order;
-    long long grid, items, cut, parts;   // cut: items that may be cut, parts: their parts
-    size_t ws_bytes;
-};
-
-template <int D>
-PackedPlan plan_packed(const cdna4_packed_cfg& c, bool with_ws) {
-    PackedPlan p{};
-    p.kernel = CDNA4_KERNEL_PACKED;
-    p.waves = 4;
-    // Query heads of one kv head side by side, up to one per wave: a block then has 128, 64 or 32 tokens, its
-    // waves end at the same key or nearly so (with 128 tokens they pass the last two tiles as a staircase), and
-    // short sequences fill it.
-    const int G = c.nQHeads / c.nKVHeads;
-    p.hp = G % 4 == 0 ? 2 : G % 2 == 0 ? 1 : 0;
-    // sum of ceil(len / rows) is at most total / rows + the sequences that are not empty
-    auto items = [&](int rows) { return (long long)(c.nQHeads >> p.hp) * (c.total / rows + std::min(c.batch, c.total)); };
-    const long long cus = device_cus() & ~7;
-    const long long slots = resident<D, 2>() * cus;   // resident workgroups: the grid is one round of them
-    // Blocks of half as many rows for calls of about one round of blocks and less, whose time is that of their
-    // longest block: one sequence of 1,024 tokens, 32/8 heads D 128, 21.4 against 25.7 us; above that they read K and V
-    // more often and fill the matrix cores less: four of 512-1,024 (808 blocks of 128) 40.0 against 34.8 us. Half a
-    // block per sequence is taken for the last ones.
-    p.qt = (long long)(c.nQHeads >> p.hp) * (2LL * c.total / (128 >> p.hp) + std::min(c.batch, c.total)) <= 4 * cus ? 1 : 2;
-    p.order = kDealt;
-    // Behind a prefix, items may be cut along their keys (cut_items) where the blocks that the call probably has, or
-    // the most it can have, would be. Whole blocks where long shares leave them their better use of K and V: one
-    // sequence of 512 tokens behind 8,192 keys 82 against 88 us.
-    bool cut = false;
-    if (with_ws && c.prefix >= kMinTiles * kBc && items(128 >> p.hp) < 2 * slots && ((long long)c.total << p.hp) / 64 < kLevels) {
-        const int tiles = c.prefix / kBc, seqs = std::min(c.batch, c.total);
-        auto blocks = [&](int rows) { return (long long)(c.nQHeads >> p.hp) * (2LL * c.total / rows + seqs) / 2; };
-        const long long n = blocks(128 >> p.hp);
-        if (((long long)c.total << p.hp) >= 128LL * seqs && n <= slots / 2 && n * tiles >= 32 * slots) p.qt = 2;
-        const int round = (int)(p.qt == 2 ? slots : resident<D, 1>() * cus), rows = (64 * p.qt) >> p.hp;
-        for (long long x : {blocks(rows), items(rows)})
-            if (cut_items((int)x, round, tiles, (int)(round / cus), p.qt).tail > 0) cut = true;
-        if (cut) p.order = kDealtCut;
-    }
-    p.rows = (p.qt == 2 ? 128 : 64) >> p.hp;
-    p.items = items(p.rows);
-    const long long round = p.qt == 2 ? slots : resident<D, 1>() * cus;
-    p.grid = cut ? round : std::min(p.items, round);
-    if (cut) {
-        p.cut = std::min(p.items, round / 2);
-        p.parts = std::min(round, kMaxParts * p.cut);
-        p.ws_bytes = 256 + align256(p.cut * sizeof(int4)) + (size_t)p.parts * (64 * p.qt) * (D + 2) * sizeof(float);
-    } else if (with_ws && D == 128 && p.qt == 2 && p.items >= 2 * slots && c.batch <= kListSeqs && p.items <= kMaxItems) {
-        p.order = kFromList;
-        p.ws_bytes = sizeof(ListHead) + (size_t)p.items * sizeof(int4);
-    }
-    return p;
-}
-
 template <int D, bool kBf16>
 int launch_packed(const cdna4_packed_cfg& c, const cdna4_packed_strides& st, const void* Q, const void* K, const void* V,
                   const void* Kp, const void* Vp, void* O, const int* cu, void* ws, hipStream_t s) {
-    const PackedPlan p = plan_packed<D>(c, ws != nullptr);
+    const PackedPlan p = plan_packed<D>(c, ws != nullptr, device_cus());
     if (p.items > kMaxItems) return CDNA4_ERR_INVALID_VALUE;
     PackedArgs a;
     a.Q = (const uint16_t*)Q; a.K = (const uint16_t*)K; a.V = (const uint16_t*)V; a.O = (uint16_t*)O;
@@ -753,7 +687,7 @@ int launch_packed(const cdna4_packed_cfg& c, const cdna4_packed_strides& st, con
     if (p.order == kDealtCut) {
         a.split = (Cut*)ws;
         a.cut = (int4*)((char*)ws + 256);
-        a.part_o = (float*)((char*)a.cut + align256(p.cut * sizeof(int4)));
+        a.part_o = (float*)((char*)a.cut + align256(p.cut * kItemBytes));
         a.part_ml = a.part_o + (size_t)p.parts * (64 * p.qt) * D;
         const unsigned join = (unsigned)(p.cut * (64 * p.qt) / (1024 / D));
         if (p.qt == 2) {
@@ -806,10 +740,10 @@ extern "C" int cdna4_attn_prefill_packed_plan(const cdna4_packed_cfg* cfg, int d
     if (!cfg || !out) return CDNA4_ERR_INVALID_VALUE;
     const cdna4_packed_cfg& c = *cfg;
     if (!valid_cfg(c) || c.batch < 1 || c.total < 1 || (dtype != CDNA4_F16 && dtype != CDNA4_BF16)) return CDNA4_ERR_INVALID_VALUE;
-    const PackedPlan p = c.D == 128 ? plan_packed<128>(c, true) : plan_packed<64>(c, true);
+    const PackedPlan p = c.D == 128 ? plan_packed<128>(c, true, device_cus()) : plan_packed<64>(c, true, device_cus());
     if (p.items > kMaxItems) return CDNA4_ERR_INVALID_VALUE;
-    out->kernel = p.kernel;
-    out->waves = p.waves;
+    out->kernel = CDNA4_KERNEL_PACKED;
+    out->waves = block::kWaves;
     out->rows = p.rows;
     out->grid = p.grid;
     out->partials = 1;

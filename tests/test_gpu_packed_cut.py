@@ -50,3 +50,15 @@ def test_places_of_the_cut_items(name):
     verify(args, cfg, dtype, O, name)
     for _ in range(3):
         assert torch.equal(O, run(*args[:5], *args[6:], workspace=ws))
+
+
+@pytest.mark.parametrize("D,total,prefix", [(128, 1008, 4096), (128, 1008, 8960), (64, 791, 8192)])
+def test_workspace_of_a_call_that_needs_none(D, total, prefix):
+    """Where the size is 0, a caller's workspace changes no bit and is not written to."""
+    args = make([total], 32, 8, D, BF16, prefix=prefix, seed=prefix)
+    assert cdna4.prefill_packed_workspace_size(args[-1]) == 0
+    ws = torch.full((4096,), 255, dtype=torch.uint8, device=DEV)
+    one = run(*args[:5], *args[6:], workspace=None)
+    assert torch.equal(one, run(*args[:5], *args[6:], workspace=ws)) and torch.equal(one, run(*args[:5], *args[6:]))
+    assert bool((ws == 255).all())
+    verify(args, args[-1], BF16, one)
