@@ -228,6 +228,9 @@ struct SharedPlan {
     size_t ws_bytes;
 };
 
+// A launch has fewer than 2^32 threads, and shared_join a wave per row (four to a workgroup).
+constexpr long long kMaxRows = (1LL << 32) / 64 - 4;
+
 bool plan_shared(const cdna4_shared_decode_cfg& c, SharedPlan& p) {
     if (c.D != 64 && c.D != 128) return false;
     if (c.nQHeads < 1 || c.nKVHeads < 1 || c.nQHeads % c.nKVHeads) return false;
@@ -240,7 +243,7 @@ bool plan_shared(const cdna4_shared_decode_cfg& c, SharedPlan& p) {
     p.HB = (p.G + 15) / 16;
     const long long own_rows = (long long)c.batch * c.nKVHeads * p.HB;
     const long long rows = (long long)c.batch * p.G;
-    if (rows > 0x7fffffff - kBlockRows || (long long)c.batch * c.nQHeads > 0x7fffffff) return false;
+    if (rows > 0x7fffffff - kBlockRows || (long long)c.batch * c.nQHeads > kMaxRows) return false;
     p.blocks = (int)((rows + kBlockRows - 1) / kBlockRows);
     // prefix: parts of whole tiles
     p.Pp = 0;

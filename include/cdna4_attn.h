@@ -223,8 +223,8 @@ int cdna3_attn_decode_noalloc(const void* q, const void* K, const void* V, void*
  * initialisation) holds the parts' results; calls that overlap must not share one. A captured call replays
  * on other lengths up to max_own. The plan is sized to the current device, so query the size with the device
  * current that the call will run on. batch == 0: nothing is done.
- * Invalid: D not 64 or 128, nQHeads % nKVHeads != 0, negative sizes, a stride below its rows (0: packed),
- * q/K/V/prefix not 16-byte or o not 4-byte aligned, a missing or small workspace.
+ * Invalid: D not 64 or 128, nQHeads % nKVHeads != 0, negative sizes, 2^26 - 3 rows of q or more, a stride below its
+ * rows (0: packed), q/K/V/prefix not 16-byte or o not 4-byte aligned, a missing or small workspace.
  */
 typedef struct {
     int D;              /* 64 or 128 */
