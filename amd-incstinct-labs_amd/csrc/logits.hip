@@ -184,6 +184,8 @@ int check_logits(const cdna4_logits_args* a, int dtype) {
     if (a->M == 0) return 0;
     const uintptr_t el = dtype == CDNA4_F32 ? 3u : 1u;
     if (!a->logits || !a->out || ((uintptr_t)a->logits & el) || ((uintptr_t)a->out & 3u)) return CDNA4_ERR_INVALID_VALUE;
+    // in place only element by element: workgroups of a row write while others read
+    if (a->logits == a->out && (dtype != CDNA4_F32 || (a->M > 1 && a->logits_stride != a->out_stride))) return CDNA4_ERR_INVALID_VALUE;
     if (a->history && a->history_stride < a->history_max) return CDNA4_ERR_INVALID_VALUE;
     if (a->n_bias > 0 && (!a->bias_ids || !a->bias_values)) return CDNA4_ERR_INVALID_VALUE;
     if (a->mask && a->mask_stride < ((long long)a->V + 31) / 32) return CDNA4_ERR_INVALID_VALUE;

@@ -324,7 +324,8 @@ int cdna3_softmax_rows_f32(const float* X, float* Y, int M, int H, cdna4_stream_
 /* ---- logits for the sampler --------------------------------------------------------
  * No counterpart in the reference (its runtime takes the argmax of the logits as they are). Penalties for
  * repeated tokens, biases and a grammar mask on M rows of V logits (fp32, fp16 or bf16), computed in fp32
- * and written as fp32 (to the logits themselves where those are fp32 and out_stride == logits_stride). With
+ * and written as fp32 (to the logits themselves where those are fp32 and out_stride == logits_stride; out must not
+ * overlap the inputs otherwise). With
  * s whether token j is among the first history_len[m] entries of row m's history and c how many of them from
  * prompt_len[m] on are j:
  *   x = logit;  s: x = x > 0 ? x / repetition[m] : x * repetition[m];
@@ -335,7 +336,8 @@ int cdna3_softmax_rows_f32(const float* X, float* Y, int M, int H, cdna4_stream_
  * biases for one token the last counts. The mask holds token j of row m in bit j % 32 of word
  * mask[m * mask_stride + j / 32] (1: allowed); a row that allows nothing is all -inf. repetition must not be 0.
  * Invalid: V < 1, M < 0 or > 65,535, strides below V (mask: below ceil(V / 32); history: below history_max),
- * history_max negative or above 2^24, n_bias negative or above 8,192, null logits or out, misaligned pointers.
+ * history_max negative or above 2^24, n_bias negative or above 8,192, null logits or out, misaligned pointers, out at
+ * the logits' address with another type or stride.
  */
 typedef struct {
     const void* logits;          /* [M][logits_stride] */

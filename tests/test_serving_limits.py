@@ -3,6 +3,7 @@ anything is launched."""
 import ctypes
 
 import pytest
+import torch
 
 import cdna4
 
@@ -23,3 +24,24 @@ def test_shared_rows_fit_the_join(cfg, fits):
     assert (cdna4.decode_shared_workspace_size(c) > 0) == fits
     if not fits:
         assert cdna4.lib().cdna4_attn_decode_shared(P, P, P, P, P, P, P, ctypes.byref(c), cdna4.F16, P, 1 << 62, None) == 1
+
+
+def logits_args(**kw):
+    a = cdna4.LogitsArgs()
+    a.logits, a.out, a.M, a.V, a.logits_stride, a.out_stride = 64, 64, 3, 100, 100, 100
+    for k, v in kw.items():
+        setattr(a, k, v)
+    return a
+
+
+@pytest.mark.parametrize("dtype,kw,fits", [
+    (cdna4.F32, {}, True), (cdna4.F32, dict(M=1, out_stride=104), True), (cdna4.F32, dict(out_stride=104), False),
+    (cdna4.F16, {}, False), (cdna4.BF16, dict(logits_stride=200), False), (cdna4.F16, dict(out=4096), True),
+])
+def test_logits_in_place(dtype, kw, fits):
+    """Results over the logits themselves only where each lies where its logit was: a workgroup would overwrite what
+    another has yet to read."""
+    if fits and torch.cuda.is_available():
+        pytest.skip("would be launched on these addresses; in place on the GPU: test_gpu_logits.py")
+    rc = cdna4.lib().cdna4_process_logits(ctypes.byref(logits_args(**kw)), dtype, None)
+    assert (rc != 1) == fits      # without a GPU the device check is what refuses a valid call
