@@ -645,7 +645,7 @@ int check_packed(const cdna4_packed_cfg* cfg, const cdna4_packed_strides* st, co
     const long long out[2] = {st->o_row, st->o_head};
     for (long long x : out)
         if (x < 0 || (x & 3)) return CDNA4_ERR_INVALID_VALUE;
-    if (st->q_row < c.D || st->kv_row < c.D || st->o_row < c.D) return CDNA4_ERR_INVALID_VALUE;
+    if (st->q_row < c.D || st->kv_row < c.D || st->o_row < c.D || (c.nQHeads > 1 && st->o_head < c.D)) return CDNA4_ERR_INVALID_VALUE;
     if (c.batch == 0 || c.total == 0) return 0;
     if (!Q || !K || !V || !O || !cu || ((uintptr_t)cu & 3u)) return CDNA4_ERR_INVALID_VALUE;
     if ((((uintptr_t)Q | (uintptr_t)K | (uintptr_t)V) & 15u) || ((uintptr_t)O & 7u)) return CDNA4_ERR_INVALID_VALUE;

@@ -148,7 +148,7 @@ int cdna3_attn_prefill_strided(const void* Q, const void* K, const void* V, void
  * the call will run on.
  * batch == 0 or total == 0: nothing is done. Invalid: D not 64 or 128, nQHeads % nKVHeads != 0, negative
  * sizes, more than 2^20 sequences or 2^30 blocks of queries, max_seq > total, prefix + total near 2^31, stride_prefix (0: prefix) < prefix, Q/K/V strides not a multiple of 8
- * elements, O strides not a multiple of 4, rows shorter than D, Q/K/V/prefix not 16-byte or O not 8-byte
+ * elements, O strides not a multiple of 4, rows shorter than D, heads of O less than D apart, Q/K/V/prefix not 16-byte or O not 8-byte
  * aligned. O must not overlap the inputs.
  */
 typedef struct {

@@ -45,3 +45,14 @@ def test_logits_in_place(dtype, kw, fits):
         pytest.skip("would be launched on these addresses; in place on the GPU: test_gpu_logits.py")
     rc = cdna4.lib().cdna4_process_logits(ctypes.byref(logits_args(**kw)), dtype, None)
     assert (rc != 1) == fits      # without a GPU the device check is what refuses a valid call
+
+
+@pytest.mark.parametrize("heads,o_head,fits", [((8, 4), 64, True), ((8, 4), 60, False), ((8, 4), 0, False), ((1, 1), 0, True)])
+def test_packed_heads_of_the_output_do_not_overlap(heads, o_head, fits):
+    """Heads of O written over each other (an expanded tensor, for instance)."""
+    if fits and torch.cuda.is_available():
+        pytest.skip("would be launched on these addresses")
+    c = cdna4.PackedPrefillCfg(64, *heads, 3, 100, 50, 0, 0)
+    s = cdna4.PackedStrides(512, 64, 256, 64, 512, o_head)
+    rc = cdna4.lib().cdna4_attn_prefill_packed(P, P, P, None, None, P, P, ctypes.byref(c), ctypes.byref(s), cdna4.F16, None, 0, None)
+    assert (rc != 1) == fits
