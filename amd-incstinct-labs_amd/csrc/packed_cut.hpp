@@ -21,8 +21,8 @@ struct Cut { int rounds, tail, each; };   // rounds of whole items before the cu
 // are cut, by estimated times in eighths of a tile's (0.7 us at D = 128): a workgroup that has its CU to itself
 // takes 8 per tile, all that fit it together 13 (two) or 19 (three); the join costs five tiles for its launch and a
 // sixth per part and 64 rows for the results' way through memory (512 parts of 128 rows: 68 MB). Measured at 32/8 heads,
-// D 128, bf16: one sequence of 64 tokens behind 8,192 keys 93 -> 27 us, four of 16 behind 32,768 350 -> 59, ten of
-// 200 behind 8,192 (560 items on 512 workgroups) 369 -> 275; cut all the same, six of 70 behind 2,048 30.5 -> 48.
+// D 128, bf16: one sequence of 64 tokens behind 8,192 keys 93-95 -> 27 us, four of 16 behind 32,768 348-355 -> 56-59, ten of
+// 200 behind 8,192 (560 items on 512 workgroups) 359-369 -> 268-275; cut all the same, six of 70 behind 2,048 30.5 -> 48.
 constexpr Cut cut_items(int items, int G, int tiles, int per_cu, int qt) {
     const int rounds = items / G, tail = items - rounds * G, cus = G / per_cu;
     const int full = per_cu == 2 ? 13 : 19;

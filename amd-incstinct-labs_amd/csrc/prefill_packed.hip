@@ -7,14 +7,20 @@
 // sequence, prefix keys 0 .. P - 1 and then the sequence's own, with no padding where they meet: key k lies
 // in the prefix cache or in the packed rows, and the tile that holds both takes its addresses per lane.
 //
-// Lengths are read on the device (a captured call replays on other lengths): a workgroup finds its item,
-// one block of queries of one sequence and head, from cu alone. Blocks are ordered by their index in the
-// sequence, the last ones (the most keys) first, so that the hardware's in-order dispatch gives the chip a
-// longest-first schedule whatever the lengths are.
+// Lengths are read on the device (a captured call replays on other lengths): a workgroup finds its items,
+// blocks of queries of one sequence and group of heads, from cu alone, or takes them from a list that a launch
+// before it has made (packed_plan.hpp: which way when; packed_cut.hpp: how they are dealt out). Blocks are ordered by their
+// index in the sequence, the last ones (the most keys) first: a longest-first schedule whatever the lengths are.
 //
-// Bound by the matrix cores: four prompts of 2,011-8,192 tokens, 32/8 heads D 128 bf16, 925 us in a graph (1,220 TFLOP/s,
-// matrix cores 65 % busy), 24 of 33-2,048 148 us (865 TFLOP/s: a block's start and end take a quarter of its time), 16 of
-// 90-1,024, 12 heads D 64 fp16, 24 us (the longest block's 16 tiles one after another).
+// A weight is rounded to the inputs' 16-bit type for the P.V product, whose matrix instructions take no wider operand at
+// their rate, and the sum of a row adds the rounded weights, in fp32, so that both sides of the quotient weigh alike.
+// Maxima, sums and O are fp32. Against an fp32 product that costs the relative error of the output, which its own
+// rounding dominates, a factor of 1.0-1.2 in bf16 and 1.2-1.4 in fp16 (0.0016 -> 0.0019, 0.00021 -> 0.00029); bf16 weights
+// of the keys that rows of few keys see carry a second term (attn_tile.hpp, kLoKeys).
+//
+// Bound by the matrix cores: four prompts of 2,011-8,192 tokens, 32/8 heads D 128 bf16, 919-967 us in a graph by machine
+// (1,170-1,230 TFLOP/s, matrix cores 65 % busy), 24 of 33-2,048 145-152 us (840-880 TFLOP/s: a block's start and end take a
+// quarter of its time), 16 of 90-1,024, 12 heads D 64 fp16, 24 us (the longest block's 16 tiles one after another).
 #include <type_traits>
 #include <algorithm>
 

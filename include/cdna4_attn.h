@@ -136,20 +136,20 @@ int cdna3_attn_prefill_strided(const void* Q, const void* K, const void* V, void
  * CDNA4_F16 or CDNA4_BF16; scale 1/sqrt(D), softmax and accumulation in fp32. Rows of O that belong to no
  * sequence (before cu_seqlens[0], behind cu_seqlens[batch]) are left as they are. cu_seqlens entries
  * outside 0 .. total or decreasing read and write nothing outside the tensors; the rows that they name
- * wrongly are not defined. A value in V that is not finite reaches the rows of its sequence's earlier
- * tokens too where they share 32 keys with it (a weight of zero times infinity); K may hold any value there.
+ * wrongly are not defined. A value in V that is not finite reaches rows of up to 62 earlier tokens of its sequence
+ * too, which share a step of 32 queries and 32 keys with it (a weight of zero times infinity); K may hold any value there.
  * max_seq (0: unknown) is the longest sequence; it is checked against total, and no kernel depends on it.
  * With a workspace (cdna4_attn_prefill_packed_workspace_size(cfg) bytes, 16-byte aligned, no initialisation; calls
  * that overlap must not share one) a call of many blocks first lists them, in an order that finds K and V in the L2
  * caches, and its workgroups claim them one by one; a call of few blocks behind a prefix of 1,024 keys and more cuts
  * them along their keys and joins the parts in a second launch. Without one (NULL), or where the size is 0, the blocks
- * are dealt out in a fixed order in one launch: the bits are those of the listed blocks, and differ from the cut ones'
- * by the order of their sums. The plan is sized to the current device, so query the size with the device current that
+ * are dealt out in a fixed order in one launch: the bits are those of the listed blocks, and differ from those of a call
+ * that may cut its blocks in the last places (other sums, and blocks of another size for some sizes). The plan is sized to the current device, so query the size with the device current that
  * the call will run on.
  * batch == 0 or total == 0: nothing is done. Invalid: D not 64 or 128, nQHeads % nKVHeads != 0, negative
- * sizes, more than 2^20 sequences or 2^30 blocks of queries, max_seq > total, prefix + total near 2^31, stride_prefix (0: prefix) < prefix, Q/K/V strides not a multiple of 8
- * elements, O strides not a multiple of 4, rows shorter than D, heads of O less than D apart, Q/K/V/prefix not 16-byte or O not 8-byte
- * aligned. O must not overlap the inputs.
+ * sizes, more than 2^20 sequences or 2^30 blocks of queries, max_seq > total, prefix + total near 2^31,
+ * stride_prefix (0: prefix) < prefix, Q/K/V strides not a multiple of 8 elements, O strides not a multiple of 4, rows
+ * shorter than D, heads of O less than D apart, Q/K/V/prefix not 16-byte or O not 8-byte aligned. O must not overlap the inputs.
  */
 typedef struct {
     int D;              /* 64 or 128 */
