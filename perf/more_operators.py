@@ -285,6 +285,11 @@ def _appended(st):
 
 # ---- plain forms ----------------------------------------------------------------------------------
 
+def _power(e):
+    """2^e in 32 bits, from its bits (pow may be a bit off)."""
+    return (e.int() + 127 << 23).view(torch.float32)
+
+
 def _quantised(x, dtype):
     """(codes, scale bytes) of x in blocks of 32 along its last axis: the smallest power of two 2^e with max|x| < 7 2^e, then the
     nearest of 0, 0.5, 1, 1.5, 2, 3, 4, 6, ties to the even code."""
@@ -292,7 +297,7 @@ def _quantised(x, dtype):
     m, k = torch.frexp(b.abs().amax(-1))
     lo, hi = (-23, 13) if dtype == "f16" else (-125, 125)
     e = torch.where(m == 0, torch.full_like(k, lo), k - 3 + (m >= 0.875).int()).clamp_(lo, hi)
-    y = torch.ldexp(b, -e[..., None].to(b.dtype))
+    y = b * _power(-e)[..., None].to(b.dtype)
     a = y.abs()
     code = ((a > 0.25).to(torch.uint8) + (a >= 0.75) + (a > 1.25) + (a >= 1.75) + (a > 2.5) + (a >= 3.5) + (a > 5)).to(torch.uint8)
     return (code | torch.signbit(y).to(torch.uint8) << 3).flatten(-2), (e + 127).to(torch.uint8)
@@ -303,7 +308,7 @@ def _values(code, scale):
     grid = torch.tensor([0, 0.5, 1, 1.5, 2, 3, 4, 6], device=DEV)
     grid = torch.cat([grid, -grid])
     x = grid[code.int()].unflatten(-1, (-1, 32))
-    return torch.ldexp(x, (scale.float() - 127)[..., None]).flatten(-2)
+    return (x * _power(scale.int() - 127)[..., None]).flatten(-2)
 
 
 def _turned(st, x, weight):
@@ -465,9 +470,9 @@ def _cached(st, name, at):
         nib[..., 0::2], nib[..., 1::2] = byte % 16, byte // 16
         mag = nib % 8
         # 1 bit of fraction under an implicit one, exponents from 2^0 on; below it steps of a half
-        val = torch.where(mag < 2, mag.to(torch.float64) / 2, (1 + (mag % 2).to(torch.float64) / 2) * torch.exp2((mag // 2 - 1).to(torch.float64)))
+        val = torch.where(mag < 2, mag.to(torch.float64) / 2, (1 + (mag % 2).to(torch.float64) / 2) * (1 << (mag // 2 - 1).clamp(min=0)).to(torch.float64))
         val = torch.where(nib >= 8, -val, val)
-        power = torch.exp2(pool[:, :, page * D // 2:].reshape(-1, HK, page, D // 32).to(torch.float64) - 127)
+        power = (pool[:, :, page * D // 2:].reshape(-1, HK, page, D // 32).long() + (1023 - 127) << 52).view(torch.float64)
         pool = val * power.repeat_interleave(32, -1)
     return pool.to(torch.float64).permute(1, 0, 2, 3).reshape(HK, -1, D)
 
@@ -492,10 +497,11 @@ def _exact_append(st):
         def held(x):
             b = x.reshape(*x.shape[:-1], D // 32, 32)
             top = b.abs().amax(-1, keepdim=True)
-            e = torch.ceil(torch.log2(top / 7))
-            e = torch.where(top >= 7 * torch.exp2(e), e + 1, torch.where(top < 7 * torch.exp2(e - 1), e - 1, e))
+            two = lambda e: (e.long() + 1023 << 52).view(torch.float64)
+            e = torch.ceil(torch.log2(top / 7)).clamp(-1000, 1000)
+            e = torch.where(top >= 7 * two(e), e + 1, torch.where(top < 7 * two(e - 1), e - 1, e))
             lo, hi = (-23, 13) if c["dtype"] == "f16" else (-125, 125)
-            s = torch.exp2(e.clamp(lo, hi))
+            s = two(e.clamp(lo, hi))
             y = b.abs() / s
             j = torch.searchsorted(grid, y.contiguous()).clamp(1, 7)                       # grid[j - 1] < y <= grid[j]
             down, up = grid[j - 1], grid[j]
