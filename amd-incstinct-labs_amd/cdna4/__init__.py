@@ -40,7 +40,9 @@ __all__ = [
     "PlanInfo", "prefill_plan", "decode_plan", "scan_status", "KERNEL_NAMES", "decode_noalloc",
     "decode_noalloc_max_bytes", "softmax_rows_f32", "PackedPrefillCfg", "PackedStrides", "prefill_packed",
     "prefill_packed_plan", "prefill_packed_workspace_size", "LogitsArgs", "process_logits", "SharedDecodeCfg",
-    "decode_shared", "decode_shared_plan", "decode_shared_workspace_size",
+    "decode_shared", "decode_shared_plan", "decode_shared_workspace_size", "KV_16BIT", "KV_MXFP4", "PagedCache",
+    "PagedDecodeCfg", "paged_pool_shape", "rope_append_paged", "decode_paged", "decode_paged_workspace_size", "decode_paged_plan",
+    "paged_reorder", "beam_select", "beam_select_workspace_size",
 ]
 
 # Element types and operators (include/cdna4_attn.h).
@@ -114,6 +116,38 @@ class LogitsArgs(ctypes.Structure):
                 ("mask_stride", ctypes.c_longlong)]
 
 
+KV_16BIT, KV_MXFP4 = 0, 1   # formats of a paged cache (CDNA4_KV_*)
+
+
+class PagedCache(ctypes.Structure):
+    """cdna4_paged_cache: pools of `pages` pages of `page` rows (16, 32, .. 256) for each kv head, in 16 bits or MXFP4;
+    tables of max_pages entries per sequence (table_stride apart, 0 = packed)."""
+    _fields_ = [(n, ctypes.c_int) for n in ("D", "nKVHeads", "page", "pages", "format", "max_pages")] + [
+        ("table_stride", ctypes.c_longlong)]
+
+
+class PagedDecodeCfg(ctypes.Structure):
+    """cdna4_paged_decode_cfg: nq queries (1 .. 16) of each of `batch` sequences."""
+    _fields_ = [(n, ctypes.c_int) for n in ("nQHeads", "batch", "nq")]
+
+    def __init__(self, nQHeads=0, batch=0, nq=1):
+        super().__init__(nQHeads, batch, nq)
+
+
+class AppendArgs(ctypes.Structure):
+    """cdna4_append_args: the pointers, sizes and token strides of one cdna4_rope_append_paged call."""
+    _fields_ = [(n, ctypes.c_void_p) for n in ("q", "k", "v", "q_out", "k_out", "v_out", "K_pages", "V_pages", "tables", "seqs",
+                                               "positions", "cos_tab", "sin_tab", "q_norm", "k_norm")] + [
+        ("eps", ctypes.c_double)] + [(n, ctypes.c_int) for n in ("T", "nQHeads", "batch", "max_pos")] + [
+        (n, ctypes.c_longlong) for n in ("q_row", "k_row", "v_row", "q_out_row", "k_out_row", "v_out_row")]
+
+
+class BeamArgs(ctypes.Structure):
+    """cdna4_beam_args: the pointers and sizes of one cdna4_beam_select call."""
+    _fields_ = [(n, ctypes.c_void_p) for n in ("logits", "cum", "done", "scores", "parents", "tokens")] + [
+        (n, ctypes.c_int) for n in ("groups", "beams", "n", "V", "eos")] + [("logits_stride", ctypes.c_longlong)]
+
+
 class ModelCfg(ctypes.Structure):
     """cdna3_model_cfg: the reference's ModelConfig (runtime/model_loader.hpp:52-61) plus the
     qkv_bias flag and the norm kind and epsilon."""
@@ -140,7 +174,7 @@ class PlanInfo(ctypes.Structure):
 
 # CDNA4_KERNEL_* (include/cdna4_attn.h)
 KERNEL_NAMES = {1: "fa_mfma_8w", 2: "fa_mfma_4w", 3: "fa_small", 4: "fa_f32", 5: "decode_split", 6: "decode_wg",
-                7: "fa_mfma_keys", 8: "fa_packed", 9: "decode_shared"}
+                7: "fa_mfma_keys", 8: "fa_packed", 9: "decode_shared", 10: "decode_paged"}
 
 
 def DecodeDmeCfg(D: int, N: int, nQHeads: int, nKVHeads: int, stride_kv: int, batch: int = 1) -> DecodeCfg:
@@ -190,6 +224,14 @@ def _declare(l: ctypes.CDLL) -> None:
         "cdna4_attn_decode_shared": (c_int, [vp] * 7 + [ctypes.POINTER(SharedDecodeCfg), c_int, vp, c_size, vp]),
         "cdna4_attn_decode_shared_plan": (c_int, [ctypes.POINTER(SharedDecodeCfg), c_int, ctypes.POINTER(PlanInfo)]),
         "cdna4_process_logits": (c_int, [ctypes.POINTER(LogitsArgs), c_int, vp]),
+        "cdna4_rope_append_paged": (c_int, [ctypes.POINTER(AppendArgs), ctypes.POINTER(PagedCache), c_int, vp]),
+        "cdna4_attn_decode_paged_workspace_size": (c_size, [ctypes.POINTER(PagedCache), ctypes.POINTER(PagedDecodeCfg)]),
+        "cdna4_attn_decode_paged": (c_int, [vp] * 6 + [ctypes.POINTER(PagedCache), ctypes.POINTER(PagedDecodeCfg), c_int, vp, c_size, vp]),
+        "cdna4_attn_decode_paged_plan": (c_int, [ctypes.POINTER(PagedCache), ctypes.POINTER(PagedDecodeCfg), c_int,
+                                                 ctypes.POINTER(PlanInfo)]),
+        "cdna4_paged_reorder": (c_int, [vp] * 8 + [ctypes.POINTER(PagedCache), c_int, c_int, c_int, ctypes.c_longlong, vp]),
+        "cdna4_beam_select_workspace_size": (c_size, [c_int] * 4),
+        "cdna4_beam_select": (c_int, [ctypes.POINTER(BeamArgs), c_int, vp, c_size, vp]),
         "cdna3_rmsnorm_f32": (c_int, [vp, vp, vp, c_int, c_int, c_float, vp]),
         "cdna3_layernorm_f32": (c_int, [vp, vp, vp, vp, c_int, c_int, c_float, vp]),
         "cdna4_gemm_f16_nt": (c_int, [vp, vp, vp, c_int, c_int, c_int, c_int, c_int, c_int, vp]),
@@ -712,6 +754,191 @@ def process_logits(logits: torch.Tensor, out: Optional[torch.Tensor] = None, *,
     rc = lib().cdna4_process_logits(ctypes.byref(a), dt, torch._C._cuda_getCurrentRawStream(dev))
     if rc:
         raise CDNA4Error("cdna4_process_logits", rc)
+    return out
+
+
+# ---- paged KV cache and beams -----------------------------------------------------------------
+
+def paged_pool_shape(cache: PagedCache) -> tuple:
+    """Shape of one layer's K (or V) pool: [pages][nKVHeads][page][D] of 16-bit elements, or, MXFP4, of bytes, a page's rows
+    of one head as codes, then scales."""
+    if cache.format == KV_MXFP4:
+        return (cache.pages, cache.nKVHeads, cache.page * (cache.D // 2 + cache.D // 32))
+    return (cache.pages, cache.nKVHeads, cache.page, cache.D)
+
+
+def _pools(K: torch.Tensor, V: torch.Tensor, cache: PagedCache, dtype, dev: int, layers: int = 1):
+    n = layers * cache.pages * cache.nKVHeads * cache.page
+    if cache.format == KV_MXFP4:
+        dtype, n = torch.uint8, n * (cache.D // 2 + cache.D // 32)
+    else:
+        n *= cache.D
+    return _arg("K_pages", K, dtype, n, dev), _arg("V_pages", V, dtype, n, dev)
+
+
+def _table_size(cache: PagedCache, rows: int) -> int:
+    """Entries that the tables of `rows` sequences span."""
+    return (rows - 1) * (cache.table_stride or cache.max_pages) + cache.max_pages if rows > 0 else 0
+
+
+def rope_append_paged(q: Optional[torch.Tensor], k: torch.Tensor, v: torch.Tensor, K_pages: torch.Tensor, V_pages: torch.Tensor,
+                      tables: torch.Tensor, positions: torch.Tensor, cache: PagedCache, q_out: Optional[torch.Tensor] = None, *,
+                      seqs: Optional[torch.Tensor] = None, cos: Optional[torch.Tensor] = None, sin: Optional[torch.Tensor] = None,
+                      q_norm: Optional[torch.Tensor] = None, k_norm: Optional[torch.Tensor] = None, eps: float = 1e-6,
+                      k_out: Optional[torch.Tensor] = None, v_out: Optional[torch.Tensor] = None, stream=None) -> Optional[torch.Tensor]:
+    """T tokens' projections q [T][nQH][D], k, v [T][nKVH][D] (fp16 or bf16, any token stride with contiguous heads: parts of one
+    projection's output) into a paged cache: queries and keys normed per head (q_norm, k_norm [D], optional) and rotated
+    (cos, sin fp32 [max_pos][D], optional), keys and values to row positions[t] of sequence seqs[t] (int32 [T]; seqs None: t), queries to
+    q_out (None: allocated), which is returned. k_out, v_out [T][nKVH][D], optional: what the cache now holds for the
+    tokens. tables int32 [batch][max_pages]. Padding tokens have a position or a sequence of -1. q None: keys and values
+    alone. The formulas: cdna4_rope_append_paged in cdna4_attn.h."""
+    dev, dtype = _gpu_of(k), k.dtype
+    if _elsewhere(dev, stream):
+        with _entered(dev, stream):
+            return rope_append_paged(q, k, v, K_pages, V_pages, tables, positions, cache, q_out, seqs=seqs, cos=cos, sin=sin,
+                                     q_norm=q_norm, k_norm=k_norm, eps=eps, k_out=k_out, v_out=v_out)
+    dt = _dtype(k)
+    T, HK, D = k.shape[0], cache.nKVHeads, cache.D
+
+    def rows(name, t, heads):
+        if t is None:
+            return 0, 0
+        if t.dtype is not dtype or t.get_device() != dev or t.shape[0] != T:
+            raise ValueError(f"{name} must have the dtype, GPU and tokens of k")
+        row, head = _token_major(name, t, T, heads, D)
+        if head != D:
+            raise ValueError(f"{name} must have its heads side by side")
+        return t.data_ptr(), row
+
+    HQ = 0
+    if q is not None:
+        HQ = q.shape[1] if q.dim() == 3 else 0
+        if q_out is None:
+            q_out = torch.empty((T, HQ, D), dtype=dtype, device=k.device)
+    elif q_out is not None or q_norm is not None:
+        raise ValueError("q_out and q_norm need q")
+    (qp, qr), (kp, kr), (vp, vr) = rows("q", q, HQ), rows("k", k, HK), rows("v", v, HK)
+    (qo, qor), (ko, kor), (vo, vor) = rows("q_out", q_out, HQ), rows("k_out", k_out, HK), rows("v_out", v_out, HK)
+    Kp, Vp = _pools(K_pages, V_pages, cache, dtype, dev)
+    batch = tables.shape[0] if tables.dim() == 2 else 0
+    if seqs is None and batch < T:
+        raise ValueError("without seqs there must be a table for every token")
+    max_pos = c = s = 0
+    if cos is not None or sin is not None:
+        max_pos = cos.shape[0] if cos is not None else 0
+        c, s = _arg("cos", cos, _F32, max_pos * D, dev), _arg("sin", sin, _F32, max_pos * D, dev)
+        if cos.shape[-1] != D or max_pos * D == 0:
+            raise ValueError("cos and sin must be [max_pos][D]")
+    a = AppendArgs(qp, kp, vp, qo, ko, vo, Kp, Vp, _arg("tables", tables, _I32, _table_size(cache, batch), dev),
+                   0 if seqs is None else _arg("seqs", seqs, _I32, T, dev), _arg("positions", positions, _I32, T, dev), c, s,
+                   0 if q_norm is None else _arg("q_norm", q_norm, dtype, D, dev),
+                   0 if k_norm is None else _arg("k_norm", k_norm, dtype, D, dev), eps, T, HQ, batch, max_pos, qr, kr, vr, qor, kor, vor)
+    rc = lib().cdna4_rope_append_paged(ctypes.byref(a), ctypes.byref(cache), dt, torch._C._cuda_getCurrentRawStream(dev))
+    if rc:
+        raise CDNA4Error("cdna4_rope_append_paged", rc)
+    return q_out
+
+
+def decode_paged_workspace_size(cache: PagedCache, cfg: PagedDecodeCfg) -> int:
+    return int(lib().cdna4_attn_decode_paged_workspace_size(ctypes.byref(cache), ctypes.byref(cfg)))
+
+
+def decode_paged(q: torch.Tensor, K_pages: torch.Tensor, V_pages: torch.Tensor, tables: torch.Tensor, lens: torch.Tensor,
+                 o: torch.Tensor, cache: PagedCache, cfg: PagedDecodeCfg, workspace="auto", stream=None) -> None:
+    """The queries of each sequence's last nq tokens over its rows of a paged cache: q, o [batch][nq][nQH][D] (fp16 or bf16, also
+    the type of a 16-bit cache); tables int32 [batch][max_pages], lens int32 [batch] (rows, the new tokens' among them) on the device.
+    `workspace`: "auto" allocates decode_paged_workspace_size(cache, cfg) bytes on the stream the call launches on; a uint8 tensor is
+    used as given."""
+    dev, dtype = _gpu_of(q), q.dtype
+    if _elsewhere(dev, stream):
+        with _entered(dev, stream):
+            return decode_paged(q, K_pages, V_pages, tables, lens, o, cache, cfg, workspace)
+    dt, B = _dtype(q), cfg.batch
+    n = B * cfg.nq * cfg.nQHeads * cache.D
+    qp, op = _arg("q", q, dtype, n, dev), _arg("o", o, dtype, n, dev)
+    Kp, Vp = _pools(K_pages, V_pages, cache, dtype, dev)
+    tp, lp = _arg("tables", tables, _I32, _table_size(cache, B), dev), _arg("lens", lens, _I32, B, dev)
+    if workspace is None or (isinstance(workspace, str) and workspace != "auto"):
+        raise ValueError("workspace must be 'auto' or a uint8 tensor")
+    if isinstance(workspace, str):
+        workspace = torch.empty(max(1, decode_paged_workspace_size(cache, cfg)), dtype=torch.uint8, device=q.device)
+    rc = lib().cdna4_attn_decode_paged(qp, Kp, Vp, tp, lp, op, ctypes.byref(cache), ctypes.byref(cfg), dt,
+                                       _arg("workspace", workspace, torch.uint8, 0, dev), workspace.numel(),
+                                       torch._C._cuda_getCurrentRawStream(dev))
+    if rc:
+        raise CDNA4Error("cdna4_attn_decode_paged", rc)
+
+
+def decode_paged_plan(cache: PagedCache, cfg: PagedDecodeCfg, dtype=F16) -> PlanInfo:
+    """The kernels cdna4_attn_decode_paged would launch on the current device."""
+    if isinstance(dtype, torch.dtype):
+        dtype = _TORCH_DTYPES[dtype]
+    out = PlanInfo()
+    _check(lib().cdna4_attn_decode_paged_plan(ctypes.byref(cache), ctypes.byref(cfg), dtype, ctypes.byref(out)),
+           "cdna4_attn_decode_paged_plan")
+    return out
+
+
+def paged_reorder(parents: torch.Tensor, tables: torch.Tensor, lens: torch.Tensor, fresh: torch.Tensor, tables_out: torch.Tensor,
+                  lens_out: torch.Tensor, K_pages: torch.Tensor, V_pages: torch.Tensor, cache: PagedCache, stream=None) -> None:
+    """The cache after beam_select: row i goes on from row parents[i] (int32; -1: unused). tables, tables_out int32 [rows][max_pages],
+    lens, lens_out int32 [rows]; a last page that is not full is copied to page fresh[i] (int32) in K and V of every layer. K_pages,
+    V_pages: one layer's pools, or those of several layers in one tensor (a dimension more)."""
+    dev = _gpu_of(parents)
+    if _elsewhere(dev, stream):
+        with _entered(dev, stream):
+            return paged_reorder(parents, tables, lens, fresh, tables_out, lens_out, K_pages, V_pages, cache)
+    rows, rows_in = parents.numel(), tables.shape[0]
+    layers = K_pages.shape[0] if K_pages.dim() == len(paged_pool_shape(cache)) + 1 else 1
+    dtype = K_pages.dtype
+    if cache.format != KV_MXFP4 and dtype not in (torch.float16, torch.bfloat16):
+        raise ValueError("pools must be fp16 or bf16")
+    Kp, Vp = _pools(K_pages, V_pages, cache, dtype, dev, layers)
+    rc = lib().cdna4_paged_reorder(_arg("parents", parents, _I32, rows, dev), _arg("tables", tables, _I32, _table_size(cache, rows_in), dev),
+                                   _arg("lens", lens, _I32, rows_in, dev), _arg("fresh", fresh, _I32, rows, dev),
+                                   _arg("tables_out", tables_out, _I32, _table_size(cache, rows), dev),
+                                   _arg("lens_out", lens_out, _I32, rows, dev), Kp, Vp, ctypes.byref(cache), rows, rows_in, layers, 0,
+                                   torch._C._cuda_getCurrentRawStream(dev))
+    if rc:
+        raise CDNA4Error("cdna4_paged_reorder", rc)
+
+
+def beam_select_workspace_size(rows: int, V: int, beams: int, n: int) -> int:
+    return int(lib().cdna4_beam_select_workspace_size(rows, V, beams, n))
+
+
+def beam_select(logits: torch.Tensor, cum: torch.Tensor, beams: int, n: Optional[int] = None, *, done: Optional[torch.Tensor] = None,
+                eos: int = -1, out=None, workspace="auto", stream=None):
+    """The n (default: beams) best continuations of each group of `beams` rows of logits [rows][V] (fp32, fp16 or bf16; rows may be apart)
+    by cum[row] + log softmax, cum fp32 [rows]: (scores fp32, parents int32, tokens int32), each [rows / beams][n], best first; into
+    `out` if given. done int32 [rows], optional: rows that have ended and go on with `eos` alone. Places that nothing fills: -inf, -1,
+    -1. The rules: cdna4_beam_select in cdna4_attn.h."""
+    dev = _gpu_of(logits)
+    if _elsewhere(dev, stream):
+        with _entered(dev, stream):
+            return beam_select(logits, cum, beams, n, done=done, eos=eos, out=out, workspace=workspace)
+    dt = _dtype(logits)
+    M, V = logits.shape if logits.dim() == 2 else (-1, 0)
+    n = beams if n is None else n
+    if M < 0 or beams < 1 or M % beams or n < 1:
+        raise ValueError("logits must be [groups * beams][V]")
+    row, one = logits.stride()
+    if one != 1 and M and V > 1:
+        raise ValueError("logits must have contiguous rows")
+    G = M // beams
+    if out is None:
+        out = tuple(torch.empty((G, n), dtype=d, device=logits.device) for d in (_F32, _I32, _I32))
+    if isinstance(workspace, str) and workspace == "auto":
+        workspace = torch.empty(max(1, beam_select_workspace_size(M, V, beams, n)), dtype=torch.uint8, device=logits.device)
+    elif workspace is None or isinstance(workspace, str):
+        raise ValueError("workspace must be 'auto' or a uint8 tensor")
+    a = BeamArgs(logits.data_ptr(), _arg("cum", cum, _F32, M, dev), 0 if done is None else _arg("done", done, _I32, M, dev),
+                 _arg("scores", out[0], _F32, G * n, dev), _arg("parents", out[1], _I32, G * n, dev), _arg("tokens", out[2], _I32, G * n, dev),
+                 G, beams, n, V, eos, row if M > 1 else V)
+    rc = lib().cdna4_beam_select(ctypes.byref(a), dt, _arg("workspace", workspace, torch.uint8, 0, dev), workspace.numel(),
+                                 torch._C._cuda_getCurrentRawStream(dev))
+    if rc:
+        raise CDNA4Error("cdna4_beam_select", rc)
     return out
 
 

@@ -1,0 +1,273 @@
+// Beam search's selection (gfx950): the n best continuations of each group of beams over beams x vocabulary.
+//
+//   score = cum[row] + x_v - log sum_u e^(x_u) = cum[row] + (x_v - M) - log S,  M = max x, S = sum_u e^(x_u - M)
+//
+// Within a row the order of the scores is that of the logits, so one pass over them finds both a row's (M, S) and its n best.
+// Launch 1: a wave takes a range of a row. Its lanes hold the running (m, s) of what they read, and the range's best keys so
+// far sorted over the lanes (n <= 64), key = (logit's order, lowest token first) in 64 bits. What is above the n-th best key of
+// the list, or of a first bound for it, is inserted one by one, which random logits need about n ln(range / n) times.
+// Launch 2: a workgroup takes a group: (M, S) and the n best of each row from its ranges, scores in fp64, the n best of those.
+#include <algorithm>
+#include <math.h>
+
+#include "common.hpp"
+#include "wave_primitives/detail/xlane.hpp"
+
+namespace cdna4 {
+namespace {
+
+using wave::xlane::allreduce;
+using wave::xlane::Max;
+using wave::xlane::Sum;
+
+typedef uint32_t u32x2_u __attribute__((ext_vector_type(2), aligned(2)));   // rows of odd length start anywhere
+typedef float f32x4_u __attribute__((ext_vector_type(4), aligned(4)));
+
+constexpr int kMost = 64;      // beams of a group, continuations of a group
+constexpr int kVec = 4;        // logits per load of a lane
+constexpr int kUnroll = 4;     // loads of a lane in flight
+constexpr int kStep = 64 * kVec * kUnroll;   // logits of a wave at a time
+constexpr float kLowest = -3.402823466e38f, kLargest = 3.402823466e38f;
+
+struct RangeSum { double s; float m; int pad; };   // sum of e^(x - m) over a range
+
+struct BeamArgs {
+    cdna4_beam_args p;
+    int parts, range;        // ranges of a row, logits of a range (a multiple of 4)
+    uint64_t* keys;          // [rows][parts][n], 0: none
+    RangeSum* sums;          // [rows][parts]
+};
+
+// A finite float's order as an unsigned number above 0, and back.
+__device__ __forceinline__ uint32_t order_of(float x) {
+    const uint32_t b = __builtin_bit_cast(uint32_t, x);
+    return b ^ (b >> 31 ? 0xffffffffu : 0x80000000u);
+}
+__device__ __forceinline__ float of_order(uint32_t o) {
+    return f32_from_bits(o ^ (o >> 31 ? 0x80000000u : 0xffffffffu));
+}
+__device__ __forceinline__ uint64_t key_of(float x, int token) {
+    // -0 and 0 are one value
+    return (uint64_t)order_of(x + 0.f) << 32 | (uint32_t)~token;
+}
+
+__device__ __forceinline__ uint64_t read_lane(uint64_t v, int lane) {
+    const uint32_t lo = (uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)v, lane);
+    const uint32_t hi = (uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)(v >> 32), lane);
+    return (uint64_t)hi << 32 | lo;
+}
+
+// The list's lanes hold keys in descending order; a new key takes its place and moves those below by one.
+__device__ __forceinline__ uint64_t insert(uint64_t list, uint64_t key, int lane) {
+    const int at = __popcll(__builtin_amdgcn_ballot_w64(list > key));
+    const uint64_t up = __shfl_up((unsigned long long)list, 1);
+    return lane < at ? list : lane == at ? key : up;
+}
+
+__device__ __forceinline__ float logit(const cdna4_beam_args& p, int dtype, size_t at) {
+    if (dtype == CDNA4_F32) return ((const float*)p.logits)[at];
+    const uint32_t b = ((const uint16_t*)p.logits)[at];
+    return dtype == CDNA4_BF16 ? bf16_bits_to_f32(b) : f16_bits_to_f32(b);
+}
+
+// NaN as -inf, +inf as the largest value.
+__device__ __forceinline__ float cleaned(float x) { return x != x ? -INFINITY : fminf(x, kLargest); }
+
+__device__ __forceinline__ bool has_own(const cdna4_beam_args& p, int row) {   // continuations from its logits
+    const float c = p.cum[row];
+    return !(p.done && p.done[row]) && c > -INFINITY && c < INFINITY;
+}
+
+// e^d for d <= 0: v_exp_f32 of d log2(e) with the product's second term, so that a bias of the constant stays out of the sums.
+__device__ __forceinline__ float exp_of(float d) {
+    constexpr float kHi = 1.44269502f, kLo = 1.92596303e-8f;
+    return __builtin_amdgcn_exp2f(fmaf(d, kHi, d * kLo));
+}
+
+template <int kDtype>
+__global__ __launch_bounds__(256) void beam_ranges(BeamArgs a) {
+    const int lane = (int)(threadIdx.x & 63u);
+    const long long item = (long long)blockIdx.x * 4 + __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
+    const int row = (int)(item / a.parts), part = (int)(item % a.parts);
+    if (row >= a.p.groups * a.p.beams || !has_own(a.p, row)) return;
+    const int n = a.p.n, begin = part * a.range, len = min(a.range, a.p.V - begin);
+    const size_t base = (size_t)row * a.p.logits_stride + begin;
+    float m = kLowest, s = 0.f;
+    uint64_t list = 0;
+    for (int i0 = 0; i0 < len; i0 += kStep) {
+        float x[kUnroll * kVec];
+#pragma unroll
+        for (int u = 0; u < kUnroll; ++u) {
+            const int i = i0 + (u * 64 + lane) * kVec;
+#pragma unroll
+            for (int e = 0; e < kVec; ++e) x[u * kVec + e] = i + e < len ? cleaned(logit(a.p, kDtype, base + i + e)) : -INFINITY;
+        }
+        float top = x[0];
+#pragma unroll
+        for (int k = 1; k < kUnroll * kVec; ++k) top = fmaxf(top, x[k]);
+        if (top > m) {
+            s *= exp_of(m - top);
+            m = top;
+        }
+#pragma unroll
+        for (int k = 0; k < kUnroll * kVec; ++k) s += exp_of(x[k] - m);
+#pragma unroll
+        for (int k = 0; k < kUnroll * kVec; ++k) {
+            const int token = begin + i0 + ((k / kVec) * 64 + lane) * kVec + k % kVec;
+            const uint64_t key = x[k] > -INFINITY ? key_of(x[k], token) : 0;
+            uint64_t need = __builtin_amdgcn_ballot_w64(key > read_lane(list, n - 1));
+            while (need) {
+                const uint64_t c = read_lane(key, __builtin_ctzll(need));
+                if (c > read_lane(list, n - 1)) list = insert(list, c, lane);
+                need &= need - 1;
+            }
+        }
+    }
+    const float M = allreduce(m, Max{});
+    const double S = allreduce((double)s * (double)exp_of(m - M), Sum{});
+    if (lane < n) a.keys[((size_t)row * a.parts + part) * n + lane] = list;
+    if (lane == 0) a.sums[(size_t)row * a.parts + part] = RangeSum{S, M, 0};
+}
+
+// Candidate i of a group, row i / n: by score, then lowest row, then lowest token.
+__device__ __forceinline__ bool before(double sx, int rx, int tx, double sy, int ry, int ty) {
+    if (sx != sy) return sx > sy;
+    return rx != ry ? rx < ry : tx < ty;
+}
+
+__global__ __launch_bounds__(1024) void beam_join(BeamArgs a) {
+    __shared__ double score[kMost * kMost];
+    __shared__ int token[kMost * kMost];   // -1: none
+    __shared__ int filled;
+    const int lane = (int)(threadIdx.x & 63u), wave = __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
+    const int waves = (int)blockDim.x >> 6, n = a.p.n, beams = a.p.beams, row0 = (int)blockIdx.x * beams;
+    if (threadIdx.x == 0) filled = 0;
+    for (int b = wave; b < beams; b += waves) {
+        const int row = row0 + b;
+        const float cum = a.p.cum[row];
+        double sc = -INFINITY;
+        int tok = -1;
+        if (a.p.done && a.p.done[row]) {
+            if (lane == 0 && cum > -INFINITY && cum < INFINITY) {
+                sc = cum;
+                tok = a.p.eos;
+            }
+        } else if (has_own(a.p, row)) {
+            float M = kLowest;
+            for (int i = lane; i < a.parts; i += 64) M = fmaxf(M, a.sums[(size_t)row * a.parts + i].m);
+            M = allreduce(M, Max{});
+            double S = 0.0;
+            for (int i = lane; i < a.parts; i += 64) {
+                const RangeSum r = a.sums[(size_t)row * a.parts + i];
+                S += r.s * exp((double)r.m - (double)M);
+            }
+            S = allreduce(S, Sum{});
+            uint64_t list = 0;
+            const uint64_t* keys = a.keys + (size_t)row * a.parts * n;
+            for (int i0 = 0; i0 < a.parts * n; i0 += 64) {
+                const uint64_t key = i0 + lane < a.parts * n ? keys[i0 + lane] : 0;
+                uint64_t need = __builtin_amdgcn_ballot_w64(key > read_lane(list, n - 1));
+                while (need) {
+                    const uint64_t k = read_lane(key, __builtin_ctzll(need));
+                    if (k > read_lane(list, n - 1)) list = insert(list, k, lane);
+                    need &= need - 1;
+                }
+            }
+            if (list) {
+                sc = (double)cum + ((double)of_order((uint32_t)(list >> 32)) - (double)M) - log(S);
+                tok = (int)~(uint32_t)list;
+            }
+        }
+        if (lane < n) {
+            score[b * n + lane] = sc;
+            token[b * n + lane] = tok;
+        }
+    }
+    __syncthreads();
+    const int all = beams * n;
+    int mine = 0;
+    for (int i = (int)threadIdx.x; i < all; i += (int)blockDim.x) {
+        if (token[i] < 0) continue;
+        ++mine;
+        int rank = 0;
+        for (int j = 0; j < all && rank < n; ++j) rank += token[j] >= 0 && before(score[j], j / n, token[j], score[i], i / n, token[i]) ? 1 : 0;
+        if (rank < n) {
+            const size_t at = (size_t)blockIdx.x * n + rank;
+            a.p.scores[at] = (float)score[i];
+            a.p.parents[at] = row0 + i / n;
+            a.p.tokens[at] = token[i];
+        }
+    }
+    if (mine) atomicAdd(&filled, mine);
+    __syncthreads();
+    for (int i = filled + (int)threadIdx.x; i < n; i += (int)blockDim.x) {   // places that nothing fills
+        const size_t at = (size_t)blockIdx.x * n + i;
+        a.p.scores[at] = -INFINITY;
+        a.p.parents[at] = -1;
+        a.p.tokens[at] = -1;
+    }
+}
+
+// Ranges of a row: enough of them for eight waves per CU, none shorter than a wave's step.
+struct BeamPlan { int parts, range; size_t ws_bytes; };
+
+bool plan_beam(long long rows, int V, int beams, int n, BeamPlan& p) {
+    if (rows < 0 || rows >= 1 << 24 || V < 1 || V > 0x7fffffff - 65536 || beams < 1 || beams > kMost || n < 1 || n > kMost) return false;
+    const long long waves = 8LL * device_cus();
+    const long long want = rows ? std::max(1LL, waves / rows) : 1;
+    long long range = std::max((V + want - 1) / want, (long long)kStep);
+    range = (range + 3) & ~3LL;
+    p.range = (int)range;
+    p.parts = (int)((V + range - 1) / range);
+    p.ws_bytes = (size_t)rows * p.parts * (n * sizeof(uint64_t) + sizeof(RangeSum)) + 16;
+    return (rows * p.parts + 3) / 4 * 256 <= 0xffffffffLL;
+}
+
+int check_beam(const cdna4_beam_args* a, int dtype) {
+    if (!a) return CDNA4_ERR_INVALID_VALUE;
+    if (dtype != CDNA4_F32 && dtype != CDNA4_F16 && dtype != CDNA4_BF16) return CDNA4_ERR_INVALID_VALUE;
+    if (a->groups < 0 || a->logits_stride < a->V) return CDNA4_ERR_INVALID_VALUE;
+    if (a->done && (a->eos < 0 || a->eos >= a->V)) return CDNA4_ERR_INVALID_VALUE;
+    if (a->groups == 0) return 0;
+    const uintptr_t el = dtype == CDNA4_F32 ? 3u : 1u;
+    if (!a->logits || ((uintptr_t)a->logits & el)) return CDNA4_ERR_INVALID_VALUE;
+    const void* words[5] = {a->cum, a->scores, a->parents, a->tokens, a->done};
+    for (int i = 0; i < 5; ++i)
+        if ((i < 4 && !words[i]) || ((uintptr_t)words[i] & 3u)) return CDNA4_ERR_INVALID_VALUE;
+    return 0;
+}
+
+}  // namespace
+}  // namespace cdna4
+
+using namespace cdna4;
+
+extern "C" size_t cdna4_beam_select_workspace_size(int rows, int V, int beams, int n) {
+    BeamPlan p;
+    return plan_beam(rows, V, beams, n, p) ? p.ws_bytes : 0;
+}
+
+extern "C" int cdna4_beam_select(const cdna4_beam_args* args, int dtype, void* workspace, size_t ws_bytes, cdna4_stream_t stream) {
+    if (int e = check_beam(args, dtype)) return e;
+    const cdna4_beam_args& p = *args;
+    BeamPlan plan;
+    if (!plan_beam((long long)p.groups * p.beams, p.V, p.beams, p.n, plan)) return CDNA4_ERR_INVALID_VALUE;
+    if (p.groups == 0) return 0;
+    if (!workspace || ((uintptr_t)workspace & 15u) || ws_bytes < plan.ws_bytes) return CDNA4_ERR_INVALID_VALUE;
+    if (int e = check_device()) return e;
+    hipStream_t s = (hipStream_t)stream;
+    BeamArgs a;
+    a.p = p;
+    a.parts = plan.parts;
+    a.range = plan.range;
+    a.sums = (RangeSum*)workspace;
+    a.keys = (uint64_t*)(a.sums + (size_t)p.groups * p.beams * plan.parts);
+    const unsigned grid = ceil_div((size_t)p.groups * p.beams * plan.parts, 4);
+    if (dtype == CDNA4_F32) beam_ranges<CDNA4_F32><<<grid, 256, 0, s>>>(a);
+    else if (dtype == CDNA4_BF16) beam_ranges<CDNA4_BF16><<<grid, 256, 0, s>>>(a);
+    else beam_ranges<CDNA4_F16><<<grid, 256, 0, s>>>(a);
+    if (int e = launch_status()) return e;
+    const int waves = std::min(16, p.beams);
+    beam_join<<<(unsigned)p.groups, 64 * waves, 0, s>>>(a);
+    return launch_status();
+}

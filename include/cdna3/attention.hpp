@@ -167,6 +167,26 @@ inline hipError_t decode_shared(const __hip_bfloat16* q, const __hip_bfloat16* K
                                                 (cdna4_stream_t)stream);
 }
 
+// New: decode over a paged KV cache (cdna4_attn_decode_paged): q, o [batch][nq][nQH][D], pools of pages in the 16-bit type of q or in
+// MXFP4 (PagedCache::format), tables and lens in device memory; a workspace of decode_paged_workspace_size(cache, cfg) bytes.
+using PagedCache = cdna4_paged_cache;
+using PagedDecodeCfg = cdna4_paged_decode_cfg;
+inline size_t decode_paged_workspace_size(const PagedCache& cache, const PagedDecodeCfg& cfg) {
+    return cdna4_attn_decode_paged_workspace_size(&cache, &cfg);
+}
+inline hipError_t decode_paged(const __half* q, const void* K_pages, const void* V_pages, const int* tables, const int* lens,
+                               __half* o, const PagedCache& cache, const PagedDecodeCfg& cfg, void* workspace, size_t ws_bytes,
+                               hipStream_t stream = nullptr) {
+    return (hipError_t)cdna4_attn_decode_paged(q, K_pages, V_pages, tables, lens, o, &cache, &cfg, CDNA4_F16, workspace, ws_bytes,
+                                               (cdna4_stream_t)stream);
+}
+inline hipError_t decode_paged(const __hip_bfloat16* q, const void* K_pages, const void* V_pages, const int* tables,
+                               const int* lens, __hip_bfloat16* o, const PagedCache& cache, const PagedDecodeCfg& cfg,
+                               void* workspace, size_t ws_bytes, hipStream_t stream = nullptr) {
+    return (hipError_t)cdna4_attn_decode_paged(q, K_pages, V_pages, tables, lens, o, &cache, &cfg, CDNA4_BF16, workspace, ws_bytes,
+                                               (cdna4_stream_t)stream);
+}
+
 }  // namespace attn
 }  // namespace cdna3
 

@@ -74,5 +74,25 @@ inline hipError_t rope_append_kv_f16(const __half* q, const __half* k, const __h
                                                 max_seq, (cdna4_stream_t)stream);
 }
 
+// New: the paged KV cache's writers and beam search's selection (cdna4_rope_append_paged, cdna4_paged_reorder, cdna4_beam_select).
+using PagedCache = cdna4_paged_cache;
+using AppendArgs = cdna4_append_args;
+using BeamArgs = cdna4_beam_args;
+inline hipError_t rope_append_paged(const AppendArgs& args, const PagedCache& cache, int dtype, hipStream_t stream = nullptr) {
+    return (hipError_t)cdna4_rope_append_paged(&args, &cache, dtype, (cdna4_stream_t)stream);
+}
+inline hipError_t paged_reorder(const int* parents, const int* tables, const int* lens, const int* fresh, int* tables_out,
+                                int* lens_out, void* K_pages, void* V_pages, const PagedCache& cache, int rows, int rows_in,
+                                int layers = 1, long long layer_stride = 0, hipStream_t stream = nullptr) {
+    return (hipError_t)cdna4_paged_reorder(parents, tables, lens, fresh, tables_out, lens_out, K_pages, V_pages, &cache, rows,
+                                           rows_in, layers, layer_stride, (cdna4_stream_t)stream);
+}
+inline size_t beam_select_workspace_size(int rows, int V, int beams, int n) {
+    return cdna4_beam_select_workspace_size(rows, V, beams, n);
+}
+inline hipError_t beam_select(const BeamArgs& args, int dtype, void* workspace, size_t ws_bytes, hipStream_t stream = nullptr) {
+    return (hipError_t)cdna4_beam_select(&args, dtype, workspace, ws_bytes, (cdna4_stream_t)stream);
+}
+
 }  // namespace runtime
 }  // namespace cdna3

@@ -259,7 +259,8 @@ enum {
                                           split over 2, 4 or 8 groups of waves */
     CDNA4_KERNEL_PACKED = 8,           /* fa_packed: 4 waves x 32 or 16 queries, `rows` tokens of 128 / rows or 64 /
                                           rows query heads */
-    CDNA4_KERNEL_DECODE_SHARED = 9     /* shared_parts + shared_join */
+    CDNA4_KERNEL_DECODE_SHARED = 9,    /* shared_parts + shared_join */
+    CDNA4_KERNEL_DECODE_PAGED = 10     /* paged_parts + paged_join */
 };
 
 typedef struct {
@@ -358,6 +359,130 @@ typedef struct {
 } cdna4_logits_args;
 
 int cdna4_process_logits(const cdna4_logits_args* args, int dtype, cdna4_stream_t stream);
+
+/* ---- paged KV cache ------------------------------------------------------------------
+ * No counterpart in the reference, whose cache is one slot per layer (cdna3-prims/include/cdna3/runtime/kv_cache.hpp:19-52).
+ * The cache of one layer is two pools, K and V, of `pages` pages of `page` rows; row j of sequence b lies in row j % page
+ * of page tables[b * table_stride + j / page] (int32, device memory, read when a kernel runs). Formats:
+ *   CDNA4_KV_16     [pages][nKVHeads][page][D] fp16 or bf16, the type of the call
+ *   CDNA4_KV_MXFP4  [pages][nKVHeads][page * (D / 2 + D / 32)] bytes: the page's rows of one head as 4-bit codes (element 2 i in the
+ *                   low half of byte i), then their scales, a byte for each 32 elements of a row. A code is sign and magnitude
+ *                   0, 0.5, 1, 1.5, 2, 3, 4, 6, a scale byte x is 2^(x - 127), 255: the block's 32 values are NaN.
+ * Pages may be shared by sequences (a common prompt). Invalid for every call: D not 64 or 128, page not 16, 32, 64, 128 or 256,
+ * sizes below 1, max_pages * page of 2^31 - 1024 rows and more, table_stride below max_pages, an unknown format, pools not 16-byte
+ * aligned.
+ */
+enum { CDNA4_KV_16 = 0, CDNA4_KV_MXFP4 = 1 };
+
+typedef struct {
+    int D;                   /* 64 or 128 */
+    int nKVHeads;
+    int page;                /* rows per page: 16, 32, 64, 128 or 256 */
+    int pages;               /* pages of a pool */
+    int format;              /* CDNA4_KV_* */
+    int max_pages;           /* table entries of a sequence that may be read */
+    long long table_stride;  /* entries between the tables of two sequences, 0 = max_pages */
+} cdna4_paged_cache;
+
+/* cdna4_rope_append_paged: T tokens' projections made ready and put into the cache, in one launch. Token t belongs to sequence seqs[t]
+ * (NULL: t), at row positions[t]. Queries and keys of each head are normed, x rsqrt(mean(x^2) + eps) w, where q_norm (k_norm) [D]
+ * is given, then rotated in halves (d, d + D/2) by row positions[t] of cos_tab, sin_tab [max_pos][D] (cdna3_rope_table_f32)
+ * where those are given; keys and values go to their places in the pools, queries to q_out, rows of k_out and v_out (NULL: not
+ * wanted) get what the cache now holds for the token, for a prompt's own attention. Computed in fp32 and rounded once
+ * to the type of the call (fp16 keys without a norm: the bits of cdna3_rope_append_kv_f16). MXFP4: each 32 elements of a row take the
+ * smallest scale 2^e with max|x| < 7 2^e (e cut to -23 .. 13 for fp16, -125 .. 125 for bf16, so that every code's value is one of the
+ * type's), and the nearest codes, ties to even, of the exact values: keys are computed in fp64 for it. A block with a value that is not
+ * finite becomes NaN.
+ * q, k, v, q_out, k_out, v_out: [T][heads][D], heads D elements apart, *_row elements between tokens (0: packed). q_out may be q,
+ * k_out k and v_out v (the same address and row stride); outputs must not overlap inputs otherwise. nQHeads == 0: keys and
+ * values alone (q, q_out NULL).
+ * A token with a sequence outside 0 .. batch - 1 or a position outside 0 .. max_pages * page - 1 (or max_pos - 1) is padding:
+ * nothing is written for it. One whose table entry is outside 0 .. pages - 1 gets its outputs, and nothing is written to
+ * the pools. Two tokens of a call must not have the same place. T == 0: nothing is done.
+ * Invalid: negative sizes, T above 2^26 - 8, more than 2^20 query heads, a negative eps, one of cos_tab and sin_tab alone, q without q_out, rows shorter
+ * than the heads, rows not a multiple of 4 elements, tensors not 8-byte, tables of angles not 16-byte aligned, batch below 1.
+ */
+typedef struct {
+    const void *q, *k, *v;
+    void *q_out, *k_out, *v_out;
+    void *K_pages, *V_pages;
+    const int *tables, *seqs, *positions;
+    const float *cos_tab, *sin_tab;      /* [max_pos][D] */
+    const void *q_norm, *k_norm;         /* [D], the type of the call */
+    double eps;
+    int T, nQHeads, batch, max_pos;
+    long long q_row, k_row, v_row, q_out_row, k_out_row, v_out_row;
+} cdna4_append_args;
+
+int cdna4_rope_append_paged(const cdna4_append_args* args, const cdna4_paged_cache* cache, int dtype, cdna4_stream_t stream);
+
+/* cdna4_attn_decode_paged: nq queries per sequence, those of its last nq tokens, over the cache: query i of sequence b sees rows
+ * 0 .. lens[b] - nq + i (lens: int32, device memory, cut to 0 .. max_pages * page; a query that sees no row gets zeros). q, o:
+ * [batch][nq][nQHeads][D], dtype CDNA4_F16 or CDNA4_BF16, also the type of a CDNA4_KV_16 cache; query head h reads kv head
+ * h / (nQHeads / nKVHeads); scale 1/sqrt(D), softmax and sums in fp32. Table entries past the last row's are not read into a
+ * result; entries outside 0 .. pages - 1 of those before read some page of the pool (nothing outside it). Rows from lens[b] on
+ * may hold anything. A value in V that is not finite reaches the queries of up to nq - 1 tokens before it. The work is cut into
+ * equal shares of keys whatever the lengths are, so a captured call replays on other lengths, tables and pages. The workspace
+ * (cdna4_attn_decode_paged_workspace_size bytes, 16-byte aligned, no initialisation) holds what shares leave of rows that they
+ * cut; calls that overlap must not share one. The plan is sized to the current device, so query the size with the device
+ * current that the call will run on. batch == 0: nothing is done.
+ * Invalid: nQHeads % nKVHeads != 0, nq not 1 .. 16, 2^24 sequences and more, 2^26 - 3 rows of q or more, q not 16-byte or o not 4-byte
+ * aligned, a missing or small workspace.
+ */
+typedef struct {
+    int nQHeads;   /* nQHeads % nKVHeads == 0 */
+    int batch;
+    int nq;        /* queries per sequence */
+} cdna4_paged_decode_cfg;
+
+/* cdna4_attn_decode_paged_plan (introspection): `rows` rows of a row block, `partials` shares of keys, `grid` workgroups of the
+ * first launch. */
+int cdna4_attn_decode_paged_plan(const cdna4_paged_cache* cache, const cdna4_paged_decode_cfg* cfg, int dtype, cdna3_plan_info* out);
+size_t cdna4_attn_decode_paged_workspace_size(const cdna4_paged_cache* cache, const cdna4_paged_decode_cfg* cfg);
+int cdna4_attn_decode_paged(const void* q, const void* K_pages, const void* V_pages, const int* tables, const int* lens,
+                            void* o, const cdna4_paged_cache* cache, const cdna4_paged_decode_cfg* cfg, int dtype,
+                            void* workspace, size_t ws_bytes, cdna4_stream_t stream);
+
+/* cdna4_paged_reorder: the cache after a selection of beams (cdna4_beam_select): row i of the new batch goes on from row
+ * p = parents[i] of the old one (0 .. rows_in - 1): lens_out[i] = lens[p], tables_out[i] = tables[p], and where the last page is not
+ * full, its rows are copied to page fresh[i] in K and V of every layer, and that page takes its place in tables_out[i]; full
+ * pages are shared. fresh[i] may be the parent's own last page (nothing is copied: a beam's only successor); else it must be a
+ * page that no row's table names, another one for each i. parents[i] outside 0 .. rows_in - 1: an unused row, lens_out 0 and table
+ * entries -1. Pages outside 0 .. pages - 1: nothing is copied. K_pages, V_pages: layers pools, layer_stride bytes apart
+ * (0: packed). All arrays int32 in device memory, tables_out with the strides of tables; tables_out and lens_out must not overlap the
+ * inputs. rows == 0: nothing is done. Invalid: rows negative or above 65,535, rows_in or layers below 1, a layer_stride that is not a
+ * multiple of 16 or below a pool's bytes, null pointers, tables_out or lens_out at the inputs' address.
+ */
+int cdna4_paged_reorder(const int* parents, const int* tables, const int* lens, const int* fresh, int* tables_out,
+                        int* lens_out, void* K_pages, void* V_pages, const cdna4_paged_cache* cache, int rows, int rows_in,
+                        int layers, long long layer_stride, cdna4_stream_t stream);
+
+/* ---- beam search -------------------------------------------------------------------------
+ * No counterpart in the reference. `groups` groups of `beams` rows of V logits (fp32, fp16 or bf16; row g * beams + b): the n best of a
+ * group's beams x V continuations by
+ *   score = cum[row] + x_v - log sum_u exp(x_u),
+ * best first, equal scores by the lowest row, then the lowest token: scores [groups][n] fp32 (compared in fp64), parents (rows) and
+ * tokens int32. Sums of exponentials are taken in fp32 and joined in fp64. A logit of -inf or NaN is no continuation and adds
+ * nothing, +inf counts as the largest fp32 value; rows with cum -inf, +inf or NaN and rows that allow nothing have none. done
+ * (int32 [rows], may be NULL): rows that are not 0 there have ended and have one continuation, `eos` at the score cum. Places that no
+ * continuation fills: score -inf, parent and token -1. Logits of one row that differ by less than 2^-40 may count as equal.
+ * The workspace (cdna4_beam_select_workspace_size bytes for groups * beams rows, 16-byte aligned, no initialisation) must not be
+ * shared by calls that overlap; query its size with the device current that the call will run on. groups == 0: nothing is done.
+ * Invalid: beams or n not 1 .. 64, V < 1, groups negative, 2^24 rows and more, a logits stride below V, done with an eos outside 0 .. V - 1,
+ * null or misaligned pointers, a missing or small workspace.
+ */
+typedef struct {
+    const void* logits;        /* [groups * beams][logits_stride] */
+    const float* cum;          /* [groups * beams] */
+    const int* done;           /* [groups * beams] */
+    float* scores;             /* [groups][n] */
+    int *parents, *tokens;     /* [groups][n] */
+    int groups, beams, n, V, eos;
+    long long logits_stride;   /* elements between rows, >= V */
+} cdna4_beam_args;
+
+size_t cdna4_beam_select_workspace_size(int rows, int V, int beams, int n);
+int cdna4_beam_select(const cdna4_beam_args* args, int dtype, void* workspace, size_t ws_bytes, cdna4_stream_t stream);
 
 /* ---- runtime norms and RoPE ---------------------------------------------------
  * cdna3_rmsnorm_f32 replaces rmsnorm_f32_kernel (cdna3-prims/include/cdna3/runtime/

@@ -1,0 +1,217 @@
+"""cdna4.decode_paged against a 64-bit reference: lengths from no key to many shares, page sizes, both formats, head layouts,
+several queries, lengths and tables read on the device."""
+import pytest
+import torch
+
+import cdna4
+from paged_util import Paged, decode_reference
+from serving_util import DEV, check
+
+pytestmark = pytest.mark.gpu
+F16, BF16 = torch.float16, torch.bfloat16
+
+
+def make(lens, HQ, HK, D, dtype, page=16, fmt="16", nq=1, seed=0, scale=1.0):
+    p = Paged(lens, HK, D, dtype, page, fmt, seed)
+    q = (torch.randn(len(lens), nq, HQ, D, device=DEV, generator=p.g) * scale).to(dtype)
+    return p, q, cdna4.PagedDecodeCfg(HQ, len(lens), nq)
+
+
+def run(p, q, cfg, o=None, tables=None, lens=None, **kw):
+    o = torch.full_like(q, 7.0) if o is None else o
+    cdna4.decode_paged(q, p.K, p.V, p.tables if tables is None else tables, p.lens if lens is None else lens, o, p.cache, cfg, **kw)
+    return o
+
+
+def verify(p, q, o, what=""):
+    return check(o, *decode_reference(q, p.k, p.v, q.dtype), what)
+
+
+@pytest.mark.parametrize("fmt", ["16", "mxfp4"])
+@pytest.mark.parametrize("dtype", [F16, BF16])
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("page", [16, 32, 64, 128, 256])
+def test_lengths(page, D, dtype, fmt):
+    """Pages that end inside a chunk, at it and past it; rows behind the last one are NaN."""
+    lens = [0, 1, 15, 16, 17, 31, 32, 33, 64, 65, 100, 255, 256, 257, 300, 700]
+    p, q, cfg = make(lens, 8, 2, D, dtype, page, fmt, seed=page)
+    o = run(p, q, cfg)
+    verify(p, q, o, f"page {page}")
+    assert bool((o[0] == 0).all())
+
+
+@pytest.mark.parametrize("fmt", ["16", "mxfp4"])
+@pytest.mark.parametrize("heads", [(1, 1), (3, 1), (8, 8), (16, 2), (40, 8), (12, 12), (20, 1), (33, 1), (64, 1)])
+@pytest.mark.parametrize("D", [64, 128])
+def test_heads(heads, D, fmt):
+    p, q, cfg = make([70, 0, 129], *heads, D, F16, 32, fmt, seed=heads[0])
+    verify(p, q, run(p, q, cfg))
+
+
+@pytest.mark.parametrize("fmt", ["16", "mxfp4"])
+@pytest.mark.parametrize("nq", [2, 3, 5, 8, 16])
+@pytest.mark.parametrize("heads", [(4, 4), (8, 2), (20, 2)])
+def test_several_queries(heads, nq, fmt):
+    """Sequences shorter than the queries leave the first ones nothing to see: zeros."""
+    lens = [0, 1, nq - 1, nq, 31, 32, 33, 40, 95, 300]
+    p, q, cfg = make(lens, *heads, 64 if nq == 3 else 128, BF16 if nq == 2 else F16, 16, fmt, nq, seed=nq)
+    # a query whose row sees nothing gets 0 times the sequence's values, which are finite here
+    o = run(p, q, cfg)
+    verify(p, q, o)
+    for b, n in enumerate(lens):
+        assert bool((o[b, :max(nq - n, 0)] == 0).all())
+
+
+@pytest.mark.parametrize("B", [1, 2, 63, 64, 65, 130, 1000, 4099])
+def test_batches(B):
+    """More sequences than a wave's lanes, and than 64 lanes of 64, most of them empty."""
+    g = torch.Generator().manual_seed(B)
+    lens = torch.randint(0, 90, (B,), generator=g)
+    lens[torch.rand(B, generator=g) < (0.3 if B < 1000 else 0.9)] = 0
+    lens = lens.tolist()
+    p, q, cfg = make(lens, 4, 1, 64, BF16, 16, seed=B)
+    verify(p, q, run(p, q, cfg))
+
+
+@pytest.mark.parametrize("fmt", ["16", "mxfp4"])
+def test_long(fmt):
+    """Shares of many chunks, items cut into many shares, page ids past a wave's 64."""
+    lens = [40000, 17, 9000, 0, 2500, 33]
+    for D, dtype, page in ((128, BF16, 16), (64, F16, 64)):
+        p, q, cfg = make(lens, 8, 2, D, dtype, page, fmt, seed=2)
+        verify(p, q, run(p, q, cfg))
+
+
+def test_one_long_among_short():
+    lens = [30] * 100 + [20000] + [50] * 27
+    p, q, cfg = make(lens, 4, 2, 64, F16, 32, seed=3)
+    verify(p, q, run(p, q, cfg))
+
+
+@pytest.mark.parametrize("fmt", ["16", "mxfp4"])
+@pytest.mark.parametrize("scale", [0.0, 8.0])
+@pytest.mark.parametrize("dtype", [F16, BF16])
+def test_peaked_and_flat(scale, dtype, fmt):
+    p, q, cfg = make([300, 0, 64], 8, 2, 128, dtype, 32, fmt, seed=4, scale=scale)
+    verify(p, q, run(p, q, cfg))
+
+
+def test_lengths_are_cut_and_tables_clamped():
+    """Lengths outside the table's rows are cut to them; entries outside the pool read some page of it and touch no other sequence."""
+    lens = [100, 0, 96, 60]
+    p, q, cfg = make(lens, 4, 2, 64, F16, 16, seed=5)
+    p.cache.max_pages, p.cache.table_stride = 6, p.tables.shape[1]          # 96 rows
+    o = run(p, q, cfg, lens=torch.tensor([2 ** 31 - 1, -2 ** 31, 97, 60], dtype=torch.int32, device=DEV))
+    p.k, p.v = [x[:, :96] for x in p.k], [x[:, :96] for x in p.v]
+    verify(p, q, o)
+    t = p.tables.clone()
+    t[3, 1], t[3, 2] = -5, 2 ** 30
+    o2 = run(p, q, cfg, tables=t, lens=torch.tensor([100, 0, 100, 60], dtype=torch.int32, device=DEV))
+    assert torch.equal(o2[:3], o[:3])
+
+
+def test_shared_pages_equal_copies():
+    """Two tables naming the same pages give the same bits as each alone."""
+    p, q, cfg = make([200], 8, 2, 128, BF16, 32, seed=6)
+    t, l = p.tables.repeat(3, 1), p.lens.repeat(3)
+    q3 = q.repeat(3, 1, 1, 1)
+    o = torch.empty_like(q3)
+    cdna4.decode_paged(q3, p.K, p.V, t, l, o, p.cache, cdna4.PagedDecodeCfg(8, 3, 1))
+    verify(p, q, o[:1])
+    ref, bound = decode_reference(q, p.k, p.v, BF16)
+    for i in (1, 2):
+        check(o[i:i + 1], ref, bound)
+
+
+def test_as_decode_of_a_contiguous_cache():
+    lens = [777] * 3
+    p, q, cfg = make(lens, 8, 2, 128, F16, 64, seed=7)
+    o = run(p, q, cfg)
+    u = torch.empty(3, 8, 128, dtype=F16, device=DEV)
+    K, V = torch.stack(p.k).to(F16), torch.stack(p.v).to(F16)
+    cdna4.decode(q[:, 0].contiguous(), K, V, u, cdna4.DecodeCfg(128, 777, 8, 2, 3, 0))
+    _, bound = decode_reference(q, p.k, p.v, F16)
+    check(o[:, 0], u.double(), 2 * bound[:, 0])
+
+
+def test_masked_keys_that_are_not_finite():
+    """K rows that some queries must not see may hold anything; a V that is not finite stays with the queries that see it and those of up
+    to nq - 1 tokens before it."""
+    p, q, cfg = make([50, 70], 4, 2, 64, F16, 16, nq=3, seed=8)
+    ref, bound = decode_reference(q, p.k, p.v, F16)
+    last = int(p.tables[0, 49 // 16])
+    p.K[last, :, 49 % 16] = float("nan")                     # row 49: queries 0 and 1 must not see it
+    o = run(p, q, cfg)
+    check(o[0, :2], ref[0, :2], bound[0, :2])
+    check(o[1], ref[1], bound[1])
+    assert bool(o[0, 2].isnan().all())
+
+
+def test_workspace_contents_do_not_matter():
+    p, q, cfg = make([40, 0, 2000], 8, 2, 128, F16, 32, seed=9)
+    need = cdna4.decode_paged_workspace_size(p.cache, cfg)
+    a = run(p, q, cfg)
+    for fill in (0, 255):
+        ws = torch.full((need + 64,), fill, dtype=torch.uint8, device=DEV)
+        assert torch.equal(a, run(p, q, cfg, workspace=ws[:need]))
+        assert bool((ws[need:] == fill).all())
+    with pytest.raises(cdna4.CDNA4Error):
+        run(p, q, cfg, workspace=ws[:need - 1])
+    for bad in (None, "none"):
+        with pytest.raises(ValueError):
+            run(p, q, cfg, workspace=bad)
+    with pytest.raises(ValueError):
+        run(p, q, cfg, tables=p.tables[:2])
+    with pytest.raises(ValueError):
+        run(p, q.to(BF16), cfg)
+
+
+def test_two_streams_at_once():
+    a, b = make([400, 30, 0], 8, 2, 128, BF16, 16, seed=10), make([77, 500], 12, 12, 64, F16, 32, "mxfp4", seed=11)
+    oa, ob = torch.empty_like(a[1]), torch.empty_like(b[1])
+    torch.cuda.synchronize()
+    s1, s2 = torch.cuda.Stream(), torch.cuda.Stream()
+    for _ in range(5):
+        run(*a, o=oa, stream=s1)
+        run(*b, o=ob, stream=s2)
+    torch.cuda.synchronize()
+    verify(a[0], a[1], oa)
+    verify(b[0], b[1], ob)
+
+
+@pytest.mark.parametrize("fmt", ["16", "mxfp4"])
+def test_captured_call_replays_on_other_lengths(fmt):
+    p, q, cfg = make([600] * 4, 8, 2, 128, F16, 32, fmt, seed=12)
+    full_k, full_v = p.k, p.v
+    ws = torch.empty(cdna4.decode_paged_workspace_size(p.cache, cfg), dtype=torch.uint8, device=DEV)
+    o = torch.empty_like(q)
+    run(p, q, cfg, o=o, workspace=ws)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        run(p, q, cfg, o=o, workspace=ws)
+    for lens in ([0, 0, 0, 0], [1, 600, 33, 64], [599, 2, 0, 300], [600] * 4):
+        p.lens.copy_(torch.tensor(lens, dtype=torch.int32))
+        o.fill_(7.0)
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(o, run(p, q, cfg))
+        p.k, p.v = [x[:, :n] for x, n in zip(full_k, lens)], [x[:, :n] for x, n in zip(full_v, lens)]
+        verify(p, q, o, str(lens))
+
+
+@pytest.mark.parametrize("fmt", ["16", "mxfp4"])
+def test_pools_past_32_bit_offsets(fmt):
+    """The rows of interest lie in the last pages of a pool of more than 4 GiB."""
+    HK, D, page = 8, 128, 256
+    pages = 2 ** 32 // (HK * page * (256 if fmt == "16" else 68)) + 40
+    p, q, cfg = make([900, 300], 16, HK, D, F16, page, fmt, seed=13)
+    small = p.cache.pages
+    for name in ("K", "V"):
+        old = getattr(p, name)
+        pool = torch.zeros((pages,) + tuple(old.shape[1:]), dtype=old.dtype, device=DEV)
+        pool[pages - small:] = old
+        setattr(p, name, pool)
+    p.cache.pages = pages
+    p.tables = torch.where(p.tables >= 0, p.tables + (pages - small), p.tables)
+    verify(p, q, run(p, q, cfg))
