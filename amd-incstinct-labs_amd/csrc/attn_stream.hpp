@@ -37,11 +37,16 @@ __device__ __forceinline__ void dma16(const void* gsrc, const void* lds_dst) {
 // spilled SGPR, v_readfirstlane) needs 5 wait states before a vector memory instruction reads that
 // SGPR, and the compiler does not know the copy reads it; so the base is first moved by the SALU
 // (which waits for VALU-written SGPRs by itself) into a fresh pair that only the copy reads.
+template <bool kNT = false>
 __device__ __forceinline__ void dma16_s(const void* sbase, uint32_t voff, const void* lds_dst) {
     const uint32_t base = (uint32_t)(uintptr_t)(const tile::LDS_AS_T*)lds_dst;
     const void* b;
-    asm volatile("s_mov_b64 %0, %2\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %0"
-                 : "=&s"(b) : "v"(voff), "s"(sbase), "{m0}"(base) : "memory");
+    if constexpr (kNT)
+        asm volatile("s_mov_b64 %0, %2\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %0 nt"
+                     : "=&s"(b) : "v"(voff), "s"(sbase), "{m0}"(base) : "memory");
+    else
+        asm volatile("s_mov_b64 %0, %2\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %0"
+                     : "=&s"(b) : "v"(voff), "s"(sbase), "{m0}"(base) : "memory");
 }
 
 // Wait until at most Y of this wave's newest copy groups (kCopies copies each) are in flight.

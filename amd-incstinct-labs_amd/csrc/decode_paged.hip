@@ -62,48 +62,48 @@ struct Window {
     }
 };
 
-// Finds the sequence that holds chunk x of the axis of one item (0 <= x < all): each level narrows the sequences to a lane's.
-__device__ __forceinline__ Place find(const PagedArgs& a, long long x, Window& w, int lane) {
-    int lo = 0, n = a.batch;
-    long long before = 0;
-    for (;;) {
+// What a share holds: chunks begin .. end - 1 of the axis, the first of them in sequence `at`.
+struct Share { long long per, begin, end; Place at; };
+
+// Equal shares of all chunks, but none below kMinChunks, and no item in more than about kMaxParts: each lane counts the chunks of a
+// run of sequences, a scan over the lanes finds the one in whose run the share begins, and so on within that run.
+__device__ __forceinline__ Share share_of(const PagedArgs& a, int share, Window& w, int lane) {
+    int lo = 0, n = a.batch, most = 0;
+    long long x = 0, before = 0;
+    Share s{0, 0, 0, Place{0, 0, 0}};
+    for (bool first = true;; first = false) {
         const int step = (n + 63) / 64;   // sequences of a lane
+        long long c = 0;
         if (step == 1) {
             w.load(a, lo, lane);
-            const long long c = lane < n ? chunks_of(w.len) : 0;
-            const long long upto = wave::xlane::scan_inclusive(c, Sum{}) + before;
-            const uint64_t here = __builtin_amdgcn_ballot_w64(upto > x);
-            const int l = here ? __builtin_ctzll(here) : 63;
-            return Place{lo + l, __builtin_amdgcn_readlane(w.len, l), scalar(__shfl(upto - c, l))};
-        }
-        long long c = 0;
-        for (int i = 0; i < step; ++i) {
-            const int at = lane * step + i;
-            if (at < n) c += chunks_of(length_of(a, lo + at));
+            if (lane < n) c = chunks_of(w.len);
+            most = max(most, (int)c);
+        } else {
+            for (int i = 0; i < step; ++i) {
+                const int at = lane * step + i, m = at < n ? chunks_of(length_of(a, lo + at)) : 0;
+                c += m;
+                most = max(most, m);
+            }
         }
         const long long upto = wave::xlane::scan_inclusive(c, Sum{}) + before;
-        const uint64_t here = __builtin_amdgcn_ballot_w64(upto > x);
-        const int l = here ? __builtin_ctzll(here) : 63;
+        if (first) {
+            const long long all = scalar(__shfl(upto, 63)) * a.items;
+            most = scalar(allreduce(most, Max{}));
+            s.per = max((all + a.shares - 1) / a.shares, (long long)max(kMinChunks, (most + kMaxParts - 1) / kMaxParts));
+            s.begin = share * s.per;
+            s.end = min(s.begin + s.per, all);
+            if (s.begin >= s.end) return s;
+            x = s.begin / a.items;
+        }
+        const int l = __builtin_ctzll(__builtin_amdgcn_ballot_w64(upto > x));   // some lane's is: x lies below the run's end
         before = scalar(__shfl(upto - c, l));
         lo += l * step;
+        if (step == 1) {
+            s.at = Place{lo, __builtin_amdgcn_readlane(w.len, l), before};
+            return s;
+        }
         n = min(step, n - l * step);
-        if (n < 1) { lo = 0; n = 1; }   // not reached: x lies below the last lane's sum
     }
-}
-
-// Chunks of a share: equal shares of all, but none below kMinChunks, and no item in more than about kMaxParts.
-__device__ __forceinline__ long long share_of(const PagedArgs& a, long long& all, int lane) {
-    long long c = 0;
-    int most = 0;
-    for (int b = lane; b < a.batch; b += 64) {
-        const int n = chunks_of(length_of(a, b));
-        c += n;
-        most = max(most, n);
-    }
-    all = scalar(allreduce(c, Sum{})) * a.items;
-    most = scalar(allreduce(most, Max{}));
-    const long long even = (all + a.shares - 1) / a.shares;
-    return max(even, (long long)max(kMinChunks, (most + kMaxParts - 1) / kMaxParts));
 }
 
 // Pages of a sequence, 64 table entries at a time, one per lane; entries past its rows are not read.
@@ -116,24 +116,103 @@ struct Pages {
     }
 };
 
-// The address of key k's row of one head in lane-by-lane form; the row's page is in the loaded entries.
-__device__ __forceinline__ size_t row_at(const PagedArgs& a, const Pages& pg, int k, int kvh, int head_bytes, int rbytes) {
-    const int id = __shfl(pg.ids, (k >> a.lp) - pg.first);
-    return ((size_t)id * a.HK + kvh) * head_bytes + (size_t)(k & (a.page - 1)) * rbytes;
+// The page of key k, whose entry is among the loaded ones: lane by lane, or for a k that all lanes share.
+__device__ __forceinline__ int page_of(const PagedArgs& a, const Pages& pg, int k) { return __shfl(pg.ids, (k >> a.lp) - pg.first); }
+__device__ __forceinline__ int page_of_all(const PagedArgs& a, const Pages& pg, int k) {
+    return __builtin_amdgcn_readlane(pg.ids, (k >> a.lp) - pg.first);
 }
 
-// Copies one chunk's K or V rows into a ring stage; rows past the last re-read it (masked).
-template <int D, bool kIsK>
+// One chunk's K and V rows into a ring stage (K first), 16-bit rows. A chunk lies in one page, or, with pages of 16 rows, in two: the copies
+// of a whole chunk take their bases from the scalar unit, and a lane's offset within them differs from copy to copy by the swizzle
+// alone. The last chunk of a sequence goes row by row; rows past the end re-read the last one (masked).
+template <int D, bool kNT>
 __device__ __forceinline__ void copy_chunk(const PagedArgs& a, const Pages& pg, int kb, int len, int kvh, uint16_t* stage, int lane) {
-    constexpr int CPR = D / 8, NI = kKeys * CPR / 64;
-    const int head_bytes = a.page * 2 * D;
-    const char* pool = kIsK ? a.K : a.V;
+    constexpr int CPR = D / 8, NI = kKeys * CPR / 64, kRows = 64 / CPR;   // copies of K, rows of a copy
+    uint16_t* const vstage = stage + kKeys * D;
+    const size_t head = (size_t)a.page * 2 * D;
+    const int mask = a.page - 1;
+    if (kb + kKeys <= len) {
+        size_t at[2];
+#pragma unroll
+        for (int h = 0; h < 2; ++h)
+            at[h] = ((size_t)page_of_all(a, pg, kb + 16 * h) * a.HK + kvh) * head + (size_t)((kb + 16 * h) & mask) * 2 * D;
+        const int r = lane / CPR, c = lane % CPR;
+        const uint32_t ko = (uint32_t)(r * 2 * D + (c ^ swz_k<D>(r)) * 16), vo = (uint32_t)(r * 2 * D + (c ^ swz_v<D>(r)) * 16);
+#pragma unroll
+        for (int j = 0; j < NI; ++j)
+            stream::dma16_s<kNT>(a.K + at[j / (NI / 2)] + j % (NI / 2) * 1024, ko ^ (uint32_t)(swz_k<D>(j * kRows) << 4), stage + j * 512);
+#pragma unroll
+        for (int j = 0; j < NI; ++j)
+            stream::dma16_s<kNT>(a.V + at[j / (NI / 2)] + j % (NI / 2) * 1024, vo ^ (uint32_t)(swz_v<D>(j * kRows) << 4), vstage + j * 512);
+        return;
+    }
 #pragma unroll
     for (int j = 0; j < NI; ++j) {
-        const int p = j * 64 + lane, r = p / CPR;
-        const size_t at = row_at(a, pg, min(kb + r, len - 1), kvh, head_bytes, 2 * D);
-        stream::dma16<false>(pool + at + ((p % CPR) ^ swz<D, kIsK>(r)) * 16, stage + j * 512);
+        const int p = j * 64 + lane, r = p / CPR, k = min(kb + r, len - 1);
+        const size_t at = ((size_t)page_of(a, pg, k) * a.HK + kvh) * head + (size_t)(k & mask) * 2 * D;
+        stream::dma16<kNT>(a.K + at + ((p % CPR) ^ swz_k<D>(r)) * 16, stage + j * 512);
+        stream::dma16<kNT>(a.V + at + ((p % CPR) ^ swz_v<D>(r)) * 16, vstage + j * 512);
     }
+}
+
+// MXFP4 rows in registers. K: lane (li, g) holds its g-th quarter of the rows that it has in the two K operand tiles, D / 4
+// values that lie in one block; operand c is 8 of them, so query operands take the same D / 4 g + 8 c. V: blocks of 32 values,
+// lane by lane in the order of memory.
+template <int D>
+struct Codes {
+    static constexpr int KW = D / 32;            // dwords of a quarter row
+    static constexpr int VB = kKeys * D / 2048;  // blocks of V per lane
+    uint32_t k[2][KW];
+    u32x4 v[VB];
+    uint32_t ks[2], vs[VB];
+};
+
+template <int D, bool kNT>
+__device__ __forceinline__ void load_codes(const PagedArgs& a, const Pages& pg, int kb, int len, int kvh, Codes<D>& x, int li, int g, int lane) {
+    constexpr int KW = Codes<D>::KW, VB = Codes<D>::VB, BPR = D / 32;   // blocks of a row
+    const size_t head = (size_t)a.page * (D / 2 + BPR);
+    const int mask = a.page - 1, scales = a.page * (D / 2);
+    auto get = [&](auto* p) {
+        if constexpr (kNT) return __builtin_nontemporal_load(p);
+        else return *p;
+    };
+    using KV = uint32_t __attribute__((ext_vector_type(KW)));
+    auto put = [&](const char* kp, int row, int u) {   // K: a row's quarter and its scale
+        const KV w = get((const KV*)(kp + row * (D / 2) + g * (D / 8)));
+#pragma unroll
+        for (int i = 0; i < KW; ++i) x.k[u][i] = w[i];
+        x.ks[u] = *(const uint8_t*)(kp + scales + row * BPR + g * BPR / 4);
+    };
+    auto put_v = [&](const char* vp, int row, int blk, int j) {
+        x.v[j] = get((const u32x4*)(vp + row * (D / 2) + blk * 16));
+        x.vs[j] = *(const uint8_t*)(vp + scales + row * BPR + blk);
+    };
+    // K rows 8 (li / 4) + li % 4 + 4 u: lanes li < 8 in the first half of the chunk; V rows (64 j + lane) / BPR
+    const int kr = 8 * (li >> 2) + (li & 3);
+    if (kb + kKeys <= len && a.page > 16) {
+        const size_t at = ((size_t)page_of_all(a, pg, kb) * a.HK + kvh) * head;
+        const int row0 = kb & mask;
+#pragma unroll
+        for (int u = 0; u < 2; ++u) put(a.K + at, row0 + kr + 4 * u, u);
+#pragma unroll
+        for (int j = 0; j < VB; ++j) put_v(a.V + at, row0 + (64 * j + lane) / BPR, lane % BPR, j);
+        return;
+    }
+#pragma unroll
+    for (int u = 0; u < 2; ++u) {
+        const int k = min(kb + kr + 4 * u, len - 1);
+        put(a.K + ((size_t)page_of(a, pg, k) * a.HK + kvh) * head, k & mask, u);
+    }
+#pragma unroll
+    for (int j = 0; j < VB; ++j) {
+        const int k = min(kb + (64 * j + lane) / BPR, len - 1);
+        put_v(a.V + ((size_t)page_of(a, pg, k) * a.HK + kvh) * head, k & mask, lane % BPR, j);
+    }
+}
+
+template <bool kBf16>
+__device__ __forceinline__ u32x4 decode8(uint32_t c, float scale) {
+    return u32x4{decode2<kBf16, 0>(c, scale), decode2<kBf16, 1>(c, scale), decode2<kBf16, 2>(c, scale), decode2<kBf16, 3>(c, scale)};
 }
 
 // Scores that a row must not see are masked by the row's own limit.
@@ -157,29 +236,36 @@ __device__ __forceinline__ bool check_limits(f32x4 (&s)[RT][2], const float (&m)
     return need;
 }
 
-template <int D, int RT, bool kBf16, bool kFp4>
-__global__ __launch_bounds__(64) void paged_parts(PagedArgs a) {
-    constexpr int ND = D / 32, NDT = D / 16, kStage = kKeys * D;
-    __shared__ __attribute__((aligned(16))) uint16_t lds[4 * kStage];
+// Waves that a CU holds: 16-bit rows as many as have a ring in its LDS, MXFP4 as the registers allow.
+constexpr int waves_per_cu(int D, int RT, bool fp4) { return fp4 ? (RT == 2 ? 8 : D == 128 ? 12 : 16) : D == 128 ? 5 : 10; }
+
+template <int D, int RT, bool kBf16, bool kFp4, bool kNT>
+__global__ __launch_bounds__(64, (waves_per_cu(D, RT, kFp4) + 3) / 4) void paged_parts(PagedArgs a) {
+    constexpr int ND = D / 32, NDT = D / 16, kStage = 2 * kKeys * D;
+    constexpr int kCopies = 2 * kKeys * (D / 8) / 64;
+    // 16 bits: a ring of two chunks of K and V. MXFP4: one chunk of V as 16-bit values.
+    __shared__ __attribute__((aligned(16))) uint16_t lds[kFp4 ? kKeys * D : 2 * kStage];
     const int lane = (int)threadIdx.x, li = lane & 15, g = lane >> 4, share = (int)blockIdx.x;
-    long long all;
-    const long long per = share_of(a, all, lane);
-    if (share == 0 && lane == 0) a.head[0] = per;
-    long long at = share * per;
-    const long long end = min(at + per, all);
-    if (at >= end) return;
     Window w;
-    Place pl = find(a, at / a.items, w, lane);
+    const Share sh = share_of(a, share, w, lane);
+    if (share == 0 && lane == 0) a.head[0] = sh.per;
+    if (sh.begin >= sh.end) return;
+    long long at = sh.begin;
+    Place pl = sh.at;
     const LdsOffsets off = lds_offsets<D>(li, g);
     const size_t slot0 = (size_t)share * 2 * a.rows;
-    while (at < end) {
+    const int R = a.nq * a.G;
+    while (at < sh.end) {
         const int n = chunks_of(pl.len);
         const long long in_seq = at - pl.before * a.items;
-        const int item = (int)(in_seq / n), c0 = (int)(in_seq % n), c1 = (int)min((long long)n, c0 + (end - at));
+        const int item = (int)(in_seq / n), c0 = (int)(in_seq - (long long)item * n), c1 = (int)min((long long)n, c0 + (sh.end - at));
         if (item == 0 && c0 == 0 && lane == 0) a.head[1 + pl.b] = pl.before;
         const int kvh = item / a.HB, hb = item % a.HB;
+        Pages pg;
+        pg.table = a.tables + pl.b * a.table_stride;
+        pg.most = (pl.len + a.page - 1) >> a.lp;
+        pg.load(a, (c0 * kKeys) >> a.lp, lane);
         // row r of the item: query r / G, head kvh G + r % G
-        const int R = a.nq * a.G;
         int limit[RT];
         u32x4 qb[RT][ND];
 #pragma unroll
@@ -192,12 +278,9 @@ __global__ __launch_bounds__(64) void paged_parts(PagedArgs a) {
                 limit[t] = pl.len - a.nq + 1 + i;
                 const uint16_t* q = a.q + (((size_t)pl.b * a.nq + i) * a.nQH + (size_t)kvh * a.G + r % a.G) * D;
 #pragma unroll
-                for (int c = 0; c < ND; ++c) qb[t][c] = *(const u32x4*)(q + c * 32 + g * 8);
+                for (int c = 0; c < ND; ++c) qb[t][c] = *(const u32x4*)(q + (kFp4 ? g * (D / 4) + c * 8 : c * 32 + g * 8));
             }
         }
-        Pages pg;
-        pg.table = a.tables + pl.b * a.table_stride;
-        pg.most = (pl.len + a.page - 1) >> a.lp;
         f32x4 o[RT][NDT], lacc[RT];
         float m[RT];
 #pragma unroll
@@ -207,41 +290,12 @@ __global__ __launch_bounds__(64) void paged_parts(PagedArgs a) {
 #pragma unroll
             for (int d = 0; d < NDT; ++d) o[t][d] = f32x4{0.f, 0.f, 0.f, 0.f};
         }
-        pg.load(a, (c0 * kKeys) >> a.lp, lane);
-        for (int c = c0; c < c1; ++c) {
-            const int kb = c * kKeys;
-            if (((min(kb + kKeys, pl.len) - 1) >> a.lp) - pg.first >= 64) pg.load(a, kb >> a.lp, lane);
-            __syncthreads();
-            if constexpr (kFp4) {
-                const int head_bytes = a.page * (D / 2 + D / 32);
-                // 16 codes to a lane: half a block
-#pragma unroll
-                for (int kv = 0; kv < 2; ++kv)
-#pragma unroll
-                    for (int j = 0; j < kKeys * D / 16 / 64; ++j) {
-                        const int p = j * 64 + lane, r = p / (D / 16), x = p % (D / 16);
-                        const int k = min(kb + r, pl.len - 1);
-                        const char* pool = (kv ? a.V : a.K) + row_at(a, pg, 0 + k, kvh, head_bytes, 0) - 0;
-                        const char* headp = pool;
-                        const int row = k & (a.page - 1);
-                        const uint2 c2 = *(const uint2*)(headp + row * (D / 2) + x * 8);
-                        const float f = f32_from_bits((uint32_t)*(const uint8_t*)(headp + a.page * (D / 2) + row * (D / 32) + x / 2) << 23);
-                        u32x4 lo{decode2<kBf16, 0>(c2.x, f), decode2<kBf16, 1>(c2.x, f), decode2<kBf16, 2>(c2.x, f), decode2<kBf16, 3>(c2.x, f)};
-                        u32x4 hi{decode2<kBf16, 0>(c2.y, f), decode2<kBf16, 1>(c2.y, f), decode2<kBf16, 2>(c2.y, f), decode2<kBf16, 3>(c2.y, f)};
-                        uint16_t* dst = lds + kv * kStage + r * D;
-                        const int z = kv ? swz_v<D>(r) : swz_k<D>(r);
-                        *(u32x4*)(dst + ((2 * x) ^ z) * 8) = lo;
-                        *(u32x4*)(dst + ((2 * x + 1) ^ z) * 8) = hi;
-                    }
-            } else {
-                copy_chunk<D, true>(a, pg, kb, pl.len, kvh, lds, lane);
-                copy_chunk<D, false>(a, pg, kb, pl.len, kvh, lds + kStage, lane);
-                asm volatile("s_waitcnt vmcnt(0)" : : : "memory");
-            }
-            __syncthreads();
-            const char *Kt = (const char*)lds, *Vt = (const char*)(lds + kStage);
-            f32x4 s[RT][2];
-            qk_chunk<D, RT, kBf16>(Kt, off, qb, s, 0);
+        auto pages_for = [&](int c) {   // the entries of chunk c's pages
+            const int last = (min((c + 1) * kKeys, pl.len) - 1) >> a.lp;
+            if (last - pg.first >= 64) pg.load(a, (c * kKeys) >> a.lp, lane);
+        };
+        // scores of a chunk to weights, weights times V
+        auto chunk = [&](f32x4 (&s)[RT][2], int kb, const char* Vt) {
             float lm[RT];
             const bool need = check_limits<RT>(s, m, lm, kb, limit, kb + kKeys > pl.len - a.nq + 1, a.sc, g);
             if (__builtin_amdgcn_ballot_w64(need)) rescale_rows<D, RT>(lm, m, o, lacc, a.sc);
@@ -249,10 +303,60 @@ __global__ __launch_bounds__(64) void paged_parts(PagedArgs a) {
             softmax_chunk<RT, kBf16>(s, m, pb, a.sc);
             pv_chunk<D, RT, kBf16>(Vt, off, pb, o, lacc, 0);
             if constexpr (kBf16) {
-                if (kb < kLoKeys) {
+                if (kb < kLoKeys) {   // the first keys: the weights' second bf16 term
                     softmax_lo_chunk<RT>(s, m, pb, a.sc);
                     pv_chunk<D, RT, true>(Vt, off, pb, o, lacc, 0);
                 }
+            }
+        };
+        if constexpr (kFp4) {
+            Codes<D> x, y;
+            load_codes<D, kNT>(a, pg, c0 * kKeys, pl.len, kvh, x, li, g, lane);
+            for (int c = c0; c < c1; ++c) {
+                const int kb = c * kKeys;
+                if (c + 1 < c1) {
+                    pages_for(c + 1);
+                    load_codes<D, kNT>(a, pg, kb + kKeys, pl.len, kvh, y, li, g, lane);
+                }
+                // V's values to LDS, where the P.V product reads them transposed
+#pragma unroll
+                for (int j = 0; j < Codes<D>::VB; ++j) {
+                    const int r = (64 * j + lane) / ND, blk = lane % ND;
+                    const float f = f32_from_bits(x.vs[j] << 23);
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) *(u32x4*)(lds + r * D + ((4 * blk + i) ^ swz_v<D>(r)) * 8) = decode8<kBf16>(x.v[j][i], f);
+                }
+                f32x4 s[RT][2];
+#pragma unroll
+                for (int t = 0; t < RT; ++t)
+#pragma unroll
+                    for (int u = 0; u < 2; ++u) s[t][u] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+                for (int u = 0; u < 2; ++u) {
+                    const float f = f32_from_bits(x.ks[u] << 23);
+#pragma unroll
+                    for (int i = 0; i < ND; ++i) {
+                        const u32x4 ka = decode8<kBf16>(x.k[u][i], f);
+#pragma unroll
+                        for (int t = 0; t < RT; ++t) s[t][u] = mfma<kBf16>(ka, qb[t][i], s[t][u]);
+                    }
+                }
+                chunk(s, kb, (const char*)lds);
+                x = y;
+            }
+        } else {
+            copy_chunk<D, kNT>(a, pg, c0 * kKeys, pl.len, kvh, lds, lane);
+            for (int c = c0, st = 0; c < c1; ++c, st ^= 1) {
+                if (c + 1 < c1) {
+                    pages_for(c + 1);
+                    copy_chunk<D, kNT>(a, pg, (c + 1) * kKeys, pl.len, kvh, lds + (st ^ 1) * kStage, lane);
+                    asm volatile("s_waitcnt vmcnt(%0)" : : "n"(kCopies) : "memory");
+                } else {
+                    asm volatile("s_waitcnt vmcnt(0)" : : : "memory");
+                }
+                f32x4 s[RT][2];
+                qk_chunk<D, RT, kBf16>((const char*)(lds + st * kStage), off, qb, s, 0);
+                chunk(s, c * kKeys, (const char*)(lds + st * kStage + kKeys * D));
             }
         }
         const bool whole = c0 == 0 && c1 == n;
@@ -277,7 +381,7 @@ __global__ __launch_bounds__(64) void paged_parts(PagedArgs a) {
             }
         }
         at += c1 - c0;
-        if (at < end && c1 == n && item + 1 == a.items) {   // on to the next sequence that has keys
+        if (at < sh.end && c1 == n && item + 1 == a.items) {   // on to the next sequence that has keys
             pl.before += n;
             int l = pl.b + 1 - w.first;
             for (;;) {
@@ -352,21 +456,29 @@ bool plan_paged(const cdna4_paged_cache& k, const cdna4_paged_decode_cfg& c, Pag
     p.items = k.nKVHeads * p.HB;
     p.rows = std::min(R, 16 * p.RT);
     if ((long long)c.batch * p.items * 256 > 0xffffffffLL) return false;
-    p.shares = device_cus() * (k.D == 64 ? 10 : 5);
+    p.shares = device_cus() * waves_per_cu(k.D, p.RT, k.format == CDNA4_KV_MXFP4);
     p.head_bytes = align256(((size_t)c.batch + 1) * sizeof(long long));
     p.ml_bytes = align256((size_t)p.shares * 2 * p.rows * 2 * sizeof(float));
     p.ws_bytes = p.head_bytes + p.ml_bytes + (size_t)p.shares * 2 * p.rows * k.D * sizeof(float);
     return true;
 }
 
+template <int D, int RT, bool kBf16, bool kFp4>
+void launch_parts(const PagedArgs& a, bool nt, hipStream_t s) {
+    if (nt) paged_parts<D, RT, kBf16, kFp4, true><<<a.shares, 64, 0, s>>>(a);
+    else paged_parts<D, RT, kBf16, kFp4, false><<<a.shares, 64, 0, s>>>(a);
+}
+
 template <int D, bool kBf16>
 int launch_paged(const PagedArgs& a, const PagedPlan& p, bool fp4, hipStream_t s) {
+    // pools larger than the Infinity Cache are read past it (stream::dma16)
+    const bool nt = 2.0 * a.pages * a.HK * a.page * row_bytes(D, fp4) > 256.0 * 1024 * 1024;
     if (p.RT == 2) {
-        if (fp4) paged_parts<D, 2, kBf16, true><<<p.shares, 64, 0, s>>>(a);
-        else paged_parts<D, 2, kBf16, false><<<p.shares, 64, 0, s>>>(a);
+        if (fp4) launch_parts<D, 2, kBf16, true>(a, nt, s);
+        else launch_parts<D, 2, kBf16, false>(a, nt, s);
     } else {
-        if (fp4) paged_parts<D, 1, kBf16, true><<<p.shares, 64, 0, s>>>(a);
-        else paged_parts<D, 1, kBf16, false><<<p.shares, 64, 0, s>>>(a);
+        if (fp4) launch_parts<D, 1, kBf16, true>(a, nt, s);
+        else launch_parts<D, 1, kBf16, false>(a, nt, s);
     }
     if (int e = launch_status()) return e;
     paged_join<D, kBf16><<<(unsigned)((size_t)a.batch * a.items), 256, 0, s>>>(a);
