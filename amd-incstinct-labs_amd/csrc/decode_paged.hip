@@ -50,6 +50,12 @@ __device__ __forceinline__ long long scalar(long long x) {
 __device__ __forceinline__ int length_of(const PagedArgs& a, int b) { return b < a.batch ? min(max(a.lens[b], 0), a.max_len) : 0; }
 __device__ __forceinline__ int chunks_of(int len) { return (len + kKeys - 1) / kKeys; }
 
+// Quotients of numbers that are nearly always below 2^32, where a division takes a third of the time.
+__device__ __forceinline__ long long quotient(long long x, long long y) {
+    if (((uint64_t)x | (uint64_t)y) >> 32 == 0) return (long long)((uint32_t)x / (uint32_t)y);
+    return x / y;
+}
+
 // Where a wave stands: sequence b of len keys, `before` chunks of one item in the sequences before it.
 struct Place { int b, len; long long before; };
 
@@ -89,11 +95,11 @@ __device__ __forceinline__ Share share_of(const PagedArgs& a, int share, Window&
         if (first) {
             const long long all = scalar(__shfl(upto, 63)) * a.items;
             most = scalar(allreduce(most, Max{}));
-            s.per = max((all + a.shares - 1) / a.shares, (long long)max(kMinChunks, (most + kMaxParts - 1) / kMaxParts));
+            s.per = max(quotient(all + a.shares - 1, a.shares), (long long)max(kMinChunks, (most + kMaxParts - 1) / kMaxParts));
             s.begin = share * s.per;
             s.end = min(s.begin + s.per, all);
             if (s.begin >= s.end) return s;
-            x = s.begin / a.items;
+            x = quotient(s.begin, a.items);
         }
         const int l = __builtin_ctzll(__builtin_amdgcn_ballot_w64(upto > x));   // some lane's is: x lies below the run's end
         before = scalar(__shfl(upto - c, l));
@@ -258,7 +264,7 @@ __global__ __launch_bounds__(64, (waves_per_cu(D, RT, kFp4) + 3) / 4) void paged
     while (at < sh.end) {
         const int n = chunks_of(pl.len);
         const long long in_seq = at - pl.before * a.items;
-        const int item = (int)(in_seq / n), c0 = (int)(in_seq - (long long)item * n), c1 = (int)min((long long)n, c0 + (sh.end - at));
+        const int item = (int)quotient(in_seq, n), c0 = (int)(in_seq - (long long)item * n), c1 = (int)min((long long)n, c0 + (sh.end - at));
         if (item == 0 && c0 == 0 && lane == 0) a.head[1 + pl.b] = pl.before;
         const int kvh = item / a.HB, hb = item % a.HB;
         Pages pg;
@@ -310,14 +316,11 @@ __global__ __launch_bounds__(64, (waves_per_cu(D, RT, kFp4) + 3) / 4) void paged
             }
         };
         if constexpr (kFp4) {
-            Codes<D> x, y;
-            load_codes<D, kNT>(a, pg, c0 * kKeys, pl.len, kvh, x, li, g, lane);
-            for (int c = c0; c < c1; ++c) {
-                const int kb = c * kKeys;
-                if (c + 1 < c1) {
-                    pages_for(c + 1);
-                    load_codes<D, kNT>(a, pg, kb + kKeys, pl.len, kvh, y, li, g, lane);
-                }
+            auto load = [&](Codes<D>& x, int c) {
+                pages_for(c);
+                load_codes<D, kNT>(a, pg, c * kKeys, pl.len, kvh, x, li, g, lane);
+            };
+            auto use = [&](const Codes<D>& x, int c) {
                 // V's values to LDS, where the P.V product reads them transposed
 #pragma unroll
                 for (int j = 0; j < Codes<D>::VB; ++j) {
@@ -341,8 +344,17 @@ __global__ __launch_bounds__(64, (waves_per_cu(D, RT, kFp4) + 3) / 4) void paged
                         for (int t = 0; t < RT; ++t) s[t][u] = mfma<kBf16>(ka, qb[t][i], s[t][u]);
                     }
                 }
-                chunk(s, kb, (const char*)lds);
-                x = y;
+                chunk(s, c * kKeys, (const char*)lds);
+            };
+            Codes<D> x, y;   // in turn: the next chunk's codes are on their way while one is used
+            load(x, c0);
+            for (int c = c0;; c += 2) {
+                if (c + 1 < c1) load(y, c + 1);
+                use(x, c);
+                if (c + 1 >= c1) break;
+                if (c + 2 < c1) load(x, c + 2);
+                use(y, c + 1);
+                if (c + 2 >= c1) break;
             }
         } else {
             copy_chunk<D, kNT>(a, pg, c0 * kKeys, pl.len, kvh, lds, lane);
@@ -400,39 +412,72 @@ __global__ __launch_bounds__(64, (waves_per_cu(D, RT, kFp4) + 3) / 4) void paged
     }
 }
 
-// A workgroup per sequence and item: its rows from the parts that its shares left, zeros where the sequence has no keys.
+// A workgroup per row of q: from the parts that its item's shares left, D / 4 lanes for each of 1024 / D parts at a time; zeros where
+// the sequence has no keys.
 template <int D, bool kBf16>
 __global__ __launch_bounds__(256) void paged_join(PagedArgs a) {
-    const int b = (int)(blockIdx.x / a.items), item = (int)(blockIdx.x % a.items), hb = item % a.HB, kvh = item / a.HB;
+    constexpr int kLanes = D / 4, kGroups = 256 / kLanes, kFlight = 4;
+    __shared__ __attribute__((aligned(16))) f32x4 acc_s[kGroups][kLanes];
+    __shared__ float2 ml_s[kGroups];
+    const int R = a.nq * a.G;
+    const int b = (int)(blockIdx.x / (a.HK * R)), kvh = (int)(blockIdx.x / R % a.HK), rr = (int)(blockIdx.x % R);
+    const int r = rr % a.rows, item = kvh * a.HB + rr / a.rows;
     const int n = chunks_of(length_of(a, b));
-    long long first = 0, parts = 0;
+    const long long per = a.head[0], before = a.head[1 + b];   // of no meaning where n is 0
+    int parts = 0;
+    long long first = 0;
     if (n > 0) {
-        const long long per = a.head[0], begin = a.head[1 + b] * a.items + (long long)item * n;
-        first = begin / per;
-        parts = (begin + n - 1) / per - first + 1;
+        const long long begin = before * a.items + (long long)item * n;
+        first = quotient(begin, per);
+        parts = (int)(quotient(begin + n - 1, per) - first) + 1;
         if (parts == 1) return;   // written by its share
     }
-    const int R = a.nq * a.G, rows = min(a.rows, R - hb * a.rows);
-    for (int x = (int)threadIdx.x; x < rows * (D / 4); x += 256) {
-        const int r = x / (D / 4), d = x % (D / 4) * 4;
-        float M = kInitM, L = 0.f;
-        f32x4 acc{0.f, 0.f, 0.f, 0.f};
-        for (long long i = 0; i < parts; ++i) {
-            // the first part begins its item, the others go on with it
-            const size_t idx = ((size_t)(first + i) * 2 + (i == 0 ? 1 : 0)) * a.rows + r;
-            const float2 ml = *(const float2*)(a.part_ml + idx * 2);
-            const f32x4 v = *(const f32x4*)(a.part_o + idx * D + d);
-            const float top = fmaxf(M, ml.x), w0 = __builtin_amdgcn_exp2f(M - top), w1 = __builtin_amdgcn_exp2f(ml.x - top);
-            M = top;
-            L = L * w0 + ml.y * w1;
-            acc = acc * w0 + v * w1;
+    const int grp = (int)threadIdx.x / kLanes, d = (int)threadIdx.x % kLanes * 4;
+    // the first part begins its item, the others go on with it
+    auto place = [&](int i) { return ((size_t)(first + i) * 2 + (i == 0 ? 1 : 0)) * a.rows + r; };
+    float M = kInitM, L = 0.f;
+    f32x4 acc{0.f, 0.f, 0.f, 0.f};
+    for (int i0 = grp; i0 < parts; i0 += kGroups * kFlight) {   // parts in flight; those past the last re-read it, weighted 0
+        float2 ml[kFlight];
+        f32x4 v[kFlight];
+#pragma unroll
+        for (int k = 0; k < kFlight; ++k) {
+            const size_t idx = place(min(i0 + k * kGroups, parts - 1));
+            ml[k] = *(const float2*)(a.part_ml + idx * 2);
+            v[k] = *(const f32x4*)(a.part_o + idx * D + d);
         }
-        const float inv = L > 0.f ? 1.f / L : 1.f;
-        const int rr = hb * a.rows + r;
-        uint16_t* dst = a.o + (((size_t)b * a.nq + rr / a.G) * a.nQH + (size_t)kvh * a.G + rr % a.G) * D + d;
-        ((uint32_t*)dst)[0] = pack2<kBf16>(acc[0] * inv, acc[1] * inv);
-        ((uint32_t*)dst)[1] = pack2<kBf16>(acc[2] * inv, acc[3] * inv);
+        float top = M;
+#pragma unroll
+        for (int k = 0; k < kFlight; ++k) top = fmaxf(top, ml[k].x);
+        const float old = __builtin_amdgcn_exp2f(M - top);
+        M = top;
+        L *= old;
+        acc *= old;
+#pragma unroll
+        for (int k = 0; k < kFlight; ++k) {
+            const float w = i0 + k * kGroups < parts ? __builtin_amdgcn_exp2f(ml[k].x - M) : 0.f;
+            L = fmaf(w, ml[k].y, L);
+            acc += v[k] * w;
+        }
     }
+    acc_s[grp][d / 4] = acc;
+    if (d == 0) ml_s[grp] = make_float2(M, L);
+    __syncthreads();
+    if (grp > 0) return;
+#pragma unroll
+    for (int k = 1; k < kGroups; ++k) M = fmaxf(M, ml_s[k].x);
+    L = 0.f;
+    acc = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int k = 0; k < kGroups; ++k) {
+        const float w = __builtin_amdgcn_exp2f(ml_s[k].x - M);
+        L = fmaf(w, ml_s[k].y, L);
+        acc += acc_s[k][d / 4] * w;
+    }
+    const float inv = L > 0.f ? 1.f / L : 1.f;
+    uint16_t* dst = a.o + (((size_t)b * a.nq + rr / a.G) * a.nQH + (size_t)kvh * a.G + rr % a.G) * D + d;
+    ((uint32_t*)dst)[0] = pack2<kBf16>(acc[0] * inv, acc[1] * inv);
+    ((uint32_t*)dst)[1] = pack2<kBf16>(acc[2] * inv, acc[3] * inv);
 }
 
 // ---- plan -----------------------------------------------------------------------------------------
@@ -448,14 +493,13 @@ bool plan_paged(const cdna4_paged_cache& k, const cdna4_paged_decode_cfg& c, Pag
     if (c.nQHeads < 1 || c.nQHeads % k.nKVHeads || c.nq < 1 || c.nq > 16) return false;
     if (c.batch < 0 || c.batch >= 1 << 24) return false;
     const long long qrows = (long long)c.batch * c.nq * c.nQHeads;
-    if (c.nQHeads > 1 << 20 || qrows > (1LL << 26) - 4) return false;
+    if (c.nQHeads > 1 << 20 || qrows >= 1LL << 24) return false;   // a launch has fewer than 2^32 threads: 256 per row of q
     p.G = c.nQHeads / k.nKVHeads;
     const int R = p.G * c.nq;
     p.RT = R > 16 ? 2 : 1;
     p.HB = (R + 16 * p.RT - 1) / (16 * p.RT);
     p.items = k.nKVHeads * p.HB;
     p.rows = std::min(R, 16 * p.RT);
-    if ((long long)c.batch * p.items * 256 > 0xffffffffLL) return false;
     p.shares = device_cus() * waves_per_cu(k.D, p.RT, k.format == CDNA4_KV_MXFP4);
     p.head_bytes = align256(((size_t)c.batch + 1) * sizeof(long long));
     p.ml_bytes = align256((size_t)p.shares * 2 * p.rows * 2 * sizeof(float));
@@ -481,7 +525,7 @@ int launch_paged(const PagedArgs& a, const PagedPlan& p, bool fp4, hipStream_t s
         else launch_parts<D, 1, kBf16, false>(a, nt, s);
     }
     if (int e = launch_status()) return e;
-    paged_join<D, kBf16><<<(unsigned)((size_t)a.batch * a.items), 256, 0, s>>>(a);
+    paged_join<D, kBf16><<<(unsigned)((size_t)a.batch * a.nq * a.nQH), 256, 0, s>>>(a);
     return launch_status();
 }
 

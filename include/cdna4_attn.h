@@ -426,7 +426,7 @@ int cdna4_rope_append_paged(const cdna4_append_args* args, const cdna4_paged_cac
  * (cdna4_attn_decode_paged_workspace_size bytes, 16-byte aligned, no initialisation) holds what shares leave of rows that they
  * cut; calls that overlap must not share one. The plan is sized to the current device, so query the size with the device
  * current that the call will run on. batch == 0: nothing is done.
- * Invalid: nQHeads % nKVHeads != 0, nq not 1 .. 16, 2^24 sequences and more, 2^26 - 3 rows of q or more, q not 16-byte or o not 4-byte
+ * Invalid: nQHeads % nKVHeads != 0, nq not 1 .. 16, 2^24 rows of q (batch nq nQHeads) and more, q not 16-byte or o not 4-byte
  * aligned, a missing or small workspace.
  */
 typedef struct {
