@@ -26,7 +26,7 @@ using wave::xlane::Sum;
 
 constexpr int kKeys = 32;         // keys of a chunk
 constexpr int kMinChunks = 2;     // a share's chunks at least
-constexpr int kMaxParts = 64;     // shares that an item is cut into, but for the two at its ends
+constexpr int kMaxParts = 512;    // shares that an item is cut into, but for the two at its ends
 
 struct PagedArgs {
     const uint16_t* q;
@@ -412,11 +412,11 @@ __global__ __launch_bounds__(64, (waves_per_cu(D, RT, kFp4) + 3) / 4) void paged
     }
 }
 
-// A workgroup per row of q: from the parts that its item's shares left, D / 4 lanes for each of 1024 / D parts at a time; zeros where
+// A workgroup per row of q: from the parts that its item's shares left, D / 4 lanes for a part; zeros where
 // the sequence has no keys.
-template <int D, bool kBf16>
-__global__ __launch_bounds__(256) void paged_join(PagedArgs a) {
-    constexpr int kLanes = D / 4, kGroups = 256 / kLanes, kFlight = 4;
+template <int D, bool kBf16, int kThreads>
+__global__ __launch_bounds__(kThreads) void paged_join(PagedArgs a) {
+    constexpr int kLanes = D / 4, kGroups = kThreads / kLanes, kFlight = kThreads == 64 ? 2 : 8;
     __shared__ __attribute__((aligned(16))) f32x4 acc_s[kGroups][kLanes];
     __shared__ float2 ml_s[kGroups];
     const int R = a.nq * a.G;
@@ -437,14 +437,18 @@ __global__ __launch_bounds__(256) void paged_join(PagedArgs a) {
     auto place = [&](int i) { return ((size_t)(first + i) * 2 + (i == 0 ? 1 : 0)) * a.rows + r; };
     float M = kInitM, L = 0.f;
     f32x4 acc{0.f, 0.f, 0.f, 0.f};
-    for (int i0 = grp; i0 < parts; i0 += kGroups * kFlight) {   // parts in flight; those past the last re-read it, weighted 0
+    for (int i0 = grp; i0 < parts; i0 += kGroups * kFlight) {   // parts in flight
         float2 ml[kFlight];
         f32x4 v[kFlight];
 #pragma unroll
         for (int k = 0; k < kFlight; ++k) {
-            const size_t idx = place(min(i0 + k * kGroups, parts - 1));
-            ml[k] = *(const float2*)(a.part_ml + idx * 2);
-            v[k] = *(const f32x4*)(a.part_o + idx * D + d);
+            ml[k] = make_float2(kInitM, 0.f);
+            v[k] = f32x4{0.f, 0.f, 0.f, 0.f};
+            if (i0 + k * kGroups < parts) {
+                const size_t idx = place(i0 + k * kGroups);
+                ml[k] = *(const float2*)(a.part_ml + idx * 2);
+                v[k] = *(const f32x4*)(a.part_o + idx * D + d);
+            }
         }
         float top = M;
 #pragma unroll
@@ -455,7 +459,7 @@ __global__ __launch_bounds__(256) void paged_join(PagedArgs a) {
         acc *= old;
 #pragma unroll
         for (int k = 0; k < kFlight; ++k) {
-            const float w = i0 + k * kGroups < parts ? __builtin_amdgcn_exp2f(ml[k].x - M) : 0.f;
+            const float w = __builtin_amdgcn_exp2f(ml[k].x - M);
             L = fmaf(w, ml[k].y, L);
             acc += v[k] * w;
         }
@@ -516,7 +520,7 @@ void launch_parts(const PagedArgs& a, bool nt, hipStream_t s) {
 template <int D, bool kBf16>
 int launch_paged(const PagedArgs& a, const PagedPlan& p, bool fp4, hipStream_t s) {
     // pools larger than the Infinity Cache are read past it (stream::dma16)
-    const bool nt = 2.0 * a.pages * a.HK * a.page * row_bytes(D, fp4) > 256.0 * 1024 * 1024;
+    const bool nt = 2.0 * a.pages * a.HK * a.page * row_bytes(D, fp4) > 0.0;
     if (p.RT == 2) {
         if (fp4) launch_parts<D, 2, kBf16, true>(a, nt, s);
         else launch_parts<D, 2, kBf16, false>(a, nt, s);
@@ -525,7 +529,9 @@ int launch_paged(const PagedArgs& a, const PagedPlan& p, bool fp4, hipStream_t s
         else launch_parts<D, 1, kBf16, false>(a, nt, s);
     }
     if (int e = launch_status()) return e;
-    paged_join<D, kBf16><<<(unsigned)((size_t)a.batch * a.nq * a.nQH), 256, 0, s>>>(a);
+    const unsigned rows = (unsigned)((size_t)a.batch * a.nq * a.nQH);
+    if (a.shares < 4LL * a.batch * a.items) paged_join<D, kBf16, 64><<<rows, 64, 0, s>>>(a);   // few parts to an item
+    else paged_join<D, kBf16, 256><<<rows, 256, 0, s>>>(a);
     return launch_status();
 }
 

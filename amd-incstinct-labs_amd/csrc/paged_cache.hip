@@ -3,6 +3,8 @@
 // Append, for each head row x of a token: x' = x rsqrt(mean(x^2) + eps) w, then the pair (d, d + D/2) turned by the angle of its
 // position, y_lo = c_lo x'_lo - s_lo x'_hi, y_hi = c_hi x'_hi + s_hi x'_lo; queries go to q_out, keys and values to row
 // position % page of page tables[sequence][position / page].
+#include <algorithm>
+
 #include "paged.hpp"
 #include "wave_primitives/detail/xlane.hpp"
 
@@ -49,12 +51,14 @@ __device__ __forceinline__ uint2 narrow4(const float (&x)[4]) {
 
 // A row in D / 8 lanes: lane i holds elements 4 i .. 4 i + 3 of its lower half and the same of its upper one, so that
 // the pairs of the rotation are in one lane and a block of 32 in 8 neighbouring ones.
+constexpr int kAhead = 4;   // rounds whose loads a wave has in flight
 struct Angles { f32x4 c_lo, s_lo, c_hi, s_hi; };
 
-// Norm (w: null for none) and rotation in F.
+// Norm and rotation in F.
 template <class F, int D>
-__device__ __forceinline__ void norm_rope(F (&lo)[4], F (&hi)[4], const float (*w)[4], double eps, bool turn, const Angles& an) {
-    if (w) {
+__device__ __forceinline__ void norm_rope(F (&lo)[4], F (&hi)[4], bool norm, const float (&w_lo)[4], const float (&w_hi)[4], double eps, bool turn,
+                                          const Angles& an) {
+    if (norm) {
         F s = 0;
 #pragma unroll
         for (int e = 0; e < 4; ++e) s = fma(lo[e], lo[e], fma(hi[e], hi[e], s));
@@ -64,8 +68,8 @@ __device__ __forceinline__ void norm_rope(F (&lo)[4], F (&hi)[4], const float (*
         else r = 1.f / sqrtf(s * (1.f / D) + (float)eps);
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
-            lo[e] = lo[e] * r * (F)w[0][e];
-            hi[e] = hi[e] * r * (F)w[1][e];
+            lo[e] = lo[e] * r * (F)w_lo[e];
+            hi[e] = hi[e] * r * (F)w_hi[e];
         }
     }
     if (turn) {
@@ -111,13 +115,25 @@ __global__ __launch_bounds__(256) void append_paged(AppendArgs a) {
     }
     const size_t page_bytes = (size_t)a.page * row_bytes(D, kFp4);
     const size_t place = ((size_t)(placed ? page : 0) * a.HK) * page_bytes;
-    for (int j = 0; j < a.per_wave; ++j) {
-        const int slot = (chunk * a.per_wave + j) * kRows + lane / kLanes;
-        if (slot >= slots) break;
+    const uint16_t *q = (const uint16_t*)a.p.q + t * a.p.q_row, *k = (const uint16_t*)a.p.k + t * a.p.k_row, *v = (const uint16_t*)a.p.v + t * a.p.v_row;
+    const int slot0 = chunk * a.per_wave * kRows + lane / kLanes;
+    for (int j0 = 0; j0 < a.per_wave; j0 += kAhead) {
+      if (slot0 - lane / kLanes + j0 * kRows >= slots) break;
+      uint2 in_lo[kAhead], in_hi[kAhead];
+#pragma unroll
+      for (int j = 0; j < kAhead; ++j) {   // rows past the last re-read it
+        const int slot = min(slot0 + (j0 + j) * kRows, slots - 1);
+        const uint16_t* src = slot < a.p.nQHeads ? q + slot * D : slot < a.p.nQHeads + a.HK ? k + (slot - a.p.nQHeads) * D : v + (slot - a.p.nQHeads - a.HK) * D;
+        in_lo[j] = *(const uint2*)(src + 4 * i);
+        in_hi[j] = *(const uint2*)(src + D / 2 + 4 * i);
+      }
+#pragma unroll
+      for (int j = 0; j < kAhead; ++j) {
+        const int slot = slot0 + (j0 + j) * kRows;
+        if (slot >= slots || j0 + j >= a.per_wave) break;
         const bool is_q = slot < a.p.nQHeads, is_k = !is_q && slot < a.p.nQHeads + a.HK;
         const int h = is_q ? slot : is_k ? slot - a.p.nQHeads : slot - a.p.nQHeads - a.HK;
-        const uint16_t* src = is_q ? (const uint16_t*)a.p.q + t * a.p.q_row : is_k ? (const uint16_t*)a.p.k + t * a.p.k_row : (const uint16_t*)a.p.v + t * a.p.v_row;
-        const uint2 u_lo = *(const uint2*)(src + h * D + 4 * i), u_hi = *(const uint2*)(src + h * D + D / 2 + 4 * i);
+        const uint2 u_lo = in_lo[j], u_hi = in_hi[j];
         float lo[4], hi[4];
         widen4<kBf16>(u_lo, lo);
         widen4<kBf16>(u_hi, hi);
@@ -131,7 +147,7 @@ __global__ __launch_bounds__(256) void append_paged(AppendArgs a) {
                 double dlo[4], dhi[4];
 #pragma unroll
                 for (int e = 0; e < 4; ++e) { dlo[e] = lo[e]; dhi[e] = hi[e]; }
-                norm_rope<double, D>(dlo, dhi, a.p.k_norm ? wk : nullptr, a.p.eps, turn, an);
+                norm_rope<double, D>(dlo, dhi, a.p.k_norm != nullptr, wk[0], wk[1], a.p.eps, turn, an);
 #pragma unroll
                 for (int e = 0; e < 4; ++e) { lo[e] = round_to_odd(dlo[e]); hi[e] = round_to_odd(dhi[e]); }
             }
@@ -172,7 +188,13 @@ __global__ __launch_bounds__(256) void append_paged(AppendArgs a) {
                     r_lo = make_uint2(p[0] | p[1] << 16, p[2] | p[3] << 16);
                     r_hi = make_uint2(q[0] | q[1] << 16, q[2] | q[3] << 16);
                 } else if (normed || turn) {
-                    norm_rope<float, D>(lo, hi, normed ? (is_q ? wq : wk) : nullptr, a.p.eps, turn, an);
+                    float w_lo[4], w_hi[4];
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        w_lo[e] = is_q ? wq[0][e] : wk[0][e];
+                        w_hi[e] = is_q ? wq[1][e] : wk[1][e];
+                    }
+                    norm_rope<float, D>(lo, hi, normed, w_lo, w_hi, a.p.eps, turn, an);
                     r_lo = narrow4<kBf16>(lo);
                     r_hi = narrow4<kBf16>(hi);
                 }
@@ -187,6 +209,7 @@ __global__ __launch_bounds__(256) void append_paged(AppendArgs a) {
                 *(uint2*)(out + D / 2) = r_hi;
             }
         }
+      }
     }
 }
 
@@ -241,7 +264,9 @@ int launch_append(const cdna4_append_args& p, const cdna4_paged_cache& c, int dt
     a.HK = c.nKVHeads; a.page = c.page; a.lp = log2_of(c.page); a.pages = c.pages; a.max_pages = c.max_pages;
     a.table_stride = table_stride(c);
     const int rounds = (p.nQHeads + 2 * c.nKVHeads + kRows - 1) / kRows;
-    a.per_wave = (long long)p.T * rounds > kMaxTokens ? rounds : 1;
+    // a wave takes as many of its token's heads as leave the chip 16 waves per CU
+    const long long waves = 16LL * device_cus();
+    a.per_wave = (int)std::min<long long>(rounds, std::max<long long>(1, (long long)p.T * rounds / waves));
     a.chunks = (rounds + a.per_wave - 1) / a.per_wave;
     const unsigned grid = ceil_div((size_t)p.T * a.chunks, 4);
     const bool bf = dtype == CDNA4_BF16, fp4 = c.format == CDNA4_KV_MXFP4;
