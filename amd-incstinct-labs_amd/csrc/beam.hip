@@ -20,13 +20,12 @@ using wave::xlane::allreduce;
 using wave::xlane::Max;
 using wave::xlane::Sum;
 
-typedef uint32_t u32x2_u __attribute__((ext_vector_type(2), aligned(2)));   // rows of odd length start anywhere
-typedef float f32x4_u __attribute__((ext_vector_type(4), aligned(4)));
+typedef uint32_t u32x4_u __attribute__((ext_vector_type(4), aligned(2)));   // rows of odd length start anywhere
 
 constexpr int kMost = 64;      // beams of a group, continuations of a group
-constexpr int kVec = 4;        // logits per load of a lane
-constexpr int kUnroll = 4;     // loads of a lane in flight
-constexpr int kStep = 64 * kVec * kUnroll;   // logits of a wave at a time
+constexpr int kValues = 32;    // logits of a lane at a time
+template <int kDtype> constexpr int vec() { return kDtype == CDNA4_F32 ? 4 : 8; }   // logits of a load: 16 bytes
+constexpr int kStep = 64 * kValues;                                                   // logits of a wave at a time
 constexpr float kLowest = -3.402823466e38f, kLargest = 3.402823466e38f;
 
 struct RangeSum { double s; float m; int pad; };   // sum of e^(x - m) over a range
@@ -57,11 +56,47 @@ __device__ __forceinline__ uint64_t read_lane(uint64_t v, int lane) {
     return (uint64_t)hi << 32 | lo;
 }
 
-// The list's lanes hold keys in descending order; a new key takes its place and moves those below by one.
+// The list's lanes hold keys in descending order; a new key takes its place and moves those below by one lane.
 __device__ __forceinline__ uint64_t insert(uint64_t list, uint64_t key, int lane) {
     const int at = __popcll(__builtin_amdgcn_ballot_w64(list > key));
-    const uint64_t up = __shfl_up((unsigned long long)list, 1);
-    return lane < at ? list : lane == at ? key : up;
+    constexpr int kWaveShr1 = 0x138;
+    const uint32_t lo = (uint32_t)__builtin_amdgcn_update_dpp(0, (int)(uint32_t)list, kWaveShr1, 0xf, 0xf, false);
+    const uint32_t hi = (uint32_t)__builtin_amdgcn_update_dpp(0, (int)(uint32_t)(list >> 32), kWaveShr1, 0xf, 0xf, false);
+    return lane < at ? list : lane == at ? key : (uint64_t)hi << 32 | lo;
+}
+
+// The n-th largest of the lanes' values, bit by bit from the top.
+__device__ __forceinline__ uint32_t nth_largest(uint32_t v, int n) {
+    uint32_t t = 0;
+#pragma unroll 1
+    for (uint32_t bit = 0x80000000u; bit; bit >>= 1) {
+        const int c = __popcll(__builtin_amdgcn_ballot_w64(v >= (t | bit)));
+        if (c >= n) t |= bit;
+        if (c == n) break;   // no lower bit changes which n these are
+    }
+    return t;
+}
+
+// Keys of a lane into the list. Only what can be among the n best goes one by one: what is above the n-th best so far, or, before
+// there are n, what is no less than the n-th best of the lanes' largest (`top`: the order of a lane's largest).
+template <int kCount, class KeyAt, class OrderAt>
+__device__ __forceinline__ uint64_t merge(uint64_t list, int n, uint32_t top, KeyAt key_at, OrderAt order_at, int lane) {
+    const uint64_t nth = read_lane(list, n - 1);
+    const uint32_t floor = (uint32_t)(nth >> 32);
+    if (!__builtin_amdgcn_ballot_w64(top > floor || (nth != 0 && top == floor))) return list;
+    const uint32_t bound = nth ? floor : max(nth_largest(top, n), order_of(kLowest));
+#pragma unroll
+    for (int k = 0; k < kCount; ++k) {
+        uint64_t need = __builtin_amdgcn_ballot_w64(order_at(k) >= bound);
+        if (!need) continue;
+        const uint64_t key = key_at(k);
+        while (need) {
+            const uint64_t c = read_lane(key, __builtin_ctzll(need));
+            if (c > read_lane(list, n - 1)) list = insert(list, c, lane);
+            need &= need - 1;
+        }
+    }
+    return list;
 }
 
 __device__ __forceinline__ float logit(const cdna4_beam_args& p, int dtype, size_t at) {
@@ -70,8 +105,8 @@ __device__ __forceinline__ float logit(const cdna4_beam_args& p, int dtype, size
     return dtype == CDNA4_BF16 ? bf16_bits_to_f32(b) : f16_bits_to_f32(b);
 }
 
-// NaN as -inf, +inf as the largest value.
-__device__ __forceinline__ float cleaned(float x) { return x != x ? -INFINITY : fminf(x, kLargest); }
+// NaN as -inf, +inf as the largest value: the middle of the three, the least where one is NaN.
+__device__ __forceinline__ float cleaned(float x) { return __builtin_amdgcn_fmed3f(x, -INFINITY, kLargest); }
 
 __device__ __forceinline__ bool has_own(const cdna4_beam_args& p, int row) {   // continuations from its logits
     const float c = p.cum[row];
@@ -86,6 +121,7 @@ __device__ __forceinline__ float exp_of(float d) {
 
 template <int kDtype>
 __global__ __launch_bounds__(256) void beam_ranges(BeamArgs a) {
+    constexpr int kVec = vec<kDtype>(), kLoads = kValues / kVec;
     const int lane = (int)(threadIdx.x & 63u);
     const long long item = (long long)blockIdx.x * 4 + __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
     const int row = (int)(item / a.parts), part = (int)(item % a.parts);
@@ -95,44 +131,63 @@ __global__ __launch_bounds__(256) void beam_ranges(BeamArgs a) {
     float m = kLowest, s = 0.f;
     uint64_t list = 0;
     for (int i0 = 0; i0 < len; i0 += kStep) {
-        float x[kUnroll * kVec];
+        float x[kValues];
+        int from[kLoads];   // of each load, its first logit in the range
+        // Loads past the end are moved back to end with it; their logits before the lane's place are another lane's.
+        const bool tail = i0 + kStep > len;
+        if (a.p.V >= kVec) {
+            u32x4_u raw[kLoads];
 #pragma unroll
-        for (int u = 0; u < kUnroll; ++u) {
-            const int i = i0 + (u * 64 + lane) * kVec;
+            for (int u = 0; u < kLoads; ++u) {
+                const int i = i0 + (u * 64 + lane) * kVec;
+                from[u] = tail ? min(i, len - kVec) : i;
+                if constexpr (kDtype == CDNA4_F32) raw[u] = *(const u32x4_u*)((const float*)a.p.logits + ((long long)base + from[u]));
+                else raw[u] = *(const u32x4_u*)((const uint16_t*)a.p.logits + ((long long)base + from[u]));
+            }
 #pragma unroll
-            for (int e = 0; e < kVec; ++e) x[u * kVec + e] = i + e < len ? cleaned(logit(a.p, kDtype, base + i + e)) : -INFINITY;
+            for (int u = 0; u < kLoads; ++u)
+#pragma unroll
+                for (int e = 0; e < kVec; ++e) {
+                    const uint32_t w = raw[u][kDtype == CDNA4_F32 ? e : e / 2];
+                    x[u * kVec + e] = kDtype == CDNA4_F32 ? f32_from_bits(w)
+                                    : kDtype == CDNA4_BF16 ? f32_from_bits(e & 1 ? w & 0xffff0000u : w << 16)
+                                                           : f16_bits_to_f32(e & 1 ? w >> 16 : w & 0xffffu);
+                }
+        } else {   // a vocabulary below a load
+#pragma unroll
+            for (int u = 0; u < kLoads; ++u) {
+                from[u] = i0 + (u * 64 + lane) * kVec;
+#pragma unroll
+                for (int e = 0; e < kVec; ++e) {
+                    const int i = from[u] + e;
+                    x[u * kVec + e] = i < len ? logit(a.p, kDtype, base + i) : -INFINITY;
+                }
+            }
+        }
+#pragma unroll
+        for (int k = 0; k < kValues; ++k) x[k] = cleaned(x[k]);
+        if (tail) {
+#pragma unroll
+            for (int k = 0; k < kValues; ++k)
+                if (from[k / kVec] + k % kVec < i0 + (k / kVec * 64 + lane) * kVec) x[k] = -INFINITY;
         }
         float top = x[0];
 #pragma unroll
-        for (int k = 1; k < kUnroll * kVec; ++k) top = fmaxf(top, x[k]);
+        for (int k = 1; k < kValues; ++k) top = fmaxf(top, x[k]);
         if (top > m) {
             s *= exp_of(m - top);
             m = top;
         }
 #pragma unroll
-        for (int k = 0; k < kUnroll * kVec; ++k) s += exp_of(x[k] - m);
-#pragma unroll
-        for (int k = 0; k < kUnroll * kVec; ++k) {
-            const int token = begin + i0 + ((k / kVec) * 64 + lane) * kVec + k % kVec;
-            const uint64_t key = x[k] > -INFINITY ? key_of(x[k], token) : 0;
-            uint64_t need = __builtin_amdgcn_ballot_w64(key > read_lane(list, n - 1));
-            while (need) {
-                const uint64_t c = read_lane(key, __builtin_ctzll(need));
-                if (c > read_lane(list, n - 1)) list = insert(list, c, lane);
-                need &= need - 1;
-            }
-        }
+        for (int k = 0; k < kValues; ++k) s += exp_of(x[k] - m);
+        list = merge<kValues>(list, n, order_of(top + 0.f),
+                              [&](int k) { return key_of(x[k], begin + from[k / kVec] + k % kVec); },
+                              [&](int k) { return order_of(x[k] + 0.f); }, lane);
     }
     const float M = allreduce(m, Max{});
     const double S = allreduce((double)s * (double)exp_of(m - M), Sum{});
     if (lane < n) a.keys[((size_t)row * a.parts + part) * n + lane] = list;
     if (lane == 0) a.sums[(size_t)row * a.parts + part] = RangeSum{S, M, 0};
-}
-
-// Candidate i of a group, row i / n: by score, then lowest row, then lowest token.
-__device__ __forceinline__ bool before(double sx, int rx, int tx, double sy, int ry, int ty) {
-    if (sx != sy) return sx > sy;
-    return rx != ry ? rx < ry : tx < ty;
 }
 
 __global__ __launch_bounds__(1024) void beam_join(BeamArgs a) {
@@ -164,14 +219,16 @@ __global__ __launch_bounds__(1024) void beam_join(BeamArgs a) {
             S = allreduce(S, Sum{});
             uint64_t list = 0;
             const uint64_t* keys = a.keys + (size_t)row * a.parts * n;
-            for (int i0 = 0; i0 < a.parts * n; i0 += 64) {
-                const uint64_t key = i0 + lane < a.parts * n ? keys[i0 + lane] : 0;
-                uint64_t need = __builtin_amdgcn_ballot_w64(key > read_lane(list, n - 1));
-                while (need) {
-                    const uint64_t k = read_lane(key, __builtin_ctzll(need));
-                    if (k > read_lane(list, n - 1)) list = insert(list, k, lane);
-                    need &= need - 1;
+            const int all = a.parts * n;
+            for (int i0 = 0; i0 < all; i0 += 256) {
+                uint64_t key[4];
+#pragma unroll
+                for (int k = 0; k < 4; ++k) {
+                    const uint64_t x = keys[min(i0 + 64 * k + lane, all - 1)];
+                    key[k] = i0 + 64 * k + lane < all ? x : 0;
                 }
+                const uint64_t top = max(max(key[0], key[1]), max(key[2], key[3]));
+                list = merge<4>(list, n, (uint32_t)(top >> 32), [&](int k) { return key[k]; }, [&](int k) { return (uint32_t)(key[k] >> 32); }, lane);
             }
             if (list) {
                 sc = (double)cum + ((double)of_order((uint32_t)(list >> 32)) - (double)M) - log(S);
@@ -184,18 +241,29 @@ __global__ __launch_bounds__(1024) void beam_join(BeamArgs a) {
         }
     }
     __syncthreads();
-    const int all = beams * n;
+    // A candidate's place is the number of those before it, by score, then by row and place in the row's list: eight lanes count.
+    const int all = beams * n, sub = (int)threadIdx.x & 7;
     int mine = 0;
-    for (int i = (int)threadIdx.x; i < all; i += (int)blockDim.x) {
-        if (token[i] < 0) continue;
-        ++mine;
+    for (int i = (int)threadIdx.x >> 3; i < all; i += (int)blockDim.x >> 3) {
+        const double sc = score[i];
+        const bool there = token[i] >= 0;
         int rank = 0;
-        for (int j = 0; j < all && rank < n; ++j) rank += token[j] >= 0 && before(score[j], j / n, token[j], score[i], i / n, token[i]) ? 1 : 0;
-        if (rank < n) {
-            const size_t at = (size_t)blockIdx.x * n + rank;
-            a.p.scores[at] = (float)score[i];
-            a.p.parents[at] = row0 + i / n;
-            a.p.tokens[at] = token[i];
+        if (there)
+            for (int j = sub; j < all; j += 8) {
+                const double o = score[j];   // -inf where there is none
+                rank += o > sc || (o == sc && j < i) ? 1 : 0;
+            }
+        rank += wave::xlane::dpp_full<wave::xlane::kQuadXor1>(rank);
+        rank += wave::xlane::dpp_full<wave::xlane::kQuadXor2>(rank);
+        rank += wave::xlane::dpp_full<wave::xlane::kRowHalfMirror>(rank);
+        if (there && sub == 0) {
+            ++mine;
+            if (rank < n) {
+                const size_t at = (size_t)blockIdx.x * n + rank;
+                a.p.scores[at] = (float)sc;
+                a.p.parents[at] = row0 + i / n;
+                a.p.tokens[at] = token[i];
+            }
         }
     }
     if (mine) atomicAdd(&filled, mine);
@@ -215,8 +283,8 @@ bool plan_beam(long long rows, int V, int beams, int n, BeamPlan& p) {
     if (rows < 0 || rows >= 1 << 24 || V < 1 || V > 0x7fffffff - 65536 || beams < 1 || beams > kMost || n < 1 || n > kMost) return false;
     const long long waves = 8LL * device_cus();
     const long long want = rows ? std::max(1LL, waves / rows) : 1;
-    long long range = std::max((V + want - 1) / want, (long long)kStep);
-    range = (range + 3) & ~3LL;
+    long long range = std::max((V + want - 1) / want, (long long)kStep / 2);
+    range = (range + 511) & ~511LL;   // whole loads of a wave
     p.range = (int)range;
     p.parts = (int)((V + range - 1) / range);
     p.ws_bytes = (size_t)rows * p.parts * (n * sizeof(uint64_t) + sizeof(RangeSum)) + 16;
@@ -267,7 +335,7 @@ extern "C" int cdna4_beam_select(const cdna4_beam_args* args, int dtype, void* w
     else if (dtype == CDNA4_BF16) beam_ranges<CDNA4_BF16><<<grid, 256, 0, s>>>(a);
     else beam_ranges<CDNA4_F16><<<grid, 256, 0, s>>>(a);
     if (int e = launch_status()) return e;
-    const int waves = std::min(16, p.beams);
+    const int waves = std::max(4, std::min(16, p.beams));
     beam_join<<<(unsigned)p.groups, 64 * waves, 0, s>>>(a);
     return launch_status();
 }
