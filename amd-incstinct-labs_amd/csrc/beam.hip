@@ -90,9 +90,8 @@ __device__ __forceinline__ uint64_t merge(uint64_t list, int n, uint32_t top, Ke
         uint64_t need = __builtin_amdgcn_ballot_w64(order_at(k) >= bound);
         if (!need) continue;
         const uint64_t key = key_at(k);
-        while (need) {
-            const uint64_t c = read_lane(key, __builtin_ctzll(need));
-            if (c > read_lane(list, n - 1)) list = insert(list, c, lane);
+        while (need) {   // a key that is none of the n best goes behind them, or past the last lane
+            list = insert(list, read_lane(key, __builtin_ctzll(need)), lane);
             need &= need - 1;
         }
     }
@@ -113,11 +112,8 @@ __device__ __forceinline__ bool has_own(const cdna4_beam_args& p, int row) {   /
     return !(p.done && p.done[row]) && c > -INFINITY && c < INFINITY;
 }
 
-// e^d for d <= 0: v_exp_f32 of d log2(e) with the product's second term, so that a bias of the constant stays out of the sums.
-__device__ __forceinline__ float exp_of(float d) {
-    constexpr float kHi = 1.44269502f, kLo = 1.92596303e-8f;
-    return __builtin_amdgcn_exp2f(fmaf(d, kHi, d * kLo));
-}
+// e^d for d <= 0. The constant's rounding (1.3e-8 of it) moves a sum by 1.3e-8 times the mean of -d, alike in all rows.
+__device__ __forceinline__ float exp_of(float d) { return __builtin_amdgcn_exp2f(d * 1.44269502f); }
 
 template <int kDtype>
 __global__ __launch_bounds__(256) void beam_ranges(BeamArgs a) {
@@ -130,22 +126,34 @@ __global__ __launch_bounds__(256) void beam_ranges(BeamArgs a) {
     const size_t base = (size_t)row * a.p.logits_stride + begin;
     float m = kLowest, s = 0.f;
     uint64_t list = 0;
-    for (int i0 = 0; i0 < len; i0 += kStep) {
+    // Loads past the end are moved back to end with it; their logits before the lane's place are another lane's. A vocabulary
+    // below a load is read one by one.
+    const bool vectors = a.p.V >= kVec;
+    u32x4_u raw[kLoads];   // of the next step
+    auto place = [&](int i0, int u) { return i0 + (u * 64 + lane) * kVec; };
+    auto load = [&](int i0) {
+        if (!vectors) return;
+#pragma unroll
+        for (int u = 0; u < kLoads; ++u) {
+            const long long at = (long long)base + min(place(i0, u), len - kVec);
+            if constexpr (kDtype == CDNA4_F32) raw[u] = *(const u32x4_u*)((const float*)a.p.logits + at);
+            else raw[u] = *(const u32x4_u*)((const uint16_t*)a.p.logits + at);
+        }
+    };
+    // Logits that are NaN or +inf make the sum NaN: the range is then read once more with a look at each.
+    for (bool careful = false;; careful = true) {
+      m = kLowest;
+      s = 0.f;
+      list = 0;
+      load(0);
+      for (int i0 = 0; i0 < len; i0 += kStep) {
         float x[kValues];
         int from[kLoads];   // of each load, its first logit in the range
-        // Loads past the end are moved back to end with it; their logits before the lane's place are another lane's.
         const bool tail = i0 + kStep > len;
-        if (a.p.V >= kVec) {
-            u32x4_u raw[kLoads];
+        if (vectors) {
 #pragma unroll
             for (int u = 0; u < kLoads; ++u) {
-                const int i = i0 + (u * 64 + lane) * kVec;
-                from[u] = tail ? min(i, len - kVec) : i;
-                if constexpr (kDtype == CDNA4_F32) raw[u] = *(const u32x4_u*)((const float*)a.p.logits + ((long long)base + from[u]));
-                else raw[u] = *(const u32x4_u*)((const uint16_t*)a.p.logits + ((long long)base + from[u]));
-            }
-#pragma unroll
-            for (int u = 0; u < kLoads; ++u)
+                from[u] = min(place(i0, u), len - kVec);
 #pragma unroll
                 for (int e = 0; e < kVec; ++e) {
                     const uint32_t w = raw[u][kDtype == CDNA4_F32 ? e : e / 2];
@@ -153,23 +161,24 @@ __global__ __launch_bounds__(256) void beam_ranges(BeamArgs a) {
                                     : kDtype == CDNA4_BF16 ? f32_from_bits(e & 1 ? w & 0xffff0000u : w << 16)
                                                            : f16_bits_to_f32(e & 1 ? w >> 16 : w & 0xffffu);
                 }
-        } else {   // a vocabulary below a load
+            }
+            if (!tail) load(i0 + kStep);   // clamped to the end where the range ends with this step
+        } else {
 #pragma unroll
             for (int u = 0; u < kLoads; ++u) {
-                from[u] = i0 + (u * 64 + lane) * kVec;
+                from[u] = place(i0, u);
 #pragma unroll
-                for (int e = 0; e < kVec; ++e) {
-                    const int i = from[u] + e;
-                    x[u * kVec + e] = i < len ? logit(a.p, kDtype, base + i) : -INFINITY;
-                }
+                for (int e = 0; e < kVec; ++e) x[u * kVec + e] = from[u] + e < len ? logit(a.p, kDtype, base + from[u] + e) : -INFINITY;
             }
         }
+        if (careful) {
 #pragma unroll
-        for (int k = 0; k < kValues; ++k) x[k] = cleaned(x[k]);
+            for (int k = 0; k < kValues; ++k) x[k] = cleaned(x[k]);
+        }
         if (tail) {
 #pragma unroll
             for (int k = 0; k < kValues; ++k)
-                if (from[k / kVec] + k % kVec < i0 + (k / kVec * 64 + lane) * kVec) x[k] = -INFINITY;
+                if (from[k / kVec] + k % kVec < place(i0, k / kVec)) x[k] = -INFINITY;
         }
         float top = x[0];
 #pragma unroll
@@ -183,6 +192,8 @@ __global__ __launch_bounds__(256) void beam_ranges(BeamArgs a) {
         list = merge<kValues>(list, n, order_of(top + 0.f),
                               [&](int k) { return key_of(x[k], begin + from[k / kVec] + k % kVec); },
                               [&](int k) { return order_of(x[k] + 0.f); }, lane);
+      }
+      if (careful || !__builtin_amdgcn_ballot_w64(s != s)) break;
     }
     const float M = allreduce(m, Max{});
     const double S = allreduce((double)s * (double)exp_of(m - M), Sum{});
@@ -199,34 +210,40 @@ __global__ __launch_bounds__(1024) void beam_join(BeamArgs a) {
     if (threadIdx.x == 0) filled = 0;
     for (int b = wave; b < beams; b += waves) {
         const int row = row0 + b;
+        // all that the row needs is on its way at once; what a row without continuations of its own left there is not used
         const float cum = a.p.cum[row];
+        const int ended = a.p.done ? a.p.done[row] : 0;
+        const RangeSum* sums = a.sums + (size_t)row * a.parts;
+        const RangeSum first = sums[min(lane, a.parts - 1)];
+        const uint64_t* keys = a.keys + (size_t)row * a.parts * n;
+        const int all = a.parts * n;
+        uint64_t key[4];
+        auto load = [&](int i0) {
+#pragma unroll
+            for (int k = 0; k < 4; ++k) key[k] = keys[min(i0 + 64 * k + lane, all - 1)];
+        };
+        load(0);
         double sc = -INFINITY;
         int tok = -1;
-        if (a.p.done && a.p.done[row]) {
-            if (lane == 0 && cum > -INFINITY && cum < INFINITY) {
+        const bool fine = cum > -INFINITY && cum < INFINITY;
+        if (ended) {
+            if (lane == 0 && fine) {
                 sc = cum;
                 tok = a.p.eos;
             }
-        } else if (has_own(a.p, row)) {
-            float M = kLowest;
-            for (int i = lane; i < a.parts; i += 64) M = fmaxf(M, a.sums[(size_t)row * a.parts + i].m);
+        } else if (fine) {
+            float M = first.m;
+            for (int i = lane + 64; i < a.parts; i += 64) M = fmaxf(M, sums[i].m);
             M = allreduce(M, Max{});
-            double S = 0.0;
-            for (int i = lane; i < a.parts; i += 64) {
-                const RangeSum r = a.sums[(size_t)row * a.parts + i];
-                S += r.s * exp((double)r.m - (double)M);
-            }
+            double S = lane < a.parts ? first.s * exp((double)first.m - (double)M) : 0.0;
+            for (int i = lane + 64; i < a.parts; i += 64) S += sums[i].s * exp((double)sums[i].m - (double)M);
             S = allreduce(S, Sum{});
             uint64_t list = 0;
-            const uint64_t* keys = a.keys + (size_t)row * a.parts * n;
-            const int all = a.parts * n;
             for (int i0 = 0; i0 < all; i0 += 256) {
-                uint64_t key[4];
+                if (i0) load(i0);
 #pragma unroll
-                for (int k = 0; k < 4; ++k) {
-                    const uint64_t x = keys[min(i0 + 64 * k + lane, all - 1)];
-                    key[k] = i0 + 64 * k + lane < all ? x : 0;
-                }
+                for (int k = 0; k < 4; ++k)
+                    if (i0 + 64 * k + lane >= all) key[k] = 0;
                 const uint64_t top = max(max(key[0], key[1]), max(key[2], key[3]));
                 list = merge<4>(list, n, (uint32_t)(top >> 32), [&](int k) { return key[k]; }, [&](int k) { return (uint32_t)(key[k] >> 32); }, lane);
             }
@@ -249,6 +266,7 @@ __global__ __launch_bounds__(1024) void beam_join(BeamArgs a) {
         const bool there = token[i] >= 0;
         int rank = 0;
         if (there)
+#pragma unroll 4
             for (int j = sub; j < all; j += 8) {
                 const double o = score[j];   // -inf where there is none
                 rank += o > sc || (o == sc && j < i) ? 1 : 0;
@@ -276,12 +294,12 @@ __global__ __launch_bounds__(1024) void beam_join(BeamArgs a) {
     }
 }
 
-// Ranges of a row: enough of them for eight waves per CU, none shorter than a wave's step.
+// Ranges of a row: enough of them for sixteen waves per CU, none shorter than a wave's step.
 struct BeamPlan { int parts, range; size_t ws_bytes; };
 
 bool plan_beam(long long rows, int V, int beams, int n, BeamPlan& p) {
     if (rows < 0 || rows >= 1 << 24 || V < 1 || V > 0x7fffffff - 65536 || beams < 1 || beams > kMost || n < 1 || n > kMost) return false;
-    const long long waves = 8LL * device_cus();
+    const long long waves = 16LL * device_cus();
     const long long want = rows ? std::max(1LL, waves / rows) : 1;
     long long range = std::max((V + want - 1) / want, (long long)kStep / 2);
     range = (range + 511) & ~511LL;   // whole loads of a wave
