@@ -79,15 +79,16 @@ __device__ __forceinline__ uint32_t nth_largest(uint32_t v, int n) {
 
 // Keys of a lane into the list. Only what can be among the n best goes one by one: what is above the n-th best so far, or, before
 // there are n, what is no less than the n-th best of the lanes' largest (`top`: the order of a lane's largest).
-template <int kCount, class KeyAt, class OrderAt>
-__device__ __forceinline__ uint64_t merge(uint64_t list, int n, uint32_t top, KeyAt key_at, OrderAt order_at, int lane) {
+// key_at(k): a lane's k-th key; reaches(b): a test of whether the k-th is of order b or more.
+template <int kCount, class KeyAt, class Reaches>
+__device__ __forceinline__ uint64_t merge(uint64_t list, int n, uint32_t top, KeyAt key_at, Reaches reaches, int lane) {
     const uint64_t nth = read_lane(list, n - 1);
     const uint32_t floor = (uint32_t)(nth >> 32);
     if (!__builtin_amdgcn_ballot_w64(top > floor || (nth != 0 && top == floor))) return list;
-    const uint32_t bound = nth ? floor : max(nth_largest(top, n), order_of(kLowest));
+    const auto test = reaches(nth ? floor : max(nth_largest(top, n), order_of(kLowest)));
 #pragma unroll
     for (int k = 0; k < kCount; ++k) {
-        uint64_t need = __builtin_amdgcn_ballot_w64(order_at(k) >= bound);
+        uint64_t need = __builtin_amdgcn_ballot_w64(test(k));
         if (!need) continue;
         const uint64_t key = key_at(k);
         while (need) {   // a key that is none of the n best goes behind them, or past the last lane
@@ -121,7 +122,8 @@ __global__ __launch_bounds__(256) void beam_ranges(BeamArgs a) {
     const int lane = (int)(threadIdx.x & 63u);
     const long long item = (long long)blockIdx.x * 4 + __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
     const int row = (int)(item / a.parts), part = (int)(item % a.parts);
-    if (row >= a.p.groups * a.p.beams || !has_own(a.p, row)) return;
+    if (row >= a.p.groups * a.p.beams) return;
+    const bool own = has_own(a.p, row);   // waited for behind the first logits
     const int n = a.p.n, begin = part * a.range, len = min(a.range, a.p.V - begin);
     const size_t base = (size_t)row * a.p.logits_stride + begin;
     float m = kLowest, s = 0.f;
@@ -141,11 +143,13 @@ __global__ __launch_bounds__(256) void beam_ranges(BeamArgs a) {
         }
     };
     // Logits that are NaN or +inf make the sum NaN: the range is then read once more with a look at each.
+    load(0);
+    if (!own) return;
     for (bool careful = false;; careful = true) {
       m = kLowest;
       s = 0.f;
       list = 0;
-      load(0);
+      if (careful) load(0);
       for (int i0 = 0; i0 < len; i0 += kStep) {
         float x[kValues];
         int from[kLoads];   // of each load, its first logit in the range
@@ -191,7 +195,7 @@ __global__ __launch_bounds__(256) void beam_ranges(BeamArgs a) {
         for (int k = 0; k < kValues; ++k) s += exp_of(x[k] - m);
         list = merge<kValues>(list, n, order_of(top + 0.f),
                               [&](int k) { return key_of(x[k], begin + from[k / kVec] + k % kVec); },
-                              [&](int k) { return order_of(x[k] + 0.f); }, lane);
+                              [&](uint32_t b) { return [&x, f = of_order(b)](int k) { return x[k] >= f; }; }, lane);
       }
       if (careful || !__builtin_amdgcn_ballot_w64(s != s)) break;
     }
@@ -245,7 +249,7 @@ __global__ __launch_bounds__(1024) void beam_join(BeamArgs a) {
                 for (int k = 0; k < 4; ++k)
                     if (i0 + 64 * k + lane >= all) key[k] = 0;
                 const uint64_t top = max(max(key[0], key[1]), max(key[2], key[3]));
-                list = merge<4>(list, n, (uint32_t)(top >> 32), [&](int k) { return key[k]; }, [&](int k) { return (uint32_t)(key[k] >> 32); }, lane);
+                list = merge<4>(list, n, (uint32_t)(top >> 32), [&](int k) { return key[k]; }, [&](uint32_t b) { return [&key, b](int k) { return (uint32_t)(key[k] >> 32) >= b; }; }, lane);
             }
             if (list) {
                 sc = (double)cum + ((double)of_order((uint32_t)(list >> 32)) - (double)M) - log(S);
