@@ -77,15 +77,14 @@ __device__ __forceinline__ uint32_t nth_largest(uint32_t v, int n) {
     return t;
 }
 
-// Keys of a lane into the list. Only what can be among the n best goes one by one: what is above the n-th best so far, or, before
-// there are n, what is no less than the n-th best of the lanes' largest (`top`: the order of a lane's largest).
-// key_at(k): a lane's k-th key; reaches(b): a test of whether the k-th is of order b or more.
+// Keys of a lane into the list, those whose order reaches `least` and that of the n-th best so far, one by one.
+// top: the order of the lane's largest; key_at(k): its k-th key; reaches(b): a test of whether the k-th is of order b or more.
 template <int kCount, class KeyAt, class Reaches>
-__device__ __forceinline__ uint64_t merge(uint64_t list, int n, uint32_t top, KeyAt key_at, Reaches reaches, int lane) {
+__device__ __forceinline__ uint64_t merge(uint64_t list, int n, uint32_t least, uint32_t top, KeyAt key_at, Reaches reaches, int lane) {
     const uint64_t nth = read_lane(list, n - 1);
-    const uint32_t floor = (uint32_t)(nth >> 32);
-    if (!__builtin_amdgcn_ballot_w64(top > floor || (nth != 0 && top == floor))) return list;
-    const auto test = reaches(nth ? floor : max(nth_largest(top, n), order_of(kLowest)));
+    const uint32_t bound = max(max(least, (uint32_t)(nth >> 32)), order_of(kLowest));
+    if (!__builtin_amdgcn_ballot_w64(top >= bound)) return list;
+    const auto test = reaches(bound);
 #pragma unroll
     for (int k = 0; k < kCount; ++k) {
         uint64_t need = __builtin_amdgcn_ballot_w64(test(k));
@@ -105,8 +104,8 @@ __device__ __forceinline__ float logit(const cdna4_beam_args& p, int dtype, size
     return dtype == CDNA4_BF16 ? bf16_bits_to_f32(b) : f16_bits_to_f32(b);
 }
 
-// NaN as -inf, +inf as the largest value: the middle of the three, the least where one is NaN.
-__device__ __forceinline__ float cleaned(float x) { return __builtin_amdgcn_fmed3f(x, -INFINITY, kLargest); }
+// NaN as -inf, +inf as the largest value.
+__device__ __forceinline__ float cleaned(float x) { return x != x ? -INFINITY : fminf(x, kLargest); }
 
 __device__ __forceinline__ bool has_own(const cdna4_beam_args& p, int row) {   // continuations from its logits
     const float c = p.cum[row];
@@ -126,6 +125,11 @@ __global__ __launch_bounds__(256) void beam_ranges(BeamArgs a) {
     const bool own = has_own(a.p, row);   // waited for behind the first logits
     const int n = a.p.n, begin = part * a.range, len = min(a.range, a.p.V - begin);
     const size_t base = (size_t)row * a.p.logits_stride + begin;
+    // Where a workgroup's four ranges are one row's, its waves share a bound: n logits of theirs, a quarter in each, are no less than
+    // the least of the waves' (n / 4)-th best so far. What the others have published may be old: a bound that is too low.
+    __shared__ volatile uint32_t quarter[4];
+    const bool shared = (a.parts & 3) == 0;
+    const int wave = __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
     float m = kLowest, s = 0.f;
     uint64_t list = 0;
     // Loads past the end are moved back to end with it; their logits before the lane's place are another lane's. A vocabulary
@@ -144,13 +148,14 @@ __global__ __launch_bounds__(256) void beam_ranges(BeamArgs a) {
     };
     // Logits that are NaN or +inf make the sum NaN: the range is then read once more with a look at each.
     load(0);
-    if (!own) return;
+    if (!own) return;   // all waves of a shared row
     for (bool careful = false;; careful = true) {
       m = kLowest;
       s = 0.f;
       list = 0;
       if (careful) load(0);
-      for (int i0 = 0; i0 < len; i0 += kStep) {
+      uint32_t least = 0;
+      for (int i0 = 0; i0 == 0 || i0 < len; i0 += kStep) {   // once also where the range is empty
         float x[kValues];
         int from[kLoads];   // of each load, its first logit in the range
         const bool tail = i0 + kStep > len;
@@ -193,9 +198,23 @@ __global__ __launch_bounds__(256) void beam_ranges(BeamArgs a) {
         }
 #pragma unroll
         for (int k = 0; k < kValues; ++k) s += exp_of(x[k] - m);
-        list = merge<kValues>(list, n, order_of(top + 0.f),
+        const uint32_t top_order = order_of(cleaned(top) + 0.f);
+        const bool share = shared && !careful;
+        if (i0 == 0) {
+            least = nth_largest(top_order, share ? (n + 3) / 4 : n);
+            if (share) {
+                if (lane == 0) quarter[wave] = least;
+                __syncthreads();   // every wave of the workgroup comes here once: a row's four
+            }
+        }
+        if (share) least = min(min(quarter[0], quarter[1]), min(quarter[2], quarter[3]));
+        list = merge<kValues>(list, n, least, top_order,
                               [&](int k) { return key_of(x[k], begin + from[k / kVec] + k % kVec); },
                               [&](uint32_t b) { return [&x, f = of_order(b)](int k) { return x[k] >= f; }; }, lane);
+        if (share) {
+            const uint32_t best = (uint32_t)(read_lane(list, (n + 3) / 4 - 1) >> 32);
+            if (lane == 0 && best > quarter[wave]) quarter[wave] = best;
+        }
       }
       if (careful || !__builtin_amdgcn_ballot_w64(s != s)) break;
     }
@@ -206,12 +225,18 @@ __global__ __launch_bounds__(256) void beam_ranges(BeamArgs a) {
 }
 
 __global__ __launch_bounds__(1024) void beam_join(BeamArgs a) {
+    // Candidates that can be among the group's n best: no less than the least of the rows' q-th best, q rows' share of n, of which
+    // the group has n.
     __shared__ double score[kMost * kMost];
-    __shared__ int token[kMost * kMost];   // -1: none
+    __shared__ int token[kMost * kMost], place[kMost * kMost];   // place: row n + place in the row's list
+    __shared__ double share[kMost];
     __shared__ int filled;
     const int lane = (int)(threadIdx.x & 63u), wave = __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
     const int waves = (int)blockDim.x >> 6, n = a.p.n, beams = a.p.beams, row0 = (int)blockIdx.x * beams;
     if (threadIdx.x == 0) filled = 0;
+    double held[kMost / 16];   // a wave has up to four rows (16 waves)
+    int said[kMost / 16];
+#pragma unroll 1
     for (int b = wave; b < beams; b += waves) {
         const int row = row0 + b;
         // all that the row needs is on its way at once; what a row without continuations of its own left there is not used
@@ -243,54 +268,64 @@ __global__ __launch_bounds__(1024) void beam_join(BeamArgs a) {
             for (int i = lane + 64; i < a.parts; i += 64) S += sums[i].s * exp((double)sums[i].m - (double)M);
             S = allreduce(S, Sum{});
             uint64_t list = 0;
+            uint32_t least = 0;
             for (int i0 = 0; i0 < all; i0 += 256) {
                 if (i0) load(i0);
 #pragma unroll
                 for (int k = 0; k < 4; ++k)
                     if (i0 + 64 * k + lane >= all) key[k] = 0;
                 const uint64_t top = max(max(key[0], key[1]), max(key[2], key[3]));
-                list = merge<4>(list, n, (uint32_t)(top >> 32), [&](int k) { return key[k]; }, [&](uint32_t b) { return [&key, b](int k) { return (uint32_t)(key[k] >> 32) >= b; }; }, lane);
+                if (i0 == 0) least = nth_largest((uint32_t)(top >> 32), n);
+                list = merge<4>(list, n, least, (uint32_t)(top >> 32), [&](int k) { return key[k]; }, [&](uint32_t b) { return [&key, b](int k) { return (uint32_t)(key[k] >> 32) >= b; }; }, lane);
             }
             if (list) {
                 sc = (double)cum + ((double)of_order((uint32_t)(list >> 32)) - (double)M) - log(S);
                 tok = (int)~(uint32_t)list;
             }
         }
-        if (lane < n) {
-            score[b * n + lane] = sc;
-            token[b * n + lane] = tok;
+        const int q = (n + beams - 1) / beams;
+        if (lane == q - 1) share[b] = sc;
+        held[b / waves] = sc;   // of the rows that this wave has
+        said[b / waves] = tok;
+    }
+    __syncthreads();
+    double least = lane < beams ? share[lane] : INFINITY;
+    least = allreduce(least, wave::xlane::Min{});
+    for (int b = wave; b < beams; b += waves) {
+        const bool in = lane < n && said[b / waves] >= 0 && held[b / waves] >= least;
+        const uint64_t mask = __builtin_amdgcn_ballot_w64(in);
+        int at = 0;
+        if (lane == 0) at = atomicAdd(&filled, __popcll(mask));
+        at = __builtin_amdgcn_readfirstlane(at) + __builtin_amdgcn_mbcnt_hi((uint32_t)(mask >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)mask, 0u));
+        if (in) {
+            score[at] = held[b / waves];
+            token[at] = said[b / waves];
+            place[at] = b * n + lane;
         }
     }
     __syncthreads();
     // A candidate's place is the number of those before it, by score, then by row and place in the row's list: eight lanes count.
-    const int all = beams * n, sub = (int)threadIdx.x & 7;
-    int mine = 0;
+    const int all = filled, sub = (int)threadIdx.x & 7;
     for (int i = (int)threadIdx.x >> 3; i < all; i += (int)blockDim.x >> 3) {
         const double sc = score[i];
-        const bool there = token[i] >= 0;
+        const int pl = place[i];
         int rank = 0;
-        if (there)
 #pragma unroll 4
-            for (int j = sub; j < all; j += 8) {
-                const double o = score[j];   // -inf where there is none
-                rank += o > sc || (o == sc && j < i) ? 1 : 0;
-            }
+        for (int j = sub; j < all; j += 8) {
+            const double o = score[j];
+            rank += o > sc || (o == sc && place[j] < pl) ? 1 : 0;
+        }
         rank += wave::xlane::dpp_full<wave::xlane::kQuadXor1>(rank);
         rank += wave::xlane::dpp_full<wave::xlane::kQuadXor2>(rank);
         rank += wave::xlane::dpp_full<wave::xlane::kRowHalfMirror>(rank);
-        if (there && sub == 0) {
-            ++mine;
-            if (rank < n) {
-                const size_t at = (size_t)blockIdx.x * n + rank;
-                a.p.scores[at] = (float)sc;
-                a.p.parents[at] = row0 + i / n;
-                a.p.tokens[at] = token[i];
-            }
+        if (sub == 0 && rank < n) {
+            const size_t at = (size_t)blockIdx.x * n + rank;
+            a.p.scores[at] = (float)sc;
+            a.p.parents[at] = row0 + pl / n;
+            a.p.tokens[at] = token[i];
         }
     }
-    if (mine) atomicAdd(&filled, mine);
-    __syncthreads();
-    for (int i = filled + (int)threadIdx.x; i < n; i += (int)blockDim.x) {   // places that nothing fills
+    for (int i = all + (int)threadIdx.x; i < n; i += (int)blockDim.x) {   // places that nothing fills
         const size_t at = (size_t)blockIdx.x * n + i;
         a.p.scores[at] = -INFINITY;
         a.p.parents[at] = -1;
@@ -298,17 +333,15 @@ __global__ __launch_bounds__(1024) void beam_join(BeamArgs a) {
     }
 }
 
-// Ranges of a row: enough of them for sixteen waves per CU, none shorter than a wave's step.
+// Ranges of a row: enough of them for sixteen waves per CU, none shorter than 1,024 logits.
 struct BeamPlan { int parts, range; size_t ws_bytes; };
 
 bool plan_beam(long long rows, int V, int beams, int n, BeamPlan& p) {
     if (rows < 0 || rows >= 1 << 24 || V < 1 || V > 0x7fffffff - 65536 || beams < 1 || beams > kMost || n < 1 || n > kMost) return false;
-    const long long waves = 16LL * device_cus();
-    const long long want = rows ? std::max(1LL, waves / rows) : 1;
-    long long range = std::max((V + want - 1) / want, (long long)kStep / 2);
-    range = (range + 511) & ~511LL;   // whole loads of a wave
-    p.range = (int)range;
-    p.parts = (int)((V + range - 1) / range);
+    // four waves of a workgroup on one row, unless it is short: they share a bound
+    p.parts = 1;
+    if (V >= 4096) p.parts = (int)std::max(4LL, std::min<long long>(V / 1024, rows ? 16LL * device_cus() / rows : 1) & ~3LL);
+    p.range = (int)(((long long)V + p.parts - 1) / p.parts + 7) & ~7;   // the last ranges may be empty
     p.ws_bytes = (size_t)rows * p.parts * (n * sizeof(uint64_t) + sizeof(RangeSum)) + 16;
     return (rows * p.parts + 3) / 4 * 256 <= 0xffffffffLL;
 }

@@ -114,6 +114,40 @@ def test_masks_and_values_that_are_not_finite():
     assert torch.equal(got[1][:, 0], torch.arange(0, 16, 4, dtype=torch.int32, device=DEV))
 
 
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("V", [4095, 4096, 4100, 5003, 40000])
+def test_ranges_of_a_row(V, dtype):
+    """Rows cut into ranges that share what they know: best logits all in one range, ranges of NaN or -inf, +inf in some, ends."""
+    x, cum = make(3, 6, V, dtype, seed=V)
+    q = V // 4
+    x[0, :q] += 40                                           # all best ones in the first range, in the last, at both ends
+    x[1, -q:] += 40
+    x[2, 0], x[2, -1] = 60.0, 60.0
+    x[3, :q] = float("nan")                                  # a range without any
+    x[4, q:] = float("nan")                                  # few left
+    x[5, q:2 * q] = -math.inf
+    x[6, 2 * q:] = -math.inf
+    x[7, 5::1000] = math.inf
+    x[8, 3 * q + 5] = math.inf
+    x[9] = -math.inf
+    x[9, V - 3] = 1.0
+    x[10, 1:] = float("nan")
+    x[11] = 2.0                                              # equal everywhere
+    x[12] = torch.linspace(-5, 5, V, device=DEV).to(dtype)   # the best ones come last
+    x[13] = torch.linspace(5, -5, V, device=DEV).to(dtype)
+    for n in (1, 5, 12, 64):
+        verify(x, cum, 6, n)
+
+
+@pytest.mark.parametrize("beams,n,V", [(64, 64, 9001), (1, 64, 50001), (16, 3, 6000), (17, 64, 5000)])
+def test_many_wanted(beams, n, V):
+    x, cum = make(2, beams, V, BF16, seed=n)
+    cum[1] = -math.inf
+    verify(x, cum, beams, n)
+    cum[:beams - 1] = -math.inf                              # one row has them all
+    verify(x, cum, beams, n)
+
+
 def test_beams_that_have_ended():
     x, cum = make(3, 4, 2000, F16, seed=3)
     done = torch.tensor([0, 1, 0, 5, 1, 1, 1, 1, 0, 0, 0, 0], dtype=torch.int32, device=DEV)
