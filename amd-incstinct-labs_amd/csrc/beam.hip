@@ -33,7 +33,7 @@ struct RangeSum { double s; float m; int pad; };   // sum of e^(x - m) over a ra
 struct BeamArgs {
     cdna4_beam_args p;
     int parts, range;        // ranges of a row, logits of a range (a multiple of 4)
-    uint64_t* keys;          // [rows][parts][n], 0: none
+    uint64_t* keys;          // [rows][n][parts], 0: none
     RangeSum* sums;          // [rows][parts]
 };
 
@@ -220,7 +220,7 @@ __global__ __launch_bounds__(256) void beam_ranges(BeamArgs a) {
     }
     const float M = allreduce(m, Max{});
     const double S = allreduce((double)s * (double)exp_of(m - M), Sum{});
-    if (lane < n) a.keys[((size_t)row * a.parts + part) * n + lane] = list;
+    if (lane < n) a.keys[((size_t)row * n + lane) * a.parts + part] = list;   // the ranges' best ones side by side
     if (lane == 0) a.sums[(size_t)row * a.parts + part] = RangeSum{S, M, 0};
 }
 
@@ -230,12 +230,13 @@ __global__ __launch_bounds__(1024) void beam_join(BeamArgs a) {
     __shared__ double score[kMost * kMost];
     __shared__ int token[kMost * kMost], place[kMost * kMost];   // place: row n + place in the row's list
     __shared__ double share[kMost];
+    __shared__ uint64_t best[16][64];   // of each wave
     __shared__ int filled;
     const int lane = (int)(threadIdx.x & 63u), wave = __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
     const int waves = (int)blockDim.x >> 6, n = a.p.n, beams = a.p.beams, row0 = (int)blockIdx.x * beams;
     if (threadIdx.x == 0) filled = 0;
     double held[kMost / 16];   // a wave has up to four rows (16 waves)
-    int said[kMost / 16];
+    int said[kMost / 16], where[kMost / 16];
 #pragma unroll 1
     for (int b = wave; b < beams; b += waves) {
         const int row = row0 + b;
@@ -253,7 +254,8 @@ __global__ __launch_bounds__(1024) void beam_join(BeamArgs a) {
         };
         load(0);
         double sc = -INFINITY;
-        int tok = -1;
+        int tok = -1, rank = lane, i0 = 0;   // rank: a lane's place in the row
+        uint64_t mine = 0;
         const bool fine = cum > -INFINITY && cum < INFINITY;
         if (ended) {
             if (lane == 0 && fine) {
@@ -261,38 +263,66 @@ __global__ __launch_bounds__(1024) void beam_join(BeamArgs a) {
                 tok = a.p.eos;
             }
         } else if (fine) {
+            rank = 0;
             float M = first.m;
             for (int i = lane + 64; i < a.parts; i += 64) M = fmaxf(M, sums[i].m);
             M = allreduce(M, Max{});
             double S = lane < a.parts ? first.s * exp((double)first.m - (double)M) : 0.0;
             for (int i = lane + 64; i < a.parts; i += 64) S += sums[i].s * exp((double)sums[i].m - (double)M);
             S = allreduce(S, Sum{});
-            uint64_t list = 0;
-            uint32_t least = 0;
-            for (int i0 = 0; i0 < all; i0 += 256) {
-                if (i0) load(i0);
+            // The keys that reach the n-th best of the lanes' largest, a few more than n as a rule: each lane takes one and counts
+            // those before it. Where they are more than 64 (equal logits), or the row's keys more than a load, into a list one by one.
+            auto tops = [&]() {
 #pragma unroll
                 for (int k = 0; k < 4; ++k)
-                    if (i0 + 64 * k + lane >= all) key[k] = 0;
-                const uint64_t top = max(max(key[0], key[1]), max(key[2], key[3]));
-                if (i0 == 0) least = nth_largest((uint32_t)(top >> 32), n);
-                list = merge<4>(list, n, least, (uint32_t)(top >> 32), [&](int k) { return key[k]; }, [&](uint32_t b) { return [&key, b](int k) { return (uint32_t)(key[k] >> 32) >= b; }; }, lane);
+                    if (64 * k + lane >= all - i0) key[k] = 0;
+                return (uint32_t)(max(max(key[0], key[1]), max(key[2], key[3])) >> 32);
+            };
+            const uint32_t least = max(nth_largest(tops(), n), order_of(kLowest));
+            int count = 0;
+            if (all <= 256) {
+#pragma unroll
+                for (int k = 0; k < 4; ++k) {
+                    const uint64_t in = __builtin_amdgcn_ballot_w64((uint32_t)(key[k] >> 32) >= least);
+                    const int at = count + (int)__builtin_amdgcn_mbcnt_hi((uint32_t)(in >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)in, 0u));
+                    if ((in >> lane & 1) && at < 64) best[wave][at] = key[k];
+                    count += __popcll(in);
+                }
             }
-            if (list) {
-                sc = (double)cum + ((double)of_order((uint32_t)(list >> 32)) - (double)M) - log(S);
-                tok = (int)~(uint32_t)list;
+            if (all <= 256 && count <= 64) {
+                __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");   // the other lanes' keys
+                __builtin_amdgcn_wave_barrier();
+                mine = lane < count ? best[wave][lane] : 0;
+#pragma unroll 4
+                for (int j = 0; j < count; ++j) rank += best[wave][j] > mine ? 1 : 0;
+            } else {
+                for (;;) {
+                    mine = merge<4>(mine, n, least, tops(), [&](int k) { return key[k]; },
+                                    [&](uint32_t b) { return [&key, b](int k) { return (uint32_t)(key[k] >> 32) >= b; }; }, lane);
+                    i0 += 256;
+                    if (i0 >= all) break;
+                    load(i0);
+                }
+                rank = lane;
+            }
+            if (mine) {
+                sc = (double)cum + ((double)of_order((uint32_t)(mine >> 32)) - (double)M) - log(S);
+                tok = (int)~(uint32_t)mine;
             }
         }
         const int q = (n + beams - 1) / beams;
-        if (lane == q - 1) share[b] = sc;
+        if (lane == 0) share[b] = -INFINITY;
+        __builtin_amdgcn_wave_barrier();
+        if (tok >= 0 && rank == q - 1) share[b] = sc;
         held[b / waves] = sc;   // of the rows that this wave has
-        said[b / waves] = tok;
+        said[b / waves] = rank < n ? tok : -1;
+        where[b / waves] = b * n + rank;
     }
     __syncthreads();
     double least = lane < beams ? share[lane] : INFINITY;
     least = allreduce(least, wave::xlane::Min{});
     for (int b = wave; b < beams; b += waves) {
-        const bool in = lane < n && said[b / waves] >= 0 && held[b / waves] >= least;
+        const bool in = said[b / waves] >= 0 && held[b / waves] >= least;
         const uint64_t mask = __builtin_amdgcn_ballot_w64(in);
         int at = 0;
         if (lane == 0) at = atomicAdd(&filled, __popcll(mask));
@@ -300,7 +330,7 @@ __global__ __launch_bounds__(1024) void beam_join(BeamArgs a) {
         if (in) {
             score[at] = held[b / waves];
             token[at] = said[b / waves];
-            place[at] = b * n + lane;
+            place[at] = where[b / waves];
         }
     }
     __syncthreads();
