@@ -78,15 +78,17 @@ __device__ __forceinline__ uint32_t nth_largest(uint32_t v, int n) {
 }
 
 // Keys of a lane into the list, those whose order reaches `least` and that of the n-th best so far, one by one.
-// top: the order of the lane's largest; key_at(k): its k-th key; reaches(b): a test of whether the k-th is of order b or more.
+// top: the order of the lane's largest; key_at(k): its k-th key; reaches(b): a test of whether the k-th is of order b or more. Of
+// kCount keys the first `count` are looked at, a multiple of 8.
 template <int kCount, class KeyAt, class Reaches>
-__device__ __forceinline__ uint64_t merge(uint64_t list, int n, uint32_t least, uint32_t top, KeyAt key_at, Reaches reaches, int lane) {
+__device__ __forceinline__ uint64_t merge(uint64_t list, int n, uint32_t least, uint32_t top, KeyAt key_at, Reaches reaches, int lane, int count = kCount) {
     const uint64_t nth = read_lane(list, n - 1);
     const uint32_t bound = max(max(least, (uint32_t)(nth >> 32)), order_of(kLowest));
     if (!__builtin_amdgcn_ballot_w64(top >= bound)) return list;
     const auto test = reaches(bound);
 #pragma unroll
     for (int k = 0; k < kCount; ++k) {
+        if (k % 8 == 0 && k >= count) break;
         uint64_t need = __builtin_amdgcn_ballot_w64(test(k));
         if (!need) continue;
         const uint64_t key = key_at(k);
@@ -159,45 +161,48 @@ __global__ __launch_bounds__(256) void beam_ranges(BeamArgs a) {
         float x[kValues];
         int from[kLoads];   // of each load, its first logit in the range
         const bool tail = i0 + kStep > len;
-        if (vectors) {
+        // Logits of the step, lane by lane, in eights: a range's last step has fewer, and what a wave does goes by them.
+        const int count = max(min(kValues, ((len - i0 + 64 * kVec - 1) / (64 * kVec) * kVec + 7) & ~7), 8);
+        const bool look = careful || !vectors;
+        float top = -INFINITY;
 #pragma unroll
-            for (int u = 0; u < kLoads; ++u) {
-                from[u] = min(place(i0, u), len - kVec);
+        for (int u = 0; u < kLoads; ++u) {
+            from[u] = vectors ? min(place(i0, u), len - kVec) : place(i0, u);
+            if (u * kVec >= count) continue;
+#pragma unroll
+            for (int e = 0; e < kVec; ++e) {
+                const uint32_t w = raw[u][kDtype == CDNA4_F32 ? e : e / 2];
+                x[u * kVec + e] = kDtype == CDNA4_F32 ? f32_from_bits(w)
+                                : kDtype == CDNA4_BF16 ? f32_from_bits(e & 1 ? w & 0xffff0000u : w << 16)
+                                                       : f16_bits_to_f32(e & 1 ? w >> 16 : w & 0xffffu);
+            }
+            if (look) {
 #pragma unroll
                 for (int e = 0; e < kVec; ++e) {
-                    const uint32_t w = raw[u][kDtype == CDNA4_F32 ? e : e / 2];
-                    x[u * kVec + e] = kDtype == CDNA4_F32 ? f32_from_bits(w)
-                                    : kDtype == CDNA4_BF16 ? f32_from_bits(e & 1 ? w & 0xffff0000u : w << 16)
-                                                           : f16_bits_to_f32(e & 1 ? w >> 16 : w & 0xffffu);
+                    float& y = x[u * kVec + e];
+                    if (!vectors) y = from[u] + e < len ? logit(a.p, kDtype, base + from[u] + e) : -INFINITY;
+                    y = cleaned(y);
                 }
             }
-            if (!tail) load(i0 + kStep);   // clamped to the end where the range ends with this step
-        } else {
+            if (tail) {
 #pragma unroll
-            for (int u = 0; u < kLoads; ++u) {
-                from[u] = place(i0, u);
-#pragma unroll
-                for (int e = 0; e < kVec; ++e) x[u * kVec + e] = from[u] + e < len ? logit(a.p, kDtype, base + from[u] + e) : -INFINITY;
+                for (int e = 0; e < kVec; ++e)
+                    if (from[u] + e < place(i0, u)) x[u * kVec + e] = -INFINITY;
             }
-        }
-        if (careful) {
 #pragma unroll
-            for (int k = 0; k < kValues; ++k) x[k] = cleaned(x[k]);
+            for (int e = 0; e < kVec; ++e) top = fmaxf(top, x[u * kVec + e]);
         }
-        if (tail) {
-#pragma unroll
-            for (int k = 0; k < kValues; ++k)
-                if (from[k / kVec] + k % kVec < place(i0, k / kVec)) x[k] = -INFINITY;
-        }
-        float top = x[0];
-#pragma unroll
-        for (int k = 1; k < kValues; ++k) top = fmaxf(top, x[k]);
+        if (!tail) load(i0 + kStep);   // clamped to the end where the range ends with this step
         if (top > m) {
             s *= exp_of(m - top);
             m = top;
         }
 #pragma unroll
-        for (int k = 0; k < kValues; ++k) s += exp_of(x[k] - m);
+        for (int u = 0; u < kLoads; ++u) {
+            if (u * kVec >= count) continue;
+#pragma unroll
+            for (int e = 0; e < kVec; ++e) s += exp_of(x[u * kVec + e] - m);
+        }
         const uint32_t top_order = order_of(cleaned(top) + 0.f);
         const bool share = shared && !careful;
         if (i0 == 0) {
@@ -210,7 +215,7 @@ __global__ __launch_bounds__(256) void beam_ranges(BeamArgs a) {
         if (share) least = min(min(quarter[0], quarter[1]), min(quarter[2], quarter[3]));
         list = merge<kValues>(list, n, least, top_order,
                               [&](int k) { return key_of(x[k], begin + from[k / kVec] + k % kVec); },
-                              [&](uint32_t b) { return [&x, f = of_order(b)](int k) { return x[k] >= f; }; }, lane);
+                              [&](uint32_t b) { return [&x, f = of_order(b)](int k) { return x[k] >= f; }; }, lane, count);
         if (share) {
             const uint32_t best = (uint32_t)(read_lane(list, (n + 3) / 4 - 1) >> 32);
             if (lane == 0 && best > quarter[wave]) quarter[wave] = best;
