@@ -768,17 +768,27 @@ def paged_pool_shape(cache: PagedCache) -> tuple:
 
 
 def _pools(K: torch.Tensor, V: torch.Tensor, cache: PagedCache, dtype, dev: int, layers: int = 1):
-    n = layers * cache.pages * cache.nKVHeads * cache.page
+    n = layers * cache.pages * cache.nKVHeads * cache.page * cache.D
     if cache.format == KV_MXFP4:
-        dtype, n = torch.uint8, n * (cache.D // 2 + cache.D // 32)
-    else:
-        n *= cache.D
+        dtype, n = torch.uint8, n // 2 + n // 32
     return _arg("K_pages", K, dtype, n, dev), _arg("V_pages", V, dtype, n, dev)
 
 
 def _table_size(cache: PagedCache, rows: int) -> int:
     """Entries that the tables of `rows` sequences span."""
-    return (rows - 1) * (cache.table_stride or cache.max_pages) + cache.max_pages if rows > 0 else 0
+    most = cache.max_pages
+    return (rows - 1) * (cache.table_stride or most) + most if rows > 0 else 0
+
+
+def _rows(name: str, t: torch.Tensor, dtype, dev: int, shape) -> int:
+    """Token stride of t [T][heads][D] with its heads side by side, 0 where it does not matter."""
+    if t.dtype is not dtype or t.get_device() != dev or t.shape != shape:
+        raise ValueError(f"{name} must be {dtype} {list(shape)} on GPU {dev}")
+    row, head, one = t.stride()
+    if one != 1 or (head != shape[2] and shape[1] > 1):
+        if t.numel():
+            raise ValueError(f"{name} must have its heads side by side")
+    return row if shape[0] > 1 else 0
 
 
 def rope_append_paged(q: Optional[torch.Tensor], k: torch.Tensor, v: torch.Tensor, K_pages: torch.Tensor, V_pages: torch.Tensor,
@@ -797,42 +807,42 @@ def rope_append_paged(q: Optional[torch.Tensor], k: torch.Tensor, v: torch.Tenso
         with _entered(dev, stream):
             return rope_append_paged(q, k, v, K_pages, V_pages, tables, positions, cache, q_out, seqs=seqs, cos=cos, sin=sin,
                                      q_norm=q_norm, k_norm=k_norm, eps=eps, k_out=k_out, v_out=v_out)
-    dt = _dtype(k)
-    T, HK, D = k.shape[0], cache.nKVHeads, cache.D
-
-    def rows(name, t, heads):
-        if t is None:
-            return 0, 0
-        if t.dtype is not dtype or t.get_device() != dev or t.shape[0] != T:
-            raise ValueError(f"{name} must have the dtype, GPU and tokens of k")
-        row, head = _token_major(name, t, T, heads, D)
-        if head != D:
-            raise ValueError(f"{name} must have its heads side by side")
-        return t.data_ptr(), row
-
-    HQ = 0
+    dt, D = _dtype(k), cache.D
+    T = k.shape[0]
+    kv, HQ = (T, cache.nKVHeads, D), 0
+    qp = qr = qo = qor = ko = kor = vo = vor = c = sn = max_pos = sp = qn = kn = 0
     if q is not None:
-        HQ = q.shape[1] if q.dim() == 3 else 0
+        qs = q.shape
+        HQ = qs[1] if len(qs) == 3 else 0
+        qs = (T, HQ, D)
+        qp, qr = q.data_ptr(), _rows("q", q, dtype, dev, qs)
         if q_out is None:
-            q_out = torch.empty((T, HQ, D), dtype=dtype, device=k.device)
+            q_out = torch.empty(qs, dtype=dtype, device=k.device)
+        qo, qor = q_out.data_ptr(), _rows("q_out", q_out, dtype, dev, qs)
     elif q_out is not None or q_norm is not None:
         raise ValueError("q_out and q_norm need q")
-    (qp, qr), (kp, kr), (vp, vr) = rows("q", q, HQ), rows("k", k, HK), rows("v", v, HK)
-    (qo, qor), (ko, kor), (vo, vor) = rows("q_out", q_out, HQ), rows("k_out", k_out, HK), rows("v_out", v_out, HK)
+    kr, vr = _rows("k", k, dtype, dev, kv), _rows("v", v, dtype, dev, kv)
+    if k_out is not None:
+        ko, kor = k_out.data_ptr(), _rows("k_out", k_out, dtype, dev, kv)
+    if v_out is not None:
+        vo, vor = v_out.data_ptr(), _rows("v_out", v_out, dtype, dev, kv)
     Kp, Vp = _pools(K_pages, V_pages, cache, dtype, dev)
     batch = tables.shape[0] if tables.dim() == 2 else 0
-    if seqs is None and batch < T:
+    if seqs is not None:
+        sp = _arg("seqs", seqs, _I32, T, dev)
+    elif batch < T:
         raise ValueError("without seqs there must be a table for every token")
-    max_pos = c = s = 0
     if cos is not None or sin is not None:
-        max_pos = cos.shape[0] if cos is not None else 0
-        c, s = _arg("cos", cos, _F32, max_pos * D, dev), _arg("sin", sin, _F32, max_pos * D, dev)
-        if cos.shape[-1] != D or max_pos * D == 0:
+        if cos is None or sin is None or cos.dim() != 2 or cos.shape[1] != D or cos.shape[0] == 0:
             raise ValueError("cos and sin must be [max_pos][D]")
-    a = AppendArgs(qp, kp, vp, qo, ko, vo, Kp, Vp, _arg("tables", tables, _I32, _table_size(cache, batch), dev),
-                   0 if seqs is None else _arg("seqs", seqs, _I32, T, dev), _arg("positions", positions, _I32, T, dev), c, s,
-                   0 if q_norm is None else _arg("q_norm", q_norm, dtype, D, dev),
-                   0 if k_norm is None else _arg("k_norm", k_norm, dtype, D, dev), eps, T, HQ, batch, max_pos, qr, kr, vr, qor, kor, vor)
+        max_pos = cos.shape[0]
+        c, sn = _arg("cos", cos, _F32, max_pos * D, dev), _arg("sin", sin, _F32, max_pos * D, dev)
+    if q_norm is not None:
+        qn = _arg("q_norm", q_norm, dtype, D, dev)
+    if k_norm is not None:
+        kn = _arg("k_norm", k_norm, dtype, D, dev)
+    a = AppendArgs(qp, k.data_ptr(), v.data_ptr(), qo, ko, vo, Kp, Vp, _arg("tables", tables, _I32, _table_size(cache, batch), dev), sp,
+                   _arg("positions", positions, _I32, T, dev), c, sn, qn, kn, eps, T, HQ, batch, max_pos, qr, kr, vr, qor, kor, vor)
     rc = lib().cdna4_rope_append_paged(ctypes.byref(a), ctypes.byref(cache), dt, torch._C._cuda_getCurrentRawStream(dev))
     if rc:
         raise CDNA4Error("cdna4_rope_append_paged", rc)
@@ -888,10 +898,9 @@ def paged_reorder(parents: torch.Tensor, tables: torch.Tensor, lens: torch.Tenso
     if _elsewhere(dev, stream):
         with _entered(dev, stream):
             return paged_reorder(parents, tables, lens, fresh, tables_out, lens_out, K_pages, V_pages, cache)
-    rows, rows_in = parents.numel(), tables.shape[0]
-    layers = K_pages.shape[0] if K_pages.dim() == len(paged_pool_shape(cache)) + 1 else 1
-    dtype = K_pages.dtype
-    if cache.format != KV_MXFP4 and dtype not in (torch.float16, torch.bfloat16):
+    rows, rows_in, dtype = parents.numel(), tables.shape[0], K_pages.dtype
+    layers = K_pages.shape[0] if K_pages.dim() == (4 if cache.format == KV_MXFP4 else 5) else 1
+    if cache.format != KV_MXFP4 and dtype is not torch.float16 and dtype is not torch.bfloat16:
         raise ValueError("pools must be fp16 or bf16")
     Kp, Vp = _pools(K_pages, V_pages, cache, dtype, dev, layers)
     rc = lib().cdna4_paged_reorder(_arg("parents", parents, _I32, rows, dev), _arg("tables", tables, _I32, _table_size(cache, rows_in), dev),
