@@ -252,7 +252,7 @@ __device__ __forceinline__ bool check_limits(f32x4 (&s)[RT][2], const float (&m)
 }
 
 // Waves that a CU holds: 16-bit rows as many as have a ring in its LDS, MXFP4 as the registers allow.
-constexpr int waves_per_cu(int D, int RT, bool fp4) { return fp4 ? (RT == 2 ? 8 : D == 128 ? 12 : 16) : D == 128 ? 5 : 10; }
+constexpr int waves_per_cu(int D, int RT, bool fp4) { return fp4 ? (RT == 2 ? 8 : D == 128 ? 12 : 16) : D == 128 ? 4 : 8; }
 
 // What a wave does next: chunks c0 .. c1 - 1 of an item's n, and the pages they begin in.
 struct Segment { int b, len, kvh, hb, c0, c1, n; Pages pg; };
