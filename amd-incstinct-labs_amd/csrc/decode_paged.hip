@@ -121,53 +121,46 @@ __device__ __forceinline__ Share share_of(const PagedArgs& a, int share, Window&
 
 // Pages of a sequence, 64 table entries at a time, one per lane; entries past its rows are not read.
 struct Pages {
-    const int* table;
-    int first, ids, most;   // most: entries with rows
-    __device__ __forceinline__ void load(const PagedArgs& a, int f, int lane) {
+    int first, ids;
+    __device__ __forceinline__ void load(const PagedArgs& a, int b, int len, int f, int lane) {
         first = f;
-        ids = min(max(table[min(f + lane, most - 1)], 0), a.pages - 1);
+        const int* table = a.tables + b * a.table_stride;
+        ids = min(max(table[min(f + lane, (len - 1) >> a.lp)], 0), a.pages - 1);
     }
 };
 
-// The page of key k, whose entry is among the loaded ones: lane by lane, or for a k that all lanes share.
-__device__ __forceinline__ int page_of(const PagedArgs& a, const Pages& pg, int k) { return __shfl(pg.ids, (k >> a.lp) - pg.first); }
-__device__ __forceinline__ int page_of_all(const PagedArgs& a, const Pages& pg, int k) {
-    return __builtin_amdgcn_readlane(pg.ids, (k >> a.lp) - pg.first);
+// Where the 16 rows of a head from key k on begin in the pools, k the same in every lane and its entry among the loaded ones. Rows past
+// the last one lie in its page or, past that, in some page of the sequence: they are read and come to nothing.
+__device__ __forceinline__ size_t rows_at(const PagedArgs& a, const Pages& pg, int k, int kvh, int head_bytes, int row_bytes) {
+    const int id = __builtin_amdgcn_readlane(pg.ids, (k >> a.lp) - pg.first);
+    return ((size_t)id * a.HK + kvh) * head_bytes + (size_t)((k & (a.page - 1)) * row_bytes);
 }
 
 // One chunk's K and V rows into a ring stage (K first), 16-bit rows. A chunk lies in one page, or, with pages of 16 rows, in two: the copies
-// of a whole chunk take their bases from the scalar unit, and a lane's offset within them differs from copy to copy by the swizzle
-// alone. The last chunk of a sequence goes row by row; rows past the end re-read the last one (masked).
+// take their bases from the scalar unit, and a lane's offset within them differs from copy to copy by the swizzle alone.
 template <int D, bool kNT>
-__device__ __forceinline__ void copy_chunk(const PagedArgs& a, const Pages& pg, int kb, int len, int kvh, uint16_t* stage, int lane) {
+__device__ __forceinline__ void copy_chunk(const PagedArgs& a, const Pages& pg, int kb, int kvh, uint16_t* stage, int lane) {
     constexpr int CPR = D / 8, NI = kKeys * CPR / 64, kRows = 64 / CPR;   // copies of K, rows of a copy
     uint16_t* const vstage = stage + kKeys * D;
-    const size_t head = (size_t)a.page * 2 * D;
-    const int mask = a.page - 1;
-    kb = scalar(kb);
-    kvh = scalar(kvh);
-    if (kb + kKeys <= len) {
-        size_t at[2];
+    size_t at[2];
 #pragma unroll
-        for (int h = 0; h < 2; ++h)
-            at[h] = ((size_t)page_of_all(a, pg, kb + 16 * h) * a.HK + kvh) * head + (size_t)((kb + 16 * h) & mask) * 2 * D;
-        const int r = lane / CPR, c = lane % CPR;
-        const uint32_t ko = (uint32_t)(r * 2 * D + (c ^ swz_k<D>(r)) * 16), vo = (uint32_t)(r * 2 * D + (c ^ swz_v<D>(r)) * 16);
+    for (int h = 0; h < 2; ++h) at[h] = rows_at(a, pg, scalar(kb) + 16 * h, scalar(kvh), a.page * 2 * D, 2 * D);
+    const int r = lane / CPR, c = lane % CPR;
+    const uint32_t ko = (uint32_t)(r * 2 * D + (c ^ swz_k<D>(r)) * 16), vo = (uint32_t)(r * 2 * D + (c ^ swz_v<D>(r)) * 16);
 #pragma unroll
-        for (int j = 0; j < NI; ++j)
-            stream::dma16_s<kNT>(a.K + at[j / (NI / 2)] + j % (NI / 2) * 1024, ko ^ (uint32_t)(swz_k<D>(j * kRows) << 4), stage + j * 512);
+    for (int j = 0; j < NI; ++j)
+        stream::dma16_s<kNT>(a.K + at[j / (NI / 2)] + j % (NI / 2) * 1024, ko ^ (uint32_t)(swz_k<D>(j * kRows) << 4), stage + j * 512);
 #pragma unroll
-        for (int j = 0; j < NI; ++j)
-            stream::dma16_s<kNT>(a.V + at[j / (NI / 2)] + j % (NI / 2) * 1024, vo ^ (uint32_t)(swz_v<D>(j * kRows) << 4), vstage + j * 512);
-        return;
-    }
+    for (int j = 0; j < NI; ++j)
+        stream::dma16_s<kNT>(a.V + at[j / (NI / 2)] + j % (NI / 2) * 1024, vo ^ (uint32_t)(swz_v<D>(j * kRows) << 4), vstage + j * 512);
+}
+
+// V rows of a chunk from the `live`-th on, which may hold anything: zeros, since their weights of zero do not undo what is not finite.
+template <int D>
+__device__ __forceinline__ void clear_rows(uint16_t* vstage, int live, int lane) {
 #pragma unroll
-    for (int j = 0; j < NI; ++j) {
-        const int p = j * 64 + lane, r = p / CPR, k = min(kb + r, len - 1);
-        const size_t at = ((size_t)page_of(a, pg, k) * a.HK + kvh) * head + (size_t)(k & mask) * 2 * D;
-        stream::dma16<kNT>(a.K + at + ((p % CPR) ^ swz_k<D>(r)) * 16, stage + j * 512);
-        stream::dma16<kNT>(a.V + at + ((p % CPR) ^ swz_v<D>(r)) * 16, vstage + j * 512);
-    }
+    for (int j = 0; j < kKeys * D / 512; ++j)
+        if ((j * 64 + lane) / (D / 8) >= live) *(u32x4*)(vstage + (j * 64 + lane) * 8) = u32x4{0u, 0u, 0u, 0u};
 }
 
 // MXFP4 rows in registers. K: lane (li, g) holds its g-th quarter of the rows that it has in the two K operand tiles, D / 4
@@ -185,43 +178,44 @@ struct Codes {
 template <int D, bool kNT>
 __device__ __forceinline__ void load_codes(const PagedArgs& a, const Pages& pg, int kb, int len, int kvh, Codes<D>& x, int li, int g, int lane) {
     constexpr int KW = Codes<D>::KW, VB = Codes<D>::VB, BPR = D / 32;   // blocks of a row
-    const size_t head = (size_t)a.page * (D / 2 + BPR);
-    const int mask = a.page - 1, scales = a.page * (D / 2);
     auto get = [&](auto* p) {
         if constexpr (kNT) return __builtin_nontemporal_load(p);
         else return *p;
     };
     using KV = uint32_t __attribute__((ext_vector_type(KW)));
-    auto put = [&](const char* kp, int row, int u) {   // K: a row's quarter and its scale
-        const KV w = get((const KV*)(kp + row * (D / 2) + g * (D / 8)));
+    // the first row of each half of the chunk: its codes, its scales
+    size_t at[2], sc[2];
 #pragma unroll
-        for (int i = 0; i < KW; ++i) x.k[u][i] = w[i];
-        x.ks[u] = *(const uint8_t*)(kp + scales + row * BPR + g * BPR / 4);
-    };
-    auto put_v = [&](const char* vp, int row, int blk, int j) {
-        x.v[j] = get((const u32x4*)(vp + row * (D / 2) + blk * 16));
-        x.vs[j] = *(const uint8_t*)(vp + scales + row * BPR + blk);
-    };
-    // K rows 8 (li / 4) + li % 4 + 4 u: lanes li < 8 in the first half of the chunk; V rows (64 j + lane) / BPR
-    const int kr = 8 * (li >> 2) + (li & 3);
-    if (kb + kKeys <= len && a.page > 16) {
-        const size_t at = ((size_t)page_of_all(a, pg, kb) * a.HK + kvh) * head;
-        const int row0 = kb & mask;
-#pragma unroll
-        for (int u = 0; u < 2; ++u) put(a.K + at, row0 + kr + 4 * u, u);
-#pragma unroll
-        for (int j = 0; j < VB; ++j) put_v(a.V + at, row0 + (64 * j + lane) / BPR, lane % BPR, j);
-        return;
+    for (int h = 0; h < 2; ++h) {
+        const int k = scalar(kb) + 16 * h;
+        const size_t head = rows_at(a, pg, k, scalar(kvh), a.page * (D / 2 + BPR), 0);
+        at[h] = head + (k & (a.page - 1)) * (D / 2);
+        sc[h] = head + a.page * (D / 2) + (k & (a.page - 1)) * BPR;
     }
+    // K rows 8 (li / 4) + li % 4 + 4 u: lanes li < 8 in the first half of the chunk
+    const int kr = 8 * (li >> 2 & 1) + (li & 3);
+    const char *kc = a.K + (li < 8 ? at[0] : at[1]), *ksc = a.K + (li < 8 ? sc[0] : sc[1]);
 #pragma unroll
     for (int u = 0; u < 2; ++u) {
-        const int k = min(kb + kr + 4 * u, len - 1);
-        put(a.K + ((size_t)page_of(a, pg, k) * a.HK + kvh) * head, k & mask, u);
+        const KV w = get((const KV*)(kc + ((kr + 4 * u) * (D / 2) + g * (D / 8))));
+#pragma unroll
+        for (int i = 0; i < KW; ++i) x.k[u][i] = w[i];
+        x.ks[u] = *(const uint8_t*)(ksc + ((kr + 4 * u) * BPR + g * BPR / 4));
     }
+    // V rows (64 j + lane) / BPR: copy j of D 128 is half j, lanes below 32 of D 64 are the first half
 #pragma unroll
     for (int j = 0; j < VB; ++j) {
-        const int k = min(kb + (64 * j + lane) / BPR, len - 1);
-        put_v(a.V + ((size_t)page_of(a, pg, k) * a.HK + kvh) * head, k & mask, lane % BPR, j);
+        const int r = (64 * j + lane) / BPR;
+        const bool second = VB == 2 ? j == 1 : lane >= 32;
+        const char *vc = a.V + (second ? at[1] : at[0]), *vsc = a.V + (second ? sc[1] : sc[0]);
+        x.v[j] = get((const u32x4*)(vc + ((r & 15) * (D / 2) + lane % BPR * 16)));
+        x.vs[j] = *(const uint8_t*)(vsc + ((r & 15) * BPR + lane % BPR));
+    }
+    if (kb + kKeys > len) {   // rows past the last: values of next to nothing whatever they hold, since their weights of zero do not undo
+                              // what is not finite
+#pragma unroll
+        for (int j = 0; j < VB; ++j)
+            if (kb + (64 * j + lane) / BPR >= len) x.vs[j] = 0;
     }
 }
 
@@ -261,7 +255,6 @@ template <int D, int RT, bool kBf16, bool kFp4, bool kNT>
 __global__ __launch_bounds__(64, (waves_per_cu(D, RT, kFp4) + 3) / 4) void paged_parts(PagedArgs a) {
     constexpr int ND = D / 32, NDT = D / 16, kStage = 2 * kKeys * D;
     constexpr int kCopies = 2 * kKeys * (D / 8) / 64;
-    constexpr bool kQueriesAhead = !kFp4 && RT == 1;   // a second set of query operands in registers
     // 16 bits: a ring of two chunks of K and V. MXFP4: one chunk of V as 16-bit values.
     __shared__ __attribute__((aligned(16))) uint16_t lds[kFp4 ? kKeys * D : 2 * kStage];
     const int lane = (int)threadIdx.x, li = lane & 15, g = lane >> 4, share = (int)blockIdx.x;
@@ -294,9 +287,7 @@ __global__ __launch_bounds__(64, (waves_per_cu(D, RT, kFp4) + 3) / 4) void paged
         s.c0 = c_next;
         s.c1 = min(n, c_next + left);
         if (item == 0 && c_next == 0 && lane == 0) a.head[1 + pl.b] = pl.before;
-        s.pg.table = a.tables + pl.b * a.table_stride;
-        s.pg.most = (pl.len + a.page - 1) >> a.lp;
-        s.pg.load(a, (s.c0 * kKeys) >> a.lp, lane);
+        s.pg.load(a, s.b, s.len, (s.c0 * kKeys) >> a.lp, lane);
         left -= s.c1 - s.c0;
         c_next = 0;
         if (left > 0 && ++item == a.items) {   // on to the next sequence that has keys
@@ -338,8 +329,8 @@ __global__ __launch_bounds__(64, (waves_per_cu(D, RT, kFp4) + 3) / 4) void paged
         }
     };
     auto pages_for = [&](Segment& s, int c) {   // the entries of chunk c's pages
-        const int last = (min((c + 1) * kKeys, s.len) - 1) >> a.lp;
-        if (last - s.pg.first >= 64) s.pg.load(a, (c * kKeys) >> a.lp, lane);
+        const int last = ((c + 1) * kKeys - 1) >> a.lp;
+        if (last - s.pg.first >= 64) s.pg.load(a, s.b, s.len, (c * kKeys) >> a.lp, lane);
     };
 
     Segment cur;
@@ -429,37 +420,50 @@ __global__ __launch_bounds__(64, (waves_per_cu(D, RT, kFp4) + 3) / 4) void paged
             }
             chunk(s, c * kKeys, (const char*)lds);
         };
-        do {
-            next_segment(cur);
-            Codes<D> x, y;   // in turn: the next chunk's codes are on their way while one is used
-            load(x, cur.c0);
+        // The next segment's pages are loaded a segment ahead, its first codes while the last ones of this are used.
+        Segment nxt;
+        Codes<D> x, y;   // in turn: the next chunk's codes are on their way while one is used
+        next_segment(cur);
+        load_codes<D, kNT>(a, cur.pg, cur.c0 * kKeys, cur.len, cur.kvh, x, li, g, lane);
+        for (;;) {
             load_q(cur, qb);
+            const bool more = left > 0;
+            if (more) next_segment(nxt);
             begin();
+            auto ahead = [&](Codes<D>& z, int c) {
+                if (c < cur.c1) load(z, c);
+                else if (more) load_codes<D, kNT>(a, nxt.pg, nxt.c0 * kKeys, nxt.len, nxt.kvh, z, li, g, lane);
+            };
+            bool in_y;   // where the next segment's codes are
             for (int c = cur.c0;; c += 2) {
-                if (c + 1 < cur.c1) load(y, c + 1);
+                ahead(y, c + 1);
                 use(x, c);
-                if (c + 1 >= cur.c1) break;
-                if (c + 2 < cur.c1) load(x, c + 2);
+                in_y = c + 1 >= cur.c1;
+                if (in_y) break;
+                ahead(x, c + 2);
                 use(y, c + 1);
                 if (c + 2 >= cur.c1) break;
             }
             finish();
-        } while (left > 0);
+            if (!more) break;
+            if (in_y) x = y;
+            cur = nxt;
+        }
     } else {
         // The copies go on across segments: the next one's first chunk is on its way while the last chunk of this is used, so
-        // its pages, and where registers allow its queries, are loaded a segment ahead.
+        // its pages and queries are loaded a segment ahead.
         Segment nxt;
-        u32x4 qn[kQueriesAhead ? RT : 1][ND];
+        u32x4 qn[RT][ND];
         bool more = false;   // nxt is there
         auto look_ahead = [&]() {
             more = left > 0;
             if (!more) return;
             next_segment(nxt);
-            if constexpr (kQueriesAhead) load_q(nxt, qn);
+            load_q(nxt, qn);
         };
         next_segment(cur);
         load_q(cur, qb);
-        copy_chunk<D, kNT>(a, cur.pg, cur.c0 * kKeys, cur.len, cur.kvh, lds, lane);
+        copy_chunk<D, kNT>(a, cur.pg, cur.c0 * kKeys, cur.kvh, lds, lane);
         begin();
         look_ahead();
         ready(qb);
@@ -469,12 +473,13 @@ __global__ __launch_bounds__(64, (waves_per_cu(D, RT, kFp4) + 3) / 4) void paged
             const bool last = c + 1 == cur.c1;
             if (!last) {
                 pages_for(cur, c + 1);
-                copy_chunk<D, kNT>(a, cur.pg, (c + 1) * kKeys, cur.len, cur.kvh, there, lane);
+                copy_chunk<D, kNT>(a, cur.pg, (c + 1) * kKeys, cur.kvh, there, lane);
                 asm volatile("s_waitcnt vmcnt(%0)" : : "n"(kCopies) : "memory");
             } else {
                 asm volatile("s_waitcnt vmcnt(0)" : : : "memory");
-                if (more) copy_chunk<D, kNT>(a, nxt.pg, nxt.c0 * kKeys, nxt.len, nxt.kvh, there, lane);
+                if (more) copy_chunk<D, kNT>(a, nxt.pg, nxt.c0 * kKeys, nxt.kvh, there, lane);
             }
+            if ((c + 1) * kKeys > cur.len) clear_rows<D>(here + kKeys * D, cur.len - c * kKeys, lane);
             f32x4 s[RT][2];
             qk_chunk<D, RT, kBf16>((const char*)here, off, qb, s, 0);
             chunk(s, c * kKeys, (const char*)(here + kKeys * D));
@@ -486,15 +491,12 @@ __global__ __launch_bounds__(64, (waves_per_cu(D, RT, kFp4) + 3) / 4) void paged
             if (!more) break;
             cur = nxt;
             c = cur.c0;
-            if constexpr (kQueriesAhead) {
 #pragma unroll
-                for (int i = 0; i < ND; ++i) qb[0][i] = qn[0][i];
-            } else {
-                load_q(cur, qb);
-            }
+            for (int t = 0; t < RT; ++t)
+#pragma unroll
+                for (int i = 0; i < ND; ++i) qb[t][i] = qn[t][i];
             begin();
             look_ahead();
-            if constexpr (!kQueriesAhead) ready(qb);
         }
     }
 }
@@ -618,7 +620,9 @@ int launch_paged(const PagedArgs& a, const PagedPlan& p, bool fp4, hipStream_t s
     }
     if (int e = launch_status()) return e;
     const unsigned rows = (unsigned)((size_t)a.batch * a.nq * a.nQH);
-    if (a.shares < 4LL * a.batch * a.items) paged_join<D, kBf16, 64><<<rows, 64, 0, s>>>(a);   // few parts to an item
+    // few parts to an item; more, and more rows than the chip holds workgroups of four waves
+    if (a.shares < 4LL * a.batch * a.items) paged_join<D, kBf16, 64><<<rows, 64, 0, s>>>(a);
+    else if (rows > 8u * (unsigned)device_cus()) paged_join<D, kBf16, 128><<<rows, 128, 0, s>>>(a);
     else paged_join<D, kBf16, 256><<<rows, 256, 0, s>>>(a);
     return launch_status();
 }
