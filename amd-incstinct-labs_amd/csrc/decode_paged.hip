@@ -176,7 +176,8 @@ struct Codes {
 };
 
 template <int D, bool kNT>
-__device__ __forceinline__ void load_codes(const PagedArgs& a, const Pages& pg, int kb, int len, int kvh, Codes<D>& x, int li, int g, int lane) {
+__device__ __forceinline__ void load_codes(const PagedArgs& a, const Pages& pg, int kb, int len, int kvh, Codes<D>& x, int lane) {
+    const int li = lane & 15, g = lane >> 4;
     constexpr int KW = Codes<D>::KW, VB = Codes<D>::VB, BPR = D / 32;   // blocks of a row
     auto get = [&](auto* p) {
         if constexpr (kNT) return __builtin_nontemporal_load(p);
@@ -248,23 +249,152 @@ __device__ __forceinline__ bool check_limits(f32x4 (&s)[RT][2], const float (&m)
 // Waves that a CU holds: 16-bit rows as many as have a ring in its LDS, MXFP4 as the registers allow.
 constexpr int waves_per_cu(int D, int RT, bool fp4) { return fp4 ? (RT == 2 ? 8 : D == 128 ? 12 : 16) : D == 128 ? 4 : 8; }
 
+// LDS of a wave, elements. 16 bits: a ring of two chunks of K and V. MXFP4: one chunk of V as 16-bit values.
+template <int D> constexpr int stage_elems() { return 2 * kKeys * D; }
+template <int D, bool kFp4> constexpr int wave_lds() { return kFp4 ? kKeys * D : 2 * stage_elems<D>(); }
+
+// A row block in a wave: queries, running maxima, sums and outputs. Row r of a kv head: query r / G, head kvh G + r % G.
+template <int D, int RT, bool kBf16, bool kFp4>
+struct RowBlock {
+    static constexpr int ND = D / 32, NDT = D / 16;
+    using Queries = u32x4[RT][ND];
+    const PagedArgs& a;
+    const int lane, li, g, R;
+    const LdsOffsets off;
+    Queries q;
+    int limit[RT];
+    f32x4 o[RT][NDT], lacc[RT];
+    float m[RT];
+
+    __device__ __forceinline__ RowBlock(const PagedArgs& args, int l)
+        : a(args), lane(l), li(l & 15), g(l >> 4), R(args.nq * args.G), off(lds_offsets<D>(l & 15, l >> 4)) {}
+
+    __device__ __forceinline__ size_t row_of(int b, int kvh, int r) const {
+        const int i = r / a.G;
+        return (((size_t)b * a.nq + i) * a.nQH + (size_t)kvh * a.G + (r - i * a.G)) * D;
+    }
+    __device__ __forceinline__ void load_q(int b, int kvh, int hb, Queries& to) const {
+#pragma unroll
+        for (int t = 0; t < RT; ++t) {
+            const uint16_t* src = a.q + row_of(b, kvh, min(hb * RT * 16 + t * 16 + li, R - 1));   // rows past the last repeat it, unused
+#pragma unroll
+            for (int c = 0; c < ND; ++c) to[t][c] = *(const u32x4*)(src + (kFp4 ? g * (D / 4) + c * 8 : c * 32 + g * 8));
+        }
+    }
+    __device__ __forceinline__ void ready() {   // the compiler waits for the queries here
+#pragma unroll
+        for (int t = 0; t < RT; ++t) {
+            if constexpr (ND == 4) asm volatile("" : "+v"(q[t][0]), "+v"(q[t][1]), "+v"(q[t][2]), "+v"(q[t][3]));
+            else asm volatile("" : "+v"(q[t][0]), "+v"(q[t][1]));
+        }
+    }
+    __device__ __forceinline__ void begin(int len, int hb) {
+#pragma unroll
+        for (int t = 0; t < RT; ++t) {
+            const int r = hb * RT * 16 + t * 16 + li;
+            limit[t] = r < R ? len - a.nq + 1 + r / a.G : len;
+            m[t] = kInitM;
+            lacc[t] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+            for (int d = 0; d < NDT; ++d) o[t][d] = f32x4{0.f, 0.f, 0.f, 0.f};
+        }
+    }
+    // scores of a chunk to weights, weights times V
+    __device__ __forceinline__ void weigh(f32x4 (&s)[RT][2], int kb, int len, const char* Vt) {
+        float lm[RT];
+        const bool need = check_limits<RT>(s, m, lm, kb, limit, kb + kKeys > len - a.nq + 1, a.sc, g);
+        if (__builtin_amdgcn_ballot_w64(need)) rescale_rows<D, RT>(lm, m, o, lacc, a.sc);
+        u32x4 pb[RT];
+        softmax_chunk<RT, kBf16>(s, m, pb, a.sc);
+        pv_chunk<D, RT, kBf16>(Vt, off, pb, o, lacc, 0);
+        if constexpr (kBf16) {
+            if (kb < kLoKeys) {   // the first keys: the weights' second bf16 term
+                softmax_lo_chunk<RT>(s, m, pb, a.sc);
+                pv_chunk<D, RT, true>(Vt, off, pb, o, lacc, 0);
+            }
+        }
+    }
+    // A chunk of 16-bit rows that is in a ring stage.
+    __device__ __forceinline__ void use(uint16_t* stage, int kb, int len) {
+        if (kb + kKeys > len) clear_rows<D>(stage + kKeys * D, len - kb, lane);
+        f32x4 s[RT][2];
+        qk_chunk<D, RT, kBf16>((const char*)stage, off, q, s, 0);
+        weigh(s, kb, len, (const char*)(stage + kKeys * D));
+    }
+    // A chunk of codes; V's values go to LDS, where the P.V product reads them transposed.
+    __device__ __forceinline__ void use(const Codes<D>& x, int kb, int len, uint16_t* vlds) {
+#pragma unroll
+        for (int j = 0; j < Codes<D>::VB; ++j) {
+            const int r = (64 * j + lane) / ND, blk = lane % ND;
+            const float f = f32_from_bits(x.vs[j] << 23);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) *(u32x4*)(vlds + r * D + ((4 * blk + i) ^ swz_v<D>(r)) * 8) = decode8<kBf16>(x.v[j][i], f);
+        }
+        f32x4 s[RT][2];
+#pragma unroll
+        for (int t = 0; t < RT; ++t)
+#pragma unroll
+            for (int u = 0; u < 2; ++u) s[t][u] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int u = 0; u < 2; ++u) {
+            const float f = f32_from_bits(x.ks[u] << 23);
+#pragma unroll
+            for (int i = 0; i < ND; ++i) {
+                const u32x4 ka = decode8<kBf16>(x.k[u][i], f);
+#pragma unroll
+                for (int t = 0; t < RT; ++t) s[t][u] = mfma<kBf16>(ka, q[t][i], s[t][u]);
+            }
+        }
+        weigh(s, kb, len, (const char*)vlds);
+    }
+    __device__ __forceinline__ void store(int b, int kvh, int hb) const {
+#pragma unroll
+        for (int t = 0; t < RT; ++t) {
+            const int r = hb * RT * 16 + t * 16 + li;
+            if (r >= R) continue;
+            const float inv = lacc[t][0] > 0.f ? 1.f / lacc[t][0] : 1.f;
+            uint16_t* dst = a.o + row_of(b, kvh, r) + g * 4;
+#pragma unroll
+            for (int d = 0; d < NDT; ++d) {
+                ((uint32_t*)(dst + d * 16))[0] = pack2<kBf16>(o[t][d][0] * inv, o[t][d][1] * inv);
+                ((uint32_t*)(dst + d * 16))[1] = pack2<kBf16>(o[t][d][2] * inv, o[t][d][3] * inv);
+            }
+        }
+    }
+    // (m, l, O) as they are: rows `first` on of ml and out, up to `rows` of them
+    __device__ __forceinline__ void store_part(float* ml, float* out, size_t first, int rows) const {
+#pragma unroll
+        for (int t = 0; t < RT; ++t) {
+            if (t * 16 + li >= rows) continue;
+            const size_t idx = first + t * 16 + li;
+            float* dst = out + idx * D + g * 4;
+#pragma unroll
+            for (int d = 0; d < NDT; ++d) *(f32x4*)(dst + d * 16) = o[t][d];
+            if (g == 0) *(float2*)(ml + idx * 2) = make_float2(m[t], lacc[t][0]);
+        }
+    }
+};
+
+template <int D> constexpr int copies() { return 2 * kKeys * (D / 8) / 64; }   // of a chunk's K and V
+
 // What a wave does next: chunks c0 .. c1 - 1 of an item's n, and the pages they begin in.
 struct Segment { int b, len, kvh, hb, c0, c1, n; Pages pg; };
 
+// The entries of chunk c's pages, loaded if they are not.
+__device__ __forceinline__ void pages_for(const PagedArgs& a, Segment& s, int c, int lane) {
+    const int last = ((c + 1) * kKeys - 1) >> a.lp;
+    if (last - s.pg.first >= 64) s.pg.load(a, s.b, s.len, (c * kKeys) >> a.lp, lane);
+}
+
+// ---- equal shares of all keys -----------------------------------------------------------------------
 template <int D, int RT, bool kBf16, bool kFp4, bool kNT>
 __global__ __launch_bounds__(64, (waves_per_cu(D, RT, kFp4) + 3) / 4) void paged_parts(PagedArgs a) {
-    constexpr int ND = D / 32, NDT = D / 16, kStage = 2 * kKeys * D;
-    constexpr int kCopies = 2 * kKeys * (D / 8) / 64;
-    // 16 bits: a ring of two chunks of K and V. MXFP4: one chunk of V as 16-bit values.
-    __shared__ __attribute__((aligned(16))) uint16_t lds[kFp4 ? kKeys * D : 2 * kStage];
-    const int lane = (int)threadIdx.x, li = lane & 15, g = lane >> 4, share = (int)blockIdx.x;
+    __shared__ __attribute__((aligned(16))) uint16_t lds[wave_lds<D, kFp4>()];
+    const int lane = (int)threadIdx.x, share = (int)blockIdx.x;
     Window w;
     const Share sh = share_of(a, share, w, lane);
     if (share == 0 && lane == 0) a.head[0] = sh.per;
     if (sh.begin >= sh.end) return;
-    const LdsOffsets off = lds_offsets<D>(li, g);
-    const size_t slot0 = (size_t)share * 2 * a.rows;
-    const int R = a.nq * a.G;
 
     // The share's segments one after another; their table entries are loaded as they are found.
     // The same in every lane, as all that follows from it; the compiler is told, and keeps it in scalar registers.
@@ -311,137 +441,39 @@ __global__ __launch_bounds__(64, (waves_per_cu(D, RT, kFp4) + 3) / 4) void paged
             }
         }
     };
-    // row r of a kv head: query r / G, head kvh G + r % G
-    auto load_q = [&](const Segment& s, u32x4 (&q)[RT][ND]) {
-#pragma unroll
-        for (int t = 0; t < RT; ++t) {
-            const int r = min(s.hb * RT * 16 + t * 16 + li, R - 1), i = r / a.G;   // rows past the last repeat it, unused
-            const uint16_t* src = a.q + (((size_t)s.b * a.nq + i) * a.nQH + (size_t)s.kvh * a.G + (r - i * a.G)) * D;
-#pragma unroll
-            for (int c = 0; c < ND; ++c) q[t][c] = *(const u32x4*)(src + (kFp4 ? g * (D / 4) + c * 8 : c * 32 + g * 8));
-        }
-    };
-    auto ready = [&](u32x4 (&q)[RT][ND]) {   // the compiler waits for the loads here
-#pragma unroll
-        for (int t = 0; t < RT; ++t) {
-            if constexpr (ND == 4) asm volatile("" : "+v"(q[t][0]), "+v"(q[t][1]), "+v"(q[t][2]), "+v"(q[t][3]));
-            else asm volatile("" : "+v"(q[t][0]), "+v"(q[t][1]));
-        }
-    };
-    auto pages_for = [&](Segment& s, int c) {   // the entries of chunk c's pages
-        const int last = ((c + 1) * kKeys - 1) >> a.lp;
-        if (last - s.pg.first >= 64) s.pg.load(a, s.b, s.len, (c * kKeys) >> a.lp, lane);
-    };
-
-    Segment cur;
-    u32x4 qb[RT][ND];
-    int limit[RT];
-    f32x4 o[RT][NDT], lacc[RT];
-    float m[RT];
-    auto begin = [&]() {
-#pragma unroll
-        for (int t = 0; t < RT; ++t) {
-            const int r = cur.hb * RT * 16 + t * 16 + li;
-            limit[t] = r < R ? cur.len - a.nq + 1 + r / a.G : cur.len;
-            m[t] = kInitM;
-            lacc[t] = f32x4{0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-            for (int d = 0; d < NDT; ++d) o[t][d] = f32x4{0.f, 0.f, 0.f, 0.f};
-        }
-    };
-    // scores of a chunk to weights, weights times V
-    auto chunk = [&](f32x4 (&s)[RT][2], int kb, const char* Vt) {
-        float lm[RT];
-        const bool need = check_limits<RT>(s, m, lm, kb, limit, kb + kKeys > cur.len - a.nq + 1, a.sc, g);
-        if (__builtin_amdgcn_ballot_w64(need)) rescale_rows<D, RT>(lm, m, o, lacc, a.sc);
-        u32x4 pb[RT];
-        softmax_chunk<RT, kBf16>(s, m, pb, a.sc);
-        pv_chunk<D, RT, kBf16>(Vt, off, pb, o, lacc, 0);
-        if constexpr (kBf16) {
-            if (kb < kLoKeys) {   // the first keys: the weights' second bf16 term
-                softmax_lo_chunk<RT>(s, m, pb, a.sc);
-                pv_chunk<D, RT, true>(Vt, off, pb, o, lacc, 0);
-            }
-        }
-    };
+    RowBlock<D, RT, kBf16, kFp4> rb(a, lane);
+    Segment cur, nxt;
+    bool more;   // nxt is there
     auto finish = [&]() {
-        const bool whole = cur.c0 == 0 && cur.c1 == cur.n;
-#pragma unroll
-        for (int t = 0; t < RT; ++t) {
-            const int r16 = t * 16 + li, r = cur.hb * RT * 16 + r16;
-            if (r >= R) continue;
-            if (whole) {
-                const float inv = lacc[t][0] > 0.f ? 1.f / lacc[t][0] : 1.f;
-                const int i = r / a.G;
-                uint16_t* dst = a.o + (((size_t)cur.b * a.nq + i) * a.nQH + (size_t)cur.kvh * a.G + (r - i * a.G)) * D + g * 4;
-#pragma unroll
-                for (int d = 0; d < NDT; ++d) {
-                    ((uint32_t*)(dst + d * 16))[0] = pack2<kBf16>(o[t][d][0] * inv, o[t][d][1] * inv);
-                    ((uint32_t*)(dst + d * 16))[1] = pack2<kBf16>(o[t][d][2] * inv, o[t][d][3] * inv);
-                }
-            } else {
-                const size_t idx = slot0 + (cur.c0 == 0 ? a.rows : 0) + r16;
-                float* dst = a.part_o + idx * D + g * 4;
-#pragma unroll
-                for (int d = 0; d < NDT; ++d) *(f32x4*)(dst + d * 16) = o[t][d];
-                if (g == 0) *(float2*)(a.part_ml + idx * 2) = make_float2(m[t], lacc[t][0]);
-            }
-        }
+        if (cur.c0 == 0 && cur.c1 == cur.n) rb.store(cur.b, cur.kvh, cur.hb);
+        else rb.store_part(a.part_ml, a.part_o, ((size_t)share * 2 + (cur.c0 == 0 ? 1 : 0)) * a.rows, min(a.rows, rb.R - cur.hb * RT * 16));
     };
-
+    next_segment(cur);
     if constexpr (kFp4) {
-        auto load = [&](Codes<D>& x, int c) {
-            pages_for(cur, c);
-            load_codes<D, kNT>(a, cur.pg, c * kKeys, cur.len, cur.kvh, x, li, g, lane);
-        };
-        auto use = [&](const Codes<D>& x, int c) {
-            // V's values to LDS, where the P.V product reads them transposed
-#pragma unroll
-            for (int j = 0; j < Codes<D>::VB; ++j) {
-                const int r = (64 * j + lane) / ND, blk = lane % ND;
-                const float f = f32_from_bits(x.vs[j] << 23);
-#pragma unroll
-                for (int i = 0; i < 4; ++i) *(u32x4*)(lds + r * D + ((4 * blk + i) ^ swz_v<D>(r)) * 8) = decode8<kBf16>(x.v[j][i], f);
-            }
-            f32x4 s[RT][2];
-#pragma unroll
-            for (int t = 0; t < RT; ++t)
-#pragma unroll
-                for (int u = 0; u < 2; ++u) s[t][u] = f32x4{0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-            for (int u = 0; u < 2; ++u) {
-                const float f = f32_from_bits(x.ks[u] << 23);
-#pragma unroll
-                for (int i = 0; i < ND; ++i) {
-                    const u32x4 ka = decode8<kBf16>(x.k[u][i], f);
-#pragma unroll
-                    for (int t = 0; t < RT; ++t) s[t][u] = mfma<kBf16>(ka, qb[t][i], s[t][u]);
-                }
-            }
-            chunk(s, c * kKeys, (const char*)lds);
-        };
         // The next segment's pages are loaded a segment ahead, its first codes while the last ones of this are used.
-        Segment nxt;
         Codes<D> x, y;   // in turn: the next chunk's codes are on their way while one is used
-        next_segment(cur);
-        load_codes<D, kNT>(a, cur.pg, cur.c0 * kKeys, cur.len, cur.kvh, x, li, g, lane);
+        load_codes<D, kNT>(a, cur.pg, cur.c0 * kKeys, cur.len, cur.kvh, x, lane);
         for (;;) {
-            load_q(cur, qb);
-            const bool more = left > 0;
+            rb.load_q(cur.b, cur.kvh, cur.hb, rb.q);
+            more = left > 0;
             if (more) next_segment(nxt);
-            begin();
+            rb.begin(cur.len, cur.hb);
             auto ahead = [&](Codes<D>& z, int c) {
-                if (c < cur.c1) load(z, c);
-                else if (more) load_codes<D, kNT>(a, nxt.pg, nxt.c0 * kKeys, nxt.len, nxt.kvh, z, li, g, lane);
+                if (c < cur.c1) {
+                    pages_for(a, cur, c, lane);
+                    load_codes<D, kNT>(a, cur.pg, c * kKeys, cur.len, cur.kvh, z, lane);
+                } else if (more) {
+                    load_codes<D, kNT>(a, nxt.pg, nxt.c0 * kKeys, nxt.len, nxt.kvh, z, lane);
+                }
             };
             bool in_y;   // where the next segment's codes are
             for (int c = cur.c0;; c += 2) {
                 ahead(y, c + 1);
-                use(x, c);
+                rb.use(x, c * kKeys, cur.len, lds);
                 in_y = c + 1 >= cur.c1;
                 if (in_y) break;
                 ahead(x, c + 2);
-                use(y, c + 1);
+                rb.use(y, (c + 1) * kKeys, cur.len, lds);
                 if (c + 2 >= cur.c1) break;
             }
             finish();
@@ -452,37 +484,30 @@ __global__ __launch_bounds__(64, (waves_per_cu(D, RT, kFp4) + 3) / 4) void paged
     } else {
         // The copies go on across segments: the next one's first chunk is on its way while the last chunk of this is used, so
         // its pages and queries are loaded a segment ahead.
-        Segment nxt;
-        u32x4 qn[RT][ND];
-        bool more = false;   // nxt is there
+        typename RowBlock<D, RT, kBf16, kFp4>::Queries qn;
         auto look_ahead = [&]() {
             more = left > 0;
             if (!more) return;
             next_segment(nxt);
-            load_q(nxt, qn);
+            rb.load_q(nxt.b, nxt.kvh, nxt.hb, qn);
         };
-        next_segment(cur);
-        load_q(cur, qb);
+        rb.load_q(cur.b, cur.kvh, cur.hb, rb.q);
         copy_chunk<D, kNT>(a, cur.pg, cur.c0 * kKeys, cur.kvh, lds, lane);
-        begin();
+        rb.begin(cur.len, cur.hb);
         look_ahead();
-        ready(qb);
+        rb.ready();
         for (int c = cur.c0, st = 0;; st ^= 1) {
-            uint16_t* const here = lds + st * kStage;
-            uint16_t* const there = lds + (st ^ 1) * kStage;
+            uint16_t* const there = lds + (st ^ 1) * stage_elems<D>();
             const bool last = c + 1 == cur.c1;
             if (!last) {
-                pages_for(cur, c + 1);
+                pages_for(a, cur, c + 1, lane);
                 copy_chunk<D, kNT>(a, cur.pg, (c + 1) * kKeys, cur.kvh, there, lane);
-                asm volatile("s_waitcnt vmcnt(%0)" : : "n"(kCopies) : "memory");
+                asm volatile("s_waitcnt vmcnt(%0)" : : "n"(copies<D>()) : "memory");
             } else {
                 asm volatile("s_waitcnt vmcnt(0)" : : : "memory");
                 if (more) copy_chunk<D, kNT>(a, nxt.pg, nxt.c0 * kKeys, nxt.kvh, there, lane);
             }
-            if ((c + 1) * kKeys > cur.len) clear_rows<D>(here + kKeys * D, cur.len - c * kKeys, lane);
-            f32x4 s[RT][2];
-            qk_chunk<D, RT, kBf16>((const char*)here, off, qb, s, 0);
-            chunk(s, c * kKeys, (const char*)(here + kKeys * D));
+            rb.use(lds + st * stage_elems<D>(), c * kKeys, cur.len);
             if (!last) {
                 ++c;
                 continue;
@@ -494,10 +519,101 @@ __global__ __launch_bounds__(64, (waves_per_cu(D, RT, kFp4) + 3) / 4) void paged
 #pragma unroll
             for (int t = 0; t < RT; ++t)
 #pragma unroll
-                for (int i = 0; i < ND; ++i) qb[t][i] = qn[t][i];
-            begin();
+                for (int i = 0; i < D / 32; ++i) rb.q[t][i] = qn[t][i];
+            rb.begin(cur.len, cur.hb);
             look_ahead();
         }
+    }
+}
+
+// ---- one workgroup per item -------------------------------------------------------------------------
+// Short caches (choose_waves): W waves take an item's chunks in equal runs and join their results in LDS; one launch.
+template <int D, int RT, bool kBf16, bool kFp4, int W>
+__global__ __launch_bounds__(64 * W) void paged_whole(PagedArgs a) {
+    constexpr int kRing = wave_lds<D, kFp4>(), kRows = 16 * RT;
+    constexpr int kBytes = W == 1 ? kRing * 2 : std::max(W * kRing * 2, W * kRows * (D + 2) * 4);
+    __shared__ __attribute__((aligned(16))) char smem[kBytes];
+    const int lane = (int)(threadIdx.x & 63u), wave = scalar((int)(threadIdx.x >> 6));
+    uint16_t* const lds = (uint16_t*)smem + wave * kRing;
+    Segment s;
+    s.b = (int)(blockIdx.x / (unsigned)a.items);
+    const int item = (int)(blockIdx.x % (unsigned)a.items);
+    s.kvh = item / a.HB;
+    s.hb = item - s.kvh * a.HB;
+    RowBlock<D, RT, kBf16, kFp4> rb(a, lane);
+    rb.load_q(s.b, s.kvh, s.hb, rb.q);
+    {   // the length and the first 64 entries at once; entries past the last row's are not used for a row that is
+        int ids = a.tables[s.b * a.table_stride + min(lane, (a.max_len >> a.lp) - 1)], len = a.lens[s.b];
+        asm volatile("" : "+v"(ids), "+v"(len));
+        s.len = scalar(min(max(len, 0), a.max_len));
+        s.pg.first = 0;
+        s.pg.ids = min(max(ids, 0), a.pages - 1);
+    }
+    s.n = chunks_of(s.len);
+    s.c0 = s.n * wave / W;
+    s.c1 = s.n * (wave + 1) / W;
+    rb.begin(s.len, s.hb);
+    if (s.c0 < s.c1) {
+        pages_for(a, s, s.c0, lane);
+        if constexpr (kFp4) {
+            Codes<D> x, y;
+            load_codes<D, false>(a, s.pg, s.c0 * kKeys, s.len, s.kvh, x, lane);
+            for (int c = s.c0;; c += 2) {
+                if (c + 1 < s.c1) {
+                    pages_for(a, s, c + 1, lane);
+                    load_codes<D, false>(a, s.pg, (c + 1) * kKeys, s.len, s.kvh, y, lane);
+                }
+                rb.use(x, c * kKeys, s.len, lds);
+                if (c + 1 >= s.c1) break;
+                if (c + 2 < s.c1) {
+                    pages_for(a, s, c + 2, lane);
+                    load_codes<D, false>(a, s.pg, (c + 2) * kKeys, s.len, s.kvh, x, lane);
+                }
+                rb.use(y, (c + 1) * kKeys, s.len, lds);
+                if (c + 2 >= s.c1) break;
+            }
+        } else {
+            copy_chunk<D, false>(a, s.pg, s.c0 * kKeys, s.kvh, lds, lane);
+            rb.ready();
+            for (int c = s.c0, st = 0; c < s.c1; ++c, st ^= 1) {
+                if (c + 1 < s.c1) {
+                    pages_for(a, s, c + 1, lane);
+                    copy_chunk<D, false>(a, s.pg, (c + 1) * kKeys, s.kvh, lds + (st ^ 1) * stage_elems<D>(), lane);
+                    asm volatile("s_waitcnt vmcnt(%0)" : : "n"(copies<D>()) : "memory");
+                } else {
+                    asm volatile("s_waitcnt vmcnt(0)" : : : "memory");
+                }
+                rb.use(lds + st * stage_elems<D>(), c * kKeys, s.len);
+            }
+        }
+    }
+    if constexpr (W == 1) {
+        rb.store(s.b, s.kvh, s.hb);
+        return;
+    }
+    __syncthreads();   // every wave is done with its ring: the results over them
+    const int rows = min(kRows, rb.R - s.hb * kRows);
+    float* const po = (float*)smem;
+    float* const pml = po + W * kRows * D;
+    rb.store_part(pml, po, wave * kRows, rows);
+    __syncthreads();
+    for (int x = (int)threadIdx.x; x < rows * (D / 4); x += 64 * W) {
+        const int r = x / (D / 4), d = x % (D / 4) * 4;
+        float M = kInitM, L = 0.f;
+        f32x4 acc{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int k = 0; k < W; ++k) M = fmaxf(M, pml[(k * kRows + r) * 2]);
+#pragma unroll
+        for (int k = 0; k < W; ++k) {
+            const float2 ml = *(const float2*)(pml + (k * kRows + r) * 2);
+            const float wt = __builtin_amdgcn_exp2f(ml.x - M);
+            L = fmaf(wt, ml.y, L);
+            acc += *(const f32x4*)(po + (k * kRows + r) * D + d) * wt;
+        }
+        const float inv = L > 0.f ? 1.f / L : 1.f;
+        uint16_t* dst = a.o + rb.row_of(s.b, s.kvh, s.hb * kRows + r) + d;
+        ((uint32_t*)dst)[0] = pack2<kBf16>(acc[0] * inv, acc[1] * inv);
+        ((uint32_t*)dst)[1] = pack2<kBf16>(acc[2] * inv, acc[3] * inv);
     }
 }
 
@@ -576,8 +692,19 @@ __global__ __launch_bounds__(kThreads) void paged_join(PagedArgs a) {
 // ---- plan -----------------------------------------------------------------------------------------
 struct PagedPlan {
     int G, RT, HB, items, rows, shares;
+    int waves;   // of a workgroup per item, 0: equal shares
     size_t head_bytes, ml_bytes, ws_bytes;
 };
+
+// One launch for short caches: as many waves per item as leave each a few chunks at the longest, if the chip holds all of them at
+// once or nearly so.
+int choose_waves(long long items, int max_len, int D, bool fp4, long long resident) {
+    const int chunks = (max_len + kKeys - 1) / kKeys, most = D == 64 ? 8 : 4;
+    for (int w = 1; w <= most; w *= 2)
+        if ((chunks + w - 1) / w <= 4 && items * w <= resident) return w;
+    (void)fp4;
+    return 0;
+}
 
 size_t align256(size_t n) { return (n + 255) & ~(size_t)255; }
 
@@ -594,6 +721,7 @@ bool plan_paged(const cdna4_paged_cache& k, const cdna4_paged_decode_cfg& c, Pag
     p.items = k.nKVHeads * p.HB;
     p.rows = std::min(R, 16 * p.RT);
     p.shares = device_cus() * waves_per_cu(k.D, p.RT, k.format == CDNA4_KV_MXFP4);
+    p.waves = choose_waves((long long)c.batch * p.items, k.max_pages * k.page, k.D, k.format == CDNA4_KV_MXFP4, p.shares);
     p.head_bytes = align256(((size_t)c.batch + 1) * sizeof(long long));
     p.ml_bytes = align256((size_t)p.shares * 2 * p.rows * 2 * sizeof(float));
     p.ws_bytes = p.head_bytes + p.ml_bytes + (size_t)p.shares * 2 * p.rows * k.D * sizeof(float);
@@ -606,8 +734,25 @@ void launch_parts(const PagedArgs& a, bool nt, hipStream_t s) {
     else paged_parts<D, RT, kBf16, kFp4, false><<<a.shares, 64, 0, s>>>(a);
 }
 
+template <int D, int RT, bool kBf16, bool kFp4>
+int launch_whole(const PagedArgs& a, int waves, hipStream_t s) {
+    const unsigned grid = (unsigned)(a.batch * a.items);
+    switch (waves) {
+        case 1: paged_whole<D, RT, kBf16, kFp4, 1><<<grid, 64, 0, s>>>(a); break;
+        case 2: paged_whole<D, RT, kBf16, kFp4, 2><<<grid, 128, 0, s>>>(a); break;
+        case 4: paged_whole<D, RT, kBf16, kFp4, 4><<<grid, 256, 0, s>>>(a); break;
+        default:
+            if constexpr (D == 64) paged_whole<D, RT, kBf16, kFp4, 8><<<grid, 512, 0, s>>>(a);
+    }
+    return launch_status();
+}
+
 template <int D, bool kBf16>
 int launch_paged(const PagedArgs& a, const PagedPlan& p, bool fp4, hipStream_t s) {
+    if (p.waves) {
+        if (p.RT == 2) return fp4 ? launch_whole<D, 2, kBf16, true>(a, p.waves, s) : launch_whole<D, 2, kBf16, false>(a, p.waves, s);
+        return fp4 ? launch_whole<D, 1, kBf16, true>(a, p.waves, s) : launch_whole<D, 1, kBf16, false>(a, p.waves, s);
+    }
     // Pools of more than half the Infinity Cache are read past it (stream::dma16): K and V of 157 MB 40.6 against 44.0 us, of 267 MB
     // 48.3 against 54.6; those of 58 MB that it holds 23.6 against 21.8.
     const bool nt = 2.0 * a.pages * a.HK * a.page * row_bytes(D, fp4) > 128.0 * 1024 * 1024;
@@ -672,10 +817,10 @@ extern "C" int cdna4_attn_decode_paged_plan(const cdna4_paged_cache* cache, cons
     PagedPlan p;
     if (!cache || !cfg || !out || (dtype != CDNA4_F16 && dtype != CDNA4_BF16) || !plan_paged(*cache, *cfg, p)) return CDNA4_ERR_INVALID_VALUE;
     out->kernel = CDNA4_KERNEL_DECODE_PAGED;
-    out->waves = 1;
+    out->waves = p.waves ? p.waves : 1;
     out->rows = p.rows;
-    out->partials = p.shares;
-    out->grid = p.shares;
+    out->partials = p.waves ? 1 : p.shares;
+    out->grid = p.waves ? (long long)cfg->batch * p.items : p.shares;
     out->workspace = p.ws_bytes;
     return 0;
 }
