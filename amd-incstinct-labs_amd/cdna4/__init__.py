@@ -857,8 +857,8 @@ def decode_paged(q: torch.Tensor, K_pages: torch.Tensor, V_pages: torch.Tensor, 
                  o: torch.Tensor, cache: PagedCache, cfg: PagedDecodeCfg, workspace="auto", stream=None) -> None:
     """The queries of each sequence's last nq tokens over its rows of a paged cache: q, o [batch][nq][nQH][D] (fp16 or bf16, also
     the type of a 16-bit cache); tables int32 [batch][max_pages], lens int32 [batch] (rows, the new tokens' among them) on the device.
-    `workspace`: "auto" allocates decode_paged_workspace_size(cache, cfg) bytes on the stream the call launches on; a uint8 tensor is
-    used as given."""
+    `workspace`: "auto" allocates decode_paged_workspace_size(cache, cfg) bytes (0 for short tables) on the stream the call launches
+    on; a uint8 tensor is used as given."""
     dev, dtype = _gpu_of(q), q.dtype
     if _elsewhere(dev, stream):
         with _entered(dev, stream):
@@ -871,7 +871,7 @@ def decode_paged(q: torch.Tensor, K_pages: torch.Tensor, V_pages: torch.Tensor, 
     if workspace is None or (isinstance(workspace, str) and workspace != "auto"):
         raise ValueError("workspace must be 'auto' or a uint8 tensor")
     if isinstance(workspace, str):
-        workspace = torch.empty(max(1, decode_paged_workspace_size(cache, cfg)), dtype=torch.uint8, device=q.device)
+        workspace = torch.empty(decode_paged_workspace_size(cache, cfg), dtype=torch.uint8, device=q.device)
     rc = lib().cdna4_attn_decode_paged(qp, Kp, Vp, tp, lp, op, ctypes.byref(cache), ctypes.byref(cfg), dt,
                                        _arg("workspace", workspace, torch.uint8, 0, dev), workspace.numel(),
                                        torch._C._cuda_getCurrentRawStream(dev))

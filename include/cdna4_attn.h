@@ -260,7 +260,7 @@ enum {
     CDNA4_KERNEL_PACKED = 8,           /* fa_packed: 4 waves x 32 or 16 queries, `rows` tokens of 128 / rows or 64 /
                                           rows query heads */
     CDNA4_KERNEL_DECODE_SHARED = 9,    /* shared_parts + shared_join */
-    CDNA4_KERNEL_DECODE_PAGED = 10     /* paged_parts + paged_join */
+    CDNA4_KERNEL_DECODE_PAGED = 10     /* paged_whole, or paged_parts + paged_join */
 };
 
 typedef struct {
@@ -421,13 +421,14 @@ int cdna4_rope_append_paged(const cdna4_append_args* args, const cdna4_paged_cac
  * [batch][nq][nQHeads][D], dtype CDNA4_F16 or CDNA4_BF16, also the type of a CDNA4_KV_16 cache; query head h reads kv head
  * h / (nQHeads / nKVHeads); scale 1/sqrt(D), softmax and sums in fp32. Table entries past the last row's are not read into a
  * result; entries outside 0 .. pages - 1 of those before read some page of the pool (nothing outside it). Rows from lens[b] on
- * may hold anything. A value in V that is not finite reaches the queries of up to nq - 1 tokens before it. The work is cut into
- * equal shares of keys whatever the lengths are, so a captured call replays on other lengths, tables and pages. The workspace
- * (cdna4_attn_decode_paged_workspace_size bytes, 16-byte aligned, no initialisation) holds what shares leave of rows that they
- * cut; calls that overlap must not share one. The plan is sized to the current device, so query the size with the device
- * current that the call will run on. batch == 0: nothing is done.
- * Invalid: nQHeads % nKVHeads != 0, nq not 1 .. 16, 2^24 rows of q (batch nq nQHeads) and more, q not 16-byte or o not 4-byte
- * aligned, a missing or small workspace.
+ * may hold anything. A value in V that is not finite reaches the queries of up to nq - 1 tokens before it. The plan follows from the
+ * two structs alone, so a captured call replays on other lengths, tables and pages: tables of few pages take one launch, a workgroup
+ * per sequence and row block; longer ones equal shares of all keys, whatever the lengths are, and a second launch. The workspace
+ * (cdna4_attn_decode_paged_workspace_size bytes, 16-byte aligned, no initialisation; 0 for one launch) holds what shares leave of
+ * rows that they cut; calls that overlap must not share one. The plan is sized to the current device, so query the size with the
+ * device current that the call will run on. batch == 0: nothing is done.
+ * Invalid: nQHeads % nKVHeads != 0, nq not 1 .. 16, 2^24 rows of q (batch nq nQHeads) and more, more than 2^35 keys of tables per
+ * resident wave of the device, q not 16-byte or o not 4-byte aligned, a missing or small workspace where one is needed.
  */
 typedef struct {
     int nQHeads;   /* nQHeads % nKVHeads == 0 */
@@ -435,8 +436,8 @@ typedef struct {
     int nq;        /* queries per sequence */
 } cdna4_paged_decode_cfg;
 
-/* cdna4_attn_decode_paged_plan (introspection): `rows` rows of a row block, `partials` shares of keys, `grid` workgroups of the
- * first launch. */
+/* cdna4_attn_decode_paged_plan (introspection): `rows` rows of a row block, `partials` shares of keys (1 and no workspace: one
+ * launch), `grid` workgroups of the first launch, of `waves` waves. */
 int cdna4_attn_decode_paged_plan(const cdna4_paged_cache* cache, const cdna4_paged_decode_cfg* cfg, int dtype, cdna3_plan_info* out);
 size_t cdna4_attn_decode_paged_workspace_size(const cdna4_paged_cache* cache, const cdna4_paged_decode_cfg* cfg);
 int cdna4_attn_decode_paged(const void* q, const void* K_pages, const void* V_pages, const int* tables, const int* lens,

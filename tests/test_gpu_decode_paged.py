@@ -1,5 +1,6 @@
 """cdna4.decode_paged against a 64-bit reference: lengths from no key to many shares, page sizes, both formats, head layouts,
-several queries, lengths and tables read on the device."""
+several queries, lengths and tables read on the device. `form`: "whole", a table of few pages, a workgroup per item; "shares", one
+long enough for equal shares of all keys, whatever the lengths."""
 import pytest
 import torch
 
@@ -11,10 +12,16 @@ pytestmark = pytest.mark.gpu
 F16, BF16 = torch.float16, torch.bfloat16
 
 
-def make(lens, HQ, HK, D, dtype, page=16, fmt="16", nq=1, seed=0, scale=1.0):
-    p = Paged(lens, HK, D, dtype, page, fmt, seed)
+FORMS = pytest.mark.parametrize("form", ["whole", "shares"])
+
+
+def make(lens, HQ, HK, D, dtype, page=16, fmt="16", nq=1, seed=0, scale=1.0, form="whole"):
+    p = Paged(lens, HK, D, dtype, page, fmt, seed, room=min(2, 256 // page) if form == "whole" else 4096 // page)
     q = (torch.randn(len(lens), nq, HQ, D, device=DEV, generator=p.g) * scale).to(dtype)
-    return p, q, cdna4.PagedDecodeCfg(HQ, len(lens), nq)
+    cfg = cdna4.PagedDecodeCfg(HQ, len(lens), nq)
+    if max(lens, default=0) <= 700 and len(lens) <= 130:
+        assert (cdna4.decode_paged_plan(p.cache, cfg).workspace == 0) == (form == "whole")
+    return p, q, cfg
 
 
 def run(p, q, cfg, o=None, tables=None, lens=None, **kw):
@@ -27,34 +34,37 @@ def verify(p, q, o, what=""):
     return check(o, *decode_reference(q, p.k, p.v, q.dtype), what)
 
 
+@FORMS
 @pytest.mark.parametrize("fmt", ["16", "mxfp4"])
 @pytest.mark.parametrize("dtype", [F16, BF16])
 @pytest.mark.parametrize("D", [64, 128])
 @pytest.mark.parametrize("page", [16, 32, 64, 128, 256])
-def test_lengths(page, D, dtype, fmt):
+def test_lengths(page, D, dtype, fmt, form):
     """Pages that end inside a chunk, at it and past it; rows behind the last one are NaN."""
     lens = [0, 1, 15, 16, 17, 31, 32, 33, 64, 65, 100, 255, 256, 257, 300, 700]
-    p, q, cfg = make(lens, 8, 2, D, dtype, page, fmt, seed=page)
+    p, q, cfg = make(lens, 8, 2, D, dtype, page, fmt, seed=page, form=form)
     o = run(p, q, cfg)
     verify(p, q, o, f"page {page}")
     assert bool((o[0] == 0).all())
 
 
+@FORMS
 @pytest.mark.parametrize("fmt", ["16", "mxfp4"])
 @pytest.mark.parametrize("heads", [(1, 1), (3, 1), (8, 8), (16, 2), (40, 8), (12, 12), (20, 1), (33, 1), (64, 1)])
 @pytest.mark.parametrize("D", [64, 128])
-def test_heads(heads, D, fmt):
-    p, q, cfg = make([70, 0, 129], *heads, D, F16, 32, fmt, seed=heads[0])
+def test_heads(heads, D, fmt, form):
+    p, q, cfg = make([70, 0, 129], *heads, D, F16, 32, fmt, seed=heads[0], form=form)
     verify(p, q, run(p, q, cfg))
 
 
+@FORMS
 @pytest.mark.parametrize("fmt", ["16", "mxfp4"])
 @pytest.mark.parametrize("nq", [2, 3, 5, 8, 16])
 @pytest.mark.parametrize("heads", [(4, 4), (8, 2), (20, 2)])
-def test_several_queries(heads, nq, fmt):
+def test_several_queries(heads, nq, fmt, form):
     """Sequences shorter than the queries leave the first ones nothing to see: zeros."""
     lens = [0, 1, nq - 1, nq, 31, 32, 33, 40, 95, 300]
-    p, q, cfg = make(lens, *heads, 64 if nq == 3 else 128, BF16 if nq == 2 else F16, 16, fmt, nq, seed=nq)
+    p, q, cfg = make(lens, *heads, 64 if nq == 3 else 128, BF16 if nq == 2 else F16, 16, fmt, nq, seed=nq, form=form)
     # a query whose row sees nothing gets 0 times the sequence's values, which are finite here
     o = run(p, q, cfg)
     verify(p, q, o)
@@ -62,14 +72,15 @@ def test_several_queries(heads, nq, fmt):
         assert bool((o[b, :max(nq - n, 0)] == 0).all())
 
 
+@FORMS
 @pytest.mark.parametrize("B", [1, 2, 63, 64, 65, 130, 1000, 4099])
-def test_batches(B):
+def test_batches(B, form):
     """More sequences than a wave's lanes, and than 64 lanes of 64, most of them empty."""
     g = torch.Generator().manual_seed(B)
     lens = torch.randint(0, 90, (B,), generator=g)
     lens[torch.rand(B, generator=g) < (0.3 if B < 1000 else 0.9)] = 0
     lens = lens.tolist()
-    p, q, cfg = make(lens, 4, 1, 64, BF16, 16, seed=B)
+    p, q, cfg = make(lens, 4, 1, 64, BF16, 16, seed=B, form=form)
     verify(p, q, run(p, q, cfg))
 
 
@@ -88,31 +99,34 @@ def test_one_long_among_short():
     verify(p, q, run(p, q, cfg))
 
 
+@FORMS
 @pytest.mark.parametrize("fmt", ["16", "mxfp4"])
 @pytest.mark.parametrize("scale", [0.0, 8.0])
 @pytest.mark.parametrize("dtype", [F16, BF16])
-def test_peaked_and_flat(scale, dtype, fmt):
-    p, q, cfg = make([300, 0, 64], 8, 2, 128, dtype, 32, fmt, seed=4, scale=scale)
+def test_peaked_and_flat(scale, dtype, fmt, form):
+    p, q, cfg = make([300, 0, 64], 8, 2, 128, dtype, 32, fmt, seed=4, scale=scale, form=form)
     verify(p, q, run(p, q, cfg))
 
 
-def test_lengths_are_cut_and_tables_clamped():
+@pytest.mark.parametrize("rows", [96, 4096])
+def test_lengths_are_cut_and_tables_clamped(rows):
     """Lengths outside the table's rows are cut to them; entries outside the pool read some page of it and touch no other sequence."""
-    lens = [100, 0, 96, 60]
+    lens = [rows + 4, 0, rows, 60]
     p, q, cfg = make(lens, 4, 2, 64, F16, 16, seed=5)
-    p.cache.max_pages, p.cache.table_stride = 6, p.tables.shape[1]          # 96 rows
-    o = run(p, q, cfg, lens=torch.tensor([2 ** 31 - 1, -2 ** 31, 97, 60], dtype=torch.int32, device=DEV))
-    p.k, p.v = [x[:, :96] for x in p.k], [x[:, :96] for x in p.v]
+    p.cache.max_pages, p.cache.table_stride = rows // 16, p.tables.shape[1]
+    o = run(p, q, cfg, lens=torch.tensor([2 ** 31 - 1, -2 ** 31, rows + 1, 60], dtype=torch.int32, device=DEV))
+    p.k, p.v = [x[:, :rows] for x in p.k], [x[:, :rows] for x in p.v]
     verify(p, q, o)
     t = p.tables.clone()
     t[3, 1], t[3, 2] = -5, 2 ** 30
-    o2 = run(p, q, cfg, tables=t, lens=torch.tensor([100, 0, 100, 60], dtype=torch.int32, device=DEV))
+    o2 = run(p, q, cfg, tables=t, lens=torch.tensor([rows + 4, 0, rows + 4, 60], dtype=torch.int32, device=DEV))
     assert torch.equal(o2[:3], o[:3])
 
 
-def test_shared_pages_equal_copies():
+@FORMS
+def test_shared_pages_equal_copies(form):
     """Two tables naming the same pages give the same bits as each alone."""
-    p, q, cfg = make([200], 8, 2, 128, BF16, 32, seed=6)
+    p, q, cfg = make([200], 8, 2, 128, BF16, 32, seed=6, form=form)
     t, l = p.tables.repeat(3, 1), p.lens.repeat(3)
     q3 = q.repeat(3, 1, 1, 1)
     o = torch.empty_like(q3)
@@ -134,10 +148,11 @@ def test_as_decode_of_a_contiguous_cache():
     check(o[:, 0], u.double(), 2 * bound[:, 0])
 
 
-def test_masked_keys_that_are_not_finite():
+@FORMS
+def test_masked_keys_that_are_not_finite(form):
     """K rows that some queries must not see may hold anything; a V that is not finite stays with the queries that see it and those of up
     to nq - 1 tokens before it."""
-    p, q, cfg = make([50, 70], 4, 2, 64, F16, 16, nq=3, seed=8)
+    p, q, cfg = make([50, 70], 4, 2, 64, F16, 16, nq=3, seed=8, form=form)
     ref, bound = decode_reference(q, p.k, p.v, F16)
     last = int(p.tables[0, 49 // 16])
     p.K[last, :, 49 % 16] = float("nan")                     # row 49: queries 0 and 1 must not see it
@@ -148,7 +163,7 @@ def test_masked_keys_that_are_not_finite():
 
 
 def test_workspace_contents_do_not_matter():
-    p, q, cfg = make([40, 0, 2000], 8, 2, 128, F16, 32, seed=9)
+    p, q, cfg = make([40, 0, 2000], 8, 2, 128, F16, 32, seed=9)   # equal shares
     need = cdna4.decode_paged_workspace_size(p.cache, cfg)
     a = run(p, q, cfg)
     for fill in (0, 255):
@@ -167,7 +182,7 @@ def test_workspace_contents_do_not_matter():
 
 
 def test_two_streams_at_once():
-    a, b = make([400, 30, 0], 8, 2, 128, BF16, 16, seed=10), make([77, 500], 12, 12, 64, F16, 32, "mxfp4", seed=11)
+    a, b = make([400, 30, 0], 8, 2, 128, BF16, 16, seed=10, form="shares"), make([77, 500], 12, 12, 64, F16, 32, "mxfp4", seed=11)
     oa, ob = torch.empty_like(a[1]), torch.empty_like(b[1])
     torch.cuda.synchronize()
     s1, s2 = torch.cuda.Stream(), torch.cuda.Stream()
@@ -179,9 +194,10 @@ def test_two_streams_at_once():
     verify(b[0], b[1], ob)
 
 
+@FORMS
 @pytest.mark.parametrize("fmt", ["16", "mxfp4"])
-def test_captured_call_replays_on_other_lengths(fmt):
-    p, q, cfg = make([600] * 4, 8, 2, 128, F16, 32, fmt, seed=12)
+def test_captured_call_replays_on_other_lengths(fmt, form):
+    p, q, cfg = make([600] * 4, 8, 2, 128, F16, 32, fmt, seed=12, form=form)
     full_k, full_v = p.k, p.v
     ws = torch.empty(cdna4.decode_paged_workspace_size(p.cache, cfg), dtype=torch.uint8, device=DEV)
     o = torch.empty_like(q)
@@ -200,12 +216,13 @@ def test_captured_call_replays_on_other_lengths(fmt):
         verify(p, q, o, str(lens))
 
 
+@FORMS
 @pytest.mark.parametrize("fmt", ["16", "mxfp4"])
-def test_pools_past_32_bit_offsets(fmt):
+def test_pools_past_32_bit_offsets(fmt, form):
     """The rows of interest lie in the last pages of a pool of more than 4 GiB."""
     HK, D, page = 8, 128, 256
     pages = 2 ** 32 // (HK * page * (256 if fmt == "16" else 68)) + 40
-    p, q, cfg = make([900, 300], 16, HK, D, F16, page, fmt, seed=13)
+    p, q, cfg = make([900, 300], 16, HK, D, F16, page, fmt, seed=13, form=form)
     small = p.cache.pages
     for name in ("K", "V"):
         old = getattr(p, name)
@@ -214,4 +231,30 @@ def test_pools_past_32_bit_offsets(fmt):
         setattr(p, name, pool)
     p.cache.pages = pages
     p.tables = torch.where(p.tables >= 0, p.tables + (pages - small), p.tables)
+    verify(p, q, run(p, q, cfg))
+
+
+@pytest.mark.parametrize("fmt", ["16", "mxfp4"])
+@pytest.mark.parametrize("nq", [1, 5])
+@pytest.mark.parametrize("D, n", [(64, 60), (64, 120), (64, 250), (64, 2040), (128, 60), (128, 120), (128, 1020)])
+def test_waves_per_item(D, n, nq, fmt):
+    """One to eight waves per item; the last has 20 heads x 5 queries, several row blocks."""
+    lens = [n, 0, n // 2 + 1, 1, n - 1]
+    p, q, cfg = make(lens, 20, 2, D, BF16, 16, fmt, nq, seed=n)
+    p.cache.max_pages, p.cache.table_stride = (n + 15) // 16, p.tables.shape[1]
+    plan = cdna4.decode_paged_plan(p.cache, cfg)
+    chunks = (n + 31) // 32
+    assert plan.workspace == 0 and plan.waves == min(chunks, 8 if D == 64 else 4)
+    ws = torch.empty(0, dtype=torch.uint8, device=DEV)
+    verify(p, q, run(p, q, cfg, workspace=ws))
+
+
+@pytest.mark.parametrize("fmt", ["16", "mxfp4"])
+@pytest.mark.parametrize("D", [64, 128])
+def test_one_wave_per_item(D, fmt):
+    """More sequences than the chip holds waves: whole items to a wave, several rounds of them."""
+    lens = [(7 * i) % 65 for i in range(5000)]
+    p, q, cfg = make(lens, 2, 1, D, F16, 64, fmt, seed=14)
+    p.cache.max_pages, p.cache.table_stride = 1, p.tables.shape[1]
+    assert cdna4.decode_paged_plan(p.cache, cfg).waves == 1 and cdna4.decode_paged_plan(p.cache, cfg).grid == 5000
     verify(p, q, run(p, q, cfg))

@@ -24,7 +24,7 @@ def cache(**kw):
 
 
 def decode(c=None, cfg=(8, 3, 1), dtype=cdna4.F16, q=P, K=P, V=P, tables=P, lens=P, o=P, ws=P, n=None):
-    c, f = c or cache(), cdna4.PagedDecodeCfg(*cfg)
+    c, f = c or cache(max_pages=400), cdna4.PagedDecodeCfg(*cfg)   # a table of several workgroups per sequence
     n = cdna4.decode_paged_workspace_size(c, f) if n is None else n
     return cdna4.lib().cdna4_attn_decode_paged(q, K, V, tables, lens, o, ctypes.byref(c), ctypes.byref(f), dtype, ws, n, None)
 
@@ -54,11 +54,25 @@ def test_decode_refuses_arguments():
     for name in ("tables", "lens", "o"):
         assert decode(**{name: ODD2}) == 1, name
     assert decode(dtype=cdna4.F32) == 1 and decode(dtype=9) == 1
-    need = cdna4.decode_paged_workspace_size(cache(), cdna4.PagedDecodeCfg(8, 3, 1))
+    need = cdna4.decode_paged_workspace_size(cache(max_pages=400), cdna4.PagedDecodeCfg(8, 3, 1))
     assert need > 0 and decode(n=need - 1) == 1
     assert decode(cfg=(8, 0, 1), q=None, K=None, V=None, tables=None, lens=None, o=None, ws=None, n=0) == 0   # nothing to do
-    p = cdna4.decode_paged_plan(cache(), cdna4.PagedDecodeCfg(8, 3, 1))
-    assert p.name == "decode_paged" and p.workspace == need and p.grid * p.waves * 64 < 2 ** 32
+    p = cdna4.decode_paged_plan(cache(max_pages=400), cdna4.PagedDecodeCfg(8, 3, 1))
+    assert p.name == "decode_paged" and p.workspace == need and p.waves == 1 and p.grid == p.partials < 2 ** 26
+
+
+def test_decode_of_short_tables_needs_no_workspace():
+    c, f = cache(), cdna4.PagedDecodeCfg(8, 3, 1)
+    p = cdna4.decode_paged_plan(c, f)
+    assert (p.workspace, p.partials, p.grid, p.waves) == (0, 1, 6, 4) and cdna4.decode_paged_workspace_size(c, f) == 0
+    assert decode(c, K=None, ws=None) == 1
+
+
+def test_decode_refuses_more_keys_than_shares_count():
+    c = cache(nKVHeads=8, page=256, max_pages=2 ** 22, pages=2 ** 20)
+    for batch, ok in ((1, True), (2 ** 20, False)):
+        assert (cdna4.decode_paged_workspace_size(c, cdna4.PagedDecodeCfg(8, batch, 1)) > 0) == ok
+    assert decode(c, (8, 2 ** 20, 1), n=1 << 60) == 1
 
 
 def append(c=None, dtype=cdna4.F16, **kw):
@@ -189,7 +203,7 @@ CALLER = r"""
 #include <cdna3/runtime/forward.hpp>
 using namespace cdna3;
 int main() {
-    attn::PagedCache c{128, 2, 64, 10, CDNA4_KV_16, 4, 0};
+    attn::PagedCache c{128, 2, 64, 10, CDNA4_KV_16, 400, 0};
     attn::PagedDecodeCfg d{8, 3, 1};
     if (attn::decode_paged_workspace_size(c, d) == 0) return 1;
     const __half* h = nullptr;
