@@ -18,6 +18,7 @@ namespace {
 
 using wave::xlane::allreduce;
 using wave::xlane::Max;
+using wave::xlane::Min;
 using wave::xlane::Sum;
 
 typedef uint32_t u32x4_u __attribute__((ext_vector_type(4), aligned(2)));   // rows of odd length start anywhere
@@ -65,16 +66,13 @@ __device__ __forceinline__ uint64_t insert(uint64_t list, uint64_t key, int lane
     return lane < at ? list : lane == at ? key : (uint64_t)hi << 32 | lo;
 }
 
-// The n-th largest of the lanes' values, bit by bit from the top.
+// The n-th largest of the lanes' values: the least of those that fewer than n are above. 700 cycles; bit by bit from the top, a
+// ballot each, it took 3,000.
 __device__ __forceinline__ uint32_t nth_largest(uint32_t v, int n) {
-    uint32_t t = 0;
-#pragma unroll 1
-    for (uint32_t bit = 0x80000000u; bit; bit >>= 1) {
-        const int c = __popcll(__builtin_amdgcn_ballot_w64(v >= (t | bit)));
-        if (c >= n) t |= bit;
-        if (c == n) break;   // no lower bit changes which n these are
-    }
-    return t;
+    int above = 0;
+#pragma unroll
+    for (int l = 0; l < 64; ++l) above += (uint32_t)__builtin_amdgcn_readlane((int)v, l) > v ? 1 : 0;
+    return allreduce(above < n ? v : 0xffffffffu, Min{});
 }
 
 // Keys of a lane into the list, those whose order reaches `least` and that of the n-th best so far, one by one.
@@ -230,16 +228,18 @@ __global__ __launch_bounds__(256) void beam_ranges(BeamArgs a) {
 }
 
 __global__ __launch_bounds__(1024) void beam_join(BeamArgs a) {
-    // Candidates that can be among the group's n best: no less than the least of the rows' q-th best, q rows' share of n, of which
-    // the group has n.
+    // Candidates that can be among the group's n best: no less, rounded to fp32, than the n-th largest of a sample that has the best of
+    // each row, two to a lane where they are more than 64.
     __shared__ double score[kMost * kMost];
     __shared__ int token[kMost * kMost], place[kMost * kMost];   // place: row n + place in the row's list
-    __shared__ double share[kMost];
+    __shared__ uint32_t sample[2 * 64];
     __shared__ uint64_t best[16][64];   // of each wave
     __shared__ int filled;
     const int lane = (int)(threadIdx.x & 63u), wave = __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
     const int waves = (int)blockDim.x >> 6, n = a.p.n, beams = a.p.beams, row0 = (int)blockIdx.x * beams;
     if (threadIdx.x == 0) filled = 0;
+    const int each = max((n + beams - 1) / beams, 64 / beams);   // of a row in the sample: 128 in all at most
+    for (int i = beams * each + (int)threadIdx.x; i < 128; i += (int)blockDim.x) sample[i] = 0;
     double held[kMost / 16];   // a wave has up to four rows (16 waves)
     int said[kMost / 16], where[kMost / 16];
 #pragma unroll 1
@@ -302,6 +302,9 @@ __global__ __launch_bounds__(1024) void beam_join(BeamArgs a) {
                 for (int j = 0; j < count; ++j) rank += best[wave][j] > mine ? 1 : 0;
             } else {
                 for (;;) {
+                    // a range's keys stand in descending order, `parts` apart: none here, none from here on
+                    const uint32_t nth = max(least, (uint32_t)(read_lane(mine, n - 1) >> 32));
+                    if (a.parts <= 256 && !__builtin_amdgcn_ballot_w64(tops() >= nth)) break;
                     mine = merge<4>(mine, n, least, tops(), [&](int k) { return key[k]; },
                                     [&](uint32_t b) { return [&key, b](int k) { return (uint32_t)(key[k] >> 32) >= b; }; }, lane);
                     i0 += 256;
@@ -315,19 +318,17 @@ __global__ __launch_bounds__(1024) void beam_join(BeamArgs a) {
                 tok = (int)~(uint32_t)mine;
             }
         }
-        const int q = (n + beams - 1) / beams;
-        if (lane == 0) share[b] = -INFINITY;
+        for (int i = lane; i < each; i += 64) sample[b * each + i] = 0;
         __builtin_amdgcn_wave_barrier();
-        if (tok >= 0 && rank == q - 1) share[b] = sc;
+        if (tok >= 0 && rank < each) sample[b * each + rank] = order_of((float)sc + 0.f);
         held[b / waves] = sc;   // of the rows that this wave has
         said[b / waves] = rank < n ? tok : -1;
         where[b / waves] = b * n + rank;
     }
     __syncthreads();
-    double least = lane < beams ? share[lane] : INFINITY;
-    least = allreduce(least, wave::xlane::Min{});
+    const uint32_t least = nth_largest(max(sample[lane], sample[lane + 64]), n);
     for (int b = wave; b < beams; b += waves) {
-        const bool in = said[b / waves] >= 0 && held[b / waves] >= least;
+        const bool in = said[b / waves] >= 0 && order_of((float)held[b / waves] + 0.f) >= least;
         const uint64_t mask = __builtin_amdgcn_ballot_w64(in);
         int at = 0;
         if (lane == 0) at = atomicAdd(&filled, __popcll(mask));

@@ -621,7 +621,7 @@ __global__ __launch_bounds__(64 * W) void paged_whole(PagedArgs a) {
 // the sequence has no keys.
 template <int D, bool kBf16, int kThreads>
 __global__ __launch_bounds__(kThreads) void paged_join(PagedArgs a) {
-    constexpr int kLanes = D / 4, kGroups = kThreads / kLanes, kFlight = kThreads == 64 ? 2 : 8;
+    constexpr int kLanes = D / 4, kGroups = kThreads / kLanes, kFlight = kThreads == 64 ? 4 : 8;
     __shared__ __attribute__((aligned(16))) f32x4 acc_s[kGroups][kLanes];
     __shared__ float2 ml_s[kGroups];
     const int R = a.nq * a.G;
@@ -696,16 +696,19 @@ struct PagedPlan {
     size_t head_bytes, ml_bytes, ws_bytes;
 };
 
+// Eight waves of 16-bit rows at D 128 are more than the LDS has room for, of MXFP4 and two row tiles more than the registers.
+constexpr int most_waves(int D, int RT, bool fp4) { return D == 64 || (fp4 && RT == 1) ? 8 : 4; }
+
 // One launch for short caches: the waves per item that end soonest, a round of the chip's waves taken for five chunks' time and those
 // that a wave has; 0: equal shares. Their second launch and the walk over the lengths cost 7-10 us, which up to eight chunks a
 // wave and sixteen over its rounds (MXFP4: twenty-four) do not: 16 sequences, 32/8 heads D 128, of 120 keys 4.7 against 13.6 us, of
 // 1,000 13.0 against 18.7; 64 of 1,000 40 against 47, 256 of 250 42 against 48. Beyond, the shares' even ends win: 128 of 1,000 (32
 // chunks) 95 against 87 us; in MXFP4 30 against 40, 256 of 1,000 (24 chunks) 61 against 65.
-int choose_waves(long long items, int max_len, int D, bool fp4, long long resident) {
+int choose_waves(long long items, int max_len, int D, int RT, bool fp4, long long resident) {
     const int chunks = (max_len + kKeys - 1) / kKeys;
     int best = 0;
     long long least = 0;
-    for (int w = 1; w <= (D == 64 ? 8 : 4); w *= 2) {
+    for (int w = 1; w <= most_waves(D, RT, fp4); w *= 2) {
         const int each = (chunks + w - 1) / w;
         const long long rounds = (items * w + resident - 1) / resident, t = rounds * (5 + each);
         if (each > 8 || rounds * each > (fp4 ? 24 : 16)) continue;
@@ -733,7 +736,7 @@ bool plan_paged(const cdna4_paged_cache& k, const cdna4_paged_decode_cfg& c, Pag
     const long long items = (long long)c.batch * p.items;   // below 2^24, as the rows of q
     const int max_len = k.max_pages * k.page;
     if (items * ((max_len + kKeys - 1) / kKeys) > ((long long)p.shares << 30)) return false;   // a share's chunks are an int
-    p.waves = choose_waves(items, max_len, k.D, k.format == CDNA4_KV_MXFP4, p.shares);
+    p.waves = choose_waves(items, max_len, k.D, p.RT, k.format == CDNA4_KV_MXFP4, p.shares);
     if (p.waves) return true;   // no workspace
     p.head_bytes = align256(((size_t)c.batch + 1) * sizeof(long long));
     p.ml_bytes = align256((size_t)p.shares * 2 * p.rows * 2 * sizeof(float));
@@ -755,7 +758,7 @@ int launch_whole(const PagedArgs& a, int waves, hipStream_t s) {
         case 2: paged_whole<D, RT, kBf16, kFp4, 2><<<grid, 128, 0, s>>>(a); break;
         case 4: paged_whole<D, RT, kBf16, kFp4, 4><<<grid, 256, 0, s>>>(a); break;
         default:
-            if constexpr (D == 64) paged_whole<D, RT, kBf16, kFp4, 8><<<grid, 512, 0, s>>>(a);
+            if constexpr (most_waves(D, RT, kFp4) == 8) paged_whole<D, RT, kBf16, kFp4, 8><<<grid, 512, 0, s>>>(a);
     }
     return launch_status();
 }
@@ -778,9 +781,11 @@ int launch_paged(const PagedArgs& a, const PagedPlan& p, bool fp4, hipStream_t s
     }
     if (int e = launch_status()) return e;
     const unsigned rows = (unsigned)((size_t)a.batch * a.nq * a.nQH);
-    // few parts to an item; more, and more rows than the chip holds workgroups of four waves
-    if (a.shares < 4LL * a.batch * a.items) paged_join<D, kBf16, 64><<<rows, 64, 0, s>>>(a);
-    else if (rows > 8u * (unsigned)device_cus()) paged_join<D, kBf16, 128><<<rows, 128, 0, s>>>(a);
+    // By the parts that an item has on the average: one, 4.7 against 6.8 us with 128 threads and 9.3 with 256 (4,096 rows); six, 4.4
+    // against 5.3 and 6.5 (2,048 rows); 128, 6.6 with 256 threads against 8.2 and 16.8 (96 rows). Many rows fill the chip without.
+    const long long items = (long long)a.batch * a.items;
+    if (a.shares < 4 * items) paged_join<D, kBf16, 64><<<rows, 64, 0, s>>>(a);
+    else if (a.shares < 32 * items || rows > 8u * (unsigned)device_cus()) paged_join<D, kBf16, 128><<<rows, 128, 0, s>>>(a);
     else paged_join<D, kBf16, 256><<<rows, 256, 0, s>>>(a);
     return launch_status();
 }
