@@ -150,76 +150,76 @@ __global__ __launch_bounds__(256) void beam_ranges(BeamArgs a) {
     load(0);
     if (!own) return;   // all waves of a shared row
     for (bool careful = false;; careful = true) {
-      m = kLowest;
-      s = 0.f;
-      list = 0;
-      if (careful) load(0);
-      uint32_t least = 0;
-      for (int i0 = 0; i0 == 0 || i0 < len; i0 += kStep) {   // once also where the range is empty
-        float x[kValues];
-        int from[kLoads];   // of each load, its first logit in the range
-        const bool tail = i0 + kStep > len;
-        // Logits of the step, lane by lane, in eights: a range's last step has fewer, and what a wave does goes by them.
-        const int count = max(min(kValues, ((len - i0 + 64 * kVec - 1) / (64 * kVec) * kVec + 7) & ~7), 8);
-        const bool look = careful || !vectors;
-        float top = -INFINITY;
+        m = kLowest;
+        s = 0.f;
+        list = 0;
+        if (careful) load(0);
+        uint32_t least = 0;
+        for (int i0 = 0; i0 == 0 || i0 < len; i0 += kStep) {   // once also where the range is empty
+            float x[kValues];
+            int from[kLoads];   // of each load, its first logit in the range
+            const bool tail = i0 + kStep > len;
+            // Logits of the step, lane by lane, in eights: a range's last step has fewer, and what a wave does goes by them.
+            const int count = max(min(kValues, ((len - i0 + 64 * kVec - 1) / (64 * kVec) * kVec + 7) & ~7), 8);
+            const bool look = careful || !vectors;
+            float top = -INFINITY;
 #pragma unroll
-        for (int u = 0; u < kLoads; ++u) {
-            from[u] = vectors ? min(place(i0, u), len - kVec) : place(i0, u);
-            if (u * kVec >= count) continue;
-#pragma unroll
-            for (int e = 0; e < kVec; ++e) {
-                const uint32_t w = raw[u][kDtype == CDNA4_F32 ? e : e / 2];
-                x[u * kVec + e] = kDtype == CDNA4_F32 ? f32_from_bits(w)
-                                : kDtype == CDNA4_BF16 ? f32_from_bits(e & 1 ? w & 0xffff0000u : w << 16)
-                                                       : f16_bits_to_f32(e & 1 ? w >> 16 : w & 0xffffu);
-            }
-            if (look) {
+            for (int u = 0; u < kLoads; ++u) {
+                from[u] = vectors ? min(place(i0, u), len - kVec) : place(i0, u);
+                if (u * kVec >= count) continue;
 #pragma unroll
                 for (int e = 0; e < kVec; ++e) {
-                    float& y = x[u * kVec + e];
-                    if (!vectors) y = from[u] + e < len ? logit(a.p, kDtype, base + from[u] + e) : -INFINITY;
-                    y = cleaned(y);
+                    const uint32_t w = raw[u][kDtype == CDNA4_F32 ? e : e / 2];
+                    x[u * kVec + e] = kDtype == CDNA4_F32 ? f32_from_bits(w)
+                                    : kDtype == CDNA4_BF16 ? f32_from_bits(e & 1 ? w & 0xffff0000u : w << 16)
+                                                           : f16_bits_to_f32(e & 1 ? w >> 16 : w & 0xffffu);
+                }
+                if (look) {
+#pragma unroll
+                    for (int e = 0; e < kVec; ++e) {
+                        float& y = x[u * kVec + e];
+                        if (!vectors) y = from[u] + e < len ? logit(a.p, kDtype, base + from[u] + e) : -INFINITY;
+                        y = cleaned(y);
+                    }
+                }
+                if (tail) {
+#pragma unroll
+                    for (int e = 0; e < kVec; ++e)
+                        if (from[u] + e < place(i0, u)) x[u * kVec + e] = -INFINITY;
+                }
+#pragma unroll
+                for (int e = 0; e < kVec; ++e) top = fmaxf(top, x[u * kVec + e]);
+            }
+            if (!tail) load(i0 + kStep);   // clamped to the end where the range ends with this step
+            if (top > m) {
+                s *= exp_of(m - top);
+                m = top;
+            }
+#pragma unroll
+            for (int u = 0; u < kLoads; ++u) {
+                if (u * kVec >= count) continue;
+#pragma unroll
+                for (int e = 0; e < kVec; ++e) s += exp_of(x[u * kVec + e] - m);
+            }
+            const uint32_t top_order = order_of(cleaned(top) + 0.f);
+            const bool share = shared && !careful;
+            if (i0 == 0) {
+                least = nth_largest(top_order, share ? (n + 3) / 4 : n);
+                if (share) {
+                    if (lane == 0) quarter[wave] = least;
+                    __syncthreads();   // every wave of the workgroup comes here once: a row's four
                 }
             }
-            if (tail) {
-#pragma unroll
-                for (int e = 0; e < kVec; ++e)
-                    if (from[u] + e < place(i0, u)) x[u * kVec + e] = -INFINITY;
-            }
-#pragma unroll
-            for (int e = 0; e < kVec; ++e) top = fmaxf(top, x[u * kVec + e]);
-        }
-        if (!tail) load(i0 + kStep);   // clamped to the end where the range ends with this step
-        if (top > m) {
-            s *= exp_of(m - top);
-            m = top;
-        }
-#pragma unroll
-        for (int u = 0; u < kLoads; ++u) {
-            if (u * kVec >= count) continue;
-#pragma unroll
-            for (int e = 0; e < kVec; ++e) s += exp_of(x[u * kVec + e] - m);
-        }
-        const uint32_t top_order = order_of(cleaned(top) + 0.f);
-        const bool share = shared && !careful;
-        if (i0 == 0) {
-            least = nth_largest(top_order, share ? (n + 3) / 4 : n);
+            if (share) least = min(min(quarter[0], quarter[1]), min(quarter[2], quarter[3]));
+            list = merge<kValues>(list, n, least, top_order,
+                                  [&](int k) { return key_of(x[k], begin + from[k / kVec] + k % kVec); },
+                                  [&](uint32_t b) { return [&x, f = of_order(b)](int k) { return x[k] >= f; }; }, lane, count);
             if (share) {
-                if (lane == 0) quarter[wave] = least;
-                __syncthreads();   // every wave of the workgroup comes here once: a row's four
+                const uint32_t best = (uint32_t)(read_lane(list, (n + 3) / 4 - 1) >> 32);
+                if (lane == 0 && best > quarter[wave]) quarter[wave] = best;
             }
         }
-        if (share) least = min(min(quarter[0], quarter[1]), min(quarter[2], quarter[3]));
-        list = merge<kValues>(list, n, least, top_order,
-                              [&](int k) { return key_of(x[k], begin + from[k / kVec] + k % kVec); },
-                              [&](uint32_t b) { return [&x, f = of_order(b)](int k) { return x[k] >= f; }; }, lane, count);
-        if (share) {
-            const uint32_t best = (uint32_t)(read_lane(list, (n + 3) / 4 - 1) >> 32);
-            if (lane == 0 && best > quarter[wave]) quarter[wave] = best;
-        }
-      }
-      if (careful || !__builtin_amdgcn_ballot_w64(s != s)) break;
+        if (careful || !__builtin_amdgcn_ballot_w64(s != s)) break;
     }
     const float M = allreduce(m, Max{});
     const double S = allreduce((double)s * (double)exp_of(m - M), Sum{});

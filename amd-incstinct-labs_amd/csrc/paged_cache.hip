@@ -118,98 +118,98 @@ __global__ __launch_bounds__(256) void append_paged(AppendArgs a) {
     const uint16_t *q = (const uint16_t*)a.p.q + t * a.p.q_row, *k = (const uint16_t*)a.p.k + t * a.p.k_row, *v = (const uint16_t*)a.p.v + t * a.p.v_row;
     const int slot0 = chunk * a.per_wave * kRows + lane / kLanes;
     for (int j0 = 0; j0 < a.per_wave; j0 += kAhead) {
-      if (slot0 - lane / kLanes + j0 * kRows >= slots) break;
-      uint2 in_lo[kAhead], in_hi[kAhead];
+        if (slot0 - lane / kLanes + j0 * kRows >= slots) break;
+        uint2 in_lo[kAhead], in_hi[kAhead];
 #pragma unroll
-      for (int j = 0; j < kAhead; ++j) {   // rows past the last re-read it
-        const int slot = min(slot0 + (j0 + j) * kRows, slots - 1);
-        const uint16_t* src = slot < a.p.nQHeads ? q + slot * D : slot < a.p.nQHeads + a.HK ? k + (slot - a.p.nQHeads) * D : v + (slot - a.p.nQHeads - a.HK) * D;
-        in_lo[j] = *(const uint2*)(src + 4 * i);
-        in_hi[j] = *(const uint2*)(src + D / 2 + 4 * i);
-      }
+        for (int j = 0; j < kAhead; ++j) {   // rows past the last re-read it
+            const int slot = min(slot0 + (j0 + j) * kRows, slots - 1);
+            const uint16_t* src = slot < a.p.nQHeads ? q + slot * D : slot < a.p.nQHeads + a.HK ? k + (slot - a.p.nQHeads) * D : v + (slot - a.p.nQHeads - a.HK) * D;
+            in_lo[j] = *(const uint2*)(src + 4 * i);
+            in_hi[j] = *(const uint2*)(src + D / 2 + 4 * i);
+        }
 #pragma unroll
-      for (int j = 0; j < kAhead; ++j) {
-        const int slot = slot0 + (j0 + j) * kRows;
-        if (slot >= slots || j0 + j >= a.per_wave) break;
-        const bool is_q = slot < a.p.nQHeads, is_k = !is_q && slot < a.p.nQHeads + a.HK;
-        const int h = is_q ? slot : is_k ? slot - a.p.nQHeads : slot - a.p.nQHeads - a.HK;
-        const uint2 u_lo = in_lo[j], u_hi = in_hi[j];
-        float lo[4], hi[4];
-        widen4<kBf16>(u_lo, lo);
-        widen4<kBf16>(u_hi, hi);
-        uint16_t* out = nullptr;
-        if (is_q) out = (uint16_t*)a.p.q_out + t * a.p.q_out_row + h * D + 4 * i;
-        else if (is_k && a.p.k_out) out = (uint16_t*)a.p.k_out + t * a.p.k_out_row + h * D + 4 * i;
-        else if (!is_k && a.p.v_out) out = (uint16_t*)a.p.v_out + t * a.p.v_out_row + h * D + 4 * i;
-        char* pool = (char*)(is_k ? a.p.K_pages : a.p.V_pages) + place + h * page_bytes;
-        if (kFp4 && !is_q) {
-            if (is_k && (a.p.k_norm || turn)) {
-                double dlo[4], dhi[4];
+        for (int j = 0; j < kAhead; ++j) {
+            const int slot = slot0 + (j0 + j) * kRows;
+            if (slot >= slots || j0 + j >= a.per_wave) break;
+            const bool is_q = slot < a.p.nQHeads, is_k = !is_q && slot < a.p.nQHeads + a.HK;
+            const int h = is_q ? slot : is_k ? slot - a.p.nQHeads : slot - a.p.nQHeads - a.HK;
+            const uint2 u_lo = in_lo[j], u_hi = in_hi[j];
+            float lo[4], hi[4];
+            widen4<kBf16>(u_lo, lo);
+            widen4<kBf16>(u_hi, hi);
+            uint16_t* out = nullptr;
+            if (is_q) out = (uint16_t*)a.p.q_out + t * a.p.q_out_row + h * D + 4 * i;
+            else if (is_k && a.p.k_out) out = (uint16_t*)a.p.k_out + t * a.p.k_out_row + h * D + 4 * i;
+            else if (!is_k && a.p.v_out) out = (uint16_t*)a.p.v_out + t * a.p.v_out_row + h * D + 4 * i;
+            char* pool = (char*)(is_k ? a.p.K_pages : a.p.V_pages) + place + h * page_bytes;
+            if (kFp4 && !is_q) {
+                if (is_k && (a.p.k_norm || turn)) {
+                    double dlo[4], dhi[4];
 #pragma unroll
-                for (int e = 0; e < 4; ++e) { dlo[e] = lo[e]; dhi[e] = hi[e]; }
-                norm_rope<double, D>(dlo, dhi, a.p.k_norm != nullptr, wk[0], wk[1], a.p.eps, turn, an);
+                    for (int e = 0; e < 4; ++e) { dlo[e] = lo[e]; dhi[e] = hi[e]; }
+                    norm_rope<double, D>(dlo, dhi, a.p.k_norm != nullptr, wk[0], wk[1], a.p.eps, turn, an);
 #pragma unroll
-                for (int e = 0; e < 4; ++e) { lo[e] = round_to_odd(dlo[e]); hi[e] = round_to_odd(dhi[e]); }
-            }
-            uint32_t m_lo = 0, m_hi = 0;
-#pragma unroll
-            for (int e = 0; e < 4; ++e) {
-                m_lo = max(m_lo, __builtin_bit_cast(uint32_t, lo[e]) & 0x7fffffffu);
-                m_hi = max(m_hi, __builtin_bit_cast(uint32_t, hi[e]) & 0x7fffffffu);
-            }
-            const uint32_t b_lo = scale_byte<kBf16>(lanes_allreduce<8>(m_lo, wave::xlane::Max{}));
-            const uint32_t b_hi = scale_byte<kBf16>(lanes_allreduce<8>(m_hi, wave::xlane::Max{}));
-            const uint32_t c_lo = encode4(lo, b_lo), c_hi = encode4(hi, b_hi);
-            if (placed) {
-                uint8_t* code = (uint8_t*)pool + row * (D / 2) + 2 * i;
-                *(uint16_t*)code = (uint16_t)c_lo;
-                *(uint16_t*)(code + D / 4) = (uint16_t)c_hi;
-                if ((i & 7) == 0) {
-                    uint8_t* scale = (uint8_t*)pool + a.page * (D / 2) + row * (D / 32) + (i >> 3);
-                    scale[0] = (uint8_t)b_lo;
-                    scale[D / 64] = (uint8_t)b_hi;
+                    for (int e = 0; e < 4; ++e) { lo[e] = round_to_odd(dlo[e]); hi[e] = round_to_odd(dhi[e]); }
                 }
-            }
-            if (out) {
-                const float f_lo = f32_from_bits(b_lo << 23), f_hi = f32_from_bits(b_hi << 23);
-                *(uint2*)out = make_uint2(decode2<kBf16, 0>(c_lo, f_lo), decode2<kBf16, 1>(c_lo, f_lo));
-                *(uint2*)(out + D / 2) = make_uint2(decode2<kBf16, 0>(c_hi, f_hi), decode2<kBf16, 1>(c_hi, f_hi));
-            }
-        } else {
-            uint2 r_lo = u_lo, r_hi = u_hi;
-            if (is_q || is_k) {
-                const bool normed = is_q ? a.p.q_norm != nullptr : a.p.k_norm != nullptr;
-                if (!kBf16 && !normed && turn) {   // the bits of the other kernels that write a cache
-                    const uint32_t x[4] = {u_lo.x & 0xffffu, u_lo.x >> 16, u_lo.y & 0xffffu, u_lo.y >> 16};
-                    const uint32_t y[4] = {u_hi.x & 0xffffu, u_hi.x >> 16, u_hi.y & 0xffffu, u_hi.y >> 16};
-                    uint32_t p[4], q[4];
+                uint32_t m_lo = 0, m_hi = 0;
 #pragma unroll
-                    for (int e = 0; e < 4; ++e) rope_pair(x[e], y[e], an.c_lo[e], an.s_lo[e], an.c_hi[e], an.s_hi[e], p[e], q[e]);
-                    r_lo = make_uint2(p[0] | p[1] << 16, p[2] | p[3] << 16);
-                    r_hi = make_uint2(q[0] | q[1] << 16, q[2] | q[3] << 16);
-                } else if (normed || turn) {
-                    float w_lo[4], w_hi[4];
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) {
-                        w_lo[e] = is_q ? wq[0][e] : wk[0][e];
-                        w_hi[e] = is_q ? wq[1][e] : wk[1][e];
+                for (int e = 0; e < 4; ++e) {
+                    m_lo = max(m_lo, __builtin_bit_cast(uint32_t, lo[e]) & 0x7fffffffu);
+                    m_hi = max(m_hi, __builtin_bit_cast(uint32_t, hi[e]) & 0x7fffffffu);
+                }
+                const uint32_t b_lo = scale_byte<kBf16>(lanes_allreduce<8>(m_lo, wave::xlane::Max{}));
+                const uint32_t b_hi = scale_byte<kBf16>(lanes_allreduce<8>(m_hi, wave::xlane::Max{}));
+                const uint32_t c_lo = encode4(lo, b_lo), c_hi = encode4(hi, b_hi);
+                if (placed) {
+                    uint8_t* code = (uint8_t*)pool + row * (D / 2) + 2 * i;
+                    *(uint16_t*)code = (uint16_t)c_lo;
+                    *(uint16_t*)(code + D / 4) = (uint16_t)c_hi;
+                    if ((i & 7) == 0) {
+                        uint8_t* scale = (uint8_t*)pool + a.page * (D / 2) + row * (D / 32) + (i >> 3);
+                        scale[0] = (uint8_t)b_lo;
+                        scale[D / 64] = (uint8_t)b_hi;
                     }
-                    norm_rope<float, D>(lo, hi, normed, w_lo, w_hi, a.p.eps, turn, an);
-                    r_lo = narrow4<kBf16>(lo);
-                    r_hi = narrow4<kBf16>(hi);
                 }
-            }
-            if (!is_q && placed) {
-                uint16_t* dst = (uint16_t*)pool + row * D + 4 * i;
-                *(uint2*)dst = r_lo;
-                *(uint2*)(dst + D / 2) = r_hi;
-            }
-            if (out) {
-                *(uint2*)out = r_lo;
-                *(uint2*)(out + D / 2) = r_hi;
+                if (out) {
+                    const float f_lo = f32_from_bits(b_lo << 23), f_hi = f32_from_bits(b_hi << 23);
+                    *(uint2*)out = make_uint2(decode2<kBf16, 0>(c_lo, f_lo), decode2<kBf16, 1>(c_lo, f_lo));
+                    *(uint2*)(out + D / 2) = make_uint2(decode2<kBf16, 0>(c_hi, f_hi), decode2<kBf16, 1>(c_hi, f_hi));
+                }
+            } else {
+                uint2 r_lo = u_lo, r_hi = u_hi;
+                if (is_q || is_k) {
+                    const bool normed = is_q ? a.p.q_norm != nullptr : a.p.k_norm != nullptr;
+                    if (!kBf16 && !normed && turn) {   // the bits of the other kernels that write a cache
+                        const uint32_t x[4] = {u_lo.x & 0xffffu, u_lo.x >> 16, u_lo.y & 0xffffu, u_lo.y >> 16};
+                        const uint32_t y[4] = {u_hi.x & 0xffffu, u_hi.x >> 16, u_hi.y & 0xffffu, u_hi.y >> 16};
+                        uint32_t p[4], q[4];
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) rope_pair(x[e], y[e], an.c_lo[e], an.s_lo[e], an.c_hi[e], an.s_hi[e], p[e], q[e]);
+                        r_lo = make_uint2(p[0] | p[1] << 16, p[2] | p[3] << 16);
+                        r_hi = make_uint2(q[0] | q[1] << 16, q[2] | q[3] << 16);
+                    } else if (normed || turn) {
+                        float w_lo[4], w_hi[4];
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) {
+                            w_lo[e] = is_q ? wq[0][e] : wk[0][e];
+                            w_hi[e] = is_q ? wq[1][e] : wk[1][e];
+                        }
+                        norm_rope<float, D>(lo, hi, normed, w_lo, w_hi, a.p.eps, turn, an);
+                        r_lo = narrow4<kBf16>(lo);
+                        r_hi = narrow4<kBf16>(hi);
+                    }
+                }
+                if (!is_q && placed) {
+                    uint16_t* dst = (uint16_t*)pool + row * D + 4 * i;
+                    *(uint2*)dst = r_lo;
+                    *(uint2*)(dst + D / 2) = r_hi;
+                }
+                if (out) {
+                    *(uint2*)out = r_lo;
+                    *(uint2*)(out + D / 2) = r_hi;
+                }
             }
         }
-      }
     }
 }
 
