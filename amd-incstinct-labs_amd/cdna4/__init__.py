@@ -920,7 +920,7 @@ def beam_select(logits: torch.Tensor, cum: torch.Tensor, beams: int, n: Optional
                 eos: int = -1, out=None, workspace="auto", stream=None):
     """The n (default: beams) best continuations of each group of `beams` rows of logits [rows][V] (fp32, fp16 or bf16; rows may be apart)
     by cum[row] + log softmax, cum fp32 [rows]: (scores fp32, parents int32, tokens int32), each [rows / beams][n], best first; into
-    `out` if given. done int32 [rows], optional: rows that have ended and go on with `eos` alone. Places that nothing fills: -inf, -1,
+    `out` if given, whose scores may be cum where n == beams. done int32 [rows], optional: rows that have ended and go on with `eos` alone. Places that nothing fills: -inf, -1,
     -1. The rules: cdna4_beam_select in cdna4_attn.h."""
     dev = _gpu_of(logits)
     if _elsewhere(dev, stream):

@@ -466,7 +466,7 @@ int cdna4_paged_reorder(const int* parents, const int* tables, const int* lens, 
  * tokens int32. Sums of exponentials are taken in fp32 and joined in fp64. A logit of -inf or NaN is no continuation and adds
  * nothing, +inf counts as the largest fp32 value; rows with cum -inf, +inf or NaN and rows that allow nothing have none. done
  * (int32 [rows], may be NULL): rows that are not 0 there have ended and have one continuation, `eos` at the score cum. Places that no
- * continuation fills: score -inf, parent and token -1. Logits of one row that differ by less than 2^-40 may count as equal.
+ * continuation fills: score -inf, parent and token -1. scores may be cum where n == beams; outputs must not overlap inputs otherwise. Logits of one row that differ by less than 2^-40 may count as equal.
  * The workspace (cdna4_beam_select_workspace_size bytes for groups * beams rows, 16-byte aligned, no initialisation) must not be
  * shared by calls that overlap; query its size with the device current that the call will run on. groups == 0: nothing is done.
  * Invalid: beams or n not 1 .. 64, V < 1, groups negative, 2^24 rows and more, a logits stride below V, done with an eos outside 0 .. V - 1,

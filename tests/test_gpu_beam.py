@@ -181,6 +181,24 @@ def test_rows_apart_and_outputs_given():
         cdna4.beam_select(x, cum, 3, 65)
 
 
+@pytest.mark.parametrize("beams,n,V", [(1, 3, 400001), (2, 2, 270000), (2, 40, 300000)])
+def test_more_ranges_than_a_load_of_their_keys(beams, n, V):
+    """Over 256 ranges to a row: the best of some lie behind the first keys read."""
+    x, cum = make(1, beams, V, BF16, seed=V)
+    verify(x, cum, beams, n)
+    x[:, V - 5:] = torch.arange(20, 25, device=DEV).to(BF16)  # rising to the end
+    verify(x, cum, beams, n)
+
+
+def test_scores_in_the_place_of_cum():
+    for G, beams, V in ((1, 4, 32000), (33, 7, 3001)):
+        x, cum = make(G, beams, V, F16, seed=V)
+        want = cdna4.beam_select(x, cum.clone(), beams)
+        out = (cum, torch.empty(G, beams, dtype=torch.int32, device=DEV), torch.empty(G, beams, dtype=torch.int32, device=DEV))
+        cdna4.beam_select(x, cum, beams, out=out)
+        assert torch.equal(cum.view(G, beams), want[0]) and torch.equal(out[1], want[1]) and torch.equal(out[2], want[2])
+
+
 def test_logits_past_32_bit_offsets():
     V = 1 << 20
     x = torch.full((2100, V), -math.inf, dtype=F16, device=DEV)   # 4.4 GB
