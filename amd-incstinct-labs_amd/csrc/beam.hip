@@ -35,7 +35,7 @@ struct RangeSum { double s; float m; int pad; };   // sum of e^(x - m) over a ra
 
 struct BeamArgs {
     cdna4_beam_args p;
-    int parts, range;        // ranges of a row, logits of a range (a multiple of 4)
+    int parts, range;        // ranges of a row, logits of a range (a multiple of 8)
     uint64_t* keys;          // [rows][n][parts], 0: none
     RangeSum* sums;          // [rows][parts]
 };
@@ -125,8 +125,13 @@ __global__ __launch_bounds__(256) void beam_ranges(BeamArgs a) {
     const int row = (int)(item / a.parts), part = (int)(item % a.parts);
     if (row >= a.p.groups * a.p.beams) return;
     const bool own = has_own(a.p, row);   // waited for behind the first logits
-    const int n = a.p.n, begin = part * a.range, len = min(a.range, a.p.V - begin);
-    const size_t base = (size_t)row * a.p.logits_stride + begin;
+    const int n = a.p.n, V = a.p.V;
+    const size_t base = (size_t)row * a.p.logits_stride;
+    // Ranges begin at multiples of 16 bytes, the first one up to a load before the row (51 MB of bf16 rows of odd length are read in 14 us
+    // so, in 17 with loads that are not aligned). A vocabulary below a load is read one by one.
+    const bool vectors = V >= kVec;
+    const int back = vectors ? (int)(((uintptr_t)a.p.logits / (16 / kVec) + base) % kVec) : 0;
+    const int begin = part * a.range - back, end = min(begin + a.range, V);
     // Where a workgroup's four ranges are one row's, its waves share a bound: n logits of theirs, a quarter in each, are no less than
     // the least of the waves' (n / 4)-th best so far. What the others have published may be old: a bound that is too low.
     __shared__ volatile uint32_t quarter[4];
@@ -134,16 +139,15 @@ __global__ __launch_bounds__(256) void beam_ranges(BeamArgs a) {
     const int wave = __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
     float m = kLowest, s = 0.f;
     uint64_t list = 0;
-    // Loads past the end are moved back to end with it; their logits before the lane's place are another lane's. A vocabulary
-    // below a load is read one by one.
-    const bool vectors = a.p.V >= kVec;
+    // A load that begins before the row or ends past the range is moved into it; the lane has those of its logits that were in its place.
     u32x4_u raw[kLoads];   // of the next step
-    auto place = [&](int i0, int u) { return i0 + (u * 64 + lane) * kVec; };
+    auto place = [&](int i0, int u) { return begin + i0 + (u * 64 + lane) * kVec; };
+    auto first_of = [&](int i0, int u) { return max(min(place(i0, u), end - kVec), 0); };
     auto load = [&](int i0) {
         if (!vectors) return;
 #pragma unroll
         for (int u = 0; u < kLoads; ++u) {
-            const long long at = (long long)base + min(place(i0, u), len - kVec);
+            const size_t at = base + first_of(i0, u);
             if constexpr (kDtype == CDNA4_F32) raw[u] = *(const u32x4_u*)((const float*)a.p.logits + at);
             else raw[u] = *(const u32x4_u*)((const uint16_t*)a.p.logits + at);
         }
@@ -157,17 +161,17 @@ __global__ __launch_bounds__(256) void beam_ranges(BeamArgs a) {
         list = 0;
         if (careful) load(0);
         uint32_t least = 0;
-        for (int i0 = 0; i0 == 0 || i0 < len; i0 += kStep) {   // once also where the range is empty
+        for (int i0 = 0; i0 == 0 || begin + i0 < end; i0 += kStep) {   // once also where the range is empty
             float x[kValues];
-            int from[kLoads];   // of each load, its first logit in the range
-            const bool tail = i0 + kStep > len;
+            int from[kLoads];   // the token of each load's first logit
+            const bool more = begin + i0 + kStep <= end, edge = !more || begin + i0 < 0;
             // Logits of the step, lane by lane, in eights: a range's last step has fewer, and what a wave does goes by them.
-            const int count = max(min(kValues, ((len - i0 + 64 * kVec - 1) / (64 * kVec) * kVec + 7) & ~7), 8);
+            const int count = max(min(kValues, ((end - begin - i0 + 64 * kVec - 1) / (64 * kVec) * kVec + 7) & ~7), 8);
             const bool look = careful || !vectors;
             float top = -INFINITY;
 #pragma unroll
             for (int u = 0; u < kLoads; ++u) {
-                from[u] = vectors ? min(place(i0, u), len - kVec) : place(i0, u);
+                from[u] = vectors ? first_of(i0, u) : place(i0, u);
                 if (u * kVec >= count) continue;
 #pragma unroll
                 for (int e = 0; e < kVec; ++e) {
@@ -180,19 +184,20 @@ __global__ __launch_bounds__(256) void beam_ranges(BeamArgs a) {
 #pragma unroll
                     for (int e = 0; e < kVec; ++e) {
                         float& y = x[u * kVec + e];
-                        if (!vectors) y = from[u] + e < len ? logit(a.p, kDtype, base + from[u] + e) : -INFINITY;
+                        if (!vectors) y = from[u] + e < V ? logit(a.p, kDtype, base + from[u] + e) : -INFINITY;
                         y = cleaned(y);
                     }
                 }
-                if (tail) {
+                if (edge) {
+                    const int own0 = place(i0, u), own1 = min(own0 + kVec, end);
 #pragma unroll
                     for (int e = 0; e < kVec; ++e)
-                        if (from[u] + e < place(i0, u)) x[u * kVec + e] = -INFINITY;
+                        if (from[u] + e < own0 || from[u] + e >= own1) x[u * kVec + e] = -INFINITY;
                 }
 #pragma unroll
                 for (int e = 0; e < kVec; ++e) top = fmaxf(top, x[u * kVec + e]);
             }
-            if (!tail) load(i0 + kStep);   // clamped to the end where the range ends with this step
+            if (more) load(i0 + kStep);   // clamped to the end where the range ends with this step
             if (top > m) {
                 s *= exp_of(m - top);
                 m = top;
@@ -214,7 +219,7 @@ __global__ __launch_bounds__(256) void beam_ranges(BeamArgs a) {
             }
             if (share) least = min(min(quarter[0], quarter[1]), min(quarter[2], quarter[3]));
             list = merge<kValues>(list, n, least, top_order,
-                                  [&](int k) { return key_of(x[k], begin + from[k / kVec] + k % kVec); },
+                                  [&](int k) { return key_of(x[k], from[k / kVec] + k % kVec); },
                                   [&](uint32_t b) { return [&x, f = of_order(b)](int k) { return x[k] >= f; }; }, lane, count);
             if (share) {
                 const uint32_t best = (uint32_t)(read_lane(list, (n + 3) / 4 - 1) >> 32);
@@ -379,7 +384,7 @@ bool plan_beam(long long rows, int V, int beams, int n, BeamPlan& p) {
     // four waves of a workgroup on one row, unless it is short: they share a bound
     p.parts = 1;
     if (V >= 4096) p.parts = (int)std::max(4LL, std::min<long long>(V / 1024, rows ? 16LL * device_cus() / rows : 1) & ~3LL);
-    p.range = (int)(((long long)V + p.parts - 1) / p.parts + 7) & ~7;   // the last ranges may be empty
+    p.range = (int)(((long long)V + 7 + p.parts - 1) / p.parts + 7) & ~7;   // from up to 7 before the row; the last ranges may be empty
     p.ws_bytes = (size_t)rows * p.parts * (n * sizeof(uint64_t) + sizeof(RangeSum)) + 16;
     return (rows * p.parts + 3) / 4 * 256 <= 0xffffffffLL;
 }
