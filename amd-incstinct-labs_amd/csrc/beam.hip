@@ -7,8 +7,9 @@
 // far sorted over the lanes (n <= 64), key = (logit's order, lowest token first) in 64 bits. What is above the n-th best key of
 // the list, or of a first bound for it, is inserted one by one, which random logits need about n ln(range / n) times.
 // Launch 2: a workgroup takes a group: (M, S) and the n best of each row from its ranges, scores in fp64, the n best of those.
-// 256 rows of 100,003 bf16 logits, n = 16 (51 MB): 17.6-20 us, of which the reads alone take 17 (2.9 TB/s; all waves start at once and have 12 KB
-// each), and 6.6 in the second launch, a chain of loads, ranks and fp64 functions. Four rows of 32,000: 5.2 + 4.5.
+// 256 rows of 100,003 bf16 logits, n = 16 (51 MB): 18-19 us, of which the reads alone take 14 (3.7 TB/s; all waves start at once and have 12 KB
+// each) and the insertions most of the rest, and 6.6 in the second launch, a chain of loads, ranks and fp64 functions. Four rows of
+// 32,000: 5.2 + 4.5.
 #include <algorithm>
 #include <math.h>
 
