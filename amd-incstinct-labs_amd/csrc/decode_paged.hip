@@ -236,6 +236,16 @@ __device__ __forceinline__ u32x4 decode8(uint32_t c, float scale) {
 template <int RT>
 __device__ __forceinline__ bool check_limits(f32x4 (&s)[RT][2], const float (&m)[RT], float (&lm)[RT], int kb, const int (&limit)[RT],
                                              bool mask, float sc, int g) {
+    if (mask) {
+        asm volatile("");   // a branch of its own: the compiler has put the masks of every chunk into its arithmetic
+#pragma unroll
+        for (int t = 0; t < RT; ++t)
+#pragma unroll
+            for (int u = 0; u < 2; ++u)
+#pragma unroll
+                for (int e = 0; e < 4; ++e)
+                    if (kb + g * 8 + u * 4 + e >= limit[t]) s[t][u][e] = -INFINITY;
+    }
     bool need = false;
 #pragma unroll
     for (int t = 0; t < RT; ++t) {
@@ -243,10 +253,7 @@ __device__ __forceinline__ bool check_limits(f32x4 (&s)[RT][2], const float (&m)
 #pragma unroll
         for (int u = 0; u < 2; ++u)
 #pragma unroll
-            for (int e = 0; e < 4; ++e) {
-                if (mask && kb + g * 8 + u * 4 + e >= limit[t]) s[t][u][e] = -INFINITY;
-                v = fmaxf(v, s[t][u][e]);
-            }
+            for (int e = 0; e < 4; ++e) v = fmaxf(v, s[t][u][e]);
         lm[t] = v;
         need |= v * sc > m[t] + kTau;
     }
