@@ -46,6 +46,7 @@ struct PagedArgs {
     int nQH, HK, G, nq, batch, rows;   // rows of a row block
     int HB, items;                     // row blocks per kv head, items per sequence
     int page, lp, pages, max_len;
+    uint32_t head_bytes, page_bytes;   // of a pool's page: one head's, all heads' (below 2^31)
     int shares;
     float sc;
 };
@@ -138,9 +139,9 @@ struct Pages {
 
 // Where the 16 rows of a head from key k on begin in the pools, k the same in every lane and its entry among the loaded ones. Rows past
 // the last one lie in its page or, past that, in some page of the sequence: they are read and come to nothing.
-__device__ __forceinline__ size_t rows_at(const PagedArgs& a, const Pages& pg, int k, int kvh, int head_bytes, int row_bytes) {
-    const int id = __builtin_amdgcn_readlane(pg.ids, (k >> a.lp) - pg.first);
-    return ((size_t)id * a.HK + kvh) * head_bytes + (size_t)((k & (a.page - 1)) * row_bytes);
+__device__ __forceinline__ size_t rows_at(const PagedArgs& a, const Pages& pg, int k, int kvh, int row_bytes) {
+    const uint32_t id = (uint32_t)__builtin_amdgcn_readlane(pg.ids, (k >> a.lp) - pg.first);
+    return (size_t)id * a.page_bytes + ((uint32_t)kvh * a.head_bytes + (uint32_t)((k & (a.page - 1)) * row_bytes));
 }
 
 // One chunk's K and V rows into a ring stage (K first), 16-bit rows. A chunk lies in one page, or, with pages of 16 rows, in two: the copies
@@ -151,7 +152,7 @@ __device__ __forceinline__ void copy_chunk(const PagedArgs& a, const Pages& pg, 
     uint16_t* const vstage = stage + kKeys * D;
     size_t at[2];
 #pragma unroll
-    for (int h = 0; h < 2; ++h) at[h] = rows_at(a, pg, scalar(kb) + 16 * h, scalar(kvh), a.page * 2 * D, 2 * D);
+    for (int h = 0; h < 2; ++h) at[h] = rows_at(a, pg, scalar(kb) + 16 * h, scalar(kvh), 2 * D);
     const int r = lane / CPR, c = lane % CPR;
     const uint32_t ko = (uint32_t)(r * 2 * D + (c ^ swz_k<D>(r)) * 16), vo = (uint32_t)(r * 2 * D + (c ^ swz_v<D>(r)) * 16);
 #pragma unroll
@@ -196,9 +197,10 @@ __device__ __forceinline__ void load_codes(const PagedArgs& a, const Pages& pg, 
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
         const int k = scalar(kb) + 16 * h;
-        const size_t head = rows_at(a, pg, k, scalar(kvh), a.page * (D / 2 + BPR), 0);
-        at[h] = head + (k & (a.page - 1)) * (D / 2);
-        sc[h] = head + a.page * (D / 2) + (k & (a.page - 1)) * BPR;
+        const size_t head = rows_at(a, pg, k, scalar(kvh), 0);
+        const uint32_t row = (uint32_t)(k & (a.page - 1));
+        at[h] = head + row * (D / 2);
+        sc[h] = head + ((uint32_t)a.page * (D / 2) + row * BPR);
     }
     // K rows 8 (li / 4) + li % 4 + 4 u: lanes li < 8 in the first half of the chunk
     const int kr = 8 * (li >> 2 & 1) + (li & 3);
@@ -837,6 +839,8 @@ extern "C" int cdna4_attn_decode_paged(const void* q, const void* K_pages, const
     a.nQH = cfg->nQHeads; a.HK = cache->nKVHeads; a.G = p.G; a.nq = cfg->nq; a.batch = cfg->batch; a.rows = p.rows;
     a.HB = p.HB; a.items = p.items;
     a.page = cache->page; a.lp = log2_of(cache->page); a.pages = cache->pages; a.max_len = cache->max_pages * cache->page;
+    a.head_bytes = (uint32_t)(cache->page * paged::row_bytes(cache->D, cache->format == CDNA4_KV_MXFP4));
+    a.page_bytes = (uint32_t)cache->nKVHeads * a.head_bytes;
     a.shares = p.shares;
     a.sc = kLog2e / sqrtf((float)cache->D);
     hipStream_t s = (hipStream_t)stream;
