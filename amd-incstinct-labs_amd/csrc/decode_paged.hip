@@ -13,7 +13,7 @@
 // Weights are rounded to the inputs' 16-bit type for P.V and added up as rounded, in fp32; in bf16 the first keys' get a second term,
 // as in the other decode kernels. MXFP4 values are decoded to that type exactly.
 // Bound by HBM where there are keys enough: 128 sequences of 500-4,096 bf16 keys, 32/8 heads, D 128 (902 MB) 141 us in the first launch,
-// 6.4 TB/s, and 4.4 in the join; three of 30,000-131,072 in MXFP4 (267 MB) 49 and 6.2. A share's start (its place, its pages' entries, its
+// 6.4 TB/s, and 4.4 in the join; three of 30,000-131,072 in MXFP4 (267 MB) 46-49 and 6.2. A share's start (its place, its pages' entries, its
 // first keys: three loads behind one another) and the join's take about 15 us of any call, 22 + 4.3 us for 64 sequences of 20-4,000
 // in MXFP4 (57 MB), where a wave has four or five chunks. One launch of four sequences of up to 545 keys, 12 heads, D 64: 5.5.
 #include <algorithm>
@@ -184,7 +184,7 @@ struct Codes {
 };
 
 template <int D, bool kNT>
-__device__ __forceinline__ void load_codes(const PagedArgs& a, const Pages& pg, int kb, int len, int kvh, Codes<D>& x, int lane) {
+__device__ __forceinline__ void load_codes(const PagedArgs& a, const Pages& pg, int kb, int kvh, Codes<D>& x, int lane) {
     const int li = lane & 15, g = lane >> 4;
     constexpr int KW = Codes<D>::KW, VB = Codes<D>::VB, BPR = D / 32;   // blocks of a row
     auto get = [&](auto* p) {
@@ -220,12 +220,6 @@ __device__ __forceinline__ void load_codes(const PagedArgs& a, const Pages& pg, 
         const char *vc = a.V + (second ? at[1] : at[0]), *vsc = a.V + (second ? sc[1] : sc[0]);
         x.v[j] = get((const u32x4*)(vc + ((r & 15) * (D / 2) + lane % BPR * 16)));
         x.vs[j] = *(const uint8_t*)(vsc + ((r & 15) * BPR + lane % BPR));
-    }
-    if (kb + kKeys > len) {   // rows past the last: values of next to nothing whatever they hold, since their weights of zero do not undo
-                              // what is not finite
-#pragma unroll
-        for (int j = 0; j < VB; ++j)
-            if (kb + (64 * j + lane) / BPR >= len) x.vs[j] = 0;
     }
 }
 
@@ -342,7 +336,11 @@ struct RowBlock {
 #pragma unroll
         for (int j = 0; j < Codes<D>::VB; ++j) {
             const int r = (64 * j + lane) / ND, blk = lane % ND;
-            const float f = f32_from_bits(x.vs[j] << 23);
+            // rows past the last: values of next to nothing whatever they hold, since their weights of zero do not undo what is not
+            // finite; here and not at the load, which would wait for it
+            uint32_t scale = x.vs[j];
+            if (kb + kKeys > len && kb + r >= len) scale = 0;
+            const float f = f32_from_bits(scale << 23);
 #pragma unroll
             for (int i = 0; i < 4; ++i) *(u32x4*)(vlds + r * D + ((4 * blk + i) ^ swz_v<D>(r)) * 8) = decode8<kBf16>(x.v[j][i], f);
         }
@@ -468,7 +466,7 @@ __global__ __launch_bounds__(64, (waves_per_cu(D, RT, kFp4) + 3) / 4) void paged
     if constexpr (kFp4) {
         // The next segment's pages are loaded a segment ahead, its first codes while the last ones of this are used.
         Codes<D> x, y;   // in turn: the next chunk's codes are on their way while one is used
-        load_codes<D, kNT>(a, cur.pg, cur.c0 * kKeys, cur.len, cur.kvh, x, lane);
+        load_codes<D, kNT>(a, cur.pg, cur.c0 * kKeys, cur.kvh, x, lane);
         for (;;) {
             rb.load_q(cur.b, cur.kvh, cur.hb, rb.q);
             more = left > 0;
@@ -477,9 +475,9 @@ __global__ __launch_bounds__(64, (waves_per_cu(D, RT, kFp4) + 3) / 4) void paged
             auto ahead = [&](Codes<D>& z, int c) {
                 if (c < cur.c1) {
                     pages_for(a, cur, c, lane);
-                    load_codes<D, kNT>(a, cur.pg, c * kKeys, cur.len, cur.kvh, z, lane);
+                    load_codes<D, kNT>(a, cur.pg, c * kKeys, cur.kvh, z, lane);
                 } else if (more) {
-                    load_codes<D, kNT>(a, nxt.pg, nxt.c0 * kKeys, nxt.len, nxt.kvh, z, lane);
+                    load_codes<D, kNT>(a, nxt.pg, nxt.c0 * kKeys, nxt.kvh, z, lane);
                 }
             };
             bool in_y;   // where the next segment's codes are
@@ -570,25 +568,25 @@ __global__ __launch_bounds__(64 * W) void paged_whole(PagedArgs a) {
     s.c1 = s.n * (wave + 1) / W;
     rb.begin(s.len, s.hb);
     if (s.c0 < s.c1) {
-        pages_for(a, s, s.c0, lane);
         if constexpr (kFp4) {
+            // Chunks in pairs, the next one's codes always on their way (past the last, that one's once more): where ways with and without
+            // loads meet, the compiler waits for all that may be on its way.
             Codes<D> x, y;
-            load_codes<D, false>(a, s.pg, s.c0 * kKeys, s.len, s.kvh, x, lane);
-            for (int c = s.c0;; c += 2) {
-                if (c + 1 < s.c1) {
-                    pages_for(a, s, c + 1, lane);
-                    load_codes<D, false>(a, s.pg, (c + 1) * kKeys, s.len, s.kvh, y, lane);
-                }
+            auto load = [&](int c, Codes<D>& to) {
+                pages_for(a, s, c, lane);
+                load_codes<D, false>(a, s.pg, c * kKeys, s.kvh, to, lane);
+            };
+            load(s.c0, x);
+            int c = s.c0;
+            for (; c + 1 < s.c1; c += 2) {
+                load(c + 1, y);
                 rb.use(x, c * kKeys, s.len, lds);
-                if (c + 1 >= s.c1) break;
-                if (c + 2 < s.c1) {
-                    pages_for(a, s, c + 2, lane);
-                    load_codes<D, false>(a, s.pg, (c + 2) * kKeys, s.len, s.kvh, x, lane);
-                }
+                load(min(c + 2, s.c1 - 1), x);
                 rb.use(y, (c + 1) * kKeys, s.len, lds);
-                if (c + 2 >= s.c1) break;
             }
+            if (c < s.c1) rb.use(x, c * kKeys, s.len, lds);
         } else {
+            pages_for(a, s, s.c0, lane);
             copy_chunk<D, false>(a, s.pg, s.c0 * kKeys, s.kvh, lds, lane);
             rb.ready();
             for (int c = s.c0, st = 0; c < s.c1; ++c, st ^= 1) {
@@ -719,7 +717,7 @@ constexpr int most_waves(int D, int RT, bool fp4) { return D == 64 || (fp4 && RT
 // that a wave has; 0: equal shares. Their second launch and the walk over the lengths cost 7-10 us, which up to eight chunks a
 // wave and sixteen over its rounds (MXFP4: twenty-four) do not: 16 sequences, 32/8 heads D 128, of 120 keys 4.7 against 13.6 us, of
 // 1,000 13.0 against 18.7; 64 of 1,000 40 against 47, 256 of 250 42 against 48. Beyond, the shares' even ends win: 128 of 1,000 (32
-// chunks) 95 against 87 us; in MXFP4 30 against 40, 256 of 1,000 (24 chunks) 61 against 65.
+// chunks) 95 against 87 us; in MXFP4, where a pair of chunks has gained some 10 % since, 30 against 40, 256 of 1,000 (24 chunks) 61 against 65.
 int choose_waves(long long items, int max_len, int D, int RT, bool fp4, long long resident) {
     const int chunks = (max_len + kKeys - 1) / kKeys;
     int best = 0;
