@@ -13,8 +13,8 @@
 // Weights are rounded to the inputs' 16-bit type for P.V and added up as rounded, in fp32; in bf16 the first keys' get a second term,
 // as in the other decode kernels. MXFP4 values are decoded to that type exactly.
 // Bound by HBM where there are keys enough: 128 sequences of 500-4,096 bf16 keys, 32/8 heads, D 128 (902 MB) 141 us in the first launch,
-// 6.4 TB/s, and 4.4 in the join; three of 30,000-131,072 in MXFP4 (267 MB) 46-49 and 6.2. A share's start (its place, its pages' entries, its
-// first keys: three loads behind one another) and the join's take about 15 us of any call, 22 + 4.3 us for 64 sequences of 20-4,000
+// 6.4 TB/s, and 4.2 in the join; three of 30,000-131,072 in MXFP4 (267 MB) 46-49 and 6.2. A share's start (its place, its pages' entries, its
+// first keys: three loads behind one another) and the join's take about 15 us of any call, 20-22 + 4.2 us for 64 sequences of 20-4,000
 // in MXFP4 (57 MB), where a wave has four or five chunks. One launch of four sequences of up to 545 keys, 12 heads, D 64: 5.5.
 #include <algorithm>
 #include <math.h>
