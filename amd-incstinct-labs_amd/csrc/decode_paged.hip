@@ -715,9 +715,10 @@ constexpr int most_waves(int D, int RT, bool fp4) { return D == 64 || (fp4 && RT
 
 // One launch for short caches: the waves per item that end soonest, a round of the chip's waves taken for five chunks' time and those
 // that a wave has; 0: equal shares. Their second launch and the walk over the lengths cost 7-10 us, which up to eight chunks a
-// wave and sixteen over its rounds (MXFP4: twenty-four) do not: 16 sequences, 32/8 heads D 128, of 120 keys 4.7 against 13.6 us, of
-// 1,000 13.0 against 18.7; 64 of 1,000 40 against 47, 256 of 250 42 against 48. Beyond, the shares' even ends win: 128 of 1,000 (32
-// chunks) 95 against 87 us; in MXFP4, where a pair of chunks has gained some 10 % since, 30 against 40, 256 of 1,000 (24 chunks) 61 against 65.
+// wave, and of 16-bit rows sixteen over its rounds or four to an item, do not: 16 sequences, 32/8 heads D 128, of 120 keys 4.8 against
+// 16 us, of 1,000 13 against 19; 64 of 1,000 40 against 47, 256 of 250 41 against 49, 4,000 of 120 361 against 430. Beyond, the
+// shares' even ends win: 128 of 1,000 (32 chunks) 95 against 87 us. In MXFP4, where a share's waves have fewer registers, 128 of 1,000 26
+// against 37, 1,600 of 500 165 against 185.
 int choose_waves(long long items, int max_len, int D, int RT, bool fp4, long long resident) {
     const int chunks = (max_len + kKeys - 1) / kKeys;
     int best = 0;
@@ -725,7 +726,7 @@ int choose_waves(long long items, int max_len, int D, int RT, bool fp4, long lon
     for (int w = 1; w <= most_waves(D, RT, fp4); w *= 2) {
         const int each = (chunks + w - 1) / w;
         const long long rounds = (items * w + resident - 1) / resident, t = rounds * (5 + each);
-        if (each > 8 || rounds * each > (fp4 ? 24 : 16)) continue;
+        if (each > 8 || rounds > 1024 || (!fp4 && chunks > 4 && rounds * each > 16)) continue;   // fewer than 2^32 threads in any case
         if (best == 0 || t < least) { best = w; least = t; }
     }
     return best;

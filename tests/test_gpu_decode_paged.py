@@ -19,7 +19,7 @@ def make(lens, HQ, HK, D, dtype, page=16, fmt="16", nq=1, seed=0, scale=1.0, for
     p = Paged(lens, HK, D, dtype, page, fmt, seed, room=min(2, 256 // page) if form == "whole" else 4096 // page)
     q = (torch.randn(len(lens), nq, HQ, D, device=DEV, generator=p.g) * scale).to(dtype)
     cfg = cdna4.PagedDecodeCfg(HQ, len(lens), nq)
-    if max(lens, default=0) <= 700 and len(lens) <= 130:
+    if max(lens, default=0) <= 700 and len(lens) <= 130:     # `room` decides there
         assert (cdna4.decode_paged_plan(p.cache, cfg).workspace == 0) == (form == "whole")
     return p, q, cfg
 
