@@ -781,14 +781,18 @@ def _table_size(cache: PagedCache, rows: int) -> int:
 
 
 def _rows(name: str, t: torch.Tensor, dtype, dev: int, shape) -> int:
-    """Token stride of t [T][heads][D] with its heads side by side, 0 where it does not matter."""
+    """Token stride of t [T][heads][D] with its heads side by side, 0 (the C call's "packed") where there is one token."""
     if t.dtype is not dtype or t.get_device() != dev or t.shape != shape:
         raise ValueError(f"{name} must be {dtype} {list(shape)} on GPU {dev}")
     row, head, one = t.stride()
+    if shape[0] < 2:
+        row = 0
+    elif row < shape[1] * shape[2]:   # 0 among them, the stride of a token repeated by expand()
+        raise ValueError(f"{name}'s tokens must not lie over each other")
     if one != 1 or (head != shape[2] and shape[1] > 1):
         if t.numel():
             raise ValueError(f"{name} must have its heads side by side")
-    return row if shape[0] > 1 else 0
+    return row
 
 
 def rope_append_paged(q: Optional[torch.Tensor], k: torch.Tensor, v: torch.Tensor, K_pages: torch.Tensor, V_pages: torch.Tensor,
@@ -796,8 +800,8 @@ def rope_append_paged(q: Optional[torch.Tensor], k: torch.Tensor, v: torch.Tenso
                       seqs: Optional[torch.Tensor] = None, cos: Optional[torch.Tensor] = None, sin: Optional[torch.Tensor] = None,
                       q_norm: Optional[torch.Tensor] = None, k_norm: Optional[torch.Tensor] = None, eps: float = 1e-6,
                       k_out: Optional[torch.Tensor] = None, v_out: Optional[torch.Tensor] = None, stream=None) -> Optional[torch.Tensor]:
-    """T tokens' projections q [T][nQH][D], k, v [T][nKVH][D] (fp16 or bf16, any token stride with contiguous heads: parts of one
-    projection's output) into a paged cache: queries and keys normed per head (q_norm, k_norm [D], optional) and rotated
+    """T tokens' projections q [T][nQH][D], k, v [T][nKVH][D] (fp16 or bf16, a token's heads contiguous, tokens at any stride that
+    leaves them apart: parts of one projection's output) into a paged cache: queries and keys normed per head (q_norm, k_norm [D], optional) and rotated
     (cos, sin fp32 [max_pos][D], optional), keys and values to row positions[t] of sequence seqs[t] (int32 [T]; seqs None: t), queries to
     q_out (None: allocated), which is returned. k_out, v_out [T][nKVH][D], optional: what the cache now holds for the
     tokens. tables int32 [batch][max_pages]. Padding tokens have a position or a sequence of -1. q None: keys and values

@@ -251,6 +251,20 @@ def test_python_refuses():
         c.run(seqs=None)
 
 
+@pytest.mark.parametrize("name", ["q", "k", "v", "q_out", "k_out", "v_out"])
+def test_tokens_over_each_other_are_refused(name):
+    """One token's row repeated by expand() has a token stride of 0, which the C call would take for packed tokens."""
+    c = Call([5], [0], 4, 2, 64, F16, 16, "16", seed=10)
+    K0, V0, t = c.K.clone(), c.V.clone(), getattr(c, name)
+    setattr(c, name, t[:1].contiguous().expand(t.shape))
+    with pytest.raises(ValueError):
+        c.run()
+    assert torch.equal(c.K, K0) and torch.equal(c.V, V0)
+    # one token may have any stride
+    one = dict(seqs=c.seqs[:1], k_out=c.k_out[:1], v_out=c.v_out[:1])
+    cdna4.rope_append_paged(c.q[:1], c.k[:1], c.v[:1], c.K, c.V, c.tables, c.positions[:1], c.cache, c.q_out[:1], cos=c.cos, sin=c.sin, **one)
+
+
 def test_pools_past_32_bit_offsets():
     HK, D, page = 8, 128, 256
     pages = 2 ** 32 // (HK * page * 256) + 8

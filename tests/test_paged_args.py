@@ -174,6 +174,21 @@ def test_python_refuses_cpu_tensors():
         cdna4.beam_select(torch.zeros(4, 10), torch.zeros(4), 4)
 
 
+def test_token_strides():
+    """The C call takes a stride of 0 for packed tokens, so Python passes it only where the stride does not matter."""
+    f16, x = torch.float16, torch.zeros(16, 10, 64, dtype=torch.float16)
+    stride = lambda t, *shape: cdna4._rows("k", t, f16, -1, shape or tuple(t.shape))
+    assert stride(x) == 640 and stride(x[:, 2:5]) == 640 and stride(x[::2, :1]) == 1280 and stride(x[:1]) == 0 and stride(x[:0]) == 0
+    assert stride(x[:1, :1].expand(1, 1, 64)) == 0
+    for t in (x[:1].expand(16, 10, 64), x[:1, :1].expand(16, 1, 64), x.as_strided((3, 10, 64), (64, 64, 1)), x.as_strided((2, 1, 64), (32, 64, 1)),
+              x.as_strided((2, 10, 64), (639, 64, 1))):
+        with pytest.raises(ValueError):
+            stride(t)
+    for t in (x[:, ::2], x[:, :, ::2], x[:, :1].expand(16, 10, 64)):
+        with pytest.raises(ValueError):
+            stride(t)
+
+
 @pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
 def test_mxfp4_reference(dtype):
     """Every grid value at every scale is kept; midpoints go to the even code; a block's largest value is off by half a step at most."""
