@@ -10,8 +10,11 @@
 //     it: lengths are read on the device, and what a wave has to do does not depend on how they differ. A share that holds all
 //     chunks of an item writes the output; of an item that shares cut, each leaves (m, l, O), and a second launch joins them,
 //     o = sum_p 2^(m_p - M) O_p / sum_p 2^(m_p - M) l_p.
-// Weights are rounded to the inputs' 16-bit type for P.V and added up as rounded, in fp32; in bf16 the first keys' get a second term,
-// as in the other decode kernels. MXFP4 values are decoded to that type exactly.
+// Weights go into P.V as two terms of the inputs' 16-bit type, 16 (bf16) or 22 bits of each, and are added up as they go, in fp32: an
+// output is then off by its own rounding. With one term its error is 1.1 to 1.4 times that, over any number of keys, and the time the same
+// within 2 %: 148.4 against 148.6 us (128 sequences of 500-4,096 in bf16), 39.8 against 40.5 (two row tiles), 53.7 against 54.7 and
+// 24.9 against 23.9 (MXFP4; there the branch that gave only the first keys a second term spilled registers). MXFP4 values are decoded to
+// the 16-bit type exactly.
 // Bound by HBM where there are keys enough: 128 sequences of 500-4,096 bf16 keys, 32/8 heads, D 128 (902 MB) 141 us in the first launch,
 // 6.4 TB/s, and 4.2 in the join; three of 30,000-131,072 in MXFP4 (267 MB) 46-49 and 6.2. A share's start (its place, its pages' entries, its
 // first keys: three loads behind one another) and the join's take about 15 us of any call, 20-22 + 4.2 us for 64 sequences of 20-4,000
@@ -256,6 +259,23 @@ __device__ __forceinline__ bool check_limits(f32x4 (&s)[RT][2], const float (&m)
     return need;
 }
 
+// Weights p = 2^(s sc - m) as two 16-bit terms each, hi = round(p), lo = round(p - hi) (p - hi is exact in fp32), packed into the B
+// operands of the P.V product.
+template <int RT, bool kBf16>
+__device__ __forceinline__ void two_terms(const f32x4 (&s)[RT][2], const float (&m)[RT], u32x4 (&hi)[RT], u32x4 (&lo)[RT], float sc) {
+#pragma unroll
+    for (int t = 0; t < RT; ++t)
+#pragma unroll
+        for (int x = 0; x < 4; ++x) {
+            const float p0 = __builtin_amdgcn_exp2f(fmaf(s[t][x >> 1][(x & 1) * 2], sc, -m[t]));
+            const float p1 = __builtin_amdgcn_exp2f(fmaf(s[t][x >> 1][(x & 1) * 2 + 1], sc, -m[t]));
+            const uint32_t h = pack2<kBf16>(p0, p1);
+            hi[t][x] = h;
+            if constexpr (kBf16) lo[t][x] = pack2<true>(p0 - f32_from_bits(h << 16), p1 - f32_from_bits(h & 0xffff0000u));
+            else lo[t][x] = pack2<false>(p0 - f16_bits_to_f32(h & 0xffffu), p1 - f16_bits_to_f32(h >> 16));
+        }
+}
+
 // Waves that a CU holds: 16-bit rows as many as have a ring in its LDS, MXFP4 as the registers allow.
 constexpr int waves_per_cu(int D, int RT, bool fp4) { return fp4 ? (RT == 2 ? 8 : D == 128 ? 12 : 16) : D == 128 ? 4 : 8; }
 
@@ -314,14 +334,19 @@ struct RowBlock {
         float lm[RT];
         const bool need = check_limits<RT>(s, m, lm, kb, limit, kb + kKeys > len - a.nq + 1, a.sc, g);
         if (__builtin_amdgcn_ballot_w64(need)) rescale_rows<D, RT>(lm, m, o, lacc, a.sc);
-        u32x4 pb[RT];
-        softmax_chunk<RT, kBf16>(s, m, pb, a.sc);
-        pv_chunk<D, RT, kBf16>(Vt, off, pb, o, lacc, 0);
-        if constexpr (kBf16) {
-            if (kb < kLoKeys) {   // the first keys: the weights' second bf16 term
-                softmax_lo_chunk<RT>(s, m, pb, a.sc);
-                pv_chunk<D, RT, true>(Vt, off, pb, o, lacc, 0);
-            }
+        u32x4 hi[RT], lo[RT];
+        two_terms<RT, kBf16>(s, m, hi, lo, a.sc);
+        const uint32_t one2 = kBf16 ? 0x3F803F80u : 0x3C003C00u;   // two 16-bit 1.0
+        const u32x4 ones{one2, one2, one2, one2};
+#pragma unroll
+        for (int t = 0; t < RT; ++t) lacc[t] = mfma<kBf16>(ones, lo[t], mfma<kBf16>(ones, hi[t], lacc[t]));
+#pragma unroll
+        for (int d = 0; d < NDT; ++d) {
+            const u32x2 v0 = __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((LDS_AS s16x4*)(Vt + off.vd(d))));
+            const u32x2 v1 = __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((LDS_AS s16x4*)(Vt + off.vd(d) + 4 * D * 2)));
+            const u32x4 va{v0[0], v0[1], v1[0], v1[1]};
+#pragma unroll
+            for (int t = 0; t < RT; ++t) o[t][d] = mfma<kBf16>(va, lo[t], mfma<kBf16>(va, hi[t], o[t][d]));
         }
     }
     // A chunk of 16-bit rows that is in a ring stage.

@@ -419,9 +419,11 @@ int cdna4_rope_append_paged(const cdna4_append_args* args, const cdna4_paged_cac
 /* cdna4_attn_decode_paged: nq queries per sequence, those of its last nq tokens, over the cache: query i of sequence b sees rows
  * 0 .. lens[b] - nq + i (lens: int32, device memory, cut to 0 .. max_pages * page; a query that sees no row gets zeros). q, o:
  * [batch][nq][nQHeads][D], dtype CDNA4_F16 or CDNA4_BF16, also the type of a CDNA4_KV_16 cache; query head h reads kv head
- * h / (nQHeads / nKVHeads); scale 1/sqrt(D), softmax and sums in fp32; o must not overlap the inputs. Table entries past the last row's are not read into a
+ * h / (nQHeads / nKVHeads); scale 1/sqrt(D), softmax and sums in fp32, its weights in the product with V as two terms of dtype (16 bits
+ * of them in bf16, 22 in fp16); o must not overlap the inputs. Table entries past the last row's are not read into a
  * result; entries outside 0 .. pages - 1 of those before read some page of the pool (nothing outside it). Rows from lens[b] on
- * may hold anything. A value in V that is not finite reaches the queries of up to nq - 1 tokens before it. The plan follows from the
+ * may hold anything. An infinity or NaN in V makes NaN or
+ * infinity of its part of the outputs that see it and of those of up to nq - 1 tokens before. The plan follows from the
  * two structs alone, so a captured call replays on other lengths, tables and pages: tables of few pages take one launch, a workgroup
  * per sequence and row block; longer ones equal shares of all keys, whatever the lengths are, and a second launch. The workspace
  * (cdna4_attn_decode_paged_workspace_size bytes, 16-byte aligned, no initialisation; 0 for one launch) holds what shares leave of

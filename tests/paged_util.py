@@ -1,8 +1,10 @@
 """Paged caches for the tests: pools filled from contiguous keys and values, MXFP4 in 64 bits, references."""
+import math
+
 import torch
 
 import cdna4
-from serving_util import attend
+from serving_util import attend, unit
 
 GRID = torch.tensor([0.0, 0.5, 1.0, 1.5, 2.0, 3.0, 4.0, 6.0], dtype=torch.float64)
 
@@ -92,7 +94,30 @@ class Paged:
         self.lens = torch.tensor(lens, dtype=torch.int32, device=dev)
 
 
-def decode_reference(q, k, v, dtype):
+def attend_two_terms(q, k, v, seen, dtype):
+    """(O, bound) as serving_util.attend, for weights that enter the product with V as two 16-bit terms:
+      the weights: hi is within u of p, lo within u of p - hi, u^2 in all, or, where lo is below fp16's normal range, half of its
+      smallest step, 2^-25, as a part of a sum that is at least 1; over A + |O|, A = sum_j w_j |v_j|;
+      scores: as there, (2 D + 16) 2^-24 of sum_d |q_d k_d| / sqrt(D), as a relative error of each weight, twice;
+      sums in 32 bits: for 32 keys two matrix instructions, each of them a rounding within and one of the running sum: N / 8, and 16 for
+      the joining of parts;
+      the output's rounding: half a step of what the rest has left."""
+    q, k, v = q.double(), k.double(), v.double()
+    N, D = k.shape
+    s = ((q @ k.t().contiguous()) / math.sqrt(D)).masked_fill(~seen, -math.inf)
+    m = s.amax(1, keepdim=True)
+    w = torch.exp(s - torch.where(m == -math.inf, torch.zeros_like(m), m))
+    tot = w.sum(1, keepdim=True)
+    w = w / torch.where(tot == 0, torch.ones_like(tot), tot)
+    O, A, u, e = w @ v, w @ v.abs(), unit(dtype), 2.0 ** -24
+    mag = ((q.abs() @ k.abs().t().contiguous()) / math.sqrt(D)).masked_fill(~seen, 0.0).amax(1, keepdim=True)
+    off = (u * u + 2 * (2 * D + 16) * e * mag + (N / 8 + 16) * e) * (A + O.abs())
+    if dtype == torch.float16:
+        off = off + N * 2.0 ** -25 * v.abs().amax(0, keepdim=True)
+    return O, off + u * (O.abs() + off) + (2.0 ** -25 if dtype == torch.float16 else 0.0)
+
+
+def decode_reference(q, k, v, dtype, attend=attend):
     """(o, bound) float64 of q [B][nq][HQ][D] over lists of keys and values [HK][n][D]: query i sees all but the last nq - 1 - i."""
     B, nq, HQ, D = q.shape
     O = torch.zeros(B, nq, HQ, D, dtype=torch.float64, device=q.device)

@@ -5,7 +5,7 @@ import pytest
 import torch
 
 import cdna4
-from paged_util import Paged, decode_reference
+from paged_util import Paged, attend_two_terms, decode_reference
 from serving_util import DEV, check
 
 pytestmark = pytest.mark.gpu
@@ -258,3 +258,19 @@ def test_one_wave_per_item(D, fmt):
     p.cache.max_pages, p.cache.table_stride = 1, p.tables.shape[1]
     assert cdna4.decode_paged_plan(p.cache, cfg).waves == 1 and cdna4.decode_paged_plan(p.cache, cfg).grid == 5000
     verify(p, q, run(p, q, cfg))
+
+
+@FORMS
+@pytest.mark.parametrize("fmt", ["16", "mxfp4"])
+@pytest.mark.parametrize("nq", [1, 5])
+@pytest.mark.parametrize("dtype", [F16, BF16])
+@pytest.mark.parametrize("D", [64, 128])
+def test_outputs_are_off_by_their_own_rounding(D, dtype, nq, fmt, form):
+    """Weights of one 16-bit term would move an output as far as its rounding does. Small scores, so that the bound's part for them is
+    far below that; as many keys as a wave's and several waves' chunks."""
+    p, q, cfg = make([300, 0, 33, 250, 120], 20, 2, D, dtype, 16, fmt, nq, seed=21, form=form)
+    q /= 64
+    o = run(p, q, cfg)
+    check(o, *decode_reference(q, p.k, p.v, dtype, attend_two_terms))
+    full = torch.randn(q.shape, device=DEV, generator=p.g).to(dtype)
+    check(run(p, full, cfg), *decode_reference(full, p.k, p.v, dtype, attend_two_terms))
