@@ -121,7 +121,8 @@ KV_16BIT, KV_MXFP4 = 0, 1   # formats of a paged cache (CDNA4_KV_*)
 
 class PagedCache(ctypes.Structure):
     """cdna4_paged_cache: pools of `pages` pages of `page` rows (16, 32, .. 256) for each kv head, in 16 bits or MXFP4;
-    tables of max_pages entries per sequence (table_stride apart, 0 = packed)."""
+    tables of max_pages entries per sequence (table_stride apart, 0 = packed). A call whose sequences are all short can name fewer
+    max_pages beside the table_stride of wider tables: decode_paged then takes one launch."""
     _fields_ = [(n, ctypes.c_int) for n in ("D", "nKVHeads", "page", "pages", "format", "max_pages")] + [
         ("table_stride", ctypes.c_longlong)]
 
@@ -774,10 +775,13 @@ def _pools(K: torch.Tensor, V: torch.Tensor, cache: PagedCache, dtype, dev: int,
     return _arg("K_pages", K, dtype, n, dev), _arg("V_pages", V, dtype, n, dev)
 
 
-def _table_size(cache: PagedCache, rows: int) -> int:
-    """Entries that the tables of `rows` sequences span."""
+def _tables(name: str, t: torch.Tensor, cache: PagedCache, rows: int, dev: int) -> int:
+    """Address of the tables of `rows` sequences; where t has rows of its own, they have to be the cache's."""
     most = cache.max_pages
-    return (rows - 1) * (cache.table_stride or most) + most if rows > 0 else 0
+    stride = cache.table_stride or most
+    if rows > 0 and t is not None and t.dim() > 1 and (t.shape[-1] < most or (rows > 1 and t.shape[-1] != stride)):
+        raise ValueError(f"{name} must have rows of {stride} entries (table_stride, or max_pages where that is 0)")
+    return _arg(name, t, _I32, (rows - 1) * stride + most if rows > 0 else 0, dev)
 
 
 def _rows(name: str, t: torch.Tensor, dtype, dev: int, shape) -> int:
@@ -804,7 +808,7 @@ def rope_append_paged(q: Optional[torch.Tensor], k: torch.Tensor, v: torch.Tenso
     leaves them apart: parts of one projection's output) into a paged cache: queries and keys normed per head (q_norm, k_norm [D], optional) and rotated
     (cos, sin fp32 [max_pos][D], optional), keys and values to row positions[t] of sequence seqs[t] (int32 [T]; seqs None: t), queries to
     q_out (None: allocated), which is returned. k_out, v_out [T][nKVH][D], optional: what the cache now holds for the
-    tokens. tables int32 [batch][max_pages]. Padding tokens have a position or a sequence of -1. q None: keys and values
+    tokens. tables int32 [batch][max_pages], or rows of cache.table_stride entries. Padding tokens have a position or a sequence of -1. q None: keys and values
     alone. The formulas: cdna4_rope_append_paged in cdna4_attn.h."""
     dev, dtype = _gpu_of(k), k.dtype
     if _elsewhere(dev, stream):
@@ -845,7 +849,7 @@ def rope_append_paged(q: Optional[torch.Tensor], k: torch.Tensor, v: torch.Tenso
         qn = _arg("q_norm", q_norm, dtype, D, dev)
     if k_norm is not None:
         kn = _arg("k_norm", k_norm, dtype, D, dev)
-    a = AppendArgs(qp, k.data_ptr(), v.data_ptr(), qo, ko, vo, Kp, Vp, _arg("tables", tables, _I32, _table_size(cache, batch), dev), sp,
+    a = AppendArgs(qp, k.data_ptr(), v.data_ptr(), qo, ko, vo, Kp, Vp, _tables("tables", tables, cache, batch, dev), sp,
                    _arg("positions", positions, _I32, T, dev), c, sn, qn, kn, eps, T, HQ, batch, max_pos, qr, kr, vr, qor, kor, vor)
     rc = lib().cdna4_rope_append_paged(ctypes.byref(a), ctypes.byref(cache), dt, torch._C._cuda_getCurrentRawStream(dev))
     if rc:
@@ -860,7 +864,8 @@ def decode_paged_workspace_size(cache: PagedCache, cfg: PagedDecodeCfg) -> int:
 def decode_paged(q: torch.Tensor, K_pages: torch.Tensor, V_pages: torch.Tensor, tables: torch.Tensor, lens: torch.Tensor,
                  o: torch.Tensor, cache: PagedCache, cfg: PagedDecodeCfg, workspace="auto", stream=None) -> None:
     """The queries of each sequence's last nq tokens over its rows of a paged cache: q, o [batch][nq][nQH][D] (fp16 or bf16, also
-    the type of a 16-bit cache); tables int32 [batch][max_pages], lens int32 [batch] (rows, the new tokens' among them) on the device.
+    the type of a 16-bit cache); tables int32 [batch][max_pages], or rows of cache.table_stride entries, lens int32 [batch] (rows, the new
+    tokens' among them) on the device.
     `workspace`: "auto" allocates decode_paged_workspace_size(cache, cfg) bytes (0 for short tables) on the stream the call launches
     on; a uint8 tensor is used as given."""
     dev, dtype = _gpu_of(q), q.dtype
@@ -871,7 +876,7 @@ def decode_paged(q: torch.Tensor, K_pages: torch.Tensor, V_pages: torch.Tensor, 
     n = B * cfg.nq * cfg.nQHeads * cache.D
     qp, op = _arg("q", q, dtype, n, dev), _arg("o", o, dtype, n, dev)
     Kp, Vp = _pools(K_pages, V_pages, cache, dtype, dev)
-    tp, lp = _arg("tables", tables, _I32, _table_size(cache, B), dev), _arg("lens", lens, _I32, B, dev)
+    tp, lp = _tables("tables", tables, cache, B, dev), _arg("lens", lens, _I32, B, dev)
     if workspace is None or (isinstance(workspace, str) and workspace != "auto"):
         raise ValueError("workspace must be 'auto' or a uint8 tensor")
     if isinstance(workspace, str):
@@ -895,7 +900,8 @@ def decode_paged_plan(cache: PagedCache, cfg: PagedDecodeCfg, dtype=F16) -> Plan
 
 def paged_reorder(parents: torch.Tensor, tables: torch.Tensor, lens: torch.Tensor, fresh: torch.Tensor, tables_out: torch.Tensor,
                   lens_out: torch.Tensor, K_pages: torch.Tensor, V_pages: torch.Tensor, cache: PagedCache, stream=None) -> None:
-    """The cache after beam_select: row i goes on from row parents[i] (int32; -1: unused). tables, tables_out int32 [rows][max_pages],
+    """The cache after beam_select: row i goes on from row parents[i] (int32; -1: unused). tables, tables_out int32 [rows][max_pages]
+    (or rows of cache.table_stride entries),
     lens, lens_out int32 [rows]; a last page that is not full is copied to page fresh[i] (int32) in K and V of every layer. K_pages,
     V_pages: one layer's pools, or those of several layers in one tensor (a dimension more)."""
     dev = _gpu_of(parents)
@@ -907,9 +913,9 @@ def paged_reorder(parents: torch.Tensor, tables: torch.Tensor, lens: torch.Tenso
     if cache.format != KV_MXFP4 and dtype is not torch.float16 and dtype is not torch.bfloat16:
         raise ValueError("pools must be fp16 or bf16")
     Kp, Vp = _pools(K_pages, V_pages, cache, dtype, dev, layers)
-    rc = lib().cdna4_paged_reorder(_arg("parents", parents, _I32, rows, dev), _arg("tables", tables, _I32, _table_size(cache, rows_in), dev),
+    rc = lib().cdna4_paged_reorder(_arg("parents", parents, _I32, rows, dev), _tables("tables", tables, cache, rows_in, dev),
                                    _arg("lens", lens, _I32, rows_in, dev), _arg("fresh", fresh, _I32, rows, dev),
-                                   _arg("tables_out", tables_out, _I32, _table_size(cache, rows), dev),
+                                   _tables("tables_out", tables_out, cache, rows, dev),
                                    _arg("lens_out", lens_out, _I32, rows, dev), Kp, Vp, ctypes.byref(cache), rows, rows_in, layers, 0,
                                    torch._C._cuda_getCurrentRawStream(dev))
     if rc:

@@ -164,3 +164,37 @@ def test_step_as_a_graph(fmt):
         torch.cuda.synchronize()
         for a, b in zip(g.results(), e.results()):
             assert torch.equal(a.nan_to_num() if a.is_floating_point() else a, b.nan_to_num() if b.is_floating_point() else b), i
+
+
+def test_tables_wider_than_max_pages():
+    """Refused without a table_stride, whose rows the calls would read at the wrong places; with one, the packed tables' bits."""
+    m = Model("16", 2)
+    g = torch.Generator(device=DEV)
+    g.manual_seed(3)
+    order = torch.randperm(POOL, device=DEV, generator=g).int()
+    tables, wide = order[:ROWS * 4].view(ROWS, 4).contiguous(), torch.full((ROWS, WIDTH), -1, dtype=torch.int32, device=DEV)
+    wide[:, :4] = tables
+    n, fresh = torch.randint(1, 64, (ROWS,), device=DEV, generator=g).int(), order[ROWS * 4:ROWS * 5].contiguous()
+    parents = torch.randint(0, ROWS, (ROWS,), device=DEV, generator=g).int()
+    ids, cfg = torch.randint(0, V, (ROWS,), device=DEV, generator=g), cdna4.PagedDecodeCfg(HQ, ROWS, 1)
+    for t in range(64):                                      # rows for every length
+        m.append(ids, wide, i32([t] * ROWS))
+    K0, V0 = m.K, m.V
+
+    def step(tables, stride, outs):
+        m.cache.max_pages, m.cache.table_stride, m.K, m.V = 4, stride, K0.clone(), V0.clone()
+        lens_out, o = torch.zeros_like(n), torch.zeros(ROWS, 1, HQ, D, dtype=F16, device=DEV)
+        q = m.append(ids, tables, n - 1)
+        cdna4.decode_paged(q, m.K, m.V, tables, n, o, m.cache, cfg)
+        cdna4.paged_reorder(parents, tables, n, fresh, outs, lens_out, m.K, m.V, m.cache)
+        return q, o, outs[:, :4], lens_out, m.K.nan_to_num(), m.V.nan_to_num()
+
+    a, b = step(tables, 0, torch.zeros_like(tables)), step(wide, WIDTH, torch.zeros_like(wide))
+    assert all(torch.equal(x, y) for x, y in zip(a, b))
+    q, o = a[0], a[1]
+    m.cache.table_stride = 0
+    for call in (lambda: m.append(ids, wide, n - 1), lambda: cdna4.decode_paged(q, m.K, m.V, wide, n, o, m.cache, cfg),
+                 lambda: cdna4.paged_reorder(parents, wide, n, fresh, tables, n.clone(), m.K, m.V, m.cache),
+                 lambda: cdna4.paged_reorder(parents, tables, n, fresh, wide, n.clone(), m.K, m.V, m.cache)):
+        with pytest.raises(ValueError):
+            call()

@@ -189,6 +189,21 @@ def test_token_strides():
             stride(t)
 
 
+def test_tables_rows():
+    """Tables whose rows are not as far apart as the kernels read them would name other sequences' pages."""
+    take = lambda c, rows, *shape: cdna4._tables("tables", torch.zeros(*shape, dtype=torch.int32), c, rows, -1)
+    packed, wide = cache(), cache(table_stride=7)                # max_pages 4
+    for ok in ((packed, 3, 3, 4), (packed, 3, 5, 4), (packed, 1, 1, 7), (packed, 3, 12), (packed, 0, 3, 7), (packed, 6, 2, 3, 4), (wide, 3, 3, 7),
+               (wide, 1, 1, 4), (wide, 3, 18)):
+        take(*ok)
+    for bad in ((packed, 3, 3, 7), (packed, 2, 3, 5), (packed, 3, 6, 3), (packed, 1, 5, 2), (packed, 3, 2, 4), (packed, 3, 11), (wide, 3, 3, 8), (wide, 3, 5, 4),
+                (wide, 3, 2, 7), (wide, 3, 17)):
+        with pytest.raises(ValueError):
+            take(*bad)
+    with pytest.raises(ValueError):
+        cdna4._tables("tables", None, packed, 3, -1)
+
+
 @pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
 def test_mxfp4_reference(dtype):
     """Every grid value at every scale is kept; midpoints go to the even code; a block's largest value is off by half a step at most."""
