@@ -401,6 +401,8 @@ int check_beam(const cdna4_beam_args* a, int dtype) {
     const void* words[5] = {a->cum, a->scores, a->parents, a->tokens, a->done};
     for (int i = 0; i < 5; ++i)
         if ((i < 4 && !words[i]) || ((uintptr_t)words[i] & 3u)) return CDNA4_ERR_INVALID_VALUE;
+    // a group's scores in the place of its own cum alone: other groups' workgroups read theirs meanwhile
+    if (a->scores == a->cum && a->n != a->beams) return CDNA4_ERR_INVALID_VALUE;
     return 0;
 }
 

@@ -472,7 +472,7 @@ int cdna4_paged_reorder(const int* parents, const int* tables, const int* lens, 
  * The workspace (cdna4_beam_select_workspace_size bytes for groups * beams rows, 16-byte aligned, no initialisation) must not be
  * shared by calls that overlap; query its size with the device current that the call will run on. groups == 0: nothing is done.
  * Invalid: beams or n not 1 .. 64, V < 1, groups negative, 2^24 rows and more, a logits stride below V, done with an eos outside 0 .. V - 1,
- * null or misaligned pointers, a missing or small workspace.
+ * scores at cum's address with n != beams, null or misaligned pointers, a missing or small workspace.
  */
 typedef struct {
     const void* logits;        /* [groups * beams][logits_stride] */

@@ -199,6 +199,17 @@ def test_scores_in_the_place_of_cum():
         assert torch.equal(cum.view(G, beams), want[0]) and torch.equal(out[1], want[1]) and torch.equal(out[2], want[2])
 
 
+def test_scores_in_the_place_of_cum_of_another_number_are_refused():
+    for n in (2, 6):
+        x, cum = make(3, 4, 3000, F16, seed=n)
+        room = torch.zeros(max(12, 3 * n), device=DEV)       # both at one address, each long enough
+        room[:12] = cum
+        out = (room, torch.empty(3, n, dtype=torch.int32, device=DEV), torch.empty(3, n, dtype=torch.int32, device=DEV))
+        with pytest.raises(cdna4.CDNA4Error):
+            cdna4.beam_select(x, room, 4, n, out=out)
+        assert torch.equal(room[:12], cum)
+
+
 def test_logits_past_32_bit_offsets():
     V = 1 << 20
     x = torch.full((2100, V), -math.inf, dtype=F16, device=DEV)   # 4.4 GB

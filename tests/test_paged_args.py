@@ -160,6 +160,28 @@ def test_beam_refuses_sizes_and_workspaces():
     assert beam(dtype=cdna4.F32, logits=66) == 1
 
 
+@pytest.mark.parametrize("n", [1, 3, 5, 64])
+def test_beam_refuses_scores_over_the_cum_of_other_groups(n):
+    """scores may be cum where a group has as many of each."""
+    a = cdna4.BeamArgs(64, 128, None, 128, 256, 320, 2, 4, n, 1000, -1, 1000)
+    assert cdna4.lib().cdna4_beam_select(ctypes.byref(a), cdna4.F16, P, 1 << 40, None) == 1
+
+
+@pytest.mark.parametrize("bad", [
+    dict(groups=-1), dict(beams=0), dict(beams=65), dict(V=0), dict(V=2 ** 31 - 1), dict(logits_stride=999), dict(groups=2 ** 22), dict(done=64, eos=1000),
+    dict(done=64, eos=-1), dict(logits=None), dict(cum=None), dict(scores=None), dict(parents=None), dict(tokens=None), dict(logits=65), dict(cum=66),
+    dict(scores=66), dict(parents=66), dict(tokens=66), dict(done=66, eos=1), dict(n=0), dict(n=65), dict(dtype=cdna4.F64), dict(ws=None), dict(ws=ODD8),
+    dict(n_bytes=600)])
+def test_beam_refuses_with_scores_of_their_own(bad):
+    """Each by itself, scores and cum apart."""
+    a = cdna4.BeamArgs(64, 128, None, 192, 256, 320, 2, 4, 8, 1000, -1, 1000)
+    kw = dict(bad)
+    dtype, ws, n_bytes = kw.pop("dtype", cdna4.F16), kw.pop("ws", P), kw.pop("n_bytes", 1 << 40)
+    for k, v in kw.items():
+        setattr(a, k, v)
+    assert cdna4.lib().cdna4_beam_select(ctypes.byref(a), dtype, ws, n_bytes, None) == 1
+
+
 def test_python_refuses_cpu_tensors():
     c = cache()
     x, t = torch.zeros(3, 2, 128, dtype=torch.float16), torch.zeros(3, 4, dtype=torch.int32)
