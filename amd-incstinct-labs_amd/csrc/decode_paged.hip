@@ -58,8 +58,9 @@ __device__ __forceinline__ int scalar(int x) { return __builtin_amdgcn_readfirst
 __device__ __forceinline__ long long scalar(long long x) {
     return (long long)((uint64_t)(uint32_t)scalar((int)(x >> 32)) << 32 | (uint32_t)scalar((int)x));
 }
-// No branch, and nothing for the compiler to know of the lanes past the batch: it has followed "0 there" through ballots into
-// loops of their own for these lanes, which then took no part in the wave's copies.
+// No branch, and nothing for the compiler to know of the lanes past the batch: with a branch here it follows "0 there" through ballots
+// into loops of their own for these lanes, which then take no part in the wave's copies. tests/test_paged_waves.py follows the masks
+// through the compiled kernels.
 __device__ __forceinline__ int length_of(const PagedArgs& a, int b) {
     int len = min(max(a.lens[min(b, a.batch - 1)], 0), a.max_len);
     len = b < a.batch ? len : 0;
