@@ -274,3 +274,40 @@ def test_outputs_are_off_by_their_own_rounding(D, dtype, nq, fmt, form):
     check(o, *decode_reference(q, p.k, p.v, dtype, attend_two_terms))
     full = torch.randn(q.shape, device=DEV, generator=p.g).to(dtype)
     check(run(p, full, cfg), *decode_reference(full, p.k, p.v, dtype, attend_two_terms))
+
+
+@FORMS
+@pytest.mark.parametrize("fmt", ["16", "mxfp4"])
+@pytest.mark.parametrize("B", [131, 1000, 4099])
+def test_form_of_large_batches(B, fmt, form):
+    """Short tables take one launch at any batch, long ones equal shares, in both formats."""
+    lens = [(37 * i) % 91 if i % 3 else 0 for i in range(B)]
+    p, q, cfg = make(lens, 4, 1, 64, F16, 16, fmt, seed=B, form=form)
+    assert (cdna4.decode_paged_plan(p.cache, cfg).workspace == 0) == (form == "whole")
+    verify(p, q, run(p, q, cfg))
+
+
+@pytest.mark.parametrize("D,B,n", [(128, 600, 1280), (128, 600, 2048), (64, 800, 1600)])
+def test_rounds_of_several_waves_per_item(D, B, n):
+    """MXFP4 in one launch with more waves than the chip holds at once, five to eight chunks in each."""
+    lens = [n if i % 50 == 0 else (97 * i) % (n + 1) if i % 4 else i % 3 for i in range(B)]
+    p, q, cfg = make(lens, 8, 2, D, F16, 256, "mxfp4", seed=22)
+    p.cache.max_pages, p.cache.table_stride = (n + 255) // 256, p.tables.shape[1]
+    plan = cdna4.decode_paged_plan(p.cache, cfg)
+    assert plan.workspace == 0 and plan.waves == 8 and 5 <= p.cache.max_pages * 256 // 32 / 8 <= 8
+    assert plan.grid * plan.waves > 2 * torch.cuda.get_device_properties(DEV).multi_processor_count * 16
+    o = run(p, q, cfg)
+    verify(p, q, o)
+    assert torch.equal(o, run(p, q, cfg))
+
+
+@pytest.mark.parametrize("fmt", ["16", "mxfp4"])
+def test_sequences_alike_give_the_same_bits(fmt):
+    """A workgroup per item knows nothing of the others."""
+    p, q, cfg = make([200], 8, 2, 128, BF16, 32, fmt, seed=23)
+    q5, o = q.repeat(5, 1, 1, 1), torch.empty(5, 1, 8, 128, dtype=BF16, device=DEV)
+    five = cdna4.PagedDecodeCfg(8, 5, 1)
+    assert cdna4.decode_paged_plan(p.cache, five).workspace == 0
+    cdna4.decode_paged(q5, p.K, p.V, p.tables.repeat(5, 1), p.lens.repeat(5), o, p.cache, five)
+    assert all(torch.equal(o[:1], o[i:i + 1]) for i in range(1, 5))
+    verify(p, q, o[:1])
