@@ -15,10 +15,13 @@
 // within 2 %: 148.4 against 148.6 us (128 sequences of 500-4,096 in bf16), 39.8 against 40.5 (two row tiles), 53.7 against 54.7 and
 // 24.9 against 23.9 (MXFP4; there the branch that gave only the first keys a second term spilled registers). MXFP4 values are decoded to
 // the 16-bit type exactly.
-// Bound by HBM where there are keys enough: 128 sequences of 500-4,096 bf16 keys, 32/8 heads, D 128 (902 MB) 141 us in the first launch,
-// 6.4 TB/s, and 4.2 in the join; three of 30,000-131,072 in MXFP4 (267 MB) 46-49 and 6.2. A share's start (its place, its pages' entries, its
-// first keys: three loads behind one another) and the join's take about 15 us of any call, 20-22 + 4.2 us for 64 sequences of 20-4,000
-// in MXFP4 (57 MB), where a wave has four or five chunks. One launch of four sequences of up to 545 keys, 12 heads, D 64: 5.5.
+// More than 32 rows of a kv head (nq G) are items of their own, and each reads the keys again: 16 sequences of 8,000 16-bit keys of one
+// head (66 MB), D 128, in the first launch: 20 rows 20.5 us, 32 rows 21.2, 64 rows 27.6 (134 MB read), 160 rows 56.5 (333 MB).
+// Bound by HBM where there are keys enough: 128 sequences of 500-4,096 bf16 keys, 32/8 heads, D 128 (902 MB) 141-145 us in the first launch,
+// 6.3 TB/s, and 4.4 in the join; three of 30,000-131,072 in MXFP4 (267 MB) 47-54 and 6.2-7.4. A share's start (its place 1.1 us, its pages'
+// entries 0.5, its first keys 1.4: three loads behind one another) and the join's are most of a short call: 64 sequences of 20-4,000
+// in MXFP4 (57 MB) take 19-21 + 4.5 us, where a wave has five chunks of 1.5 us each (half of the waves end 11.4 us after the first one's start,
+// 95 % after 13.6, the last, with many short sequences, after 18). One launch of four sequences of up to 545 keys, 12 heads, D 64: 5.8.
 #include <algorithm>
 #include <math.h>
 
@@ -741,10 +744,13 @@ constexpr int most_waves(int D, int RT, bool fp4) { return D == 64 || (fp4 && RT
 
 // One launch for short caches: the waves per item that end soonest, a round of the chip's waves taken for five chunks' time and those
 // that a wave has; 0: equal shares. Their second launch and the walk over the lengths cost 7-10 us, which up to eight chunks a
-// wave, and of 16-bit rows sixteen over its rounds or four to an item, do not: 16 sequences, 32/8 heads D 128, of 120 keys 4.8 against
-// 16 us, of 1,000 13 against 19; 64 of 1,000 40 against 47, 256 of 250 41 against 49, 4,000 of 120 361 against 430. Beyond, the
-// shares' even ends win: 128 of 1,000 (32 chunks) 95 against 87 us. In MXFP4, where a share's waves have fewer registers, 128 of 1,000 26
-// against 37, 1,600 of 500 165 against 185.
+// wave, and of 16-bit rows sixteen over its rounds or four to an item, do not: 16 sequences, 32/8 heads D 128, of 120 keys 5.0 against
+// 16 us, of 1,000 13 against 19; 64 of 1,000 41 against 47, 256 of 250 41 against 49, 4,000 of 120 377 against 423. Beyond, the
+// shares' even ends win: 128 of 1,000 (32 chunks) 95 against 87 us. In MXFP4, where a share's waves have fewer registers, 128 of 1,000 29
+// against 37, 1,600 of 500 183 against 190. Those are calls that find the Infinity Cache as the one before left it. Behind other work that
+// fills it, one launch wins up to about 70 MB (16 of 1,000 27 against 32, in MXFP4 9.9 against 16 and 64 of 1,000 30 against 38) and loses
+// above (64 of 1,000 82 against 52, 256 of 250 83 against 54, in MXFP4 128 of 1,000 56 against 42), but for many short ones (4,000 of 120
+// 425 against 472); tables with more room than the sequences need (max_pages) take the shares.
 int choose_waves(long long items, int max_len, int D, int RT, bool fp4, long long resident) {
     const int chunks = (max_len + kKeys - 1) / kKeys;
     int best = 0;

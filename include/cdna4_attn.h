@@ -425,7 +425,9 @@ int cdna4_rope_append_paged(const cdna4_append_args* args, const cdna4_paged_cac
  * may hold anything. An infinity or NaN in V makes NaN or
  * infinity of its part of the outputs that see it and of those of up to nq - 1 tokens before. The plan follows from the
  * two structs alone, so a captured call replays on other lengths, tables and pages: tables of few pages take one launch, a workgroup
- * per sequence and row block; longer ones equal shares of all keys, whatever the lengths are, and a second launch. The workspace
+ * per sequence and row block; longer ones equal shares of all keys, whatever the lengths are, and a second launch. Where all lengths of a
+ * call are short, max_pages may be less than the tables have room for, their width given as table_stride, for the one launch. Row
+ * blocks are of 32 rows of a kv head (nq * nQHeads / nKVHeads of them), and each reads the keys: more rows cost as many reads. The workspace
  * (cdna4_attn_decode_paged_workspace_size bytes, 16-byte aligned, no initialisation; 0 for one launch) holds what shares leave of
  * rows that they cut; calls that overlap must not share one. The plan is sized to the current device, so query the size with the
  * device current that the call will run on. batch == 0: nothing is done.
@@ -464,7 +466,7 @@ int cdna4_paged_reorder(const int* parents, const int* tables, const int* lens, 
  * No counterpart in the reference. `groups` groups of `beams` rows of V logits (fp32, fp16 or bf16; row g * beams + b): the n best of a
  * group's beams x V continuations by
  *   score = cum[row] + x_v - log sum_u exp(x_u),
- * best first, equal scores by the lowest row, then the lowest token: scores [groups][n] fp32 (compared in fp64), parents (rows) and
+ * best first, equal scores by the lowest row, then the lowest token, a row's own continuations in the order of their logits whatever cum is: scores [groups][n] fp32 (compared in fp64), parents (rows) and
  * tokens int32. Sums of exponentials are taken in fp32 and joined in fp64. A logit of -inf or NaN is no continuation and adds
  * nothing, +inf counts as the largest fp32 value; rows with cum -inf, +inf or NaN and rows that allow nothing have none. done
  * (int32 [rows], may be NULL): rows that are not 0 there have ended and have one continuation, `eos` at the score cum. Places that no

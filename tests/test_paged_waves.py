@@ -246,3 +246,5 @@ def test_paged_decode_waves_stay_whole(tmp_path):
         body = re.search(rf"^{re.escape(name)}:.*?^\.Lfunc_end", text, re.M | re.S).group(0)
         count, bad = partial_instructions(body.split("\n"))
         assert count > 20 and not bad, f"{name}: {bad[:3]} of {count}"
+    # and nothing spills to memory
+    assert set(re.findall(r"\.amdhsa_private_segment_fixed_size (\d+)", text)) == {"0"}
