@@ -777,11 +777,14 @@ def _pools(K: torch.Tensor, V: torch.Tensor, cache: PagedCache, dtype, dev: int,
 
 def _tables(name: str, t: torch.Tensor, cache: PagedCache, rows: int, dev: int) -> int:
     """Address of the tables of `rows` sequences; where t has rows of its own, they have to be the cache's."""
-    most = cache.max_pages
-    stride = cache.table_stride or most
-    if rows > 0 and t is not None and t.dim() > 1 and (t.shape[-1] < most or (rows > 1 and t.shape[-1] != stride)):
-        raise ValueError(f"{name} must have rows of {stride} entries (table_stride, or max_pages where that is 0)")
-    return _arg(name, t, _I32, (rows - 1) * stride + most if rows > 0 else 0, dev)
+    stride = cache.table_stride or cache.max_pages
+    if t is not None:
+        s = t.shape
+        if len(s) == 2 and s[1] == stride and s[0] >= rows and t.dtype is _I32 and t.get_device() == dev and t.is_contiguous():
+            return t.data_ptr()   # what programs pass
+        if len(s) > 1 and s[-1] != stride and (rows > 1 or rows == 1 and s[-1] < cache.max_pages):
+            raise ValueError(f"{name} must have rows of {stride} entries (table_stride, or max_pages where that is 0)")
+    return _arg(name, t, _I32, (rows - 1) * stride + cache.max_pages if rows > 0 else 0, dev)
 
 
 def _rows(name: str, t: torch.Tensor, dtype, dev: int, shape) -> int:
@@ -789,13 +792,14 @@ def _rows(name: str, t: torch.Tensor, dtype, dev: int, shape) -> int:
     if t.dtype is not dtype or t.get_device() != dev or t.shape != shape:
         raise ValueError(f"{name} must be {dtype} {list(shape)} on GPU {dev}")
     row, head, one = t.stride()
-    if shape[0] < 2:
-        row = 0
-    elif row < shape[1] * shape[2]:   # 0 among them, the stride of a token repeated by expand()
-        raise ValueError(f"{name}'s tokens must not lie over each other")
-    if one != 1 or (head != shape[2] and shape[1] > 1):
+    T, heads, D = shape
+    if one != 1 or (head != D and heads > 1):
         if t.numel():
             raise ValueError(f"{name} must have its heads side by side")
+    if T < 2:
+        return 0
+    if row < heads * D:   # 0 among them, the stride of a token repeated by expand()
+        raise ValueError(f"{name}'s tokens must not lie over each other")
     return row
 
 
