@@ -466,11 +466,12 @@ int cdna4_paged_reorder(const int* parents, const int* tables, const int* lens, 
  * No counterpart in the reference. `groups` groups of `beams` rows of V logits (fp32, fp16 or bf16; row g * beams + b): the n best of a
  * group's beams x V continuations by
  *   score = cum[row] + x_v - log sum_u exp(x_u),
- * best first, equal scores by the lowest row, then the lowest token, a row's own continuations in the order of their logits whatever cum is: scores [groups][n] fp32 (compared in fp64), parents (rows) and
- * tokens int32. Sums of exponentials are taken in fp32 and joined in fp64. A logit of -inf or NaN is no continuation and adds
- * nothing, +inf counts as the largest fp32 value; rows with cum -inf, +inf or NaN and rows that allow nothing have none. done
- * (int32 [rows], may be NULL): rows that are not 0 there have ended and have one continuation, `eos` at the score cum. Places that no
- * continuation fills: score -inf, parent and token -1. scores may be cum where n == beams; outputs must not overlap inputs otherwise. Logits of one row that differ by less than 2^-40 may count as equal.
+ * best first: scores [groups][n] fp32, parents (rows) and tokens int32. Scores are compared in fp64, equal ones by the lowest row; a row's own
+ * continuations stand in the order of their logits whatever cum is, equal logits by the lowest token. Sums of exponentials are taken in fp32
+ * and joined in fp64. A logit of -inf or NaN is no continuation and adds nothing, +inf counts as the largest fp32 value; rows with cum
+ * -inf, +inf or NaN and rows that allow nothing have none. done (int32 [rows], may be NULL): rows that are not 0 there have ended and
+ * have one continuation, `eos` at the score cum. Places that no continuation fills: score -inf, parent and token -1. scores may be cum
+ * where n == beams; outputs must not overlap inputs otherwise.
  * The workspace (cdna4_beam_select_workspace_size bytes for groups * beams rows, 16-byte aligned, no initialisation) must not be
  * shared by calls that overlap; query its size with the device current that the call will run on. groups == 0: nothing is done.
  * Invalid: beams or n not 1 .. 64, V < 1, groups negative, 2^24 rows and more, a logits stride below V, done with an eos outside 0 .. V - 1,

@@ -133,6 +133,17 @@ def test_time_of_equal_logits():
     assert best[1] < 8 * best[0], best
 
 
+def test_order_within_a_row_is_that_of_its_logits():
+    """Also where a large cum leaves nothing of their differences in a score."""
+    x, _ = make(1, 2, 5000, F32, seed=9)
+    x[1] = x[0]
+    for c in (-1e9, -1e20, 1e30):
+        s, p, t = cdna4.beam_select(x, torch.full((2,), c, device=DEV), 1, 8)
+        assert torch.equal(t.long(), x.topk(8, dim=1).indices) and bool((s == c).all())
+    s, p, t = cdna4.beam_select(x, torch.full((2,), -1e20, device=DEV), 2, 8)   # equal scores: the lowest row's
+    assert bool((p == 0).all()) and torch.equal(t[0].long(), x[0].topk(8).indices)
+
+
 def test_masks_and_values_that_are_not_finite():
     x, cum = make(4, 4, 3000, F32, seed=1)
     x[0, 5:] = -math.inf                                     # few tokens allowed
